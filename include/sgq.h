@@ -360,6 +360,85 @@ int sgq_embedding(const float* indices, int64_t n, const float* weight, int64_t 
  * out = x * (1 / sqrt(sum(x^2) / D + eps)) * g.  out may be x. */
 int sgq_rms_norm(const float* x, int64_t rows, int64_t D, const float* g, float eps, float* out, void* stream);
 
+/* ---- 8-bit tokens, 8-bit channels and their product -------------------- */
+
+/* These have no counterpart in the reference: activations ("tokens", the rows of
+ * a matrix) as int8 codes with one fp32 scale per row, weights as int8 codes with
+ * one fp32 scale per output channel (column of W [K, N]), and products of the two
+ * that run on integers and are exact until the scales are applied.  Both sides use
+ * the quantizer of sgq_quantize_int8 (per-channel over rows, columns): m =
+ * max(1e-8, max|v|) where NaN never wins, scale = m / 127, code = clamp(round(v *
+ * (127 / m)), -127, 127), halves away from zero, a NaN value 127.
+ *
+ * Activations and outputs are of one of three element types, rows of `ld`
+ * elements (>= their length); any address aligned to the element will do.  Token
+ * codes: row m at codes + m * ldc, ldc a multiple of 16 of at least
+ * sgq_tokens_row_bytes(K) bytes, 16-byte aligned; the quantizers write zeros from
+ * K up to sgq_tokens_row_bytes(K), the products ignore what stands there.  K is at
+ * most 131071 (SGQ_ERR_UNSUPPORTED past it), which keeps sums exact in int32. */
+#define SGQ_F32 0
+#define SGQ_BF16 1
+#define SGQ_F16 2
+
+/* Bytes of a row of token codes: K rounded up to 128 (at least 128). */
+int64_t sgq_tokens_row_bytes(int64_t K);
+
+/* codes and scales [M] of the rows of x [M, K].  For fp32 x the codes and scales
+ * are sgq_quantize_int8's per-channel ones, bit for bit. */
+int sgq_quantize_tokens(const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, void* codes, int64_t ldc,
+                        float* scales, void* stream);
+
+/* The same of an RMSNorm's output: h = x + residual, rounded to the type, and
+ *   rms_norm(h) = h * g / sqrt(sum(h^2) / K + eps)
+ * row by row, g [K] fp32.  residual NULL: h is x, and the argument h must be NULL;
+ * else h [M, K] is written and may be x or residual itself (with its row stride).
+ * The codes are those of u = fp32(h * g) with m = max(max|u|, 1e-8 / rstd), rstd =
+ * 1 / sqrt(...): the norm's factor is common to a row and changes none of them.
+ * scale = m * rstd / 127.  A row with an infinity or a NaN has a scale of NaN. */
+int sgq_rms_norm_tokens(const void* x, int dtype, int64_t ldx, const void* residual, int64_t ldr, void* h, int64_t ldh,
+                        const float* g, float eps, int64_t M, int64_t K, void* codes, int64_t ldc, float* scales,
+                        void* stream);
+
+/* out[m, k] = code * scales[m], one multiply, rounded to the type. */
+int sgq_dequantize_tokens(const void* codes, int64_t ldc, const float* scales, int64_t M, int64_t K, void* out,
+                          int dtype, int64_t ldo, void* stream);
+
+/* Bytes of a packed [K, N] weight, and of the workspace of the two functions
+ * that build one. */
+int64_t sgq_channels_packed_bytes(int64_t K, int64_t N);
+int64_t sgq_channels_workspace_bytes(int64_t K, int64_t N);
+
+/* scales [N], and optionally the packed buffer and the fp32 codes [K, N], of w. */
+int sgq_quantize_channels(const float* w, int64_t K, int64_t N, float* qdata_f32, float* scales, void* packed,
+                          void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Packs fp32 codes [K, N].  SGQ_ERR_CODES (after synchronising `stream`) when one
+ * is not an integer in [-128, 127]. */
+int sgq_pack_channels(const float* qdata_f32, int64_t K, int64_t N, void* packed, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+
+/* fp32 codes [K, N] of a packed buffer; out[k, n] = code * scales[n]. */
+int sgq_unpack_channels(const void* packed, int64_t K, int64_t N, float* qdata_f32, void* stream);
+int sgq_dequantize_channels(const void* packed, const float* scales, int64_t K, int64_t N, float* out, void* stream);
+
+/* y[m, n] = (sum_k cx[m, k] * cw[k, n]) * x_scales[m] * w_scales[n] + bias[n], the
+ * sum in int32, the rest in fp32, rounded to the type.  bias [N] fp32 or NULL.
+ * K == 0 gives the bias.  workspace: sgq_linear_w8a8_workspace_bytes(M, K, N)
+ * bytes, 16-byte aligned, else SGQ_ERR_WORKSPACE; it needs no initialisation, and
+ * calls that overlap in time must not share one. */
+int64_t sgq_linear_w8a8_workspace_bytes(int64_t M, int64_t K, int64_t N);
+int sgq_linear_w8a8(const void* codes, int64_t ldc, const float* x_scales, int64_t M, int64_t K, int64_t N,
+                    const void* packed, const float* w_scales, const float* bias, void* y, int dtype, int64_t ldy,
+                    void* workspace, int64_t workspace_bytes, void* stream);
+
+/* h = silu(gate) * up of two such products (as sgq_swiglu_int8), in fp32 until it
+ * is rounded to the type. */
+int64_t sgq_swiglu_w8a8_workspace_bytes(int64_t M, int64_t K, int64_t N);
+int sgq_swiglu_w8a8(const void* codes, int64_t ldc, const float* x_scales, int64_t M, int64_t K, int64_t N,
+                    const void* packed_gate, const float* scales_gate, const float* bias_gate, const void* packed_up,
+                    const float* scales_up, const float* bias_up, void* h, int dtype, int64_t ldh, void* workspace,
+                    int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

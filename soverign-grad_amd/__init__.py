@@ -78,6 +78,22 @@ SIGNATURES = {
     "sgq_llama_block_decode_int4": (_int, [_vp, _vp, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp]),
     "sgq_rms_norm": (_int, [_vp, _i64, _i64, _vp, ctypes.c_float, _vp, _vp]),
     "sgq_embedding": (_int, [_vp, _i64, _vp, _i64, _i64, _vp, _vp]),
+    "sgq_tokens_row_bytes": (_i64, [_i64]),
+    "sgq_quantize_tokens": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
+    "sgq_rms_norm_tokens": (_int, [_vp, _int, _i64, _vp, _i64, _vp, _i64, _vp, ctypes.c_float, _i64, _i64, _vp, _i64,
+                                   _vp, _vp]),
+    "sgq_dequantize_tokens": (_int, [_vp, _i64, _vp, _i64, _i64, _vp, _int, _i64, _vp]),
+    "sgq_channels_packed_bytes": (_i64, [_i64, _i64]),
+    "sgq_channels_workspace_bytes": (_i64, [_i64, _i64]),
+    "sgq_quantize_channels": (_int, [_vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "sgq_pack_channels": (_int, [_vp, _i64, _i64, _vp, _vp, _i64, _vp]),
+    "sgq_unpack_channels": (_int, [_vp, _i64, _i64, _vp, _vp]),
+    "sgq_dequantize_channels": (_int, [_vp, _vp, _i64, _i64, _vp, _vp]),
+    "sgq_linear_w8a8_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "sgq_linear_w8a8": (_int, [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _int, _i64, _vp, _i64, _vp]),
+    "sgq_swiglu_w8a8_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "sgq_swiglu_w8a8": (_int, [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _int, _i64, _vp,
+                               _i64, _vp]),
 }
 
 _lib = None

@@ -208,6 +208,11 @@ DecodeWs decode_ws(int64_t B, int64_t D, int64_t H, int64_t max_len) {
     return w;
 }
 
+// Workspace of sgq_quantize_channels / sgq_pack_channels: [column maxima: N
+// floats][bad flag].
+int64_t channels_flag_off(int64_t N) { return align_up((N > 0 ? N : 1) * 4); }
+int64_t channels_ws_bytes(int64_t N) { return channels_flag_off(N) + kAlign; }
+
 bool bad_dims(int64_t a, int64_t b) { return a < 0 || b < 0 || a > kMaxDim || b > kMaxDim || a * b > ((int64_t)1 << 40); }
 
 // The forward kernels address a strip of codes, a scale column and a row of x
@@ -228,6 +233,31 @@ bool forward_fits(int bits, int64_t M, int64_t K, int64_t N, int64_t group_size)
         if (g.tiled && g.spc % 16 != 0 && g.devscale_count() * 4 >= ((int64_t)1 << 32)) return false;
     }
     return true;
+}
+
+bool bad_dtype(int t) { return t != SGQ_F32 && t != SGQ_BF16 && t != SGQ_F16; }
+bool aligned_to(const void* p, int t) { return ((uintptr_t)p) % dtype_bytes((DType)t) == 0; }
+
+// A shape of 8-bit tokens or channels.
+int check_w8a8_shape(const char* fn, int64_t M, int64_t K) {
+    if (bad_dims(M, K)) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: bad shape", fn);
+    if (K > kMaxTokenK)
+        return fail(SGQ_ERR_UNSUPPORTED, "%s: K = %lld is longer than %lld", fn, (long long)K, (long long)kMaxTokenK);
+    return SGQ_OK;
+}
+// A matrix of activations: element type, row stride, address.
+int check_rows(const char* fn, const char* what, const void* p, int dtype, int64_t ld, int64_t K) {
+    if (ld < K || ld > kMaxDim) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: bad row stride of %s", fn, what);
+    if (!p) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: null %s", fn, what);
+    if (!aligned_to(p, dtype)) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: %s is not aligned to its type", fn, what);
+    return SGQ_OK;
+}
+int check_token_codes(const char* fn, const void* codes, int64_t ldc, int64_t K) {
+    if (!codes || !aligned16(codes)) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: codes must be 16-byte aligned", fn);
+    if (ldc % 16 != 0 || ldc < round_up(K, kTokenPadK) || ldc > kMaxDim)
+        return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: rows of codes need a multiple of 16 bytes, at least %lld", fn,
+                    (long long)round_up(K, kTokenPadK));
+    return SGQ_OK;
 }
 
 int check_codes_flag(const int* dflag, hipStream_t s) {
@@ -324,6 +354,36 @@ int linear_int4(const char* fn, const float* x, int64_t M, int64_t K, int64_t N,
         if (lw != SGQ_OK) return lw;
         SGQ_HIP(launch_gemm_i4(x, M, K, N, 1, &packed, &devscales, &bias, g, {}, y, workspace, s), "gemm_i4");
     }
+    return ok();
+}
+
+// One product (ng == 1) or the gated MLP's two of 8-bit tokens.
+int product_w8a8(const char* fn, int ng, const void* codes, int64_t ldc, const float* x_scales, int64_t M, int64_t K,
+                 int64_t N, const void* const* packed, const float* const* scales, const float* const* bias, void* y,
+                 int dtype, int64_t ldy, void* workspace, int64_t workspace_bytes, void* stream) {
+    if (bad_dims(M, K) || bad_dims(K, N) || bad_dims(M, N))
+        return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: bad shape", fn);
+    int st = check_w8a8_shape(fn, M, K);
+    if (st != SGQ_OK) return st;
+    if (bad_dtype(dtype)) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: bad dtype", fn);
+    if (M == 0 || N == 0) return ok();
+    if ((st = check_rows(fn, "output", y, dtype, ldy, N)) != SGQ_OK) return st;
+    W8A8Args a{};
+    for (int q = 0; q < ng; ++q) {
+        if (K > 0 && (!packed[q] || !scales[q])) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: null weight", fn);
+        if (!aligned16(packed[q])) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: packed must be 16-byte aligned", fn);
+        a.w[q] = (const signed char*)packed[q], a.sw[q] = scales[q], a.bias[q] = bias[q];
+    }
+    if (K > 0) {
+        if (!x_scales) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: null scales", fn);
+        if ((st = check_token_codes(fn, codes, ldc, K)) != SGQ_OK) return st;
+    }
+    const int64_t need = w8a8_workspace_bytes(ng, M, K, N);
+    if ((st = check_launch_ws(fn, need, workspace, workspace_bytes)) != SGQ_OK) return st;
+    a.x = (const signed char*)codes, a.ldx = ldc, a.sx = x_scales;
+    a.M = M, a.K = K, a.N = N;
+    a.y = y, a.t = (DType)dtype, a.ldy = ldy;
+    SGQ_HIP(launch_w8a8(a, ng, workspace, (hipStream_t)stream), "w8a8");
     return ok();
 }
 
@@ -933,6 +993,163 @@ int sgq_llama_block_decode_int4(const sgq_llama_block_int4* blk, const float* x,
         SGQ_HIP(decode_project(hid, B, H, D, blk->down, ghd, h, out, split, cus, s), "project_down");
     }
     return ok();
+}
+
+// ---- 8-bit tokens and channels ------------------------------------------
+
+int64_t sgq_tokens_row_bytes(int64_t K) {
+    if (bad_dims(K, 1) || K > kMaxTokenK) return -1;
+    return K == 0 ? kTokenPadK : round_up(K, kTokenPadK);
+}
+
+int64_t sgq_channels_packed_bytes(int64_t K, int64_t N) {
+    if (bad_dims(K, N) || K > kMaxTokenK) return -1;
+    return ChannelsGeom(K, N).bytes();
+}
+
+int64_t sgq_channels_workspace_bytes(int64_t K, int64_t N) {
+    if (bad_dims(K, N) || K > kMaxTokenK) return -1;
+    return channels_ws_bytes(N);
+}
+
+int sgq_quantize_tokens(const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, void* codes, int64_t ldc,
+                        float* scales, void* stream) {
+    const char* fn = "sgq_quantize_tokens";
+    int st = check_w8a8_shape(fn, M, K);
+    if (st != SGQ_OK) return st;
+    if (bad_dtype(dtype)) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: bad dtype", fn);
+    if (M == 0) return ok();
+    if (!scales) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: null scales", fn);
+    if ((st = check_token_codes(fn, codes, ldc, K)) != SGQ_OK) return st;
+    if (K > 0 && (st = check_rows(fn, "x", x, dtype, ldx, K)) != SGQ_OK) return st;
+    SGQ_HIP(launch_tokens(x, (DType)dtype, ldx, nullptr, 0, nullptr, 0, nullptr, 0.0f, M, K, codes, ldc, scales,
+                          (hipStream_t)stream),
+            "tokens");
+    return ok();
+}
+
+int sgq_rms_norm_tokens(const void* x, int dtype, int64_t ldx, const void* residual, int64_t ldr, void* h, int64_t ldh,
+                        const float* g, float eps, int64_t M, int64_t K, void* codes, int64_t ldc, float* scales,
+                        void* stream) {
+    const char* fn = "sgq_rms_norm_tokens";
+    int st = check_w8a8_shape(fn, M, K);
+    if (st != SGQ_OK) return st;
+    if (bad_dtype(dtype)) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: bad dtype", fn);
+    if (M == 0 || K == 0) return ok();
+    if (!scales || !g) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: null pointer", fn);
+    if ((st = check_token_codes(fn, codes, ldc, K)) != SGQ_OK) return st;
+    if ((st = check_rows(fn, "x", x, dtype, ldx, K)) != SGQ_OK) return st;
+    if (residual) {
+        if ((st = check_rows(fn, "residual", residual, dtype, ldr, K)) != SGQ_OK) return st;
+        if ((st = check_rows(fn, "h", h, dtype, ldh, K)) != SGQ_OK) return st;
+        if ((h == x && ldh != ldx) || (h == residual && ldh != ldr))
+            return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: h over an input needs its row stride", fn);
+    } else if (h) {
+        return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: h without a residual", fn);
+    }
+    SGQ_HIP(launch_tokens(x, (DType)dtype, ldx, residual, ldr, h, ldh, g, eps, M, K, codes, ldc, scales,
+                          (hipStream_t)stream),
+            "tokens");
+    return ok();
+}
+
+int sgq_dequantize_tokens(const void* codes, int64_t ldc, const float* scales, int64_t M, int64_t K, void* out,
+                          int dtype, int64_t ldo, void* stream) {
+    const char* fn = "sgq_dequantize_tokens";
+    int st = check_w8a8_shape(fn, M, K);
+    if (st != SGQ_OK) return st;
+    if (bad_dtype(dtype)) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: bad dtype", fn);
+    if (M == 0 || K == 0) return ok();
+    if (!scales) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: null scales", fn);
+    if ((st = check_token_codes(fn, codes, ldc, K)) != SGQ_OK) return st;
+    if ((st = check_rows(fn, "out", out, dtype, ldo, K)) != SGQ_OK) return st;
+    SGQ_HIP(launch_tokens_values(codes, ldc, scales, M, K, out, (DType)dtype, ldo, (hipStream_t)stream),
+            "tokens_values");
+    return ok();
+}
+
+int sgq_quantize_channels(const float* w, int64_t K, int64_t N, float* qdata_f32, float* scales, void* packed,
+                          void* workspace, int64_t workspace_bytes, void* stream) {
+    const char* fn = "sgq_quantize_channels";
+    const int st = check_w8a8_shape(fn, N, K);
+    if (st != SGQ_OK) return st;
+    if (N == 0) return ok();
+    if (!scales || (K > 0 && !w)) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: null pointer", fn);
+    if (packed && !aligned16(packed)) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: packed must be 16-byte aligned", fn);
+    if (!workspace || workspace_bytes < channels_ws_bytes(N))
+        return fail(SGQ_ERR_WORKSPACE, "%s: workspace needs %lld bytes", fn, (long long)channels_ws_bytes(N));
+    if (!aligned16(workspace)) return fail(SGQ_ERR_WORKSPACE, "%s: workspace must be 16-byte aligned", fn);
+    SGQ_HIP(launch_channels_quantize(w, K, N, qdata_f32, scales, packed, workspace, (hipStream_t)stream),
+            "channels_quantize");
+    return ok();
+}
+
+int sgq_pack_channels(const float* qdata_f32, int64_t K, int64_t N, void* packed, void* workspace,
+                      int64_t workspace_bytes, void* stream) {
+    const char* fn = "sgq_pack_channels";
+    const int st = check_w8a8_shape(fn, N, K);
+    if (st != SGQ_OK) return st;
+    if (K == 0 || N == 0) return ok();
+    if (!qdata_f32 || !packed || !aligned16(packed))
+        return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: null or unaligned pointer", fn);
+    if (!workspace || workspace_bytes < channels_ws_bytes(N))
+        return fail(SGQ_ERR_WORKSPACE, "%s: workspace needs %lld bytes", fn, (long long)channels_ws_bytes(N));
+    if (!aligned16(workspace)) return fail(SGQ_ERR_WORKSPACE, "%s: workspace must be 16-byte aligned", fn);
+    int* bad = (int*)((char*)workspace + channels_flag_off(N));
+    hipStream_t s = (hipStream_t)stream;
+    SGQ_HIP(launch_fill_zero(bad, kAlign, s), "fill_zero(flag)");
+    SGQ_HIP(launch_channels_pack(qdata_f32, K, N, packed, bad, s), "channels_pack");
+    return check_codes_flag(bad, s);
+}
+
+int sgq_unpack_channels(const void* packed, int64_t K, int64_t N, float* qdata_f32, void* stream) {
+    const char* fn = "sgq_unpack_channels";
+    const int st = check_w8a8_shape(fn, N, K);
+    if (st != SGQ_OK) return st;
+    if (K == 0 || N == 0) return ok();
+    if (!packed || !aligned16(packed) || !qdata_f32)
+        return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: null or unaligned pointer", fn);
+    SGQ_HIP(launch_channels_unpack(packed, K, N, nullptr, qdata_f32, (hipStream_t)stream), "channels_unpack");
+    return ok();
+}
+
+int sgq_dequantize_channels(const void* packed, const float* scales, int64_t K, int64_t N, float* out, void* stream) {
+    const char* fn = "sgq_dequantize_channels";
+    const int st = check_w8a8_shape(fn, N, K);
+    if (st != SGQ_OK) return st;
+    if (K == 0 || N == 0) return ok();
+    if (!packed || !aligned16(packed) || !scales || !out)
+        return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: null or unaligned pointer", fn);
+    SGQ_HIP(launch_channels_unpack(packed, K, N, scales, out, (hipStream_t)stream), "channels_unpack");
+    return ok();
+}
+
+int64_t sgq_linear_w8a8_workspace_bytes(int64_t M, int64_t K, int64_t N) {
+    if (bad_dims(M, K) || bad_dims(K, N) || bad_dims(M, N) || K > kMaxTokenK) return -1;
+    return w8a8_workspace_bytes(1, M, K, N);
+}
+
+int64_t sgq_swiglu_w8a8_workspace_bytes(int64_t M, int64_t K, int64_t N) {
+    if (bad_dims(M, K) || bad_dims(K, N) || bad_dims(M, N) || K > kMaxTokenK) return -1;
+    return w8a8_workspace_bytes(2, M, K, N);
+}
+
+int sgq_linear_w8a8(const void* codes, int64_t ldc, const float* x_scales, int64_t M, int64_t K, int64_t N,
+                    const void* packed, const float* w_scales, const float* bias, void* y, int dtype, int64_t ldy,
+                    void* workspace, int64_t workspace_bytes, void* stream) {
+    return product_w8a8("sgq_linear_w8a8", 1, codes, ldc, x_scales, M, K, N, &packed, &w_scales, &bias, y, dtype, ldy,
+                        workspace, workspace_bytes, stream);
+}
+
+int sgq_swiglu_w8a8(const void* codes, int64_t ldc, const float* x_scales, int64_t M, int64_t K, int64_t N,
+                    const void* packed_gate, const float* scales_gate, const float* bias_gate, const void* packed_up,
+                    const float* scales_up, const float* bias_up, void* h, int dtype, int64_t ldh, void* workspace,
+                    int64_t workspace_bytes, void* stream) {
+    const void* packed[2] = {packed_gate, packed_up};
+    const float* scales[2] = {scales_gate, scales_up};
+    const float* bias[2] = {bias_gate, bias_up};
+    return product_w8a8("sgq_swiglu_w8a8", 2, codes, ldc, x_scales, M, K, N, packed, scales, bias, h, dtype, ldh,
+                        workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

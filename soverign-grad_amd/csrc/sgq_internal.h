@@ -106,6 +106,25 @@ struct I4Geom {
     int64_t devscale_count() const { return tiled ? nsc * Kpad : 0; }
 };
 
+// 8-bit tokens times 8-bit weights.  A row of token codes is plain row-major int8,
+// K rounded up to kTokenPadK bytes.  A weight with a scale per output channel is
+// held in chunks of 16 consecutive k of one column: chunk (column block cb, k chunk
+// kc, column c) at ((cb * KC + kc) * 16 + c) * 16, sixteen columns to a block,
+// KC = Kpad / 16; codes past K and N are 0, so what a token's row holds past K does
+// not matter.  Four consecutive k chunks of a block are the 1024 bytes of an
+// operand of v_mfma_i32_16x16x64_i8, lane t's sixteen at byte 16 t, and a column
+// block is one contiguous run over K.
+constexpr int64_t kTokenPadK = 128;
+constexpr int64_t kMaxTokenK = 131071;  // K * 128 * 128 < 2^31: sums stay exact in int32
+struct ChannelsGeom {
+    int64_t Kpad, KC, NB;
+    __host__ __device__ ChannelsGeom(int64_t k, int64_t n)
+        : Kpad(round_up(k, kTokenPadK)), KC(Kpad / 16), NB(ceil_div(n, 16)) {}
+    int64_t bytes() const { return NB * KC * 256; }
+};
+enum class DType : int { f32 = 0, bf16 = 1, f16 = 2 };
+constexpr int64_t dtype_bytes(DType t) { return t == DType::f32 ? 4 : 2; }
+
 constexpr int kGemvMaxM = 16;  // up to this many rows never run the MFMA GEMM (but see below)
 // The plain forward also runs the GEMV for batches of up to this many rows
 // (row groups of 8, one workgroup each) when the work is small: the GEMV's
@@ -489,5 +508,37 @@ int64_t attn_workspace_floats(int64_t B, int64_t D, int64_t max_len);
 hipError_t launch_attention_decode(const float* q, const float* knew, const float* vnew, int64_t ldq, int64_t B,
                                    int64_t D, float* kc, float* vc, int64_t max_tokens, const int32_t* pos,
                                    int64_t max_len, float scale, float* part, float* ctx, hipStream_t s);
+
+
+// ---- 8-bit tokens and their products (sgq_tokens.hip, sgq_w8a8.hip) ------
+// Rows of x [M, K] as codes and scales.  g (optional): of the RMSNorm of h = x + r
+// (r optional; h is then written); without g the rows of x themselves.
+hipError_t launch_tokens(const void* x, DType t, int64_t ldx, const void* r, int64_t ldr, void* h, int64_t ldh,
+                         const float* g, float eps, int64_t M, int64_t K, void* codes, int64_t ldc, float* scales,
+                         hipStream_t s);
+hipError_t launch_tokens_values(const void* codes, int64_t ldc, const float* scales, int64_t M, int64_t K, void* out,
+                                DType t, int64_t ldo, hipStream_t s);
+// Weights [K, N] with a scale per column.  top: N floats of workspace; qdata and
+// packed optional.
+hipError_t launch_channels_quantize(const float* w, int64_t K, int64_t N, float* qdata, float* scales, void* packed,
+                                    void* top, hipStream_t s);
+hipError_t launch_channels_pack(const float* codes, int64_t K, int64_t N, void* packed, int* bad, hipStream_t s);
+hipError_t launch_channels_unpack(const void* packed, int64_t K, int64_t N, const float* scales, float* out,
+                                  hipStream_t s);
+struct W8A8Args {
+    const signed char* x;  // token codes, rows of ldx bytes
+    int64_t ldx;
+    const float* sx;
+    int64_t M, K, N;
+    const signed char* w[2];  // packed weights: one, or the gated MLP's gate and up
+    const float* sw[2];
+    const float* bias[2];
+    void* y;  // [M, N] of type t, rows of ldy elements
+    DType t;
+    int64_t ldy;
+};
+// Bytes of workspace of ng products of this shape on any device.
+int64_t w8a8_workspace_bytes(int ng, int64_t M, int64_t K, int64_t N);
+hipError_t launch_w8a8(const W8A8Args& a, int ng, void* ws, hipStream_t s);
 
 }  // namespace sgq

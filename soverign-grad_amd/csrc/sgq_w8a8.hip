@@ -1,0 +1,224 @@
+// sgq_w8a8.hip -- int8 tokens times int8 weights on the matrix cores (gfx950),
+// and the layout of such weights.
+//
+// Mathematics.  acc[m,n] = sum_k cx[m,k] * cw[k,n] in int32, exact while K * 128^2
+// < 2^31, so neither the order of the sum nor a split of K changes a bit;
+// y = (acc * sx[m]) * sw[n] + bias[n] in fp32, rounded once more to the output's
+// type.  The gated form takes two such products and h = silu(gate) * up.
+#include "sgq_device.h"
+#include "sgq_internal.h"
+
+namespace sgq {
+namespace {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kWG = 256;
+
+__device__ __forceinline__ float ref_max(float m, float a) { return (a > m) ? a : m; }
+
+// ---- weights ------------------------------------------------------------
+
+constexpr int kTileK = 128, kTileN = 64;  // of the pack kernels: one workgroup
+
+// top[n] (bits of a float, starting at 1e-8) = max |w[k][n]|, NaN never winning.
+// A maximum does not depend on the order the workgroups come in, and floats of
+// one sign compare as their bits do.
+__global__ void k_channels_start(uint32_t* __restrict__ top, int64_t N) {
+    const int64_t n = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
+    if (n < N) top[n] = __float_as_uint(1e-8f);
+}
+
+__global__ __launch_bounds__(kWG) void k_channels_top(const float* __restrict__ w, int64_t K, int64_t N, int64_t rows,
+                                                      uint32_t* __restrict__ top) {
+    __shared__ float red[kWG / 64][64];
+    const int64_t n = blockIdx.x * (int64_t)64 + (threadIdx.x & 63);
+    const int64_t k0 = blockIdx.y * rows, k1 = min(K, k0 + rows);
+    float m = 0.0f;
+    if (n < N)
+#pragma unroll 8
+        for (int64_t k = k0 + (threadIdx.x >> 6); k < k1; k += kWG / 64) m = ref_max(m, fabsf(w[k * N + n]));
+    red[threadIdx.x >> 6][threadIdx.x & 63] = m;
+    __syncthreads();
+    if (threadIdx.x < 64 && n < N) {
+#pragma unroll
+        for (int q = 1; q < kWG / 64; ++q) m = ref_max(m, red[q][threadIdx.x]);
+        atomicMax(top + n, __float_as_uint(m));
+    }
+}
+
+// Codes of a kTileK x kTileN tile: FROM_CODES reads fp32 codes (validated into
+// *bad), else w with the columns' maxima in top; through LDS into the layout.
+template <bool FROM_CODES>
+__global__ __launch_bounds__(kWG) void k_channels_pack(const float* __restrict__ src, int64_t K, int64_t N, int64_t nkt,
+                                                       const uint32_t* __restrict__ top, float* __restrict__ scales,
+                                                       float* __restrict__ qdata, signed char* __restrict__ packed,
+                                                       int* __restrict__ bad) {
+#pragma clang fp contract(off)
+    __shared__ __attribute__((aligned(16))) signed char col[kTileN][kTileK + 16];
+    const int64_t kt = blockIdx.x % nkt, nt = blockIdx.x / nkt;
+    const int c = threadIdx.x & 63;
+    const int64_t n = nt * kTileN + c;
+    float inv = 0.0f;
+    if (!FROM_CODES && n < N) {
+        const float m = __uint_as_float(top[n]);
+        inv = 127.0f / m;
+        if (kt == 0 && threadIdx.x < 64) scales[n] = m / 127.0f;
+    }
+    bool wrong = false;
+    for (int r = threadIdx.x >> 6; r < kTileK; r += kWG / 64) {
+        const int64_t k = kt * kTileK + r;
+        float v = 0.0f;
+        if (k < K && n < N) {
+            v = src[k * N + n];
+            if constexpr (FROM_CODES) {
+                if (!(v == truncf(v) && v >= -128.0f && v <= 127.0f)) wrong = true, v = 0.0f;
+            } else {
+                v = roundf(v * inv);
+                v = (v < 127.0f) ? v : 127.0f;
+                v = (-127.0f < v) ? v : -127.0f;
+                if (qdata) qdata[k * N + n] = v;
+            }
+        }
+        col[c][r] = (signed char)(int)v;
+    }
+    if (wrong) atomicOr(bad, 1);
+    if (!packed) return;
+    __syncthreads();
+    // Chunk t: column t % 16 of column block t / 128, k chunk (t / 16) % 8.
+    const ChannelsGeom g(K, N);
+    for (int t = threadIdx.x; t < kTileN * kTileK / 16; t += kWG) {
+        const int cb = t >> 7, kc = (t >> 4) & 7, cc = t & 15;
+        const int64_t gcb = nt * (kTileN / 16) + cb;
+        if (gcb < g.NB)
+            *(uint4*)(packed + ((gcb * g.KC + kt * (kTileK / 16) + kc) * 16 + cc) * 16) =
+                *(const uint4*)&col[16 * cb + cc][16 * kc];
+    }
+}
+
+// out[k][n] = code (* scales[n]).
+__global__ __launch_bounds__(kWG) void k_channels_unpack(const signed char* __restrict__ packed, int64_t K, int64_t N,
+                                                         int64_t nkt, const float* __restrict__ scales,
+                                                         float* __restrict__ out) {
+    __shared__ __attribute__((aligned(16))) signed char col[kTileN][kTileK + 16];
+    const int64_t kt = blockIdx.x % nkt, nt = blockIdx.x / nkt;
+    const ChannelsGeom g(K, N);
+    for (int t = threadIdx.x; t < kTileN * kTileK / 16; t += kWG) {
+        const int cb = t >> 7, kc = (t >> 4) & 7, cc = t & 15;
+        const int64_t gcb = nt * (kTileN / 16) + cb;
+        if (gcb < g.NB)
+            *(uint4*)&col[16 * cb + cc][16 * kc] =
+                *(const uint4*)(packed + ((gcb * g.KC + kt * (kTileK / 16) + kc) * 16 + cc) * 16);
+    }
+    __syncthreads();
+    const int c = threadIdx.x & 63;
+    const int64_t n = nt * kTileN + c;
+    if (n >= N) return;
+    const float s = scales ? scales[n] : 1.0f;
+    for (int r = threadIdx.x >> 6; r < kTileK; r += kWG / 64) {
+        const int64_t k = kt * kTileK + r;
+        if (k < K) out[k * N + n] = scales ? (float)col[c][r] * s : (float)col[c][r];
+    }
+}
+
+// ---- products -----------------------------------------------------------
+
+template <typename T>
+__device__ __forceinline__ void store1(void* y, int64_t o, float v) {
+    ((T*)y)[o] = (T)v;
+}
+__device__ __forceinline__ void store_as(void* y, DType t, int64_t o, float v) {
+    if (t == DType::f32)
+        store1<float>(y, o, v);
+    else if (t == DType::bf16)
+        store1<__bf16>(y, o, v);
+    else
+        store1<_Float16>(y, o, v);
+}
+
+__device__ __forceinline__ float product(int acc, float sx, float sw, float b) {
+#pragma clang fp contract(off)
+    return ((float)acc * sx) * sw + b;
+}
+
+// A wavefront per 16 tokens by 16 columns, operands straight from memory.  A
+// lane's A operand is a chunk of the packed weight (column lane & 15, k chunk lane
+// >> 4), its B operand 16 codes of token lane & 15, so that it ends up with four
+// neighbouring columns of one token.
+template <int NG>
+__global__ __launch_bounds__(kWG) void k_w8a8_simple(const W8A8Args a) {
+    const int lane = threadIdx.x & 63, lr = lane & 15, g = lane >> 4;
+    const int64_t wave = (int64_t)blockIdx.x * (kWG / 64) + (threadIdx.x >> 6);
+    const ChannelsGeom geo(a.K, a.N);
+    if (wave >= geo.NB * ceil_div(a.M, 16)) return;
+    const int64_t cb = wave % geo.NB, mb = wave / geo.NB;
+    const int64_t m = mb * 16 + lr;
+    const signed char* x = a.x + (m < a.M ? m : a.M - 1) * a.ldx + 16 * g;
+    i32x4 acc[NG];
+#pragma unroll
+    for (int q = 0; q < NG; ++q) acc[q] = i32x4{0, 0, 0, 0};
+    for (int64_t kc = 0; kc < geo.KC; kc += 4) {
+        const i32x4 b = *(const i32x4*)(x + 16 * kc);
+#pragma unroll
+        for (int q = 0; q < NG; ++q) {
+            const i32x4 w = *(const i32x4*)(a.w[q] + ((cb * geo.KC + kc) * 16 + lane) * 16);
+            acc[q] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, b, acc[q], 0, 0, 0);
+        }
+    }
+    if (m >= a.M) return;
+    const float sx = a.K > 0 ? a.sx[m] : 0.0f;  // K = 0: the biases
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int64_t n = cb * 16 + 4 * g + r;
+        if (n >= a.N) break;
+        float v = product(acc[0][r], sx, a.K > 0 ? a.sw[0][n] : 0.0f, a.bias[0] ? a.bias[0][n] : 0.0f);
+        if constexpr (NG == 2)
+            v = silu_f32(v) * product(acc[1][r], sx, a.K > 0 ? a.sw[1][n] : 0.0f, a.bias[1] ? a.bias[1][n] : 0.0f);
+        store_as(a.y, a.t, m * a.ldy + n, v);
+    }
+}
+
+}  // namespace
+
+hipError_t launch_channels_quantize(const float* w, int64_t K, int64_t N, float* qdata, float* scales, void* packed,
+                                    void* top, hipStream_t s) {
+    k_channels_start<<<(unsigned)ceil_div(N, kWG), kWG, 0, s>>>((uint32_t*)top, N);
+    const int64_t rows = 256;
+    if (K > 0) {
+        const dim3 grid((unsigned)ceil_div(N, 64), (unsigned)ceil_div(K, rows));
+        k_channels_top<<<grid, kWG, 0, s>>>(w, K, N, rows, (uint32_t*)top);
+    }
+    const int64_t nkt = K > 0 ? ceil_div(K, kTileK) : 1;
+    k_channels_pack<false><<<(unsigned)(nkt * ceil_div(N, kTileN)), kWG, 0, s>>>(
+        w, K, N, nkt, (const uint32_t*)top, scales, qdata, K > 0 ? (signed char*)packed : nullptr, nullptr);
+    return hipGetLastError();
+}
+
+hipError_t launch_channels_pack(const float* codes, int64_t K, int64_t N, void* packed, int* bad, hipStream_t s) {
+    const int64_t nkt = ceil_div(K, kTileK);
+    k_channels_pack<true><<<(unsigned)(nkt * ceil_div(N, kTileN)), kWG, 0, s>>>(codes, K, N, nkt, nullptr, nullptr,
+                                                                               nullptr, (signed char*)packed, bad);
+    return hipGetLastError();
+}
+
+hipError_t launch_channels_unpack(const void* packed, int64_t K, int64_t N, const float* scales, float* out,
+                                  hipStream_t s) {
+    const int64_t nkt = ceil_div(K, kTileK);
+    k_channels_unpack<<<(unsigned)(nkt * ceil_div(N, kTileN)), kWG, 0, s>>>((const signed char*)packed, K, N, nkt,
+                                                                           scales, out);
+    return hipGetLastError();
+}
+
+int64_t w8a8_workspace_bytes(int, int64_t, int64_t, int64_t) { return 0; }
+
+hipError_t launch_w8a8(const W8A8Args& a, int ng, void*, hipStream_t s) {
+    const int64_t waves = ChannelsGeom(a.K, a.N).NB * ceil_div(a.M, 16);
+    const unsigned grid = (unsigned)ceil_div(waves, kWG / 64);
+    if (ng == 2)
+        k_w8a8_simple<2><<<grid, kWG, 0, s>>>(a);
+    else
+        k_w8a8_simple<1><<<grid, kWG, 0, s>>>(a);
+    return hipGetLastError();
+}
+
+}  // namespace sgq
