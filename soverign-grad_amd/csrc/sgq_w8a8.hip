@@ -178,6 +178,147 @@ __global__ __launch_bounds__(kWG) void k_w8a8_simple(const W8A8Args a) {
     }
 }
 
+
+// ---- the tile kernel ------------------------------------------------------
+
+typedef __attribute__((address_space(3))) void lds_void;
+
+constexpr int kStage = 128;  // k per stage
+
+template <int NG, int BM, int BN, int WM, int WN>
+struct TileCfg {
+    static constexpr int kThreads = 64 * WM * WN;
+    static constexpr int TM = BM / WM / 16;       // token blocks of a wavefront
+    static constexpr int TN = BN / WN / 16;       // column blocks of a wavefront, NG > 1: of all weights
+    static constexpr int kXLoads = BM * kStage / 16 / kThreads;  // 16-byte loads a thread and stage
+    static constexpr int kWLoads = BN * kStage / 16 / kThreads;
+};
+
+template <int NG, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void k_w8a8_tile(const W8A8Args a, int tiles_m, int tiles_n, int xlog) {
+    using C = TileCfg<NG, BM, BN, WM, WN>;
+    constexpr int TM = C::TM, TN = C::TN;
+    __shared__ __attribute__((aligned(128))) signed char xs0[BM * kStage], xs1[BM * kStage];
+    __shared__ __attribute__((aligned(128))) signed char ws0[BN * kStage], ws1[BN * kStage];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lr = lane & 15, g = lane >> 4;
+    const int wm = wave / WN, wn = wave % WN;
+
+    // Tiles in groups of eight rows of tiles, column by column.
+    const int b = xcd_swizzle(blockIdx.x, gridDim.x, xlog);
+    constexpr int kGroup = 8;
+    const int group = b / (kGroup * tiles_n), in = b - group * (kGroup * tiles_n);
+    const int gm = min(kGroup, tiles_m - group * kGroup);
+    const int tm = group * kGroup + in % gm, tn = in / gm;
+
+    const int64_t m0 = (int64_t)tm * BM;
+    const ChannelsGeom geo(a.K, a.N);
+    const int64_t cb0 = (int64_t)tn * (BN / 16 / NG);  // first column block of each weight
+    const int rows = (int)min((int64_t)BM, a.M - m0), ncb = (int)min((int64_t)(BN / 16 / NG), geo.NB - cb0);
+    const int ldx = (int)a.ldx, cbytes = (int)geo.KC * 256;
+    const signed char* const xp = a.x + m0 * a.ldx;
+    const uint32_t xbytes = (uint32_t)((rows - 1) * ldx) + (uint32_t)geo.Kpad, wbytes = (uint32_t)ncb * (uint32_t)cbytes;
+    const int n = (int)(geo.Kpad / kStage);
+
+    // A stage's loads.  Tokens: eight rows of 128 bytes a wavefront and load, the 16-byte
+    // chunk at place p of row r being chunk p ^ (r & 7) (no bank twice when sixteen rows
+    // are read at one k).  Weights: the layout as it is, half a column block a load.
+    const int xrow = lane >> 3, xoff = ((lane & 7) ^ xrow) * 16;
+    // Past the last stage the buffers have no bytes: the loads are issued (the compiler
+    // counts them to know which ones a read has to wait for) and fetch nothing.
+    auto load = [&](signed char* xs, signed char* ws, int s) {
+        const __amdgpu_buffer_rsrc_t rx = make_rsrc(xp, s < n ? xbytes : 0);
+#pragma unroll
+        for (int i = 0; i < C::kXLoads; ++i) {
+            const int r = (i * (C::kThreads / 64) + wave) * 8;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lds_void*)(xs + r * kStage), 16, (r + xrow) * ldx + xoff, s * kStage, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < C::kWLoads; ++i) {
+            const int u = i * (C::kThreads / 64) + wave;  // of 1024 bytes
+            const int q = NG == 1 ? 0 : i / (C::kWLoads / NG);
+            const int v = NG == 1 ? u : u - q * (BN / NG / 8);
+            const __amdgpu_buffer_rsrc_t rw = make_rsrc(a.w[q] + cb0 * cbytes, s < n ? wbytes : 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_void*)(ws + u * 1024), 16, (v >> 1) * cbytes + (v & 1) * 1024 + lane * 16, s * 2048, 0, 0);
+        }
+    };
+    // Operands of half a stage: 64 k.
+    auto read = [&](i32x4 (&x)[TM], i32x4 (&w)[TN], const signed char* xs, const signed char* ws, int h) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+            x[i] = *(const i32x4*)(xs + (wm * (BM / WM) + i * 16 + lr) * kStage + (((4 * h + g) ^ (lr & 7)) * 16));
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+            // NG weights: each wavefront has the same columns of all.
+            const int cb = NG == 1 ? wn * TN + j : (j / (TN / NG)) * (BN / 16 / NG) + wn * (TN / NG) + j % (TN / NG);
+            w[j] = *(const i32x4*)(ws + cb * 2048 + h * 1024 + lane * 16);
+        }
+    };
+    i32x4 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+    auto mfma = [&](const i32x4 (&x)[TM], const i32x4 (&w)[TN]) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int i = 0; i < TM; ++i) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[j], x[i], acc[i][j], 0, 0, 0);
+    };
+
+    i32x4 x0[TM], w0[TN], x1[TM], w1[TN];
+    load(xs0, ws0, 0);
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    load(xs1, ws1, 1);
+    read(x0, w0, xs0, ws0, 0);
+    auto step = [&](signed char* xs, signed char* ws, const signed char* xn, const signed char* wsn, int s) {
+        read(x1, w1, xs, ws, 1);
+        __builtin_amdgcn_sched_barrier(0);
+        mfma(x0, w0);
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        load(xs, ws, s + 2);
+        read(x0, w0, xn, wsn, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        mfma(x1, w1);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    for (int s = 0; s < n - 1; s += 2) {
+        step(xs0, ws0, xs1, ws1, s);
+        step(xs1, ws1, xs0, ws0, s + 1);
+    }
+    if (n & 1) step(xs0, ws0, xs1, ws1, n - 1);
+    // No load may still be writing to LDS when the workgroup's share of it is given away.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+
+    // A lane has columns 4 g .. 4 g + 3 of a block, of token lr.
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+        const int64_t m = m0 + wm * (BM / WM) + i * 16 + lr;
+        if (m >= a.M) continue;
+        const float sx = a.sx[m];
+#pragma unroll
+        for (int j = 0; j < TN / NG; ++j) {
+            const int64_t nn = (cb0 + wn * (TN / NG) + j) * 16 + 4 * g;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if (nn + r >= a.N) break;
+                float v = product(acc[i][j][r], sx, a.sw[0][nn + r], a.bias[0] ? a.bias[0][nn + r] : 0.0f);
+                if constexpr (NG == 2)
+                    v = silu_f32(v) * product(acc[i][j + TN / 2][r], sx, a.sw[1][nn + r], a.bias[1] ? a.bias[1][nn + r] : 0.0f);
+                store_as(a.y, a.t, m * a.ldy + nn + r, v);
+            }
+        }
+    }
+}
+
+template <int NG, int BM, int BN, int WM, int WN>
+hipError_t launch_tile(const W8A8Args& a, hipStream_t s) {
+    const int64_t tm = ceil_div(a.M, BM), tn = ceil_div(ChannelsGeom(a.K, a.N).NB, BN / 16 / NG);
+    k_w8a8_tile<NG, BM, BN, WM, WN><<<(unsigned)(tm * tn), 64 * WM * WN, 0, s>>>(a, (int)tm, (int)tn, xcd_log2(device_xcds(s)));
+    return hipGetLastError();
+}
+
 }  // namespace
 
 hipError_t launch_channels_quantize(const float* w, int64_t K, int64_t N, float* qdata, float* scales, void* packed,
@@ -212,6 +353,7 @@ hipError_t launch_channels_unpack(const void* packed, int64_t K, int64_t N, cons
 int64_t w8a8_workspace_bytes(int, int64_t, int64_t, int64_t) { return 0; }
 
 hipError_t launch_w8a8(const W8A8Args& a, int ng, void*, hipStream_t s) {
+    if (a.K > 0 && a.M > 128) return ng == 2 ? launch_tile<2, 256, 256, 4, 2>(a, s) : launch_tile<1, 256, 256, 4, 2>(a, s);
     const int64_t waves = ChannelsGeom(a.K, a.N).NB * ceil_div(a.M, 16);
     const unsigned grid = (unsigned)ceil_div(waves, kWG / 64);
     if (ng == 2)
