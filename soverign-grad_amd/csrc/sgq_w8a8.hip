@@ -123,29 +123,60 @@ __global__ __launch_bounds__(kWG) void k_channels_unpack(const signed char* __re
 
 // ---- products -----------------------------------------------------------
 
+// Four neighbouring values of type T at an address of T's alignment.
 template <typename T>
-__device__ __forceinline__ void store1(void* y, int64_t o, float v) {
-    ((T*)y)[o] = (T)v;
-}
-__device__ __forceinline__ void store_as(void* y, DType t, int64_t o, float v) {
-    if (t == DType::f32)
-        store1<float>(y, o, v);
-    else if (t == DType::bf16)
-        store1<__bf16>(y, o, v);
-    else
-        store1<_Float16>(y, o, v);
+struct Four {
+    typedef T type __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+};
+typedef Four<float>::type f32x4_u;
+
+// (acc * sx) * sw + bias of four neighbouring columns.
+__device__ __forceinline__ floatx4 product4(i32x4 acc, float sx, floatx4 sw, floatx4 b) {
+#pragma clang fp contract(off)
+    floatx4 v;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = ((float)acc[r] * sx) * sw[r] + b[r];
+    return v;
 }
 
-__device__ __forceinline__ float product(int acc, float sx, float sw, float b) {
-#pragma clang fp contract(off)
-    return ((float)acc * sx) * sw + b;
+// v rounded to T into columns n .. n + 3 of a row, those below N.
+template <typename T>
+__device__ __forceinline__ void store4(T* row, int64_t n, int64_t N, floatx4 v) {
+    typename Four<T>::type o;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o[r] = (T)v[r];
+    if (n + 4 <= N) {
+        *(typename Four<T>::type*)(row + n) = o;
+    } else {
+#pragma unroll
+        for (int r = 0; r < 3; ++r)
+            if (n + r < N) row[n + r] = o[r];
+    }
+}
+
+__device__ __forceinline__ floatx4 silu_mul4(floatx4 g, floatx4 u) {
+    floatx4 v;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = silu_f32(g[r]) * u[r];
+    return v;
+}
+
+// v[n .. n + 3], zeros from N on or without v.
+__device__ __forceinline__ floatx4 load4(const float* v, int64_t n, int64_t N) {
+    if (v && n + 4 <= N) return *(const f32x4_u*)(v + n);
+    floatx4 o = {0.f, 0.f, 0.f, 0.f};
+    if (v)
+#pragma unroll
+        for (int r = 0; r < 3; ++r)
+            if (n + r < N) o[r] = v[n + r];
+    return o;
 }
 
 // A wavefront per 16 tokens by 16 columns, operands straight from memory.  A
 // lane's A operand is a chunk of the packed weight (column lane & 15, k chunk lane
 // >> 4), its B operand 16 codes of token lane & 15, so that it ends up with four
 // neighbouring columns of one token.
-template <int NG>
+template <int NG, typename T>
 __global__ __launch_bounds__(kWG) void k_w8a8_simple(const W8A8Args a) {
     const int lane = threadIdx.x & 63, lr = lane & 15, g = lane >> 4;
     const int64_t wave = (int64_t)blockIdx.x * (kWG / 64) + (threadIdx.x >> 6);
@@ -166,18 +197,14 @@ __global__ __launch_bounds__(kWG) void k_w8a8_simple(const W8A8Args a) {
         }
     }
     if (m >= a.M) return;
-    const float sx = a.K > 0 ? a.sx[m] : 0.0f;  // K = 0: the biases
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int64_t n = cb * 16 + 4 * g + r;
-        if (n >= a.N) break;
-        float v = product(acc[0][r], sx, a.K > 0 ? a.sw[0][n] : 0.0f, a.bias[0] ? a.bias[0][n] : 0.0f);
-        if constexpr (NG == 2)
-            v = silu_f32(v) * product(acc[1][r], sx, a.K > 0 ? a.sw[1][n] : 0.0f, a.bias[1] ? a.bias[1][n] : 0.0f);
-        store_as(a.y, a.t, m * a.ldy + n, v);
-    }
+    const bool sums = a.K > 0;  // else the biases
+    const float sx = sums ? a.sx[m] : 0.0f;
+    const int64_t n = cb * 16 + 4 * g;
+    floatx4 v = product4(acc[0], sx, load4(sums ? a.sw[0] : nullptr, n, a.N), load4(a.bias[0], n, a.N));
+    if constexpr (NG == 2)
+        v = silu_mul4(v, product4(acc[1], sx, load4(sums ? a.sw[1] : nullptr, n, a.N), load4(a.bias[1], n, a.N)));
+    store4((T*)a.y + m * a.ldy, n, a.N, v);
 }
-
 
 // ---- the tile kernel ------------------------------------------------------
 
@@ -194,12 +221,14 @@ struct TileCfg {
     static constexpr int kWLoads = BN * kStage / 16 / kThreads;
 };
 
-template <int NG, int BM, int BN, int WM, int WN>
+template <int NG, typename T, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void k_w8a8_tile(const W8A8Args a, int tiles_m, int tiles_n, int xlog) {
     using C = TileCfg<NG, BM, BN, WM, WN>;
     constexpr int TM = C::TM, TN = C::TN;
     __shared__ __attribute__((aligned(128))) signed char xs0[BM * kStage], xs1[BM * kStage];
     __shared__ __attribute__((aligned(128))) signed char ws0[BN * kStage], ws1[BN * kStage];
+    __shared__ float esx[BM];
+    __shared__ __attribute__((aligned(16))) float esw[BN], eb[BN];  // scales and biases, as the weights' blocks lie
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lr = lane & 15, g = lane >> 4;
     const int wm = wave / WN, wn = wave % WN;
@@ -268,7 +297,14 @@ __global__ __launch_bounds__(64 * WM * WN) void k_w8a8_tile(const W8A8Args a, in
 
     i32x4 x0[TM], w0[TN], x1[TM], w1[TN];
     load(xs0, ws0, 0);
-    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    for (int t = threadIdx.x; t < BM; t += C::kThreads) esx[t] = t < rows ? a.sx[m0 + t] : 0.0f;
+    for (int t = threadIdx.x; t < BN; t += C::kThreads) {
+        const int q = t / (BN / NG);
+        const int64_t nn = cb0 * 16 + t - q * (BN / NG);
+        esw[t] = nn < a.N ? a.sw[q][nn] : 0.0f;
+        eb[t] = nn < a.N && a.bias[q] ? a.bias[q][nn] : 0.0f;
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     load(xs1, ws1, 1);
     read(x0, w0, xs0, ws0, 0);
     auto step = [&](signed char* xs, signed char* ws, const signed char* xn, const signed char* wsn, int s) {
@@ -292,31 +328,48 @@ __global__ __launch_bounds__(64 * WM * WN) void k_w8a8_tile(const W8A8Args a, in
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
     // A lane has columns 4 g .. 4 g + 3 of a block, of token lr.
+    const int col0 = wn * (TN / NG) * 16 + 4 * g;  // of the first block, in its weight
+    const int64_t nb = cb0 * 16 + col0;
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
-        const int64_t m = m0 + wm * (BM / WM) + i * 16 + lr;
-        if (m >= a.M) continue;
-        const float sx = a.sx[m];
+        const int r = wm * (BM / WM) + i * 16 + lr;
+        if (r >= rows) continue;
+        const float sx = esx[r];
+        T* row = (T*)a.y + (m0 + r) * a.ldy;
 #pragma unroll
         for (int j = 0; j < TN / NG; ++j) {
-            const int64_t nn = (cb0 + wn * (TN / NG) + j) * 16 + 4 * g;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                if (nn + r >= a.N) break;
-                float v = product(acc[i][j][r], sx, a.sw[0][nn + r], a.bias[0] ? a.bias[0][nn + r] : 0.0f);
-                if constexpr (NG == 2)
-                    v = silu_f32(v) * product(acc[i][j + TN / 2][r], sx, a.sw[1][nn + r], a.bias[1] ? a.bias[1][nn + r] : 0.0f);
-                store_as(a.y, a.t, m * a.ldy + nn + r, v);
-            }
+            const int c = col0 + 16 * j;
+            floatx4 v = product4(acc[i][j], sx, *(const floatx4*)&esw[c], *(const floatx4*)&eb[c]);
+            if constexpr (NG == 2)
+                v = silu_mul4(v, product4(acc[i][j + TN / 2], sx, *(const floatx4*)&esw[c + BN / 2],
+                                          *(const floatx4*)&eb[c + BN / 2]));
+            store4(row, nb + 16 * j, a.N, v);
         }
     }
 }
 
-template <int NG, int BM, int BN, int WM, int WN>
-hipError_t launch_tile(const W8A8Args& a, hipStream_t s) {
+template <int NG, typename T, int BM, int BN, int WM, int WN>
+void launch_tile(const W8A8Args& a, hipStream_t s) {
     const int64_t tm = ceil_div(a.M, BM), tn = ceil_div(ChannelsGeom(a.K, a.N).NB, BN / 16 / NG);
-    k_w8a8_tile<NG, BM, BN, WM, WN><<<(unsigned)(tm * tn), 64 * WM * WN, 0, s>>>(a, (int)tm, (int)tn, xcd_log2(device_xcds(s)));
+    k_w8a8_tile<NG, T, BM, BN, WM, WN>
+        <<<(unsigned)(tm * tn), 64 * WM * WN, 0, s>>>(a, (int)tm, (int)tn, xcd_log2(device_xcds(s)));
+}
+
+template <int NG, typename T>
+hipError_t launch_as(const W8A8Args& a, hipStream_t s) {
+    if (a.K > 0 && a.M > 128) {
+        launch_tile<NG, T, 256, 256, 4, 2>(a, s);
+    } else {
+        const int64_t waves = ChannelsGeom(a.K, a.N).NB * ceil_div(a.M, 16);
+        k_w8a8_simple<NG, T><<<(unsigned)ceil_div(waves, kWG / 64), kWG, 0, s>>>(a);
+    }
     return hipGetLastError();
+}
+
+template <int NG>
+hipError_t launch_ng(const W8A8Args& a, hipStream_t s) {
+    return a.t == DType::f32 ? launch_as<NG, float>(a, s)
+                             : (a.t == DType::bf16 ? launch_as<NG, __bf16>(a, s) : launch_as<NG, _Float16>(a, s));
 }
 
 }  // namespace
@@ -353,14 +406,7 @@ hipError_t launch_channels_unpack(const void* packed, int64_t K, int64_t N, cons
 int64_t w8a8_workspace_bytes(int, int64_t, int64_t, int64_t) { return 0; }
 
 hipError_t launch_w8a8(const W8A8Args& a, int ng, void*, hipStream_t s) {
-    if (a.K > 0 && a.M > 128) return ng == 2 ? launch_tile<2, 256, 256, 4, 2>(a, s) : launch_tile<1, 256, 256, 4, 2>(a, s);
-    const int64_t waves = ChannelsGeom(a.K, a.N).NB * ceil_div(a.M, 16);
-    const unsigned grid = (unsigned)ceil_div(waves, kWG / 64);
-    if (ng == 2)
-        k_w8a8_simple<2><<<grid, kWG, 0, s>>>(a);
-    else
-        k_w8a8_simple<1><<<grid, kWG, 0, s>>>(a);
-    return hipGetLastError();
+    return ng == 2 ? launch_ng<2>(a, s) : launch_ng<1>(a, s);
 }
 
 }  // namespace sgq
