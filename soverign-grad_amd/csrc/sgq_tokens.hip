@@ -19,12 +19,21 @@ namespace sgq {
 namespace {
 
 constexpr int kBlock = 256;
-__device__ __forceinline__ float ref_max(float m, float a) { return (a > m) ? a : m; }
+constexpr int kV = 8;  // elements a thread takes at a time
 
-__device__ __forceinline__ int code_of(float u, float inv) {
-    const float v = roundf(u * inv);
-    const float m = (v < 127.0f) ? v : 127.0f;  // NaN gives 127, as the weights' quantizer does
-    return (int)((-127.0f < m) ? m : -127.0f);
+// Eight elements at an address of their type's alignment.
+template <typename T>
+struct Eight {
+    typedef T type __attribute__((ext_vector_type(kV), aligned(sizeof(T))));
+};
+typedef Eight<float>::type f32x8_u;
+
+// round half away from zero(u * inv), at most 127 (as a NaN is).  |u * inv| stays
+// below 127.5 but for a NaN, and adding the float below 0.5 with its sign before
+// the truncation rounds every such value as roundf does.
+__device__ __forceinline__ uint32_t code_of(float u, float inv) {
+    const float v = fminf(u * inv, 127.0f);
+    return (uint32_t)(int)(v + copysignf(0.49999997f, v)) & 0xFFu;
 }
 
 struct TokensArgs {
@@ -34,86 +43,217 @@ struct TokensArgs {
     const float* g; // the norm's weights
     float eps;
     int64_t ldx, ldr, ldh, ldc;
-    int64_t K, Kpad;
+    int64_t M, K, Kpad;
     signed char* codes;
     float* scales;
 };
 
-// One workgroup per row, the row read again for the codes.
-template <typename T, bool NORM, bool RES>
-__global__ __launch_bounds__(kBlock) void k_tokens(const TokensArgs a) {
-    __shared__ float red[2][kBlock / 64];
-    const int64_t row = blockIdx.x;
-    const T* x = (const T*)a.x + row * a.ldx;
-    const T* r = RES ? (const T*)a.r + row * a.ldr : nullptr;
-    T* h = RES ? (T*)a.h + row * a.ldh : nullptr;
-    float ss = 0.0f, m = NORM ? 0.0f : 1e-8f;
-    for (int64_t k = threadIdx.x; k < a.K; k += kBlock) {
-        float v = (float)x[k];
-        if constexpr (RES) {
-            const T t = (T)(v + (float)r[k]);
-            h[k] = t;
-            v = (float)t;
-        }
-        if constexpr (NORM) {
-            ss = fmaf(v, v, ss);
-            v = v * a.g[k];
-        }
-        m = ref_max(m, fabsf(v));
-    }
+// Sum of ss and maximum of m over NT threads of the workgroup (a wavefront, or all).
+template <int NT>
+__device__ __forceinline__ void row_reduce(float& ss, float& m, float (*red)[16]) {
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) {
         ss += __shfl_xor(ss, o, 64);
-        m = ref_max(m, __shfl_xor(m, o, 64));
+        m = fmaxf(m, __shfl_xor(m, o, 64));
     }
-    if ((threadIdx.x & 63) == 0) red[0][threadIdx.x >> 6] = ss, red[1][threadIdx.x >> 6] = m;
-    __syncthreads();
-    ss = red[0][0], m = red[1][0];
+    if constexpr (NT > 64) {
+        __syncthreads();  // the last row's
+        if ((threadIdx.x & 63) == 0) red[0][threadIdx.x >> 6] = ss, red[1][threadIdx.x >> 6] = m;
+        __syncthreads();
+        ss = red[0][0], m = red[1][0];
 #pragma unroll
-    for (int w = 1; w < kBlock / 64; ++w) ss += red[0][w], m = ref_max(m, red[1][w]);
-    float scale;
-    if constexpr (NORM) {
-        const float rstd = 1.0f / sqrtf(ss / (float)a.K + a.eps);
-        m = ref_max(m, 1e-8f / rstd);
-        scale = m * rstd / 127.0f;
-    } else {
-        scale = m / 127.0f;
-    }
-    const float inv = 127.0f / m;
-    if (threadIdx.x == 0) a.scales[row] = scale;
-    const T* src = RES ? h : x;
-    for (int64_t k = threadIdx.x; k < a.Kpad; k += kBlock) {
-        int c = 0;
-        if (k < a.K) {
-            float v = (float)src[k];
-            if constexpr (NORM) v = v * a.g[k];
-            c = code_of(v, inv);
-        }
-        a.codes[row * a.ldc + k] = (signed char)c;
+        for (int w = 1; w < NT / 64; ++w) ss += red[0][w], m = fmaxf(m, red[1][w]);
     }
 }
 
+// Scale and inverse of a row from its sum of squares and its maximum.
+template <bool NORM>
+__device__ __forceinline__ float row_scale(float ss, float& m, float K, float eps) {
+    if constexpr (NORM) {
+        const float rstd = 1.0f / sqrtf(ss / K + eps);
+        m = fmaxf(m, 1e-8f / rstd);
+        return m * rstd / 127.0f;
+    } else {
+        m = fmaxf(m, 1e-8f);
+        return m / 127.0f;
+    }
+}
+
+// NT threads a row (a wavefront of several in a workgroup, or a workgroup), C
+// chunks of eight elements a thread: the row stays in registers.
+template <typename T, bool NORM, bool RES, int NT, int C>
+__global__ __launch_bounds__(NT < kBlock ? kBlock : NT) void k_tokens_row(const TokensArgs a) {
+    __shared__ float red[2][16];
+    constexpr int kRows = NT < kBlock ? kBlock / NT : 1;
+    typedef typename Eight<T>::type T8;
+    const int t = NT < kBlock ? threadIdx.x % NT : threadIdx.x;
+    const int K = (int)a.K, nq = (int)(a.Kpad / kV);
+    for (int64_t row = blockIdx.x * (int64_t)kRows + (NT < kBlock ? threadIdx.x / NT : 0); row < a.M;
+         row += (int64_t)gridDim.x * kRows) {
+        const T* x = (const T*)a.x + row * a.ldx;
+        const T* r = RES ? (const T*)a.r + row * a.ldr : nullptr;
+        T* h = RES ? (T*)a.h + row * a.ldh : nullptr;
+        T8 xv[C], rv[C];
+        f32x8_u gv[C];
+        auto load_g = [&](f32x8_u& v, int k) {
+            if (k + kV <= K) {
+                v = *(const f32x8_u*)(a.g + k);
+            } else {
+#pragma unroll
+                for (int e = 0; e < kV; ++e) v[e] = k + e < K ? a.g[k + e] : 0.0f;
+            }
+        };
+        // Every load is issued before the first is used.
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            const int k = (t + i * NT) * kV;
+            if (k + kV <= K) {
+                xv[i] = *(const T8*)(x + k);
+                if constexpr (RES) rv[i] = *(const T8*)(r + k);
+            } else {
+#pragma unroll
+                for (int e = 0; e < kV; ++e) {
+                    xv[i][e] = k + e < K ? x[k + e] : (T)0.0f;
+                    if constexpr (RES) rv[i][e] = k + e < K ? r[k + e] : (T)0.0f;
+                }
+            }
+            if constexpr (NORM) load_g(gv[i], k);
+        }
+        float u[C][kV], ss = 0.0f, m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            const int k = (t + i * NT) * kV;
+            if constexpr (RES) {
+#pragma unroll
+                for (int e = 0; e < kV; ++e) xv[i][e] = (T)((float)xv[i][e] + (float)rv[i][e]);
+                if (k + kV <= K) {
+                    *(T8*)(h + k) = xv[i];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < kV; ++e)
+                        if (k + e < K) h[k + e] = xv[i][e];
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < kV; ++e) {
+                float v = (float)xv[i][e];
+                if constexpr (NORM) {
+                    ss = fmaf(v, v, ss);
+                    v = v * gv[i][e];
+                }
+                u[i][e] = v;
+                m = fmaxf(m, fabsf(v));
+            }
+        }
+        row_reduce<NT>(ss, m, red);
+        const float scale = row_scale<NORM>(ss, m, (float)K, a.eps), inv = 127.0f / m;
+        if (t == 0) a.scales[row] = scale;
+        signed char* c = a.codes + row * a.ldc;
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            const int q = t + i * NT;
+            uint32_t w[2] = {0, 0};
+#pragma unroll
+            for (int e = 0; e < kV; ++e) w[e / 4] |= code_of(u[i][e], inv) << (8 * (e % 4));
+            if (q < nq) *(uint2*)(c + q * kV) = make_uint2(w[0], w[1]);
+        }
+    }
+}
+
+// Longer rows, read again (from the caches) for the codes.  With the norm that is
+// from 16384 on: x, the residual, g and u of four chunks do not fit the 128 registers
+// that sixteen wavefronts leave a thread.
+constexpr int kLoopBlock = 1024;
+template <typename T, bool NORM, bool RES>
+__global__ __launch_bounds__(kLoopBlock) void k_tokens_loop(const TokensArgs a) {
+    __shared__ float red[2][16];
+    for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
+        const T* x = (const T*)a.x + row * a.ldx;
+        const T* r = RES ? (const T*)a.r + row * a.ldr : nullptr;
+        T* h = RES ? (T*)a.h + row * a.ldh : nullptr;
+        float ss = 0.0f, m = 0.0f;
+#pragma unroll 4
+        for (int64_t k = threadIdx.x; k < a.K; k += kLoopBlock) {
+            float v = (float)x[k];
+            if constexpr (RES) {
+                const T t = (T)(v + (float)r[k]);
+                h[k] = t;
+                v = (float)t;
+            }
+            if constexpr (NORM) {
+                ss = fmaf(v, v, ss);
+                v = v * a.g[k];
+            }
+            m = fmaxf(m, fabsf(v));
+        }
+        row_reduce<kLoopBlock>(ss, m, red);
+        const float scale = row_scale<NORM>(ss, m, (float)a.K, a.eps), inv = 127.0f / m;
+        if (threadIdx.x == 0) a.scales[row] = scale;
+        const T* src = RES ? h : x;  // each thread reads what it wrote
+#pragma unroll 4
+        for (int64_t k = threadIdx.x; k < a.Kpad; k += kLoopBlock) {
+            float v = k < a.K ? (float)src[k] : 0.0f;
+            if constexpr (NORM) v = k < a.K ? v * a.g[k] : 0.0f;
+            a.codes[row * a.ldc + k] = (signed char)code_of(v, inv);
+        }
+    }
+}
+
+// Values of eight codes a thread.
 template <typename T>
 __global__ __launch_bounds__(kBlock) void k_tokens_values(const signed char* __restrict__ codes, int64_t ldc,
-                                                          const float* __restrict__ scales, int64_t M, int64_t K,
+                                                          const float* __restrict__ scales, int64_t M, int K,
                                                           T* __restrict__ out, int64_t ldo) {
+    const int k = (blockIdx.x * kBlock + threadIdx.x) * kV;
+    if (k >= K) return;
     for (int64_t row = blockIdx.y; row < M; row += gridDim.y) {
         const float s = scales[row];
-        for (int64_t k = blockIdx.x * (int64_t)kBlock + threadIdx.x; k < K; k += (int64_t)gridDim.x * kBlock)
-            out[row * ldo + k] = (T)((float)codes[row * ldc + k] * s);
+        const uint2 w = *(const uint2*)(codes + row * ldc + k);  // within the row: it holds K rounded up to 128
+        typename Eight<T>::type v;
+#pragma unroll
+        for (int e = 0; e < kV; ++e) v[e] = (T)((float)(signed char)((e < 4 ? w.x : w.y) >> (8 * (e % 4))) * s);
+        T* o = out + row * ldo + k;
+        if (k + kV <= K) {
+            *(typename Eight<T>::type*)o = v;
+        } else {
+#pragma unroll
+            for (int e = 0; e < kV - 1; ++e)
+                if (k + e < K) o[e] = v[e];
+        }
     }
 }
 
-template <typename T>
-hipError_t launch_t(const TokensArgs& a, int64_t M, hipStream_t s) {
-    const unsigned grid = (unsigned)M;
-    if (!a.g)
-        k_tokens<T, false, false><<<grid, kBlock, 0, s>>>(a);
-    else if (!a.r)
-        k_tokens<T, true, false><<<grid, kBlock, 0, s>>>(a);
-    else
-        k_tokens<T, true, true><<<grid, kBlock, 0, s>>>(a);
+constexpr int64_t kMaxRowGroups = (int64_t)1 << 20;  // workgroups of a launch (fewer than 2^32 threads)
+
+template <typename T, bool NORM, bool RES>
+hipError_t launch_rows(const TokensArgs& a, hipStream_t s) {
+    const auto grid = [&](int rows) { return (unsigned)(ceil_div(a.M, rows) < kMaxRowGroups ? ceil_div(a.M, rows) : kMaxRowGroups); };
+    const int64_t q = a.Kpad / kV;
+    if (q <= 64)
+        k_tokens_row<T, NORM, RES, 64, 1><<<grid(4), kBlock, 0, s>>>(a);
+    else if (q <= 256)
+        k_tokens_row<T, NORM, RES, 256, 1><<<grid(1), 256, 0, s>>>(a);
+    else if (q <= 512)
+        k_tokens_row<T, NORM, RES, 256, 2><<<grid(1), 256, 0, s>>>(a);
+    else if (q <= 1024)
+        k_tokens_row<T, NORM, RES, 256, 4><<<grid(1), 256, 0, s>>>(a);
+    else if (q <= 2048)
+        k_tokens_row<T, NORM, RES, 512, 4><<<grid(1), 512, 0, s>>>(a);
+    else if constexpr (!NORM) {
+        if (q <= 4096)
+            k_tokens_row<T, NORM, RES, 1024, 4><<<grid(1), 1024, 0, s>>>(a);
+        else
+            k_tokens_loop<T, NORM, RES><<<grid(1), kLoopBlock, 0, s>>>(a);
+    } else {
+        k_tokens_loop<T, NORM, RES><<<grid(1), kLoopBlock, 0, s>>>(a);
+    }
     return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_t(const TokensArgs& a, hipStream_t s) {
+    if (!a.g) return launch_rows<T, false, false>(a, s);
+    return a.r ? launch_rows<T, true, true>(a, s) : launch_rows<T, true, false>(a, s);
 }
 
 }  // namespace
@@ -124,22 +264,22 @@ hipError_t launch_tokens(const void* x, DType t, int64_t ldx, const void* r, int
     TokensArgs a{};
     a.x = x, a.r = r, a.h = h, a.g = g, a.eps = eps;
     a.ldx = ldx, a.ldr = ldr, a.ldh = ldh, a.ldc = ldc;
-    a.K = K, a.Kpad = round_up(K, kTokenPadK);
+    a.M = M, a.K = K, a.Kpad = K > 0 ? round_up(K, kTokenPadK) : kTokenPadK;
     a.codes = (signed char*)codes, a.scales = scales;
-    return t == DType::f32 ? launch_t<float>(a, M, s)
-                           : (t == DType::bf16 ? launch_t<__bf16>(a, M, s) : launch_t<_Float16>(a, M, s));
+    return t == DType::f32 ? launch_t<float>(a, s)
+                           : (t == DType::bf16 ? launch_t<__bf16>(a, s) : launch_t<_Float16>(a, s));
 }
 
 hipError_t launch_tokens_values(const void* codes, int64_t ldc, const float* scales, int64_t M, int64_t K, void* out,
                                 DType t, int64_t ldo, hipStream_t s) {
-    const dim3 grid((unsigned)(ceil_div(K, kBlock) < 1024 ? ceil_div(K, kBlock) : 1024), (unsigned)(M < 32768 ? M : 32768));
+    const dim3 grid((unsigned)ceil_div(K, kBlock * kV), (unsigned)(M < 32768 ? M : 32768));
     const signed char* c = (const signed char*)codes;
     if (t == DType::f32)
-        k_tokens_values<float><<<grid, kBlock, 0, s>>>(c, ldc, scales, M, K, (float*)out, ldo);
+        k_tokens_values<float><<<grid, kBlock, 0, s>>>(c, ldc, scales, M, (int)K, (float*)out, ldo);
     else if (t == DType::bf16)
-        k_tokens_values<__bf16><<<grid, kBlock, 0, s>>>(c, ldc, scales, M, K, (__bf16*)out, ldo);
+        k_tokens_values<__bf16><<<grid, kBlock, 0, s>>>(c, ldc, scales, M, (int)K, (__bf16*)out, ldo);
     else
-        k_tokens_values<_Float16><<<grid, kBlock, 0, s>>>(c, ldc, scales, M, K, (_Float16*)out, ldo);
+        k_tokens_values<_Float16><<<grid, kBlock, 0, s>>>(c, ldc, scales, M, (int)K, (_Float16*)out, ldo);
     return hipGetLastError();
 }
 

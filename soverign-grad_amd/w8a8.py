@@ -2,7 +2,7 @@
 
 Activations become int8 tokens (a scale per row), weights int8 channels (a scale
 per output column of W [K, N]), and products of the two run on the int8 matrix
-cores, exact until the scales are applied:
+cores, exact until the scales are applied (inference only: nothing here has a gradient):
 
     quantize_int8_tokens(x)                        x as tokens
     rms_norm_int8_tokens(x, weight)                rms_norm(x) as tokens
@@ -77,10 +77,12 @@ def _rows(x: torch.Tensor, name: str) -> torch.Tensor:
     """x as a matrix of rows on the device, its own memory wherever rows are contiguous."""
     if not x.is_cuda:
         raise ValueError("sgq: expected a device tensor")
-    if x.dim() < 2:
-        raise ValueError(f"{name} must have at least 2 dimensions")
-    if x.dim() > 2:
-        x = x.reshape(-1, x.shape[-1])
+    if x.dim() != 2:
+        if x.dim() < 2:
+            raise ValueError(f"{name} must have at least 2 dimensions")
+        x = x.flatten(0, -2)
+    if x.is_contiguous():
+        return x
     M, K = x.shape
     if (K > 1 and x.stride(1) != 1) or (M > 1 and x.stride(0) < K):
         x = x.contiguous()
@@ -102,17 +104,21 @@ def _vector(t: torch.Tensor, n: int, dev: torch.device, name: str) -> torch.Tens
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _new_tokens(M: int, K: int, dev: torch.device) -> TokensInt8:
-    row = load_library().sgq_tokens_row_bytes(K)
-    if row < 0:
+def _row_bytes(K: int) -> int:
+    """sgq_tokens_row_bytes."""
+    if K > 131071:
         raise ValueError("sgq: rows of tokens are at most 131071 long")
-    return TokensInt8(torch.empty((M, row), dtype=torch.int8, device=dev),
+    return (K + 127 & -128) or 128
+
+
+def _new_tokens(M: int, K: int, dev: torch.device) -> TokensInt8:
+    return TokensInt8(torch.empty(M, _row_bytes(K), dtype=torch.int8, device=dev),
                       torch.empty(M, dtype=torch.float32, device=dev), K)
 
 
 def _output(out: Optional[torch.Tensor], M: int, N: int, dtype: torch.dtype, dev: torch.device) -> torch.Tensor:
     if out is None:
-        return torch.empty((M, N), dtype=dtype, device=dev)
+        return torch.empty(M, N, dtype=dtype, device=dev)
     if out.dtype != dtype or out.device != dev or tuple(out.shape) != (M, N):
         raise ValueError(f"out must be a {dtype} [{M}, {N}] on {dev}")
     if (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
@@ -126,7 +132,7 @@ def quantize_int8_tokens(x: torch.Tensor) -> TokensInt8:
     M, K = x.shape
     t = _new_tokens(M, K, x.device)
     _call(x.device, load_library().sgq_quantize_tokens, x.data_ptr(), _dtype(x.dtype), _ld(x), M, K,
-          t.codes.data_ptr(), _ld(t.codes), t.scales.data_ptr())
+          t.codes.data_ptr(), _row_bytes(K), t.scales.data_ptr())
     return t
 
 
@@ -140,7 +146,7 @@ def _norm_tokens(x, residual, weight, eps, out):
     r, ldr, h, ldh = (None, 0, None, 0) if residual is None else (residual.data_ptr(), _ld(residual), out.data_ptr(),
                                                                     _ld(out))
     _call(dev, load_library().sgq_rms_norm_tokens, x.data_ptr(), _dtype(x.dtype), _ld(x), r, ldr, h, ldh,
-          g.data_ptr(), eps, M, K, t.codes.data_ptr(), _ld(t.codes), t.scales.data_ptr())
+          g.data_ptr(), eps, M, K, t.codes.data_ptr(), _row_bytes(K), t.scales.data_ptr())
     return t
 
 
@@ -158,25 +164,25 @@ def add_rms_norm_int8_tokens(x: torch.Tensor, residual: torch.Tensor, weight: to
     shape = x.shape
     x, r = _rows(x, "x"), _rows(residual, "residual")
     if out is None:
-        h = y = torch.empty(shape, dtype=x.dtype, device=x.device)
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        h = y if len(shape) == 2 else y.view(shape)
     elif out.shape != shape or out.dtype != x.dtype or out.device != x.device:
         raise ValueError("out must be alike x in shape, type and device")
     else:
         h, y = out, _rows(out, "out")
         if y.data_ptr() != out.data_ptr():
             raise ValueError("out must have contiguous rows")
-    return _norm_tokens(x, r, weight, eps, _rows(y, "out")), h
+    return _norm_tokens(x, r, weight, eps, y), h
 
 
 def dequantize_int8_tokens(t: TokensInt8, dtype: torch.dtype = torch.float32,
                            out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The values [M, K] that tokens stand for."""
-    dev = t.codes.device
-    M, K = t.codes.shape[0], t.K
+    dev, K = t.codes.device, t.K
+    codes, ldc, scales, M = _tokens(t, dev)
     y = _output(out, M, K, dtype, dev)
-    _tokens(t, dev)
-    _call(dev, load_library().sgq_dequantize_tokens, t.codes.data_ptr(), _ld(t.codes), t.scales.data_ptr(), M, K,
-          y.data_ptr(), _dtype(dtype), _ld(y))
+    _call(dev, load_library().sgq_dequantize_tokens, codes, ldc, scales, M, K, y.data_ptr(), _dtype(dtype),
+          K if out is None else _ld(y))
     return y
 
 
@@ -233,19 +239,26 @@ def dequantize_int8_channels(qw: ChannelsInt8) -> torch.Tensor:
     return out
 
 
-def _tokens(t: TokensInt8, dev: torch.device) -> None:
+def _tokens(t: TokensInt8, dev: torch.device) -> Tuple[int, int, int, int]:
+    """Address, row stride and scales' address of tokens on dev, and how many they are."""
     c, s = t.codes, t.scales
-    if not c.is_cuda or c.dtype is not torch.int8 or c.dim() != 2 or (c.shape[1] > 1 and c.stride(1) != 1):
+    if not c.is_cuda or c.dtype is not torch.int8 or c.dim() != 2:
         raise ValueError("token codes must be int8 rows on the device")
     if c.device != dev or s.device != dev:
         raise ValueError("tokens and weight must be on one device")
-    if c.shape[1] < t.K or (c.shape[0] > 1 and c.stride(0) < c.shape[1]):
-        raise ValueError("rows of token codes overlap")
-    if s.dtype is not torch.float32 or not s.is_contiguous() or s.numel() != c.shape[0]:
+    M, row = c.shape
+    ld = row
+    if not c.is_contiguous():
+        if row > 1 and c.stride(1) != 1:
+            raise ValueError("token codes must be int8 rows on the device")
+        ld = _ld(c)
+        if ld < row:
+            raise ValueError("rows of token codes overlap")
+    if s.dtype is not torch.float32 or s.numel() != M or not s.is_contiguous():
         raise ValueError("token scales must be fp32, one per row")
-    row = load_library().sgq_tokens_row_bytes(t.K)
-    if c.shape[1] < row:
-        raise ValueError(f"rows of {t.K} token codes take {row} bytes")
+    if row < _row_bytes(t.K):
+        raise ValueError(f"rows of {t.K} token codes take {_row_bytes(t.K)} bytes")
+    return c.data_ptr(), ld, s.data_ptr(), M
 
 
 def _bias(b: Optional[torch.Tensor], N: int, dev: torch.device) -> Optional[torch.Tensor]:
@@ -258,16 +271,15 @@ def quantized_matmul_w8a8(t: TokensInt8, qw: ChannelsInt8, bias: Optional[torch.
     dev = qw.packed.device
     if t.K != qw.K:
         raise ValueError("Matrix inner dimensions must match for matmul!")
-    _tokens(t, dev)
-    c, N, lib = t.codes, qw.N, load_library()
-    M = c.shape[0]
+    codes, ldc, scales, M = _tokens(t, dev)
+    N, lib = qw.N, load_library()
     b = _bias(bias, N, dev)
     y = _output(out, M, N, dtype, dev)
     need = lib.sgq_linear_w8a8_workspace_bytes(M, qw.K, N)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
-    _call(dev, lib.sgq_linear_w8a8, c.data_ptr(), _ld(c), t.scales.data_ptr(), M, qw.K, N, qw.packed.data_ptr(),
-          qw.scales.data_ptr(), None if b is None else b.data_ptr(), y.data_ptr(), _dtype(dtype), _ld(y),
-          None if ws is None else ws.data_ptr(), need)
+    _call(dev, lib.sgq_linear_w8a8, codes, ldc, scales, M, qw.K, N, qw.packed.data_ptr(),
+          qw.scales.data_ptr(), None if b is None else b.data_ptr(), y.data_ptr(), _dtype(dtype),
+          N if out is None else _ld(y), None if ws is None else ws.data_ptr(), need)
     return y
 
 
@@ -280,16 +292,16 @@ def quantized_swiglu_w8a8(t: TokensInt8, w_gate: ChannelsInt8, w_up: ChannelsInt
         raise ValueError("gate and up weights must have the same shape and device")
     if t.K != w_gate.K:
         raise ValueError("Matrix inner dimensions must match for matmul!")
-    _tokens(t, dev)
-    c, K, N, lib = t.codes, w_gate.K, w_gate.N, load_library()
-    M = c.shape[0]
+    codes, ldc, scales, M = _tokens(t, dev)
+    K, N, lib = w_gate.K, w_gate.N, load_library()
     bg, bu = _bias(bias_gate, N, dev), _bias(bias_up, N, dev)
     h = _output(out, M, N, dtype, dev)
     need = lib.sgq_swiglu_w8a8_workspace_bytes(M, K, N)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
-    _call(dev, lib.sgq_swiglu_w8a8, c.data_ptr(), _ld(c), t.scales.data_ptr(), M, K, N, w_gate.packed.data_ptr(),
+    _call(dev, lib.sgq_swiglu_w8a8, codes, ldc, scales, M, K, N, w_gate.packed.data_ptr(),
           w_gate.scales.data_ptr(), None if bg is None else bg.data_ptr(), w_up.packed.data_ptr(),
-          w_up.scales.data_ptr(), None if bu is None else bu.data_ptr(), h.data_ptr(), _dtype(dtype), _ld(h),
+          w_up.scales.data_ptr(), None if bu is None else bu.data_ptr(), h.data_ptr(), _dtype(dtype),
+          N if out is None else _ld(h),
           None if ws is None else ws.data_ptr(), need)
     return h
 
