@@ -373,7 +373,7 @@ int sgq_rms_norm(const float* x, int64_t rows, int64_t D, const float* g, float 
  * Activations and outputs are of one of three element types, rows of `ld`
  * elements (>= their length); any address aligned to the element will do.  Token
  * codes: row m at codes + m * ldc, ldc a multiple of 16 of at least
- * sgq_tokens_row_bytes(K) bytes, 16-byte aligned; the quantizers write zeros from
+ * sgq_tokens_row_bytes(K) and at most 2^21 bytes, 16-byte aligned; the quantizers write zeros from
  * K up to sgq_tokens_row_bytes(K), the products ignore what stands there.  K is at
  * most 131071 (SGQ_ERR_UNSUPPORTED past it), which keeps sums exact in int32. */
 #define SGQ_F32 0
@@ -423,21 +423,30 @@ int sgq_dequantize_channels(const void* packed, const float* scales, int64_t K, 
 
 /* y[m, n] = (sum_k cx[m, k] * cw[k, n]) * x_scales[m] * w_scales[n] + bias[n], the
  * sum in int32, the rest in fp32, rounded to the type.  bias [N] fp32 or NULL.
- * K == 0 gives the bias.  workspace: sgq_linear_w8a8_workspace_bytes(M, K, N)
- * bytes, 16-byte aligned, else SGQ_ERR_WORKSPACE; it needs no initialisation, and
- * calls that overlap in time must not share one. */
-int64_t sgq_linear_w8a8_workspace_bytes(int64_t M, int64_t K, int64_t N);
+ * K == 0 gives the bias.  workspace: sgq_linear_w8a8_workspace_bytes bytes for a
+ * device of `compute_units` CUs (0: the calling thread's current device), 16-byte
+ * aligned, else SGQ_ERR_WORKSPACE; it needs no initialisation, and calls that
+ * overlap in time must not share one. */
+int64_t sgq_linear_w8a8_workspace_bytes(int64_t M, int64_t K, int64_t N, int compute_units);
 int sgq_linear_w8a8(const void* codes, int64_t ldc, const float* x_scales, int64_t M, int64_t K, int64_t N,
                     const void* packed, const float* w_scales, const float* bias, void* y, int dtype, int64_t ldy,
                     void* workspace, int64_t workspace_bytes, void* stream);
 
 /* h = silu(gate) * up of two such products (as sgq_swiglu_int8), in fp32 until it
  * is rounded to the type. */
-int64_t sgq_swiglu_w8a8_workspace_bytes(int64_t M, int64_t K, int64_t N);
+int64_t sgq_swiglu_w8a8_workspace_bytes(int64_t M, int64_t K, int64_t N, int compute_units);
 int sgq_swiglu_w8a8(const void* codes, int64_t ldc, const float* x_scales, int64_t M, int64_t K, int64_t N,
                     const void* packed_gate, const float* scales_gate, const float* bias_gate, const void* packed_up,
                     const float* scales_up, const float* bias_up, void* h, int dtype, int64_t ldh, void* workspace,
                     int64_t workspace_bytes, void* stream);
+
+/* The kernel such a product (gated: such a gated MLP) runs on `compute_units` CUs
+ * (0: the current device's).  *form: 0 the biases alone (K == 0); 1..4 workgroups of
+ * 16 x 16, 32 x 16, 32 x 32 and 64 x 32 tokens by columns, whose wavefronts share K;
+ * 5..8 tiles of 64 x 128, 128 x 128, 128 x 256 and 256 x 256 through LDS (columns of
+ * both weights).  *k_splits: workgroups that share a tile's K, their sums added by
+ * a second kernel.  Host-only. */
+int sgq_w8a8_plan(int gated, int64_t M, int64_t K, int64_t N, int compute_units, int* form, int* k_splits);
 
 #ifdef __cplusplus
 }

@@ -89,11 +89,12 @@ SIGNATURES = {
     "sgq_pack_channels": (_int, [_vp, _i64, _i64, _vp, _vp, _i64, _vp]),
     "sgq_unpack_channels": (_int, [_vp, _i64, _i64, _vp, _vp]),
     "sgq_dequantize_channels": (_int, [_vp, _vp, _i64, _i64, _vp, _vp]),
-    "sgq_linear_w8a8_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "sgq_linear_w8a8_workspace_bytes": (_i64, [_i64, _i64, _i64, _int]),
     "sgq_linear_w8a8": (_int, [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _int, _i64, _vp, _i64, _vp]),
-    "sgq_swiglu_w8a8_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "sgq_swiglu_w8a8_workspace_bytes": (_i64, [_i64, _i64, _i64, _int]),
     "sgq_swiglu_w8a8": (_int, [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _int, _i64, _vp,
                                _i64, _vp]),
+    "sgq_w8a8_plan": (_int, [_int, _i64, _i64, _i64, _int, ctypes.POINTER(_int), ctypes.POINTER(_int)]),
 }
 
 _lib = None

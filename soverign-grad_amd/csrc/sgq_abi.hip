@@ -254,9 +254,11 @@ int check_rows(const char* fn, const char* what, const void* p, int dtype, int64
 }
 int check_token_codes(const char* fn, const void* codes, int64_t ldc, int64_t K) {
     if (!codes || !aligned16(codes)) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: codes must be 16-byte aligned", fn);
-    if (ldc % 16 != 0 || ldc < round_up(K, kTokenPadK) || ldc > kMaxDim)
+    if (ldc % 16 != 0 || ldc < round_up(K, kTokenPadK))
         return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: rows of codes need a multiple of 16 bytes, at least %lld", fn,
                     (long long)round_up(K, kTokenPadK));
+    if (ldc > kMaxTokenStride)
+        return fail(SGQ_ERR_UNSUPPORTED, "%s: rows of codes more than %lld bytes apart", fn, (long long)kMaxTokenStride);
     return SGQ_OK;
 }
 
@@ -357,6 +359,13 @@ int linear_int4(const char* fn, const float* x, int64_t M, int64_t K, int64_t N,
     return ok();
 }
 
+// Workspace of such a product on `cus` compute units (0: the current device's).
+int64_t w8a8_ws_bytes(int ng, int64_t M, int64_t K, int64_t N, int cus) {
+    if (bad_dims(M, K) || bad_dims(K, N) || bad_dims(M, N) || K > kMaxTokenK || cus < 0) return -1;
+    if (M == 0 || N == 0) return 0;
+    return w8a8_plan_bytes(w8a8_plan(ng, M, K, N, cus > 0 ? cus : device_cus(nullptr)), ng, M, K, N);
+}
+
 // One product (ng == 1) or the gated MLP's two of 8-bit tokens.
 int product_w8a8(const char* fn, int ng, const void* codes, int64_t ldc, const float* x_scales, int64_t M, int64_t K,
                  int64_t N, const void* const* packed, const float* const* scales, const float* const* bias, void* y,
@@ -378,12 +387,12 @@ int product_w8a8(const char* fn, int ng, const void* codes, int64_t ldc, const f
         if (!x_scales) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: null scales", fn);
         if ((st = check_token_codes(fn, codes, ldc, K)) != SGQ_OK) return st;
     }
-    const int64_t need = w8a8_workspace_bytes(ng, M, K, N);
-    if ((st = check_launch_ws(fn, need, workspace, workspace_bytes)) != SGQ_OK) return st;
+    const W8A8Plan p = w8a8_plan(ng, M, K, N, device_cus((hipStream_t)stream));
+    if ((st = check_launch_ws(fn, w8a8_plan_bytes(p, ng, M, K, N), workspace, workspace_bytes)) != SGQ_OK) return st;
     a.x = (const signed char*)codes, a.ldx = ldc, a.sx = x_scales;
     a.M = M, a.K = K, a.N = N;
     a.y = y, a.t = (DType)dtype, a.ldy = ldy;
-    SGQ_HIP(launch_w8a8(a, ng, workspace, (hipStream_t)stream), "w8a8");
+    SGQ_HIP(launch_w8a8(a, ng, p, workspace, (hipStream_t)stream), "w8a8");
     return ok();
 }
 
@@ -1124,14 +1133,20 @@ int sgq_dequantize_channels(const void* packed, const float* scales, int64_t K, 
     return ok();
 }
 
-int64_t sgq_linear_w8a8_workspace_bytes(int64_t M, int64_t K, int64_t N) {
-    if (bad_dims(M, K) || bad_dims(K, N) || bad_dims(M, N) || K > kMaxTokenK) return -1;
-    return w8a8_workspace_bytes(1, M, K, N);
+int64_t sgq_linear_w8a8_workspace_bytes(int64_t M, int64_t K, int64_t N, int compute_units) {
+    return w8a8_ws_bytes(1, M, K, N, compute_units);
 }
 
-int64_t sgq_swiglu_w8a8_workspace_bytes(int64_t M, int64_t K, int64_t N) {
-    if (bad_dims(M, K) || bad_dims(K, N) || bad_dims(M, N) || K > kMaxTokenK) return -1;
-    return w8a8_workspace_bytes(2, M, K, N);
+int64_t sgq_swiglu_w8a8_workspace_bytes(int64_t M, int64_t K, int64_t N, int compute_units) {
+    return w8a8_ws_bytes(2, M, K, N, compute_units);
+}
+
+int sgq_w8a8_plan(int gated, int64_t M, int64_t K, int64_t N, int compute_units, int* form, int* k_splits) {
+    if (bad_dims(M, K) || bad_dims(K, N) || bad_dims(M, N) || K > kMaxTokenK || compute_units < 0 || !form || !k_splits)
+        return fail(SGQ_ERR_INVALID_ARGUMENT, "sgq_w8a8_plan: bad argument");
+    const W8A8Plan p = w8a8_plan(gated ? 2 : 1, M, K, N, compute_units > 0 ? compute_units : device_cus(nullptr));
+    *form = (int)p.form, *k_splits = p.KS;
+    return ok();
 }
 
 int sgq_linear_w8a8(const void* codes, int64_t ldc, const float* x_scales, int64_t M, int64_t K, int64_t N,

@@ -116,6 +116,7 @@ struct I4Geom {
 // block is one contiguous run over K.
 constexpr int64_t kTokenPadK = 128;
 constexpr int64_t kMaxTokenK = 131071;  // K * 128 * 128 < 2^31: sums stay exact in int32
+constexpr int64_t kMaxTokenStride = (int64_t)1 << 21;  // 256 rows through 32-bit offsets below kOobOff
 struct ChannelsGeom {
     int64_t Kpad, KC, NB;
     __host__ __device__ ChannelsGeom(int64_t k, int64_t n)
@@ -537,8 +538,17 @@ struct W8A8Args {
     DType t;
     int64_t ldy;
 };
-// Bytes of workspace of ng products of this shape on any device.
-int64_t w8a8_workspace_bytes(int ng, int64_t M, int64_t K, int64_t N);
-hipError_t launch_w8a8(const W8A8Args& a, int ng, void* ws, hipStream_t s);
+// Forms of the product: the biases (K = 0), k_w8a8_few with row blocks x column
+// blocks of 16, k_w8a8_tile with tokens x columns.  KS: workgroups that share a
+// tile's K, whose sums a second kernel adds (each has stages of its own).
+enum class W8A8Form : int { bias, few1x1, few2x1, few2x2, few4x2, tile64x128, tile128, tile128x256, tile256 };
+struct W8A8Plan {
+    W8A8Form form = W8A8Form::bias;
+    int KS = 1;
+};
+W8A8Plan w8a8_plan(int ng, int64_t M, int64_t K, int64_t N, int64_t cus);
+// Bytes of workspace of a plan: its partial sums.
+int64_t w8a8_plan_bytes(const W8A8Plan& p, int ng, int64_t M, int64_t K, int64_t N);
+hipError_t launch_w8a8(const W8A8Args& a, int ng, const W8A8Plan& p, void* ws, hipStream_t s);
 
 }  // namespace sgq

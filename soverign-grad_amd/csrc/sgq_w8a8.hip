@@ -50,13 +50,13 @@ __global__ __launch_bounds__(kWG) void k_channels_top(const float* __restrict__ 
 // Codes of a kTileK x kTileN tile: FROM_CODES reads fp32 codes (validated into
 // *bad), else w with the columns' maxima in top; through LDS into the layout.
 template <bool FROM_CODES>
-__global__ __launch_bounds__(kWG) void k_channels_pack(const float* __restrict__ src, int64_t K, int64_t N, int64_t nkt,
+__global__ __launch_bounds__(kWG) void k_channels_pack(const float* __restrict__ src, int64_t K, int64_t N, int64_t nkt, int64_t t0,
                                                        const uint32_t* __restrict__ top, float* __restrict__ scales,
                                                        float* __restrict__ qdata, signed char* __restrict__ packed,
                                                        int* __restrict__ bad) {
 #pragma clang fp contract(off)
     __shared__ __attribute__((aligned(16))) signed char col[kTileN][kTileK + 16];
-    const int64_t kt = blockIdx.x % nkt, nt = blockIdx.x / nkt;
+    const int64_t kt = (t0 + blockIdx.x) % nkt, nt = (t0 + blockIdx.x) / nkt;
     const int c = threadIdx.x & 63;
     const int64_t n = nt * kTileN + c;
     float inv = 0.0f;
@@ -98,10 +98,10 @@ __global__ __launch_bounds__(kWG) void k_channels_pack(const float* __restrict__
 
 // out[k][n] = code (* scales[n]).
 __global__ __launch_bounds__(kWG) void k_channels_unpack(const signed char* __restrict__ packed, int64_t K, int64_t N,
-                                                         int64_t nkt, const float* __restrict__ scales,
+                                                         int64_t nkt, int64_t t0, const float* __restrict__ scales,
                                                          float* __restrict__ out) {
     __shared__ __attribute__((aligned(16))) signed char col[kTileN][kTileK + 16];
-    const int64_t kt = blockIdx.x % nkt, nt = blockIdx.x / nkt;
+    const int64_t kt = (t0 + blockIdx.x) % nkt, nt = (t0 + blockIdx.x) / nkt;
     const ChannelsGeom g(K, N);
     for (int t = threadIdx.x; t < kTileN * kTileK / 16; t += kWG) {
         const int cb = t >> 7, kc = (t >> 4) & 7, cc = t & 15;
@@ -172,38 +172,105 @@ __device__ __forceinline__ floatx4 load4(const float* v, int64_t n, int64_t N) {
     return o;
 }
 
-// A wavefront per 16 tokens by 16 columns, operands straight from memory.  A
-// lane's A operand is a chunk of the packed weight (column lane & 15, k chunk lane
-// >> 4), its B operand 16 codes of token lane & 15, so that it ends up with four
-// neighbouring columns of one token.
-template <int NG, typename T>
-__global__ __launch_bounds__(kWG) void k_w8a8_simple(const W8A8Args a) {
-    const int lane = threadIdx.x & 63, lr = lane & 15, g = lane >> 4;
-    const int64_t wave = (int64_t)blockIdx.x * (kWG / 64) + (threadIdx.x >> 6);
+// ---- few tokens -----------------------------------------------------------
+
+// A workgroup takes 16 MB tokens by 16 C columns (of NG weights); its NW wavefronts
+// share K, a step of 64 k at a time in turn, with operands straight from memory: a
+// lane's A operand is a chunk of the packed weight (column lane & 15, k chunk lane >>
+// 4: a wavefront reads 1024 contiguous bytes), its B operand 16 codes of token lane &
+// 15, so that it ends up with four neighbouring columns of one token.  The sums of
+// the wavefronts are added through LDS; integers, so in any order.
+template <int NG, typename T, int MB, int C, int NW>
+__global__ __launch_bounds__(64 * NW) void k_w8a8_few(const W8A8Args a, int mblocks, int xlog) {
+    constexpr int B = MB * C * NG;                     // 16 x 16 blocks of sums
+    constexpr int U = B >= 8 ? 1 : (B >= 4 ? 2 : 4);   // steps whose loads are in flight together
+    __shared__ i32x4 red[NW][B][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lr = lane & 15, g = lane >> 4;
     const ChannelsGeom geo(a.K, a.N);
-    if (wave >= geo.NB * ceil_div(a.M, 16)) return;
-    const int64_t cb = wave % geo.NB, mb = wave / geo.NB;
-    const int64_t m = mb * 16 + lr;
-    const signed char* x = a.x + (m < a.M ? m : a.M - 1) * a.ldx + 16 * g;
-    i32x4 acc[NG];
+    const int bs = xcd_swizzle(blockIdx.x, gridDim.x, xlog);  // row blocks of the same columns on one XCD
+    const int64_t mb = bs % mblocks, cb0 = (int64_t)(bs / mblocks) * C;
+    const int64_t m0 = mb * 16 * MB;
+    const int rows = (int)min((int64_t)(16 * MB), a.M - m0), ncb = (int)min((int64_t)C, geo.NB - cb0);
+    const int ldx = (int)a.ldx, cbytes = (int)geo.KC * 256, steps = (int)(geo.Kpad / 64);
+    const __amdgpu_buffer_rsrc_t rx = make_rsrc(a.x + m0 * a.ldx, (uint32_t)((rows - 1) * ldx) + (uint32_t)geo.Kpad);
+    __amdgpu_buffer_rsrc_t rw[NG];
 #pragma unroll
-    for (int q = 0; q < NG; ++q) acc[q] = i32x4{0, 0, 0, 0};
-    for (int64_t kc = 0; kc < geo.KC; kc += 4) {
-        const i32x4 b = *(const i32x4*)(x + 16 * kc);
+    for (int q = 0; q < NG; ++q) rw[q] = make_rsrc(a.w[q] + cb0 * cbytes, (uint32_t)ncb * (uint32_t)cbytes);
+    int xo[MB];
+#pragma unroll
+    for (int i = 0; i < MB; ++i) xo[i] = i * 16 + lr < rows ? (i * 16 + lr) * ldx + 16 * g : kOobOff;
+
+    i32x4 acc[MB][NG * C];
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int c = 0; c < NG * C; ++c) acc[i][c] = i32x4{0, 0, 0, 0};
+    for (int st = wave; st < steps; st += NW * U) {
+        i32x4 x[U][MB], w[U][NG * C];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = st + u * NW;  // past the last step: zeros (the weight's buffer ends, or the next block's codes times zeros)
+            const int wo = k < steps ? lane * 16 : kOobOff;
+#pragma unroll
+            for (int q = 0; q < NG; ++q)
+#pragma unroll
+                for (int c = 0; c < C; ++c)
+                    w[u][q * C + c] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rw[q], wo, c * cbytes + k * 1024, MB == 1 ? kStreamPolicy : 0));
+#pragma unroll
+            for (int i = 0; i < MB; ++i)
+                x[u][i] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rx, k < steps ? xo[i] : kOobOff, k * 64, 0));
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int c = 0; c < NG * C; ++c)
+#pragma unroll
+                for (int i = 0; i < MB; ++i)
+                    acc[i][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u][c], x[u][i], acc[i][c], 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int c = 0; c < NG * C; ++c) red[wave][i * NG * C + c][lane] = acc[i][c];
+    __syncthreads();
+    // A thread per four columns of a token.
+    for (int t = threadIdx.x; t < MB * C * 64; t += 64 * NW) {
+        const int b = t >> 6, i = b / C, c = b - i * C;
+        const int64_t m = m0 + i * 16 + (t & 15), n = (cb0 + c) * 16 + 4 * ((t >> 4) & 3);
+        i32x4 v[NG];
 #pragma unroll
         for (int q = 0; q < NG; ++q) {
-            const i32x4 w = *(const i32x4*)(a.w[q] + ((cb * geo.KC + kc) * 16 + lane) * 16);
-            acc[q] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, b, acc[q], 0, 0, 0);
+            v[q] = red[0][i * NG * C + q * C + c][t & 63];
+#pragma unroll 5
+            for (int w = 1; w < NW; ++w) v[q] += red[w][i * NG * C + q * C + c][t & 63];
         }
+        if (m >= a.M || n >= a.N) continue;
+        const float sx = a.sx[m];
+        floatx4 o = product4(v[0], sx, load4(a.sw[0], n, a.N), load4(a.bias[0], n, a.N));
+        if constexpr (NG == 2) o = silu_mul4(o, product4(v[1], sx, load4(a.sw[1], n, a.N), load4(a.bias[1], n, a.N)));
+        store4((T*)a.y + m * a.ldy, n, a.N, o);
     }
-    if (m >= a.M) return;
-    const bool sums = a.K > 0;  // else the biases
-    const float sx = sums ? a.sx[m] : 0.0f;
-    const int64_t n = cb * 16 + 4 * g;
-    floatx4 v = product4(acc[0], sx, load4(sums ? a.sw[0] : nullptr, n, a.N), load4(a.bias[0], n, a.N));
-    if constexpr (NG == 2)
-        v = silu_mul4(v, product4(acc[1], sx, load4(sums ? a.sw[1] : nullptr, n, a.N), load4(a.bias[1], n, a.N)));
-    store4((T*)a.y + m * a.ldy, n, a.N, v);
+}
+
+// Wavefronts of a workgroup with `blocks` 16 x 16 blocks a weight.  Up to two blocks:
+// eight where K gives sixteen less than four steps each (us, sixteen -> eight: 1 x
+// 2048 -> 2048 3.1 -> 2.5, 1 x 2048 -> 11008 7.5 -> 5.2; 1 x 4096 -> 4096 4.5 against
+// 4.9, 16 x 11008 -> 4096 11.9 against 11.7).  More blocks: what LDS holds of their sums.
+int few_waves(int blocks, int ng, int64_t K) {
+    if (blocks <= 2) return K < 4096 ? 8 : 16;
+    return (blocks <= 4 ? 16 : 8) / ng;
+}
+
+// K == 0: the biases.
+template <int NG, typename T>
+__global__ void k_w8a8_bias(const W8A8Args a) {
+    for (int64_t m = blockIdx.y; m < a.M; m += gridDim.y)
+        for (int64_t n = 4 * (blockIdx.x * (int64_t)blockDim.x + threadIdx.x); n < a.N; n += 4 * (int64_t)gridDim.x * blockDim.x) {
+            floatx4 o = load4(a.bias[0], n, a.N);
+            if constexpr (NG == 2) o = silu_mul4(o, load4(a.bias[1], n, a.N));
+            store4((T*)a.y + m * a.ldy, n, a.N, o);
+        }
 }
 
 // ---- the tile kernel ------------------------------------------------------
@@ -222,9 +289,12 @@ struct TileCfg {
 };
 
 template <int NG, typename T, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void k_w8a8_tile(const W8A8Args a, int tiles_m, int tiles_n, int xlog) {
+__global__ __launch_bounds__(64 * WM * WN) void k_w8a8_tile(const W8A8Args a, int tiles_m, int tiles_n, int xlog,
+                                                                   int KS, int* part) {
     using C = TileCfg<NG, BM, BN, WM, WN>;
-    constexpr int TM = C::TM, TN = C::TN;
+    constexpr int TM = C::TM, TN = C::TN, kQuads = TM * TN / 4, kLoads = C::kXLoads + C::kWLoads, kReads = TM + TN;
+    // Of n things issued between kQuads quads of products, those before quad q.
+    constexpr auto part_of = [](int q, int n) { return q * n / kQuads; };
     __shared__ __attribute__((aligned(128))) signed char xs0[BM * kStage], xs1[BM * kStage];
     __shared__ __attribute__((aligned(128))) signed char ws0[BN * kStage], ws1[BN * kStage];
     __shared__ float esx[BM];
@@ -234,7 +304,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_w8a8_tile(const W8A8Args a, in
     const int wm = wave / WN, wn = wave % WN;
 
     // Tiles in groups of eight rows of tiles, column by column.
-    const int b = xcd_swizzle(blockIdx.x, gridDim.x, xlog);
+    // The K splits of a tile are neighbours.
+    const int bs = xcd_swizzle(blockIdx.x, gridDim.x, xlog), b = bs / KS, split = bs - b * KS;
     constexpr int kGroup = 8;
     const int group = b / (kGroup * tiles_n), in = b - group * (kGroup * tiles_n);
     const int gm = min(kGroup, tiles_m - group * kGroup);
@@ -247,38 +318,39 @@ __global__ __launch_bounds__(64 * WM * WN) void k_w8a8_tile(const W8A8Args a, in
     const int ldx = (int)a.ldx, cbytes = (int)geo.KC * 256;
     const signed char* const xp = a.x + m0 * a.ldx;
     const uint32_t xbytes = (uint32_t)((rows - 1) * ldx) + (uint32_t)geo.Kpad, wbytes = (uint32_t)ncb * (uint32_t)cbytes;
-    const int n = (int)(geo.Kpad / kStage);
+    const int stages = (int)(geo.Kpad / kStage), per = (stages + KS - 1) / KS;
+    const int s0 = split * per, n = min(stages, s0 + per);  // stages s0 .. n - 1, at least one
 
-    // A stage's loads.  Tokens: eight rows of 128 bytes a wavefront and load, the 16-byte
-    // chunk at place p of row r being chunk p ^ (r & 7) (no bank twice when sixteen rows
-    // are read at one k).  Weights: the layout as it is, half a column block a load.
+    // A stage's loads, a 16-byte one of each thread at a time.  Tokens: eight rows of 128
+    // bytes a wavefront, the chunk at place p of row r being chunk p ^ (r & 7) (no bank
+    // twice when sixteen rows are read at one k).  Weights: the layout as it is, half a
+    // column block a wavefront.  Past the last stage the buffers have no bytes: the loads
+    // are issued (the compiler counts them to know which ones a read has to wait for)
+    // and fetch nothing.
     const int xrow = lane >> 3, xoff = ((lane & 7) ^ xrow) * 16;
-    // Past the last stage the buffers have no bytes: the loads are issued (the compiler
-    // counts them to know which ones a read has to wait for) and fetch nothing.
-    auto load = [&](signed char* xs, signed char* ws, int s) {
-        const __amdgpu_buffer_rsrc_t rx = make_rsrc(xp, s < n ? xbytes : 0);
-#pragma unroll
-        for (int i = 0; i < C::kXLoads; ++i) {
-            const int r = (i * (C::kThreads / 64) + wave) * 8;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lds_void*)(xs + r * kStage), 16, (r + xrow) * ldx + xoff, s * kStage, 0, 0);
-        }
-#pragma unroll
-        for (int i = 0; i < C::kWLoads; ++i) {
-            const int u = i * (C::kThreads / 64) + wave;  // of 1024 bytes
-            const int q = NG == 1 ? 0 : i / (C::kWLoads / NG);
-            const int v = NG == 1 ? u : u - q * (BN / NG / 8);
+    auto load1 = [&](signed char* xs, signed char* ws, int s, int l) {
+        if (l < C::kXLoads) {
+            const __amdgpu_buffer_rsrc_t rx = make_rsrc(xp, s < n ? xbytes : 0);
+            const int r = (l * (C::kThreads / 64) + wave) * 8;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lds_void*)(xs + r * kStage), 16, (r + xrow) * ldx + xoff,
+                                                     s * kStage, 0, 0);
+        } else {
+            const int i = l - C::kXLoads, u = i * (C::kThreads / 64) + wave;  // of 1024 bytes
+            const int q = NG == 1 ? 0 : i / (C::kWLoads / NG), v = NG == 1 ? u : u - q * (BN / NG / 8);
             const __amdgpu_buffer_rsrc_t rw = make_rsrc(a.w[q] + cb0 * cbytes, s < n ? wbytes : 0);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_void*)(ws + u * 1024), 16, (v >> 1) * cbytes + (v & 1) * 1024 + lane * 16, s * 2048, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_void*)(ws + u * 1024), 16,
+                                                     (v >> 1) * cbytes + (v & 1) * 1024 + lane * 16, s * 2048, 0, 0);
         }
     };
-    // Operands of half a stage: 64 k.
-    auto read = [&](i32x4 (&x)[TM], i32x4 (&w)[TN], const signed char* xs, const signed char* ws, int h) {
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
+    // An operand of half a stage, 64 k: the first columns', the tokens', then the other
+    // columns', as the products take them.
+    auto read1 = [&](i32x4 (&x)[TM], i32x4 (&w)[TN], const signed char* xs, const signed char* ws, int h, int l) {
+        if (l >= 1 && l <= TM) {
+            const int i = l - 1;
             x[i] = *(const i32x4*)(xs + (wm * (BM / WM) + i * 16 + lr) * kStage + (((4 * h + g) ^ (lr & 7)) * 16));
-#pragma unroll
-        for (int j = 0; j < TN; ++j) {
+        } else {
             // NG weights: each wavefront has the same columns of all.
+            const int j = l == 0 ? 0 : l - TM;
             const int cb = NG == 1 ? wn * TN + j : (j / (TN / NG)) * (BN / 16 / NG) + wn * (TN / NG) + j % (TN / NG);
             w[j] = *(const i32x4*)(ws + cb * 2048 + h * 1024 + lane * 16);
         }
@@ -288,15 +360,18 @@ __global__ __launch_bounds__(64 * WM * WN) void k_w8a8_tile(const W8A8Args a, in
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
-    auto mfma = [&](const i32x4 (&x)[TM], const i32x4 (&w)[TN]) {
+    // Four products of half a stage.
+    auto mfma4 = [&](const i32x4 (&x)[TM], const i32x4 (&w)[TN], int q) {
 #pragma unroll
-        for (int j = 0; j < TN; ++j)
-#pragma unroll
-            for (int i = 0; i < TM; ++i) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[j], x[i], acc[i][j], 0, 0, 0);
+        for (int p = 4 * q; p < 4 * q + 4; ++p) {
+            const int j = p / TM, i = p % TM;
+            acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[j], x[i], acc[i][j], 0, 0, 0);
+        }
     };
 
     i32x4 x0[TM], w0[TN], x1[TM], w1[TN];
-    load(xs0, ws0, 0);
+#pragma unroll
+    for (int l = 0; l < kLoads; ++l) load1(xs0, ws0, s0, l);
     for (int t = threadIdx.x; t < BM; t += C::kThreads) esx[t] = t < rows ? a.sx[m0 + t] : 0.0f;
     for (int t = threadIdx.x; t < BN; t += C::kThreads) {
         const int q = t / (BN / NG);
@@ -305,31 +380,63 @@ __global__ __launch_bounds__(64 * WM * WN) void k_w8a8_tile(const W8A8Args a, in
         eb[t] = nn < a.N && a.bias[q] ? a.bias[q][nn] : 0.0f;
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    load(xs1, ws1, 1);
-    read(x0, w0, xs0, ws0, 0);
+#pragma unroll
+    for (int l = 0; l < kLoads; ++l) load1(xs1, ws1, s0 + 1, l);
+#pragma unroll
+    for (int l = 0; l < kReads; ++l) read1(x0, w0, xs0, ws0, 0, l);
+    // A stage: the products of its first half while the operands of the second are
+    // read; all wavefronts are then done with its buffers, which the stage after the
+    // next is loaded into while the products of the second half run and the first
+    // operands of the next stage are read.  A load or read is issued every few products:
+    // all of them at once held the products back until the queues had taken them (4096
+    // x 8192 -> 4096 117 -> 107 us).
     auto step = [&](signed char* xs, signed char* ws, const signed char* xn, const signed char* wsn, int s) {
-        read(x1, w1, xs, ws, 1);
-        __builtin_amdgcn_sched_barrier(0);
-        mfma(x0, w0);
-        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int q = 0; q < kQuads; ++q) {
+#pragma unroll
+            for (int l = part_of(q, kReads); l < part_of(q + 1, kReads); ++l) read1(x1, w1, xs, ws, 1, l);
+            __builtin_amdgcn_sched_barrier(0);
+            mfma4(x0, w0, q);
+            __builtin_amdgcn_sched_barrier(0);
+        }
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        load(xs, ws, s + 2);
-        read(x0, w0, xn, wsn, 0);
-        __builtin_amdgcn_sched_barrier(0);
-        mfma(x1, w1);
-        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int q = 0; q < kQuads; ++q) {
+#pragma unroll
+            for (int l = part_of(q, kReads); l < part_of(q + 1, kReads); ++l) read1(x0, w0, xn, wsn, 0, l);
+#pragma unroll
+            for (int l = part_of(q, kLoads); l < part_of(q + 1, kLoads); ++l) load1(xs, ws, s + 2, l);
+            __builtin_amdgcn_sched_barrier(0);
+            mfma4(x1, w1, q);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     };
-    for (int s = 0; s < n - 1; s += 2) {
+    for (int s = s0; s < n - 1; s += 2) {
         step(xs0, ws0, xs1, ws1, s);
         step(xs1, ws1, xs0, ws0, s + 1);
     }
-    if (n & 1) step(xs0, ws0, xs1, ws1, n - 1);
+    if ((n - s0) & 1) step(xs0, ws0, xs1, ws1, n - 1);
     // No load may still be writing to LDS when the workgroup's share of it is given away.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
     // A lane has columns 4 g .. 4 g + 3 of a block, of token lr.
     const int col0 = wn * (TN / NG) * 16 + 4 * g;  // of the first block, in its weight
     const int64_t nb = cb0 * 16 + col0;
+    if (KS > 1) {  // partial sums, [split][weight][M][16 NB]
+        const int64_t np = geo.NB * 16;
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            const int r = wm * (BM / WM) + i * 16 + lr;
+            if (r >= rows) continue;
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+                const int q = j / (TN / NG);
+                const int64_t nn = nb + 16 * (j - q * (TN / NG));
+                if (nn < np) *(i32x4*)(part + ((split * NG + q) * a.M + m0 + r) * np + nn) = acc[i][j];
+            }
+        }
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
         const int r = wm * (BM / WM) + i * 16 + lr;
@@ -348,65 +455,207 @@ __global__ __launch_bounds__(64 * WM * WN) void k_w8a8_tile(const W8A8Args a, in
     }
 }
 
+// y of the partial sums of KS splits.
+template <int NG, typename T>
+__global__ __launch_bounds__(kWG) void k_w8a8_reduce(const W8A8Args a, int KS, const int* __restrict__ part, int64_t np) {
+    const int64_t n = 4 * (blockIdx.x * (int64_t)kWG + threadIdx.x);
+    if (n >= a.N) return;
+    for (int64_t m = blockIdx.y; m < a.M; m += gridDim.y) {
+        i32x4 v[NG];
+#pragma unroll
+        for (int q = 0; q < NG; ++q) {
+            const int* p = part + (q * a.M + m) * np + n;
+            v[q] = *(const i32x4*)p;
+            for (int s = 1; s < KS; ++s) v[q] += *(const i32x4*)(p + s * NG * a.M * np);
+        }
+        const float sx = a.sx[m];
+        floatx4 o = product4(v[0], sx, load4(a.sw[0], n, a.N), load4(a.bias[0], n, a.N));
+        if constexpr (NG == 2) o = silu_mul4(o, product4(v[1], sx, load4(a.sw[1], n, a.N), load4(a.bias[1], n, a.N)));
+        store4((T*)a.y + m * a.ldy, n, a.N, o);
+    }
+}
+
 template <int NG, typename T, int BM, int BN, int WM, int WN>
-void launch_tile(const W8A8Args& a, hipStream_t s) {
+void launch_tile(const W8A8Args& a, int KS, int* part, hipStream_t s) {
     const int64_t tm = ceil_div(a.M, BM), tn = ceil_div(ChannelsGeom(a.K, a.N).NB, BN / 16 / NG);
     k_w8a8_tile<NG, T, BM, BN, WM, WN>
-        <<<(unsigned)(tm * tn), 64 * WM * WN, 0, s>>>(a, (int)tm, (int)tn, xcd_log2(device_xcds(s)));
+        <<<(unsigned)(tm * tn * KS), 64 * WM * WN, 0, s>>>(a, (int)tm, (int)tn, xcd_log2(device_xcds(s)), KS, part);
+    if (KS > 1) {
+        const dim3 grid((unsigned)ceil_div(a.N, 4 * kWG), (unsigned)(a.M < 32768 ? a.M : 32768));
+        k_w8a8_reduce<NG, T><<<grid, kWG, 0, s>>>(a, KS, part, ChannelsGeom(a.K, a.N).NB * 16);
+    }
+}
+
+template <int NG, typename T, int MB, int C, int NW>
+void launch_few(const W8A8Args& a, hipStream_t s) {
+    const int64_t mbs = ceil_div(a.M, 16 * MB), cgs = ceil_div(ChannelsGeom(a.K, a.N).NB, C);
+    const int xlog = xcd_log2(device_xcds(s));
+    if constexpr (NW == 16) {
+        if (few_waves(MB * C, NG, a.K) == 8) {
+            k_w8a8_few<NG, T, MB, C, 8><<<(unsigned)(mbs * cgs), 64 * 8, 0, s>>>(a, (int)mbs, xlog);
+            return;
+        }
+    }
+    k_w8a8_few<NG, T, MB, C, NW><<<(unsigned)(mbs * cgs), 64 * NW, 0, s>>>(a, (int)mbs, xlog);
 }
 
 template <int NG, typename T>
-hipError_t launch_as(const W8A8Args& a, hipStream_t s) {
-    if (a.K > 0 && a.M > 128) {
-        launch_tile<NG, T, 256, 256, 4, 2>(a, s);
-    } else {
-        const int64_t waves = ChannelsGeom(a.K, a.N).NB * ceil_div(a.M, 16);
-        k_w8a8_simple<NG, T><<<(unsigned)ceil_div(waves, kWG / 64), kWG, 0, s>>>(a);
+hipError_t launch_as(const W8A8Args& a, const W8A8Plan& p, int* part, hipStream_t s) {
+    switch (p.form) {
+        case W8A8Form::bias: {
+            const dim3 grid((unsigned)min(ceil_div(a.N, 4 * kWG), (int64_t)4096), (unsigned)(a.M < 32768 ? a.M : 32768));
+            k_w8a8_bias<NG, T><<<grid, kWG, 0, s>>>(a);
+            break;
+        }
+        case W8A8Form::few1x1: launch_few<NG, T, 1, 1, 16>(a, s); break;
+        case W8A8Form::few2x1: launch_few<NG, T, 2, 1, 16>(a, s); break;
+        case W8A8Form::few2x2: launch_few<NG, T, 2, 2, 16 / NG>(a, s); break;
+        case W8A8Form::few4x2: launch_few<NG, T, 4, 2, 8 / NG>(a, s); break;
+        case W8A8Form::tile64x128: launch_tile<NG, T, 64, 128, 1, 4>(a, p.KS, part, s); break;
+        case W8A8Form::tile128: launch_tile<NG, T, 128, 128, 2, 2>(a, p.KS, part, s); break;
+        case W8A8Form::tile128x256: launch_tile<NG, T, 128, 256, 2, 4>(a, p.KS, part, s); break;
+        case W8A8Form::tile256: launch_tile<NG, T, 256, 256, 2, 4>(a, p.KS, part, s); break;
     }
     return hipGetLastError();
 }
 
 template <int NG>
-hipError_t launch_ng(const W8A8Args& a, hipStream_t s) {
-    return a.t == DType::f32 ? launch_as<NG, float>(a, s)
-                             : (a.t == DType::bf16 ? launch_as<NG, __bf16>(a, s) : launch_as<NG, _Float16>(a, s));
+hipError_t launch_ng(const W8A8Args& a, const W8A8Plan& p, int* part, hipStream_t s) {
+    return a.t == DType::f32 ? launch_as<NG, float>(a, p, part, s)
+                             : (a.t == DType::bf16 ? launch_as<NG, __bf16>(a, p, part, s)
+                                                   : launch_as<NG, _Float16>(a, p, part, s));
 }
 
 }  // namespace
 
+// A launch holds fewer than 2^32 threads: f(first tile, tiles) over nkt times the
+// column tiles.
+constexpr int64_t kPackTiles = (int64_t)1 << 23;
+template <typename F>
+static void each_tiles(int64_t nkt, int64_t N, F f) {
+    const int64_t tiles = nkt * ceil_div(N, kTileN);
+    for (int64_t t = 0; t < tiles; t += kPackTiles) f(t, (unsigned)min(kPackTiles, tiles - t));
+}
+
 hipError_t launch_channels_quantize(const float* w, int64_t K, int64_t N, float* qdata, float* scales, void* packed,
                                     void* top, hipStream_t s) {
     k_channels_start<<<(unsigned)ceil_div(N, kWG), kWG, 0, s>>>((uint32_t*)top, N);
-    const int64_t rows = 256;
     if (K > 0) {
+        constexpr int64_t rows = 256;
         const dim3 grid((unsigned)ceil_div(N, 64), (unsigned)ceil_div(K, rows));
         k_channels_top<<<grid, kWG, 0, s>>>(w, K, N, rows, (uint32_t*)top);
     }
     const int64_t nkt = K > 0 ? ceil_div(K, kTileK) : 1;
-    k_channels_pack<false><<<(unsigned)(nkt * ceil_div(N, kTileN)), kWG, 0, s>>>(
-        w, K, N, nkt, (const uint32_t*)top, scales, qdata, K > 0 ? (signed char*)packed : nullptr, nullptr);
+    each_tiles(nkt, N, [&](int64_t t0, unsigned n) {
+        k_channels_pack<false><<<n, kWG, 0, s>>>(w, K, N, nkt, t0, (const uint32_t*)top, scales, qdata,
+                                                 K > 0 ? (signed char*)packed : nullptr, nullptr);
+    });
     return hipGetLastError();
 }
 
 hipError_t launch_channels_pack(const float* codes, int64_t K, int64_t N, void* packed, int* bad, hipStream_t s) {
     const int64_t nkt = ceil_div(K, kTileK);
-    k_channels_pack<true><<<(unsigned)(nkt * ceil_div(N, kTileN)), kWG, 0, s>>>(codes, K, N, nkt, nullptr, nullptr,
-                                                                               nullptr, (signed char*)packed, bad);
+    each_tiles(nkt, N, [&](int64_t t0, unsigned n) {
+        k_channels_pack<true><<<n, kWG, 0, s>>>(codes, K, N, nkt, t0, nullptr, nullptr, nullptr, (signed char*)packed, bad);
+    });
     return hipGetLastError();
 }
 
 hipError_t launch_channels_unpack(const void* packed, int64_t K, int64_t N, const float* scales, float* out,
                                   hipStream_t s) {
     const int64_t nkt = ceil_div(K, kTileK);
-    k_channels_unpack<<<(unsigned)(nkt * ceil_div(N, kTileN)), kWG, 0, s>>>((const signed char*)packed, K, N, nkt,
-                                                                           scales, out);
+    each_tiles(nkt, N, [&](int64_t t0, unsigned n) {
+        k_channels_unpack<<<n, kWG, 0, s>>>((const signed char*)packed, K, N, nkt, t0, scales, out);
+    });
     return hipGetLastError();
 }
 
-int64_t w8a8_workspace_bytes(int, int64_t, int64_t, int64_t) { return 0; }
+int64_t w8a8_plan_bytes(const W8A8Plan& p, int ng, int64_t M, int64_t K, int64_t N) {
+    return p.KS > 1 ? (int64_t)p.KS * ng * M * ChannelsGeom(K, N).NB * 64 : 0;
+}
 
-hipError_t launch_w8a8(const W8A8Args& a, int ng, void*, hipStream_t s) {
-    return ng == 2 ? launch_ng<2>(a, s) : launch_ng<1>(a, s);
+// The form and the K splits with the least time by a model of a launch, in us: a form
+// that puts w workgroups on a CU, each with st steps of K (stages of 128 k; a
+// wavefront's steps of 64 k in the forms for few tokens), takes
+//   fixed + max(alone * st, w * (step * st + end)), and at least 2 + the weights at 4.7 TB/s,
+// a split of K 3 us and its partial sums at 3.5 TB/s more.  The constants are fitted to
+// 316 shapes (1 to 8192 tokens, K and N of 512 to 28672, one weight and two) with every
+// form timed on each; the form this picks takes 1.04 times the fastest one's time on
+// average, 1.13 times in one of ten.  For instance (us, 64 x 128 / 128 x 128 / 128 x 256 / 256 x
+// 256): 333 x 2043 -> 5001 11.7 / 14.8 / 19.0 / 32.9, 2048 x 4096 -> 4096 49 / 41 / 37 / 48,
+// 8192 x 8192 -> 28672 2380 / 1850 / 1940 / 1440; 128 x 11008 -> 4096 gated, 64 x 128 without
+// a split 60, with four 32.  The forms for few tokens read a weight once for each of
+// their row blocks, which costs them large weights: 48 x 14336 -> 28672 132 against 85.
+W8A8Plan w8a8_plan(int ng, int64_t M, int64_t K, int64_t N, int64_t cus) {
+    W8A8Plan best;
+    if (K == 0) return best;
+    if (M <= 16) {  // one row block: a read of the weight, whatever the sizes
+        best.form = W8A8Form::few1x1;
+        return best;
+    }
+    static constexpr struct {
+        W8A8Form form;
+        int few, rows, cols;                  // rows and columns (of all weights) of a workgroup, in 16s for few
+        struct { double fixed, alone, step, end; } t[2];  // one weight, two
+    } forms[] = {
+        {W8A8Form::few2x1, 1, 2, 1, {{1.0, .5, 1.0, 0.}, {.5, 1.16, 1.07, 0.}}},
+        {W8A8Form::few2x2, 1, 2, 2, {{1.95, .5, 1.08, 1.}, {2.7, .87, .86, .55}}},
+        {W8A8Form::few4x2, 1, 4, 2, {{1.4, .7, .81, 1.4}, {2.7, .7, .65, 1.2}}},
+        {W8A8Form::tile64x128, 0, 64, 128, {{2.5, .515, .30, 1.1}, {2.5, .515, .30, 1.1}}},
+        {W8A8Form::tile128, 0, 128, 128, {{3.3, .61, .464, 1.95}, {3.3, .61, .464, 1.95}}},
+        {W8A8Form::tile128x256, 0, 128, 256, {{0., .9, .853, 5.4}, {0., .9, .853, 5.4}}},
+        {W8A8Form::tile256, 0, 256, 256, {{0., 1.31, 1.3, 9.1}, {0., 1.31, 1.3, 9.1}}},
+    };
+    constexpr int64_t kFewRows = 256, kFewBytes = 100 * 1000 * 1000, kMinSplitStages = 4;
+    const ChannelsGeom g(K, N);
+    const double cu = cus < 1 ? 1.0 : (double)cus;
+    double least = 0.0;
+    for (const auto& f : forms) {
+        if (f.few && (M > kFewRows || ng * K * N > kFewBytes)) continue;
+        const auto& t = f.t[ng - 1];
+        for (int ks = 1; ks <= (f.few ? 1 : 8); ks *= 2) {
+            const int64_t stages = g.Kpad / 128, per = ceil_div(stages, ks);
+            if (ks > 1 && (per < kMinSplitStages || ceil_div(stages, per) != ks)) continue;
+            double w, st;
+            if (f.few) {
+                w = (double)(ceil_div(M, 16 * f.rows) * ceil_div(g.NB, f.cols)) / cu;
+                w = w < 1.0 ? 1.0 : w;
+                st = (double)ceil_div(2 * stages, few_waves(f.rows * f.cols, ng, K));
+            } else {
+                w = (double)ceil_div(ceil_div(M, f.rows) * ceil_div(g.NB, f.cols / 16 / ng) * ks, (int64_t)cu);
+                st = (double)per;
+            }
+            const double busy = w * (t.step * st + t.end), alone = t.alone * st;
+            double us = t.fixed + (busy > alone ? busy : alone);
+            const double read = 2.0 + (double)(ng * K) * (double)N / 4.7e6;
+            us = us > read ? us : read;
+            if (ks > 1) us += 3.0 + (double)(ks * ng * 4) * (double)M * (double)N / 3.5e6;
+            if (least == 0.0 || us < least) least = us, best.form = f.form, best.KS = ks;
+        }
+    }
+    return best;
+}
+
+hipError_t launch_w8a8(const W8A8Args& a, int ng, const W8A8Plan& p, void* ws, hipStream_t s) {
+    // A launch holds fewer than 2^32 threads: very wide or very many rows go in slices.
+    constexpr int64_t kRows = (int64_t)1 << 26, kCols = (int64_t)1 << 24;
+    if (a.M > kRows || a.N > kCols) {
+        for (int64_t m = 0; m < a.M; m += kRows)
+            for (int64_t n = 0; n < a.N; n += kCols) {
+                W8A8Args b = a;
+                b.M = min(kRows, a.M - m), b.N = min(kCols, a.N - n);
+                b.x += m * a.ldx, b.sx += m;
+                b.y = (char*)a.y + (m * a.ldy + n) * dtype_bytes(a.t);
+                for (int q = 0; q < ng; ++q) {
+                    b.w[q] += n / 16 * ChannelsGeom(a.K, a.N).KC * 256, b.sw[q] += n;
+                    if (b.bias[q]) b.bias[q] += n;
+                }
+                const hipError_t e = launch_w8a8(b, ng, p, ws, s);
+                if (e != hipSuccess) return e;
+            }
+        return hipSuccess;
+    }
+    return ng == 2 ? launch_ng<2>(a, p, (int*)ws, s) : launch_ng<1>(a, p, (int*)ws, s);
 }
 
 }  // namespace sgq

@@ -261,6 +261,18 @@ def _tokens(t: TokensInt8, dev: torch.device) -> Tuple[int, int, int, int]:
     return c.data_ptr(), ld, s.data_ptr(), M
 
 
+def _workspace(query, M: int, K: int, N: int, dev: torch.device):
+    """A workspace of its own for each call: what a graph captures stays the graph's."""
+    if M <= 16:  # such products have none
+        return None, 0
+    if dev.index == torch.cuda.current_device():
+        need = query(M, K, N, 0)
+    else:
+        with torch.cuda.device(dev):
+            need = query(M, K, N, 0)
+    return (torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None), need
+
+
 def _bias(b: Optional[torch.Tensor], N: int, dev: torch.device) -> Optional[torch.Tensor]:
     return None if b is None else _vector(b, N, dev, "bias")
 
@@ -275,8 +287,7 @@ def quantized_matmul_w8a8(t: TokensInt8, qw: ChannelsInt8, bias: Optional[torch.
     N, lib = qw.N, load_library()
     b = _bias(bias, N, dev)
     y = _output(out, M, N, dtype, dev)
-    need = lib.sgq_linear_w8a8_workspace_bytes(M, qw.K, N)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
+    ws, need = _workspace(lib.sgq_linear_w8a8_workspace_bytes, M, qw.K, N, dev)
     _call(dev, lib.sgq_linear_w8a8, codes, ldc, scales, M, qw.K, N, qw.packed.data_ptr(),
           qw.scales.data_ptr(), None if b is None else b.data_ptr(), y.data_ptr(), _dtype(dtype),
           N if out is None else _ld(y), None if ws is None else ws.data_ptr(), need)
@@ -296,8 +307,7 @@ def quantized_swiglu_w8a8(t: TokensInt8, w_gate: ChannelsInt8, w_up: ChannelsInt
     K, N, lib = w_gate.K, w_gate.N, load_library()
     bg, bu = _bias(bias_gate, N, dev), _bias(bias_up, N, dev)
     h = _output(out, M, N, dtype, dev)
-    need = lib.sgq_swiglu_w8a8_workspace_bytes(M, K, N)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
+    ws, need = _workspace(lib.sgq_swiglu_w8a8_workspace_bytes, M, K, N, dev)
     _call(dev, lib.sgq_swiglu_w8a8, codes, ldc, scales, M, K, N, w_gate.packed.data_ptr(),
           w_gate.scales.data_ptr(), None if bg is None else bg.data_ptr(), w_up.packed.data_ptr(),
           w_up.scales.data_ptr(), None if bu is None else bu.data_ptr(), h.data_ptr(), _dtype(dtype),

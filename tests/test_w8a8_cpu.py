@@ -30,8 +30,41 @@ def test_sizes(lib):
     assert lib.sgq_channels_packed_bytes(131072, 16) == -1 and lib.sgq_channels_packed_bytes(16, -1) == -1
     for fn in (lib.sgq_linear_w8a8_workspace_bytes, lib.sgq_swiglu_w8a8_workspace_bytes):
         for shape in [(0, 0, 0), (1, 1, 1), (1, 4096, 4096), (128, 1024, 1024), (2048, 4096, 11008), (3, 0, 5)]:
-            assert fn(*shape) >= 0
-        assert fn(1, 131072, 16) == -1 and fn(-1, 1, 1) == -1
+            assert fn(*shape, 256) >= 0
+        assert fn(1, 131072, 16, 256) == -1 and fn(-1, 1, 1, 256) == -1 and fn(1, 1, 1, -1) == -1
+
+
+def _plan(lib, gated, M, K, N, cus=256):
+    import ctypes
+
+    form, ks = ctypes.c_int(-1), ctypes.c_int(-1)
+    assert lib.sgq_w8a8_plan(gated, M, K, N, cus, ctypes.byref(form), ctypes.byref(ks)) == 0
+    return form.value, ks.value
+
+
+def test_plans(lib):
+    """Every form has shapes of its own, every split of K its stages of 128, and the workspace is the partial sums'."""
+    seen = set()
+    for cus in (1, 32, 64, 128, 256, 304):
+        for gated in (0, 1):
+            for K in (0, 1, 100, 640, 1024, 2043, 4096, 11008, 14336, 131071):
+                for N in (1, 40, 1024, 4096, 5001, 28672):
+                    for M in (1, 16, 17, 32, 33, 64, 100, 128, 200, 333, 512, 1000, 2048, 8192):
+                        form, ks = _plan(lib, gated, M, K, N, cus)
+                        seen.add(form)
+                        assert (form == 0) == (K == 0) and (form == 1) == (K > 0 and M <= 16)
+                        stages = -(-K // 128)
+                        assert ks == 1 or (form >= 5 and (ks - 1) * -(-stages // ks) < stages)
+                        fn = lib.sgq_swiglu_w8a8_workspace_bytes if gated else lib.sgq_linear_w8a8_workspace_bytes
+                        want = 0 if ks == 1 else ks * (1 + gated) * M * -(-N // 16) * 64
+                        assert fn(M, K, N, cus) == want
+    assert seen == set(range(9))
+    assert _plan(lib, 0, 8192, 8192, 28672) == (8, 1)
+    import ctypes
+
+    i = ctypes.c_int()
+    assert lib.sgq_w8a8_plan(0, 1, 131072, 1, 256, ctypes.byref(i), ctypes.byref(i)) == 1
+    assert lib.sgq_w8a8_plan(0, 1, 1, 1, 256, None, ctypes.byref(i)) == 1
 
 
 def test_tokens_refusals(lib):
