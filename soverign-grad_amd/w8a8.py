@@ -26,7 +26,16 @@ from typing import Optional, Tuple
 
 import torch
 
-from . import _check, _ptr, _stream, load_library
+from . import _check, _ptr, _raw_stream, _stream, load_library
+
+# torch.cuda.current_device() without its check that CUDA is initialised, which the
+# tensors of a call have shown.
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+if _raw_stream is None:
+
+    def _raw_stream(index: int) -> int:
+        return _stream(torch.device("cuda", index))
+
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # SGQ_F32, SGQ_BF16, SGQ_F16
 
@@ -57,11 +66,12 @@ class ChannelsInt8:
 
 def _call(dev: torch.device, fn, *args) -> None:
     """fn(*args, stream) on dev's current stream, with dev the current device."""
-    if dev.index == torch.cuda.current_device():
-        status = fn(*args, _stream(dev))
+    i = dev.index
+    if i == _current_device():
+        status = fn(*args, _raw_stream(i))
     else:
         with torch.cuda.device(dev):
-            status = fn(*args, _stream(dev))
+            status = fn(*args, _raw_stream(i))
     if status:
         _check(status)
 
@@ -91,7 +101,8 @@ def _rows(x: torch.Tensor, name: str) -> torch.Tensor:
 
 def _ld(x: torch.Tensor) -> int:
     """Row stride of a matrix of contiguous rows (that of a single row says nothing)."""
-    return x.stride(0) if x.shape[0] > 1 else max(x.shape[1], 1)
+    M, K = x.shape
+    return x.stride(0) if M > 1 else K or 1
 
 
 def _vector(t: torch.Tensor, n: int, dev: torch.device, name: str) -> torch.Tensor:
@@ -143,8 +154,11 @@ def _norm_tokens(x, residual, weight, eps, out):
     dev = x.device
     g = _vector(weight, K, dev, "weight")
     t = _new_tokens(M, K, dev)
-    r, ldr, h, ldh = (None, 0, None, 0) if residual is None else (residual.data_ptr(), _ld(residual), out.data_ptr(),
-                                                                    _ld(out))
+    if residual is None:
+        r = h = None
+        ldr = ldh = 0
+    else:
+        r, ldr, h, ldh = residual.data_ptr(), _ld(residual), out.data_ptr(), _ld(out)
     _call(dev, load_library().sgq_rms_norm_tokens, x.data_ptr(), _dtype(x.dtype), _ld(x), r, ldr, h, ldh,
           g.data_ptr(), eps, M, K, t.codes.data_ptr(), _row_bytes(K), t.scales.data_ptr())
     return t
@@ -159,14 +173,15 @@ def add_rms_norm_int8_tokens(x: torch.Tensor, residual: torch.Tensor, weight: to
                              out: Optional[torch.Tensor] = None) -> Tuple[TokensInt8, torch.Tensor]:
     """h = x + residual, and rms_norm(h) as int8 tokens.  h comes in x's shape, or in
     `out`, which may be x or residual itself."""
-    if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device:
+    shape, dtype, dev = x.shape, x.dtype, x.device
+    if residual.shape != shape or residual.dtype != dtype or residual.device != dev:
         raise ValueError("x and residual must be alike in shape, type and device")
-    shape = x.shape
     x, r = _rows(x, "x"), _rows(residual, "residual")
     if out is None:
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        M, K = x.shape
+        y = torch.empty(M, K, dtype=dtype, device=dev)
         h = y if len(shape) == 2 else y.view(shape)
-    elif out.shape != shape or out.dtype != x.dtype or out.device != x.device:
+    elif out.shape != shape or out.dtype != dtype or out.device != dev:
         raise ValueError("out must be alike x in shape, type and device")
     else:
         h, y = out, _rows(out, "out")
@@ -265,7 +280,7 @@ def _workspace(query, M: int, K: int, N: int, dev: torch.device):
     """A workspace of its own for each call: what a graph captures stays the graph's."""
     if M <= 16:  # such products have none
         return None, 0
-    if dev.index == torch.cuda.current_device():
+    if dev.index == _current_device():
         need = query(M, K, N, 0)
     else:
         with torch.cuda.device(dev):
