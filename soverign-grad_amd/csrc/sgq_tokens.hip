@@ -225,18 +225,28 @@ __global__ __launch_bounds__(kBlock) void k_tokens_values(const signed char* __r
 
 constexpr int64_t kMaxRowGroups = (int64_t)1 << 20;  // workgroups of a launch (fewer than 2^32 threads)
 
+// Threads of a row by its chunks q.  Measured (us, graphs; bf16 with a residual unless
+// said): a wavefront against 256 threads, 4096 x 1024 7.5 / 10.0, but 2048 x 2048 8.3 / 7.6 and
+// 8 x 2048 fp32 4.0 / 2.9; 256 threads of three chunks against four, 1023 x 5003 fp16 without
+// 7.0 / 7.9; 512 of two against 256 of four, 8192 x 8192 84 / 87, 16 x 8192 3.9 / 4.3.  HBM bounds
+// them from there: 2048 x 4096 11.3 us, 5.2 TB/s, 2048 x 11008 fp32 tokens 20.7, 5.4 TB/s (a large
+// copy reaches 5.1); a few rows are one row's latency.
 template <typename T, bool NORM, bool RES>
 hipError_t launch_rows(const TokensArgs& a, hipStream_t s) {
     const auto grid = [&](int rows) { return (unsigned)(ceil_div(a.M, rows) < kMaxRowGroups ? ceil_div(a.M, rows) : kMaxRowGroups); };
     const int64_t q = a.Kpad / kV;
     if (q <= 64)
         k_tokens_row<T, NORM, RES, 64, 1><<<grid(4), kBlock, 0, s>>>(a);
+    else if (q <= 128)
+        k_tokens_row<T, NORM, RES, 64, 2><<<grid(4), kBlock, 0, s>>>(a);
     else if (q <= 256)
         k_tokens_row<T, NORM, RES, 256, 1><<<grid(1), 256, 0, s>>>(a);
     else if (q <= 512)
         k_tokens_row<T, NORM, RES, 256, 2><<<grid(1), 256, 0, s>>>(a);
+    else if (q <= 768)
+        k_tokens_row<T, NORM, RES, 256, 3><<<grid(1), 256, 0, s>>>(a);
     else if (q <= 1024)
-        k_tokens_row<T, NORM, RES, 256, 4><<<grid(1), 256, 0, s>>>(a);
+        k_tokens_row<T, NORM, RES, 512, 2><<<grid(1), 512, 0, s>>>(a);
     else if (q <= 2048)
         k_tokens_row<T, NORM, RES, 512, 4><<<grid(1), 512, 0, s>>>(a);
     else if constexpr (!NORM) {
