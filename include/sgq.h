@@ -443,8 +443,8 @@ int sgq_swiglu_w8a8(const void* codes, int64_t ldc, const float* x_scales, int64
 /* The kernel such a product (gated: such a gated MLP) runs on `compute_units` CUs
  * (0: the current device's).  *form: 0 the biases alone (K == 0); 1..4 workgroups of
  * 16 x 16, 32 x 16, 32 x 32 and 64 x 32 tokens by columns, whose wavefronts share K;
- * 5..8 tiles of 64 x 128, 128 x 128, 128 x 256 and 256 x 256 through LDS (columns of
- * both weights).  *k_splits: workgroups that share a tile's K, their sums added by
+ * 5..9 tiles of 64 x 128, 128 x 128 (with two and with four buffers of a stage), 128 x
+ * 256 and 256 x 256 through LDS (columns of both weights).  *k_splits: workgroups that share a tile's K, their sums added by
  * a second kernel.  Host-only. */
 int sgq_w8a8_plan(int gated, int64_t M, int64_t K, int64_t N, int compute_units, int* form, int* k_splits);
 

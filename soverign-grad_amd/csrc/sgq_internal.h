@@ -541,7 +541,7 @@ struct W8A8Args {
 // Forms of the product: the biases (K = 0), k_w8a8_few with row blocks x column
 // blocks of 16, k_w8a8_tile with tokens x columns.  KS: workgroups that share a
 // tile's K, whose sums a second kernel adds (each has stages of its own).
-enum class W8A8Form : int { bias, few1x1, few2x1, few2x2, few4x2, tile64x128, tile128, tile128x256, tile256 };
+enum class W8A8Form : int { bias, few1x1, few2x1, few2x2, few4x2, tile64x128, tile128, tile128deep, tile128x256, tile256 };
 struct W8A8Plan {
     W8A8Form form = W8A8Form::bias;
     int KS = 1;

@@ -288,15 +288,20 @@ struct TileCfg {
     static constexpr int kWLoads = BN * kStage / 16 / kThreads;
 };
 
-template <int NG, typename T, int BM, int BN, int WM, int WN>
+template <int NG, typename T, int BM, int BN, int WM, int WN, int NB>
 __global__ __launch_bounds__(64 * WM * WN) void k_w8a8_tile(const W8A8Args a, int tiles_m, int tiles_n, int xlog,
                                                                    int KS, int* part) {
     using C = TileCfg<NG, BM, BN, WM, WN>;
     constexpr int TM = C::TM, TN = C::TN, kQuads = TM * TN / 4, kLoads = C::kXLoads + C::kWLoads, kReads = TM + TN;
     // Of n things issued between kQuads quads of products, those before quad q.
     constexpr auto part_of = [](int q, int n) { return q * n / kQuads; };
-    __shared__ __attribute__((aligned(128))) signed char xs0[BM * kStage], xs1[BM * kStage];
-    __shared__ __attribute__((aligned(128))) signed char ws0[BN * kStage], ws1[BN * kStage];
+    // NB buffers of a stage, objects of their own: by them the compiler tells the loads a
+    // read has to wait for from those it has not.
+    constexpr int kX = BM * kStage, kW = BN * kStage;
+    __shared__ __attribute__((aligned(128))) signed char xs0[kX], xs1[kX], xs2[NB > 2 ? kX : 16], xs3[NB > 3 ? kX : 16],
+        xs4[NB > 4 ? kX : 16], xs5[NB > 5 ? kX : 16];
+    __shared__ __attribute__((aligned(128))) signed char ws0[kW], ws1[kW], ws2[NB > 2 ? kW : 16], ws3[NB > 3 ? kW : 16],
+        ws4[NB > 4 ? kW : 16], ws5[NB > 5 ? kW : 16];
     __shared__ float esx[BM];
     __shared__ __attribute__((aligned(16))) float esw[BN], eb[BN];  // scales and biases, as the weights' blocks lie
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -370,18 +375,44 @@ __global__ __launch_bounds__(64 * WM * WN) void k_w8a8_tile(const W8A8Args a, in
     };
 
     i32x4 x0[TM], w0[TN], x1[TM], w1[TN];
+    // The first stages and the scales and biases on their way together.
+    auto load = [&](signed char* xs, signed char* ws, int s) {
 #pragma unroll
-    for (int l = 0; l < kLoads; ++l) load1(xs0, ws0, s0, l);
-    for (int t = threadIdx.x; t < BM; t += C::kThreads) esx[t] = t < rows ? a.sx[m0 + t] : 0.0f;
-    for (int t = threadIdx.x; t < BN; t += C::kThreads) {
-        const int q = t / (BN / NG);
-        const int64_t nn = cb0 * 16 + t - q * (BN / NG);
-        esw[t] = nn < a.N ? a.sw[q][nn] : 0.0f;
-        eb[t] = nn < a.N && a.bias[q] ? a.bias[q][nn] : 0.0f;
+        for (int l = 0; l < kLoads; ++l) load1(xs, ws, s, l);
+    };
+    load(xs0, ws0, s0);
+    constexpr int kEX = (BM + C::kThreads - 1) / C::kThreads, kEW = (BN + C::kThreads - 1) / C::kThreads;
+    float vx[kEX], vw[kEW], vb[kEW];
+#pragma unroll
+    for (int e = 0; e < kEX; ++e) {
+        const int t = threadIdx.x + e * C::kThreads;
+        vx[e] = t < rows ? a.sx[m0 + t] : 0.0f;
     }
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
-    for (int l = 0; l < kLoads; ++l) load1(xs1, ws1, s0 + 1, l);
+    for (int e = 0; e < kEW; ++e) {
+        const int t = threadIdx.x + e * C::kThreads, q = NG == 1 ? 0 : t / (BN / NG);
+        const int64_t c = cb0 * 16 + t - q * (BN / NG);
+        const float* sw = q == 0 ? a.sw[0] : a.sw[NG - 1];
+        const float* b = q == 0 ? a.bias[0] : a.bias[NG - 1];
+        const bool in = t < BN && c < a.N;
+        vw[e] = in ? sw[c] : 0.0f;
+        vb[e] = in && b ? b[c] : 0.0f;
+    }
+    load(xs1, ws1, s0 + 1);
+    if constexpr (NB > 2) load(xs2, ws2, s0 + 2);
+    if constexpr (NB > 3) load(xs3, ws3, s0 + 3);
+    if constexpr (NB > 4) load(xs4, ws4, s0 + 4);
+    if constexpr (NB > 5) load(xs5, ws5, s0 + 5);
+#pragma unroll
+    for (int e = 0; e < kEX; ++e)
+        if (threadIdx.x + e * C::kThreads < BM) esx[threadIdx.x + e * C::kThreads] = vx[e];
+#pragma unroll
+    for (int e = 0; e < kEW; ++e)
+        if (threadIdx.x + e * C::kThreads < BN) {
+            esw[threadIdx.x + e * C::kThreads] = vw[e];
+            eb[threadIdx.x + e * C::kThreads] = vb[e];
+        }
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"((NB - 1) * kLoads) : "memory");
 #pragma unroll
     for (int l = 0; l < kReads; ++l) read1(x0, w0, xs0, ws0, 0, l);
     // A stage: the products of its first half while the operands of the second are
@@ -399,23 +430,54 @@ __global__ __launch_bounds__(64 * WM * WN) void k_w8a8_tile(const W8A8Args a, in
             mfma4(x0, w0, q);
             __builtin_amdgcn_sched_barrier(0);
         }
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        // The next stage has come when all but the loads of the NB - 2 after it have.
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"((NB - 2) * kLoads) : "memory");
 #pragma unroll
         for (int q = 0; q < kQuads; ++q) {
 #pragma unroll
             for (int l = part_of(q, kReads); l < part_of(q + 1, kReads); ++l) read1(x0, w0, xn, wsn, 0, l);
 #pragma unroll
-            for (int l = part_of(q, kLoads); l < part_of(q + 1, kLoads); ++l) load1(xs, ws, s + 2, l);
+            for (int l = part_of(q, kLoads); l < part_of(q + 1, kLoads); ++l) load1(xs, ws, s + NB, l);
             __builtin_amdgcn_sched_barrier(0);
             mfma4(x1, w1, q);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    for (int s = s0; s < n - 1; s += 2) {
+    // The buffers in turn; what is left past the last whole turn.
+    int s = s0;
+    for (; s + NB <= n; s += NB) {
         step(xs0, ws0, xs1, ws1, s);
-        step(xs1, ws1, xs0, ws0, s + 1);
+        if constexpr (NB == 2) {
+            step(xs1, ws1, xs0, ws0, s + 1);
+        } else {
+            step(xs1, ws1, xs2, ws2, s + 1);
+            if constexpr (NB == 3) {
+                step(xs2, ws2, xs0, ws0, s + 2);
+            } else {
+                step(xs2, ws2, xs3, ws3, s + 2);
+                if constexpr (NB == 4) {
+                    step(xs3, ws3, xs0, ws0, s + 3);
+                } else {
+                    step(xs3, ws3, xs4, ws4, s + 3);
+                    if constexpr (NB == 5) {
+                        step(xs4, ws4, xs0, ws0, s + 4);
+                    } else {
+                        step(xs4, ws4, xs5, ws5, s + 4);
+                        step(xs5, ws5, xs0, ws0, s + 5);
+                    }
+                }
+            }
+        }
     }
-    if ((n - s0) & 1) step(xs0, ws0, xs1, ws1, n - 1);
+    if (s < n) step(xs0, ws0, xs1, ws1, s);
+    if constexpr (NB > 2)
+        if (s + 1 < n) step(xs1, ws1, xs2, ws2, s + 1);
+    if constexpr (NB > 3)
+        if (s + 2 < n) step(xs2, ws2, xs3, ws3, s + 2);
+    if constexpr (NB > 4)
+        if (s + 3 < n) step(xs3, ws3, xs4, ws4, s + 3);
+    if constexpr (NB > 5)
+        if (s + 4 < n) step(xs4, ws4, xs5, ws5, s + 4);
     // No load may still be writing to LDS when the workgroup's share of it is given away.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
@@ -475,10 +537,10 @@ __global__ __launch_bounds__(kWG) void k_w8a8_reduce(const W8A8Args a, int KS, c
     }
 }
 
-template <int NG, typename T, int BM, int BN, int WM, int WN>
+template <int NG, typename T, int BM, int BN, int WM, int WN, int NB>
 void launch_tile(const W8A8Args& a, int KS, int* part, hipStream_t s) {
     const int64_t tm = ceil_div(a.M, BM), tn = ceil_div(ChannelsGeom(a.K, a.N).NB, BN / 16 / NG);
-    k_w8a8_tile<NG, T, BM, BN, WM, WN>
+    k_w8a8_tile<NG, T, BM, BN, WM, WN, NB>
         <<<(unsigned)(tm * tn * KS), 64 * WM * WN, 0, s>>>(a, (int)tm, (int)tn, xcd_log2(device_xcds(s)), KS, part);
     if (KS > 1) {
         const dim3 grid((unsigned)ceil_div(a.N, 4 * kWG), (unsigned)(a.M < 32768 ? a.M : 32768));
@@ -511,10 +573,11 @@ hipError_t launch_as(const W8A8Args& a, const W8A8Plan& p, int* part, hipStream_
         case W8A8Form::few2x1: launch_few<NG, T, 2, 1, 16>(a, s); break;
         case W8A8Form::few2x2: launch_few<NG, T, 2, 2, 16 / NG>(a, s); break;
         case W8A8Form::few4x2: launch_few<NG, T, 4, 2, 8 / NG>(a, s); break;
-        case W8A8Form::tile64x128: launch_tile<NG, T, 64, 128, 1, 4>(a, p.KS, part, s); break;
-        case W8A8Form::tile128: launch_tile<NG, T, 128, 128, 2, 2>(a, p.KS, part, s); break;
-        case W8A8Form::tile128x256: launch_tile<NG, T, 128, 256, 2, 4>(a, p.KS, part, s); break;
-        case W8A8Form::tile256: launch_tile<NG, T, 256, 256, 2, 4>(a, p.KS, part, s); break;
+        case W8A8Form::tile64x128: launch_tile<NG, T, 64, 128, 1, 4, 3>(a, p.KS, part, s); break;
+        case W8A8Form::tile128: launch_tile<NG, T, 128, 128, 2, 2, 2>(a, p.KS, part, s); break;
+        case W8A8Form::tile128deep: launch_tile<NG, T, 128, 128, 2, 2, 4>(a, p.KS, part, s); break;
+        case W8A8Form::tile128x256: launch_tile<NG, T, 128, 256, 2, 4, 3>(a, p.KS, part, s); break;
+        case W8A8Form::tile256: launch_tile<NG, T, 256, 256, 2, 4, 2>(a, p.KS, part, s); break;
     }
     return hipGetLastError();
 }
@@ -577,15 +640,17 @@ int64_t w8a8_plan_bytes(const W8A8Plan& p, int ng, int64_t M, int64_t K, int64_t
 // The form and the K splits with the least time by a model of a launch, in us: a form
 // that puts w workgroups on a CU, each with st steps of K (stages of 128 k; a
 // wavefront's steps of 64 k in the forms for few tokens), takes
-//   fixed + max(alone * st, w * (step * st + end)), and at least 2 + the weights at 4.7 TB/s,
-// a split of K 3 us and its partial sums at 3.5 TB/s more.  The constants are fitted to
-// 316 shapes (1 to 8192 tokens, K and N of 512 to 28672, one weight and two) with every
-// form timed on each; the form this picks takes 1.04 times the fastest one's time on
-// average, 1.13 times in one of ten.  For instance (us, 64 x 128 / 128 x 128 / 128 x 256 / 256 x
-// 256): 333 x 2043 -> 5001 11.7 / 14.8 / 19.0 / 32.9, 2048 x 4096 -> 4096 49 / 41 / 37 / 48,
-// 8192 x 8192 -> 28672 2380 / 1850 / 1940 / 1440; 128 x 11008 -> 4096 gated, 64 x 128 without
-// a split 60, with four 32.  The forms for few tokens read a weight once for each of
-// their row blocks, which costs them large weights: 48 x 14336 -> 28672 132 against 85.
+//   fixed + max(alone * st, w * (step * st + end)), and at least 2 + the weights at 5 TB/s
+// or at 36 GB/s a workgroup; a split of K 2.5 us and its partial sums at 3.3 TB/s more.
+// The constants are fitted to 316 shapes (1 to 8192 tokens, K and N of 512 to 28672, one
+// weight and two) with every form timed on each; the form this picks takes 1.03 times
+// the fastest one's time on average, 1.11 times in one of ten.  For instance (us, 64 x
+// 128 / 128 x 128 with two buffers / with four / 128 x 256 / 256 x 256): 333 x 2043 -> 5001 9.7 /
+// 13.8 / 13.0 / 17.4 / 28.7, 1024 x 4096 -> 4096 24.4 / 25.4 / 21.3 / 26.5 / 42, 2048 x 4096 -> 4096
+// 49 / 38 / 43 / 34 / 46, 4096 x 4096 -> 4096 90 / 73 / 83 / 67 / 57; 128 x 11008 -> 4096, 64 x 128
+// without a split 26.7, with two 19.3.  The forms for few tokens read a weight once for
+// each of their row blocks, which costs them large weights: 48 x 14336 -> 28672 132
+// against 85.
 W8A8Plan w8a8_plan(int ng, int64_t M, int64_t K, int64_t N, int64_t cus) {
     W8A8Plan best;
     if (K == 0) return best;
@@ -598,13 +663,14 @@ W8A8Plan w8a8_plan(int ng, int64_t M, int64_t K, int64_t N, int64_t cus) {
         int few, rows, cols;                  // rows and columns (of all weights) of a workgroup, in 16s for few
         struct { double fixed, alone, step, end; } t[2];  // one weight, two
     } forms[] = {
-        {W8A8Form::few2x1, 1, 2, 1, {{1.0, .5, 1.0, 0.}, {.5, 1.16, 1.07, 0.}}},
-        {W8A8Form::few2x2, 1, 2, 2, {{1.95, .5, 1.08, 1.}, {2.7, .87, .86, .55}}},
-        {W8A8Form::few4x2, 1, 4, 2, {{1.4, .7, .81, 1.4}, {2.7, .7, .65, 1.2}}},
-        {W8A8Form::tile64x128, 0, 64, 128, {{2.5, .515, .30, 1.1}, {2.5, .515, .30, 1.1}}},
-        {W8A8Form::tile128, 0, 128, 128, {{3.3, .61, .464, 1.95}, {3.3, .61, .464, 1.95}}},
-        {W8A8Form::tile128x256, 0, 128, 256, {{0., .9, .853, 5.4}, {0., .9, .853, 5.4}}},
-        {W8A8Form::tile256, 0, 256, 256, {{0., 1.31, 1.3, 9.1}, {0., 1.31, 1.3, 9.1}}},
+        {W8A8Form::few2x1, 1, 2, 1, {{1.0, .48, 1.0, 0.}, {1.0, 1.09, .88, 0.}}},
+        {W8A8Form::few2x2, 1, 2, 2, {{1.75, .5, 1.07, 1.1}, {1.5, .85, .9, 1.3}}},
+        {W8A8Form::few4x2, 1, 4, 2, {{1.4, .67, .74, 1.5}, {2.7, .7, .65, 1.2}}},
+        {W8A8Form::tile64x128, 0, 64, 128, {{2.8, .224, .285, 1.25}, {2.8, .224, .285, 1.25}}},
+        {W8A8Form::tile128, 0, 128, 128, {{3.7, .6, .455, 1.85}, {3.7, .6, .455, 1.85}}},
+        {W8A8Form::tile128deep, 0, 128, 128, {{.7, .47, .435, 4.5}, {.7, .47, .435, 4.5}}},
+        {W8A8Form::tile128x256, 0, 128, 256, {{.2, .72, .716, 6.3}, {.2, .72, .716, 6.3}}},
+        {W8A8Form::tile256, 0, 256, 256, {{0., 1.35, 1.295, 8.8}, {0., 1.35, 1.295, 8.8}}},
     };
     constexpr int64_t kFewRows = 256, kFewBytes = 100 * 1000 * 1000, kMinSplitStages = 4;
     const ChannelsGeom g(K, N);
@@ -616,20 +682,23 @@ W8A8Plan w8a8_plan(int ng, int64_t M, int64_t K, int64_t N, int64_t cus) {
         for (int ks = 1; ks <= (f.few ? 1 : 8); ks *= 2) {
             const int64_t stages = g.Kpad / 128, per = ceil_div(stages, ks);
             if (ks > 1 && (per < kMinSplitStages || ceil_div(stages, per) != ks)) continue;
-            double w, st;
+            double wgs, w, st;
             if (f.few) {
-                w = (double)(ceil_div(M, 16 * f.rows) * ceil_div(g.NB, f.cols)) / cu;
-                w = w < 1.0 ? 1.0 : w;
+                wgs = (double)(ceil_div(M, 16 * f.rows) * ceil_div(g.NB, f.cols));
+                w = wgs < cu ? 1.0 : wgs / cu;
                 st = (double)ceil_div(2 * stages, few_waves(f.rows * f.cols, ng, K));
             } else {
-                w = (double)ceil_div(ceil_div(M, f.rows) * ceil_div(g.NB, f.cols / 16 / ng) * ks, (int64_t)cu);
+                const int64_t n = ceil_div(M, f.rows) * ceil_div(g.NB, f.cols / 16 / ng) * ks;
+                wgs = (double)n;
+                w = (double)ceil_div(n, (int64_t)cu);
                 st = (double)per;
             }
             const double busy = w * (t.step * st + t.end), alone = t.alone * st;
             double us = t.fixed + (busy > alone ? busy : alone);
-            const double read = 2.0 + (double)(ng * K) * (double)N / 4.7e6;
+            const double rate = wgs * 3.6e4 < 5.0e6 ? wgs * 3.6e4 : 5.0e6;  // bytes a us
+            const double read = 2.0 + (double)(ng * K) * (double)N / rate;
             us = us > read ? us : read;
-            if (ks > 1) us += 3.0 + (double)(ks * ng * 4) * (double)M * (double)N / 3.5e6;
+            if (ks > 1) us += 2.5 + (double)(ks * ng * 4) * (double)M * (double)N / 3.34e6;
             if (least == 0.0 || us < least) least = us, best.form = f.form, best.KS = ks;
         }
     }

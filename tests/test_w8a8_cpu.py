@@ -58,8 +58,8 @@ def test_plans(lib):
                         fn = lib.sgq_swiglu_w8a8_workspace_bytes if gated else lib.sgq_linear_w8a8_workspace_bytes
                         want = 0 if ks == 1 else ks * (1 + gated) * M * -(-N // 16) * 64
                         assert fn(M, K, N, cus) == want
-    assert seen == set(range(9))
-    assert _plan(lib, 0, 8192, 8192, 28672) == (8, 1)
+    assert seen == set(range(10))
+    assert _plan(lib, 0, 8192, 8192, 28672) == (9, 1)
     import ctypes
 
     i = ctypes.c_int()

@@ -262,7 +262,8 @@ PRODUCTS = [(1, 64, 16), (1, 1, 1), (1, 4096, 100), (2, 129, 40), (3, 2048, 2048
             (128, 1024, 1024), (129, 1024, 511), (200, 300, 1000), (256, 4096, 257), (257, 127, 512), (300, 5000, 640),
             (512, 2048, 2048), (513, 1023, 1025), (1000, 130, 4099), (2048, 512, 768), (1111, 2222, 3333), (40, 4099, 2050), (48, 4096, 4096), (60, 1000, 8003),
             (30, 1000, 8003), (600, 1100, 5000), (90, 14000, 1030), (130, 9000, 2000), (1030, 2048, 4096),
-            (700, 8200, 4000), (2050, 4096, 4100), (1500, 14336, 1999), (520, 8192, 9000), (300, 11008, 4096)]
+            (700, 8200, 4000), (2050, 4096, 4100), (1500, 14336, 1999), (520, 8192, 9000), (300, 11008, 4096),
+            (70, 14000, 4100), (141, 24011, 5612), (1542, 268, 2433), (20, 3267, 34), (2240, 2949, 69)]
 
 
 def test_products_take_every_form(op, sgq):
@@ -275,7 +276,7 @@ def test_products_take_every_form(op, sgq):
             form, ks = ctypes.c_int(), ctypes.c_int()
             assert sgq.load_library().sgq_w8a8_plan(gated, M, K, N, 256, ctypes.byref(form), ctypes.byref(ks)) == 0
             seen.add((form.value, ks.value > 1))
-    assert seen >= {(f, False) for f in range(1, 9)} | {(f, True) for f in range(5, 9)}, sorted(seen)
+    assert seen >= {(f, False) for f in range(1, 10)} | {(f, True) for f in (5, 7, 8, 9)}, sorted(seen)
 
 
 @pytest.mark.parametrize("M,K,N", PRODUCTS)
