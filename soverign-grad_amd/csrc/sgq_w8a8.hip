@@ -420,7 +420,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_w8a8_tile(const W8A8Args a, in
     // next is loaded into while the products of the second half run and the first
     // operands of the next stage are read.  A load or read is issued every few products:
     // all of them at once held the products back until the queues had taken them (4096
-    // x 8192 -> 4096 117 -> 107 us).
+    // x 8192 -> 4096 117 -> 104 us).
     auto step = [&](signed char* xs, signed char* ws, const signed char* xn, const signed char* wsn, int s) {
 #pragma unroll
         for (int q = 0; q < kQuads; ++q) {
@@ -478,8 +478,9 @@ __global__ __launch_bounds__(64 * WM * WN) void k_w8a8_tile(const W8A8Args a, in
         if (s + 3 < n) step(xs3, ws3, xs4, ws4, s + 3);
     if constexpr (NB > 5)
         if (s + 4 < n) step(xs4, ws4, xs5, ws5, s + 4);
-    // No load may still be writing to LDS when the workgroup's share of it is given away.
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    // No load may still be writing to LDS, which the results go through and which is
+    // given away at the end.
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
 
     // A lane has columns 4 g .. 4 g + 3 of a block, of token lr.
     const int col0 = wn * (TN / NG) * 16 + 4 * g;  // of the first block, in its weight
@@ -499,12 +500,25 @@ __global__ __launch_bounds__(64 * WM * WN) void k_w8a8_tile(const W8A8Args a, in
         }
         return;
     }
+    // Sixteen tokens at a time through a share of LDS of the wavefront's own, so that
+    // neighbouring lanes store a row's 16-byte chunks: chunk c of row r lies at place
+    // c ^ r (mod the chunks of a row).  Rows that begin with a 128-byte line are written
+    // past the L2, which would else hold them until the kernel's end and write them back
+    // at once; rows that share lines are left to the L2 to put together.  Measured (us,
+    // bf16: stores from the registers, through LDS, past the L2): 4096 x 4096 -> 4096 58.6 /
+    // 57.2 / 54.0, 2048 x 4096 -> 4096 35.2 / 34.7 / 33.0, 8192 x 8192 -> 28672 1447 / 1411 /
+    // 1402; on 256 x 256 tiles 4096 x 4096 -> 5003 101 / 91 / 96.
+    const bool whole = (((uintptr_t)a.y | (uintptr_t)(a.ldy * (int)sizeof(T))) & 127) == 0;
+    constexpr int kCols = TN / NG * 16, kRowBytes = kCols * (int)sizeof(T), kChunks = kRowBytes / 16;
+    constexpr int kRowsAt = 64 / kChunks, kPer = 16 / (int)sizeof(T);
+    static_assert(WM * WN * 16 * kRowBytes <= BN * kStage, "the wavefronts' shares are in ws0");
+    signed char* const share = ws0 + wave * 16 * kRowBytes;
+    const int at_row = lane / kChunks, at_chunk = lane % kChunks;
+    const int64_t col = cb0 * 16 + wn * kCols + at_chunk * kPer;
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
-        const int r = wm * (BM / WM) + i * 16 + lr;
-        if (r >= rows) continue;
-        const float sx = esx[r];
-        T* row = (T*)a.y + (m0 + r) * a.ldy;
+        const int r0 = wm * (BM / WM) + i * 16;
+        const float sx = esx[r0 + lr];
 #pragma unroll
         for (int j = 0; j < TN / NG; ++j) {
             const int c = col0 + 16 * j;
@@ -512,8 +526,36 @@ __global__ __launch_bounds__(64 * WM * WN) void k_w8a8_tile(const W8A8Args a, in
             if constexpr (NG == 2)
                 v = silu_mul4(v, product4(acc[i][j + TN / 2], sx, *(const floatx4*)&esw[c + BN / 2],
                                           *(const floatx4*)&eb[c + BN / 2]));
-            store4(row, nb + 16 * j, a.N, v);
+            typedef T T4 __attribute__((ext_vector_type(4)));
+            T4 o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = (T)v[e];
+            const int byte = (16 * j + 4 * g) * (int)sizeof(T);
+            *(T4*)(share + lr * kRowBytes + ((byte / 16) ^ (lr % kChunks)) * 16 + byte % 16) = o;
         }
+        asm volatile("" ::: "memory");  // a wavefront's LDS accesses are in order
+#pragma unroll
+        for (int q = 0; q < (15 + kRowsAt) / kRowsAt; ++q) {
+            const int row = q * kRowsAt + at_row;
+            if (kRowsAt > 16 && row >= 16) continue;
+            typedef T TP __attribute__((ext_vector_type(kPer)));
+            typedef T TPu __attribute__((ext_vector_type(kPer), aligned(sizeof(T))));
+            const TP o = *(const TP*)(share + row * kRowBytes + (at_chunk ^ (row % kChunks)) * 16);
+            if (r0 + row < rows) {
+                T* to = (T*)a.y + (m0 + r0 + row) * a.ldy + col;
+                if (col + kPer <= a.N) {
+                    if (whole)
+                        __builtin_nontemporal_store(o, (TPu*)to);
+                    else
+                        *(TPu*)to = o;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < kPer - 1; ++e)
+                        if (col + e < a.N) to[e] = o[e];
+                }
+            }
+        }
+        asm volatile("" ::: "memory");
     }
 }
 
@@ -641,16 +683,16 @@ int64_t w8a8_plan_bytes(const W8A8Plan& p, int ng, int64_t M, int64_t K, int64_t
 // that puts w workgroups on a CU, each with st steps of K (stages of 128 k; a
 // wavefront's steps of 64 k in the forms for few tokens), takes
 //   fixed + max(alone * st, w * (step * st + end)), and at least 2 + the weights at 5 TB/s
-// or at 36 GB/s a workgroup; a split of K 2.5 us and its partial sums at 3.3 TB/s more.
-// The constants are fitted to 316 shapes (1 to 8192 tokens, K and N of 512 to 28672, one
+// or at 36 GB/s a workgroup; a split of K 2.5 us and its partial sums at 3 TB/s more.
+// The constants are fitted to 326 shapes (1 to 8192 tokens, K and N of 512 to 28672, one
 // weight and two) with every form timed on each; the form this picks takes 1.03 times
 // the fastest one's time on average, 1.11 times in one of ten.  For instance (us, 64 x
-// 128 / 128 x 128 with two buffers / with four / 128 x 256 / 256 x 256): 333 x 2043 -> 5001 9.7 /
-// 13.8 / 13.0 / 17.4 / 28.7, 1024 x 4096 -> 4096 24.4 / 25.4 / 21.3 / 26.5 / 42, 2048 x 4096 -> 4096
-// 49 / 38 / 43 / 34 / 46, 4096 x 4096 -> 4096 90 / 73 / 83 / 67 / 57; 128 x 11008 -> 4096, 64 x 128
-// without a split 26.7, with two 19.3.  The forms for few tokens read a weight once for
-// each of their row blocks, which costs them large weights: 48 x 14336 -> 28672 132
-// against 85.
+// 128 / 128 x 128 with two buffers / with four / 128 x 256 / 256 x 256): 333 x 2043 -> 5001 9.6 /
+// 13.8 / 12.7 / 15.6 / 24.6, 1024 x 4096 -> 4096 23.4 / 24.4 / 20.2 / 23.7 / 38, 2048 x 4096 -> 4096
+// 44 / 36 / 39 / 31 / 40, 4096 x 4096 -> 4096 86 / 69 / 75 / 61 / 54; 128 x 11008 -> 4096 on 64 x
+// 128 without a split 26.4, with two 19.2.  The forms for few tokens read a weight once
+// for each of their row blocks: 48 x 4096 -> 4096 9.8 on 64 x 32 against 11.2, but 48 x
+// 14336 -> 28672 132 against 73.
 W8A8Plan w8a8_plan(int ng, int64_t M, int64_t K, int64_t N, int64_t cus) {
     W8A8Plan best;
     if (K == 0) return best;
@@ -666,11 +708,11 @@ W8A8Plan w8a8_plan(int ng, int64_t M, int64_t K, int64_t N, int64_t cus) {
         {W8A8Form::few2x1, 1, 2, 1, {{1.0, .48, 1.0, 0.}, {1.0, 1.09, .88, 0.}}},
         {W8A8Form::few2x2, 1, 2, 2, {{1.75, .5, 1.07, 1.1}, {1.5, .85, .9, 1.3}}},
         {W8A8Form::few4x2, 1, 4, 2, {{1.4, .67, .74, 1.5}, {2.7, .7, .65, 1.2}}},
-        {W8A8Form::tile64x128, 0, 64, 128, {{2.8, .224, .285, 1.25}, {2.8, .224, .285, 1.25}}},
-        {W8A8Form::tile128, 0, 128, 128, {{3.7, .6, .455, 1.85}, {3.7, .6, .455, 1.85}}},
-        {W8A8Form::tile128deep, 0, 128, 128, {{.7, .47, .435, 4.5}, {.7, .47, .435, 4.5}}},
-        {W8A8Form::tile128x256, 0, 128, 256, {{.2, .72, .716, 6.3}, {.2, .72, .716, 6.3}}},
-        {W8A8Form::tile256, 0, 256, 256, {{0., 1.35, 1.295, 8.8}, {0., 1.35, 1.295, 8.8}}},
+        {W8A8Form::tile64x128, 0, 64, 128, {{2.6, .226, .29, 1.25}, {2.6, .226, .29, 1.25}}},
+        {W8A8Form::tile128, 0, 128, 128, {{3.4, .6, .46, 1.75}, {3.4, .6, .46, 1.75}}},
+        {W8A8Form::tile128deep, 0, 128, 128, {{.2, .48, .45, 4.6}, {.2, .48, .45, 4.6}}},
+        {W8A8Form::tile128x256, 0, 128, 256, {{0., .73, .74, 5.6}, {0., .73, .74, 5.6}}},
+        {W8A8Form::tile256, 0, 256, 256, {{0., 1.33, 1.33, 7.2}, {0., 1.33, 1.33, 7.2}}},
     };
     constexpr int64_t kFewRows = 256, kFewBytes = 100 * 1000 * 1000, kMinSplitStages = 4;
     const ChannelsGeom g(K, N);
@@ -695,10 +737,10 @@ W8A8Plan w8a8_plan(int ng, int64_t M, int64_t K, int64_t N, int64_t cus) {
             }
             const double busy = w * (t.step * st + t.end), alone = t.alone * st;
             double us = t.fixed + (busy > alone ? busy : alone);
-            const double rate = wgs * 3.6e4 < 5.0e6 ? wgs * 3.6e4 : 5.0e6;  // bytes a us
+            const double rate = wgs * 3.6e4 < 5.1e6 ? wgs * 3.6e4 : 5.1e6;  // bytes a us
             const double read = 2.0 + (double)(ng * K) * (double)N / rate;
             us = us > read ? us : read;
-            if (ks > 1) us += 2.5 + (double)(ks * ng * 4) * (double)M * (double)N / 3.34e6;
+            if (ks > 1) us += 2.5 + (double)(ks * ng * 4) * (double)M * (double)N / 3.0e6;
             if (least == 0.0 || us < least) least = us, best.form = f.form, best.KS = ks;
         }
     }
