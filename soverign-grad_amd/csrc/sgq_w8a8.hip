@@ -47,6 +47,9 @@ __global__ __launch_bounds__(kWG) void k_channels_top(const float* __restrict__ 
     }
 }
 
+// HBM bounds the two passes over w: packing 4096 x 4096 fp32 codes takes 22 us, 8192 x
+// 28672 360 us (3.3 TB/s).
+//
 // Codes of a kTileK x kTileN tile: FROM_CODES reads fp32 codes (validated into
 // *bad), else w with the columns' maxima in top; through LDS into the layout.
 template <bool FROM_CODES>
@@ -179,7 +182,14 @@ __device__ __forceinline__ floatx4 load4(const float* v, int64_t n, int64_t N) {
 // lane's A operand is a chunk of the packed weight (column lane & 15, k chunk lane >>
 // 4: a wavefront reads 1024 contiguous bytes), its B operand 16 codes of token lane &
 // 15, so that it ends up with four neighbouring columns of one token.  The sums of
-// the wavefronts are added through LDS; integers, so in any order.
+// the wavefronts are added through LDS; integers, so in any order.  The weight's bytes
+// bound it (graphs of calls over weights that together pass the caches): 1 x 4096 -> 4096
+// 5.0 us, 3.3 TB/s, 16 x 4096 -> 11008 gated 18.5 us, 4.9 TB/s, 8 x 8192 -> 28672 38.5 us, 6.1
+// TB/s; below some 30 MB the launch and one latency.  With one row block a weight is read
+// once and its loads are marked as streamed: from HBM 1 x 4096 -> 4096 5.0 us against 5.6
+// without, 16 x 4096 -> 11008 gated 18.5 against 20.0 (a weight that the caches hold from
+// the call before loses by it, 16 x 11008 -> 4096 11.9 against 10.2; the layers of a model
+// come from HBM).
 template <int NG, typename T, int MB, int C, int NW>
 __global__ __launch_bounds__(64 * NW) void k_w8a8_few(const W8A8Args a, int mblocks, int xlog) {
     constexpr int B = MB * C * NG;                     // 16 x 16 blocks of sums
@@ -279,6 +289,25 @@ typedef __attribute__((address_space(3))) void lds_void;
 
 constexpr int kStage = 128;  // k per stage
 
+// A workgroup of WM x WN wavefronts computes BM tokens by BN columns (of the NG weights
+// together, so that the gated MLP's two products of an output are in one lane).  Both
+// operands go to LDS by direct loads, 128 k a stage, in NB buffers; a wavefront reads
+// each operand once for all of its products, and the weight's layout is its operands',
+// so nothing is rearranged.
+//
+// What bounds it: at 8192 x 8192 -> 28672 (256 x 256 tiles, 1.40 ms, 2.75 POP/s; a library
+// int8 product of the shape 1.66 ms) the matrix cores are busy 70% of the time with the
+// clock at 1.74 GHz, the power limit: the same instructions alone, on operands of
+// random bits, run at 3.3 to 3.4 POP/s (4.6 on zeros), and the 32 x 32 x 32 form is
+// slower (1710 us against 1530 in the first tiles).  2048 x 4096 -> 4096 (128 x 256, one
+// tile a CU, 31 us, the library 41) keeps its clock at 2.4 GHz: 22 us of stages, the rest
+// the launch, the first loads and the stores.  Smaller products wait for their stages'
+// loads: a third and a fourth buffer take a 64 x 128 stage from .51 to .23 us and a 128 x
+// 128 one from .61 to .48; where CUs hold several tiles, two buffers of 128 x 128 leave
+// room for a second workgroup and do better (2048 x 4096 -> 4096 36 us against 39).
+// Measured and not kept: a workgroup that takes its tiles one after another, the next
+// one's first loads under the last products (4096 x 4096 -> 11008 176 us against 163: the
+// loop over tiles left no registers); four wavefronts of 128 x 128 (1638 against 1449).
 template <int NG, int BM, int BN, int WM, int WN>
 struct TileCfg {
     static constexpr int kThreads = 64 * WM * WN;
@@ -298,10 +327,9 @@ __global__ __launch_bounds__(64 * WM * WN) void k_w8a8_tile(const W8A8Args a, in
     // NB buffers of a stage, objects of their own: by them the compiler tells the loads a
     // read has to wait for from those it has not.
     constexpr int kX = BM * kStage, kW = BN * kStage;
-    __shared__ __attribute__((aligned(128))) signed char xs0[kX], xs1[kX], xs2[NB > 2 ? kX : 16], xs3[NB > 3 ? kX : 16],
-        xs4[NB > 4 ? kX : 16], xs5[NB > 5 ? kX : 16];
-    __shared__ __attribute__((aligned(128))) signed char ws0[kW], ws1[kW], ws2[NB > 2 ? kW : 16], ws3[NB > 3 ? kW : 16],
-        ws4[NB > 4 ? kW : 16], ws5[NB > 5 ? kW : 16];
+    static_assert(NB >= 2 && NB <= 4, "buffers");
+    __shared__ __attribute__((aligned(128))) signed char xs0[kX], xs1[kX], xs2[NB > 2 ? kX : 16], xs3[NB > 3 ? kX : 16];
+    __shared__ __attribute__((aligned(128))) signed char ws0[kW], ws1[kW], ws2[NB > 2 ? kW : 16], ws3[NB > 3 ? kW : 16];
     __shared__ float esx[BM];
     __shared__ __attribute__((aligned(16))) float esw[BN], eb[BN];  // scales and biases, as the weights' blocks lie
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -401,8 +429,6 @@ __global__ __launch_bounds__(64 * WM * WN) void k_w8a8_tile(const W8A8Args a, in
     load(xs1, ws1, s0 + 1);
     if constexpr (NB > 2) load(xs2, ws2, s0 + 2);
     if constexpr (NB > 3) load(xs3, ws3, s0 + 3);
-    if constexpr (NB > 4) load(xs4, ws4, s0 + 4);
-    if constexpr (NB > 5) load(xs5, ws5, s0 + 5);
 #pragma unroll
     for (int e = 0; e < kEX; ++e)
         if (threadIdx.x + e * C::kThreads < BM) esx[threadIdx.x + e * C::kThreads] = vx[e];
@@ -455,17 +481,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_w8a8_tile(const W8A8Args a, in
                 step(xs2, ws2, xs0, ws0, s + 2);
             } else {
                 step(xs2, ws2, xs3, ws3, s + 2);
-                if constexpr (NB == 4) {
-                    step(xs3, ws3, xs0, ws0, s + 3);
-                } else {
-                    step(xs3, ws3, xs4, ws4, s + 3);
-                    if constexpr (NB == 5) {
-                        step(xs4, ws4, xs0, ws0, s + 4);
-                    } else {
-                        step(xs4, ws4, xs5, ws5, s + 4);
-                        step(xs5, ws5, xs0, ws0, s + 5);
-                    }
-                }
+                step(xs3, ws3, xs0, ws0, s + 3);
             }
         }
     }
@@ -474,10 +490,6 @@ __global__ __launch_bounds__(64 * WM * WN) void k_w8a8_tile(const W8A8Args a, in
         if (s + 1 < n) step(xs1, ws1, xs2, ws2, s + 1);
     if constexpr (NB > 3)
         if (s + 2 < n) step(xs2, ws2, xs3, ws3, s + 2);
-    if constexpr (NB > 4)
-        if (s + 3 < n) step(xs3, ws3, xs4, ws4, s + 3);
-    if constexpr (NB > 5)
-        if (s + 4 < n) step(xs4, ws4, xs5, ws5, s + 4);
     // No load may still be writing to LDS, which the results go through and which is
     // given away at the end.
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
@@ -594,7 +606,7 @@ template <int NG, typename T, int MB, int C, int NW>
 void launch_few(const W8A8Args& a, hipStream_t s) {
     const int64_t mbs = ceil_div(a.M, 16 * MB), cgs = ceil_div(ChannelsGeom(a.K, a.N).NB, C);
     const int xlog = xcd_log2(device_xcds(s));
-    if constexpr (NW == 16) {
+    if constexpr (MB * C <= 2) {
         if (few_waves(MB * C, NG, a.K) == 8) {
             k_w8a8_few<NG, T, MB, C, 8><<<(unsigned)(mbs * cgs), 64 * 8, 0, s>>>(a, (int)mbs, xlog);
             return;
