@@ -220,13 +220,16 @@ __global__ __launch_bounds__(64 * NW) void k_w8a8_few(const W8A8Args a, int mblo
         i32x4 x[U][MB], w[U][NG * C];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int k = st + u * NW;  // past the last step: zeros (the weight's buffer ends, or the next block's codes times zeros)
+            // Past the last step and the last column block: zeros.  What a buffer checks is the
+            // lane's offset alone, so the column block is in it.
+            const int k = st + u * NW;
             const int wo = k < steps ? lane * 16 : kOobOff;
 #pragma unroll
             for (int q = 0; q < NG; ++q)
 #pragma unroll
                 for (int c = 0; c < C; ++c)
-                    w[u][q * C + c] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rw[q], wo, c * cbytes + k * 1024, MB == 1 ? kStreamPolicy : 0));
+                    w[u][q * C + c] = __builtin_bit_cast(
+                        i32x4, __builtin_amdgcn_raw_buffer_load_b128(rw[q], wo + c * cbytes, k * 1024, MB == 1 ? kStreamPolicy : 0));
 #pragma unroll
             for (int i = 0; i < MB; ++i)
                 x[u][i] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rx, k < steps ? xo[i] : kOobOff, k * 64, 0));

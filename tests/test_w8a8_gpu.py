@@ -304,6 +304,32 @@ def test_swiglu(op, dev, M, K, N, bias):
         _check(op.quantized_swiglu_w8a8(t, wg, wu, bg, bu, dtype), s * u, tol, dtype)
 
 
+# Forms of two column blocks a workgroup, with an odd number of blocks: the last workgroup's second one is past the weight.
+ODD_BLOCKS = [(30, 1000, 8003), (60, 1000, 8003), (100, 2000, 300), (48, 1000, 5295), (59, 2048, 7278)]
+
+
+def test_few_tokens_past_the_last_column_block(op, sgq, dev):
+    import ctypes
+
+    seen = set()
+    for M, K, N in ODD_BLOCKS:
+        cx, cw, sx, sw, b = _problem(op, dev, M, K, N, M + K, True)
+        qw, t = op.pack_int8_channels(cw, sw), _tokens(op, cx, sx)
+        p, y = _exact(cx, cw, sx, sw, b)
+        _check(op.quantized_matmul_w8a8(t, qw, b), y, _error(p, y), torch.float32)
+        # The weight's buffer ends with its last block.
+        assert qw.packed.numel() == 16 * (-(-N // 16)) * 128 * (-(-K // 128)) and -(-N // 16) % 2 == 1
+        for gated in (0, 1):
+            form, ks = ctypes.c_int(), ctypes.c_int()
+            assert sgq.load_library().sgq_w8a8_plan(gated, M, K, N, 256, ctypes.byref(form), ctypes.byref(ks)) == 0
+            seen.add((gated, form.value))
+        h = op.quantized_swiglu_w8a8(t, qw, qw, b, b)
+        s = y * torch.sigmoid(y)
+        _check(h, s * y, y.abs() * (1.1 * _error(p, y) + 8 * U * s.abs()) + s.abs() * _error(p, y) + U * (s * y).abs(),
+               torch.float32)
+    assert seen >= {(0, 3), (0, 4), (1, 3), (1, 4)}, sorted(seen)
+
+
 def test_extreme_codes_and_scales(op, dev):
     """Every code -128 over the longest K: the sum comes within 128^2 of int32's end.  Scales of NaN and infinity
     reach their row or column only."""
