@@ -29,10 +29,10 @@ __global__ void k_channels_start(uint32_t* __restrict__ top, int64_t N) {
     if (n < N) top[n] = __float_as_uint(1e-8f);
 }
 
-__global__ __launch_bounds__(kWG) void k_channels_top(const float* __restrict__ w, int64_t K, int64_t N, int64_t rows,
-                                                      uint32_t* __restrict__ top) {
+__global__ __launch_bounds__(kWG) void k_channels_top(const float* __restrict__ w, int64_t K, int64_t N, int64_t n0,
+                                                      int64_t rows, uint32_t* __restrict__ top) {
     __shared__ float red[kWG / 64][64];
-    const int64_t n = blockIdx.x * (int64_t)64 + (threadIdx.x & 63);
+    const int64_t n = n0 + blockIdx.x * (int64_t)64 + (threadIdx.x & 63);
     const int64_t k0 = blockIdx.y * rows, k1 = min(K, k0 + rows);
     float m = 0.0f;
     if (n < N)
@@ -661,9 +661,11 @@ hipError_t launch_channels_quantize(const float* w, int64_t K, int64_t N, float*
                                     void* top, hipStream_t s) {
     k_channels_start<<<(unsigned)ceil_div(N, kWG), kWG, 0, s>>>((uint32_t*)top, N);
     if (K > 0) {
-        constexpr int64_t rows = 256;
-        const dim3 grid((unsigned)ceil_div(N, 64), (unsigned)ceil_div(K, rows));
-        k_channels_top<<<grid, kWG, 0, s>>>(w, K, N, rows, (uint32_t*)top);
+        constexpr int64_t rows = 256, cols = 64 * kPackTiles;
+        for (int64_t n = 0; n < N; n += cols) {
+            const dim3 grid((unsigned)ceil_div(min(cols, N - n), 64), (unsigned)ceil_div(K, rows));
+            k_channels_top<<<grid, kWG, 0, s>>>(w, K, N, n, rows, (uint32_t*)top);
+        }
     }
     const int64_t nkt = K > 0 ? ceil_div(K, kTileK) : 1;
     each_tiles(nkt, N, [&](int64_t t0, unsigned n) {

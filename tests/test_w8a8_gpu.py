@@ -226,6 +226,22 @@ def test_channels(op, dev, K, N):
         op.pack_int8_channels(bad, qw.scales)
 
 
+def test_channels_of_a_very_wide_weight(op, sgq, dev):
+    """The widest weight, which has more columns than one launch has threads for: scales and fp32 codes."""
+    N = 2**30
+    w = torch.ones(1, N, device=dev)
+    w[0, -3:] = torch.tensor([2.0, 0.0, -5.0], device=dev)
+    lib = sgq.load_library()
+    ws = torch.empty(lib.sgq_channels_workspace_bytes(1, N), dtype=torch.uint8, device=dev)
+    scales, q = torch.full((N,), -1.0, device=dev), torch.zeros(1, N, device=dev)
+    s = torch.cuda.current_stream().cuda_stream
+    assert lib.sgq_quantize_channels(w.data_ptr(), 1, N, q.data_ptr(), scales.data_ptr(), None, ws.data_ptr(), ws.numel(), s) == 0
+    one = float(np.float32(1) / np.float32(127))
+    assert bool((scales[:-3] == one).all()) and bool((q[0, :-3] == 127).all())
+    want = (np.array([2, 1e-8, 5], np.float32) / np.float32(127)).tolist()
+    assert scales[-3:].tolist() == want and q[0, -3:].tolist() == [127.0, 0.0, -127.0]
+
+
 # ---- products ---------------------------------------------------------------
 
 
