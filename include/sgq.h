@@ -391,7 +391,8 @@ int sgq_quantize_tokens(const void* x, int dtype, int64_t ldx, int64_t M, int64_
 /* The same of an RMSNorm's output: h = x + residual, rounded to the type, and
  *   rms_norm(h) = h * g / sqrt(sum(h^2) / K + eps)
  * row by row, g [K] fp32.  residual NULL: h is x, and the argument h must be NULL;
- * else h [M, K] is written and may be x or residual itself (with its row stride).
+ * else h [M, K] is written and may be x or residual itself (with its row stride);
+ * any other memory that it shares with them is refused.
  * The codes are those of u = fp32(h * g) with m = max(max|u|, 1e-8 / rstd), rstd =
  * 1 / sqrt(...): the norm's factor is common to a row and changes none of them.
  * scale = m * rstd / 127.  A row with an infinity or a NaN has a scale of NaN. */

@@ -252,6 +252,17 @@ int check_rows(const char* fn, const char* what, const void* p, int dtype, int64
     if (!aligned_to(p, dtype)) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: %s is not aligned to its type", fn, what);
     return SGQ_OK;
 }
+// Whether h [M, K] shares memory with x [M, K] without being it.  Rows of one stride may
+// lie between each other.
+bool rows_clash(const void* h, int64_t ldh, const void* x, int64_t ldx, int64_t M, int64_t K, int dtype) {
+    const int64_t size = dtype_bytes((DType)dtype);
+    const uintptr_t a = (uintptr_t)h, b = (uintptr_t)x;
+    if (a == b && ldh == ldx) return false;
+    if (a + (uintptr_t)(((M - 1) * ldh + K) * size) <= b || b + (uintptr_t)(((M - 1) * ldx + K) * size) <= a) return false;
+    if (ldh != ldx || M == 1) return true;
+    const int64_t at = (int64_t)((a > b ? a - b : b - a) / (uintptr_t)size) % ldh;
+    return at < K || at > ldh - K;
+}
 int check_token_codes(const char* fn, const void* codes, int64_t ldc, int64_t K) {
     if (!codes || !aligned16(codes)) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: codes must be 16-byte aligned", fn);
     if (ldc % 16 != 0 || ldc < round_up(K, kTokenPadK))
@@ -1051,8 +1062,8 @@ int sgq_rms_norm_tokens(const void* x, int dtype, int64_t ldx, const void* resid
     if (residual) {
         if ((st = check_rows(fn, "residual", residual, dtype, ldr, K)) != SGQ_OK) return st;
         if ((st = check_rows(fn, "h", h, dtype, ldh, K)) != SGQ_OK) return st;
-        if ((h == x && ldh != ldx) || (h == residual && ldh != ldr))
-            return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: h over an input needs its row stride", fn);
+        if (rows_clash(h, ldh, x, ldx, M, K, dtype) || rows_clash(h, ldh, residual, ldr, M, K, dtype))
+            return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: h over an input needs its address and row stride", fn);
     } else if (h) {
         return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: h without a residual", fn);
     }

@@ -172,7 +172,7 @@ def rms_norm_int8_tokens(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-
 def add_rms_norm_int8_tokens(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5,
                              out: Optional[torch.Tensor] = None) -> Tuple[TokensInt8, torch.Tensor]:
     """h = x + residual, and rms_norm(h) as int8 tokens.  h comes in x's shape, or in
-    `out`, which may be x or residual itself."""
+    `out`, which may be x or residual itself but share no other memory with them."""
     shape, dtype, dev = x.shape, x.dtype, x.device
     if residual.shape != shape or residual.dtype != dtype or residual.device != dev:
         raise ValueError("x and residual must be alike in shape, type and device")

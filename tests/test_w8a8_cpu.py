@@ -103,6 +103,24 @@ def test_norm_refusals(lib):
     assert call(M=0) == 0
 
 
+def test_norm_refuses_h_across_an_input(lib):
+    """h is an input, with its stride, or shares nothing with either."""
+    good = dict(x=P, dtype=1, ldx=64, r=16 * P, ldr=64, h=P, ldh=64, g=P, eps=1e-5, M=4, K=64, codes=P, ldc=128,
+                scales=P)
+
+    def clash(**kw):
+        st = lib.sgq_rms_norm_tokens(*{**good, **kw}.values(), None)
+        return st == 1 and b"over an input" in lib.sgq_last_error()
+
+    for d in (2, 128, 2 * 64 * 3, 2 * (64 * 3 + 63)):  # an element, a row, the last row, the last element
+        assert clash(h=P + d) and clash(h=P - d) and clash(h=16 * P + d) and clash(h=16 * P - d)
+    assert clash(h=P + 2, M=1) and clash(h=P - 126, M=1, ldx=4096, ldr=64, ldh=4096)
+    wide = dict(ldx=200, ldr=64, ldh=200)
+    for d in (1, 63, 137, 199):
+        assert clash(h=P + 2 * d, **wide) and clash(h=P - 2 * d, **wide)
+    assert clash(h=P, ldh=65) and clash(h=P + 2 * 64, ldh=65)
+
+
 def test_channels_refusals(lib):
     ws = lib.sgq_channels_workspace_bytes(64, 32)
     assert lib.sgq_quantize_channels(P, 64, 32, None, P, P, None, 0, None) == 3

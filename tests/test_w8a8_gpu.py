@@ -187,6 +187,27 @@ def test_tokens_of_views(op, dev, K, off, dtype):
     assert bool((v[:, :4] == 7).all()) and bool((v[:, 4 + K :] == 7).all())
 
 
+def test_norm_into_the_memory_around_an_input(op, dev):
+    """h between the rows of the inputs, behind them and over them is right; across them it is refused."""
+    M, K = 7, 200
+    g = 1 + 0.2 * _randn(dev, 9, K)
+    x, r = _randn(dev, 1, M, K), _randn(dev, 2, M, K)
+    want, hw = op.add_rms_norm_int8_tokens(x, r, g)
+    buf = torch.empty(2 * M, 3 * K, device=dev)
+    a, b = buf[:M, :K], buf[:M, K : 2 * K]
+    for out in (buf[:M, 2 * K :], buf[M:, :K], a, b):
+        a.copy_(x), b.copy_(r)
+        t, h = op.add_rms_norm_int8_tokens(a, b, g, out=out)
+        assert torch.equal(h, hw) and torch.equal(t.codes, want.codes) and torch.equal(t.scales, want.scales)
+    for out in (buf[1 : M + 1, :K], buf[:M, K - 1 : 2 * K - 1], buf[:M, 1 : K + 1], buf[:M, 2 * K - 1 : 3 * K - 1]):
+        with pytest.raises(RuntimeError, match="over an input"):
+            op.add_rms_norm_int8_tokens(a, b, g, out=out)
+    one, _ = op.add_rms_norm_int8_tokens(x[:1], r[:1], g, out=r[:1])
+    assert torch.equal(one.codes[0], want.codes[0])
+    with pytest.raises(RuntimeError, match="over an input"):
+        op.add_rms_norm_int8_tokens(buf[:1, :K], r[:1], g, out=buf[:1, 1 : K + 1])
+
+
 def test_tokens_without_rows_or_columns(op, dev):
     t = op.quantize_int8_tokens(torch.empty(0, 64, device=dev))
     assert t.codes.shape == (0, 128) and op.dequantize_int8_tokens(t).shape == (0, 64)
