@@ -63,6 +63,16 @@ class ChannelsInt8:
     K: int
     N: int
 
+    def __post_init__(self):
+        p, s = self.packed, self.scales
+        size = load_library().sgq_channels_packed_bytes(self.K, self.N)
+        if size < 0:
+            raise ValueError("sgq: a weight of channels has at most 131071 rows")
+        if not p.is_cuda or not p.is_contiguous() or p.numel() * p.element_size() < size:
+            raise ValueError(f"packed must be {size} contiguous bytes on the device")
+        if s.device != p.device or s.dtype is not torch.float32 or not s.is_contiguous() or s.numel() != self.N:
+            raise ValueError(f"scales must be {self.N} contiguous float32 beside packed")
+
 
 def _call(dev: torch.device, fn, *args) -> None:
     """fn(*args, stream) on dev's current stream, with dev the current device."""

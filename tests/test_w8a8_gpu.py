@@ -187,6 +187,20 @@ def test_tokens_of_views(op, dev, K, off, dtype):
     assert bool((v[:, :4] == 7).all()) and bool((v[:, 4 + K :] == 7).all())
 
 
+@pytest.mark.parametrize("K", [300, 5000, 20000])
+def test_norm_of_rows_at_the_ends_of_the_range(op, dev, K):
+    """Squares past fp32's largest value give a scale of NaN, not a wrong row; squares below its smallest are eps's."""
+    x = _randn(dev, 5, 4, K)
+    want = op.rms_norm_int8_tokens(x, torch.ones(K, device=dev))
+    x[1] *= 1e25
+    x[2] *= 1e-30
+    t = op.rms_norm_int8_tokens(x, torch.ones(K, device=dev))
+    assert torch.isnan(t.scales[1]) and torch.isnan(op.dequantize_int8_tokens(t)[1]).all()
+    assert not t.codes[2].any() and abs(float(t.scales[2]) * 127 / 1e-8 - 1) <= 32 * U
+    for i in (0, 3):
+        assert torch.equal(t.codes[i], want.codes[i]) and torch.equal(t.scales[i], want.scales[i])
+
+
 def test_norm_into_the_memory_around_an_input(op, dev):
     """h between the rows of the inputs, behind them and over them is right; across them it is refused."""
     M, K = 7, 200
@@ -478,6 +492,52 @@ def test_mlp(op, dev, M, dtype):
     assert h is x and torch.equal(first, mlp.forward(x - x + x, torch.zeros_like(x))[0])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_mlp_of_sequences(op, dev, dtype):
+    """Three dimensions, a padded batch seen through a view, and no tokens at all."""
+    D, H = 256, 600
+    _, _, mlp = _mlp(op, dev, D, H, dtype)
+    x, r = _randn(dev, 11, 3, 9, D).to(dtype), _randn(dev, 12, 3, 9, D).to(dtype)
+    out, h = mlp.forward(x[:, :5], r[:, :5])
+    flat, fh = mlp.forward(x[:, :5].reshape(15, D), r[:, :5].reshape(15, D))
+    assert out.shape == h.shape == (3, 5, D) and torch.equal(out.view(15, D), flat) and torch.equal(h.view(15, D), fh)
+    for shape in ((0, D), (2, 0, D)):
+        none = torch.empty(shape, dtype=dtype, device=dev)
+        out, h = mlp.forward(none, none)
+        assert out.shape == h.shape == shape and out.dtype == dtype
+        assert mlp.forward(none)[0].shape == shape
+
+
+def test_more_rows_and_columns_than_a_launch_takes(op, dev):
+    """Products in slices: rows past 2^26, columns past 2^24."""
+    M = 2**26 + 37
+    x = torch.zeros(M, 1, device=dev)
+    x[-40:, 0] = torch.arange(40, device=dev) - 20.0
+    t = op.quantize_int8_tokens(x)
+    w = op.pack_int8_channels(torch.tensor([[3, -2]], device=dev), torch.tensor([0.5, 1.0], device=dev))
+    b = torch.tensor([0.0, 1.0], device=dev)
+    y = op.quantized_matmul_w8a8(t, w, b, torch.bfloat16)
+    want = op.quantized_matmul_w8a8(op.TokensInt8(t.codes[-40:], t.scales[-40:], 1), w, b, torch.bfloat16)
+    assert torch.equal(y[-40:], want) and bool((want[:20, 0] < 0).all()) and bool((want[21:, 0] > 0).all())
+    assert not y[:-40, 0].any() and bool((y[:-40, 1] == 1).all())
+    del x, t, y
+    N = 2**24 + 45
+    cw = torch.zeros(1, N, dtype=torch.int8, device=dev)
+    cw[0, -60:] = torch.arange(60, device=dev) - 30
+    sw = torch.ones(N, device=dev)
+    wide = op.pack_int8_channels(cw, sw)
+    few = op.pack_int8_channels(cw[:, -60:], sw[-60:])
+    b = torch.zeros(N, device=dev)
+    b[-30:] = 0.25
+    for m in (3, 40, 300):
+        t = op.quantize_int8_tokens(_randn(dev, m, m, 1))
+        y = op.quantized_matmul_w8a8(t, wide, b, torch.float16)
+        assert torch.equal(y[:, -60:], op.quantized_matmul_w8a8(t, few, b[-60:], torch.float16)) and not y[:, :-60].any()
+        y = op.quantized_swiglu_w8a8(t, wide, wide, b, None, torch.bfloat16)
+        h = op.quantized_swiglu_w8a8(t, few, few, b[-60:], None, torch.bfloat16)
+        assert torch.equal(y[:, -60:], h) and not y[:, :-60].any()
+
+
 @pytest.mark.parametrize("M", [1, 40, 300])
 def test_graph_replays_match_eager(op, dev, M):
     """Two captured MLPs on one stream, replayed in turn on new inputs, with eager work between the replays."""
@@ -560,6 +620,11 @@ def test_refusals_on_the_device(op, dev):
         op.quantized_matmul_w8a8(op.TokensInt8(t.codes.float(), t.scales, 64), w)
     with pytest.raises(ValueError):
         op.quantized_matmul_w8a8(op.TokensInt8(t.codes, t.scales[:3], 64), w)
+    for bad in ((w.packed[:-1], w.scales, 64, 32), (w.packed, w.scales[:31], 64, 32), (w.packed, w.scales.half(), 64, 32),
+                (w.packed, w.scales, 129, 32), (w.packed, w.scales.cpu(), 64, 32), (w.packed.cpu(), w.scales, 64, 32),
+                (w.packed[::2], w.scales, 64, 16), (w.packed, w.scales, 1 << 20, 32), (w.packed, w.scales, -1, 32)):
+        with pytest.raises(ValueError):
+            op.ChannelsInt8(*bad)
     odd = torch.zeros(4, 129, dtype=torch.int8, device=dev)
     with pytest.raises(RuntimeError, match="16"):
         op.quantized_matmul_w8a8(op.TokensInt8(odd[:, :128], t.scales, 64), w)  # rows of 129 bytes
