@@ -306,19 +306,24 @@ constexpr int kStage = 128;  // k per stage
 // each operand once for all of its products, and the weight's layout is its operands',
 // so nothing is rearranged.
 //
-// What bounds it: at 8192 x 8192 -> 28672 (256 x 256 tiles, 1.40 ms, 2.75 POP/s; a library
-// int8 product of the shape 1.66 ms) the matrix cores are busy 70% of the time with the
-// clock at 1.74 GHz, the power limit: the same instructions alone, on operands of
+// What bounds it: at 8192 x 8192 -> 28672 (256 x 256 tiles, 1.35 to 1.40 ms, 2.8 POP/s; a library
+// int8 product of the shape 1.66 ms) the matrix cores are busy 73 to 75% of the time with
+// the clock at 1.65 GHz, the power limit: the same instructions alone, on operands of
 // random bits, run at 3.3 to 3.4 POP/s (4.6 on zeros), and the 32 x 32 x 32 form is
 // slower (1710 us against 1530 in the first tiles).  2048 x 4096 -> 4096 (128 x 256, one
-// tile a CU, 31 us, the library 41) keeps its clock at 2.4 GHz: 22 us of stages, the rest
-// the launch, the first loads and the stores.  Smaller products wait for their stages'
-// loads: a third and a fourth buffer take a 64 x 128 stage from .51 to .23 us and a 128 x
-// 128 one from .61 to .48; where CUs hold several tiles, two buffers of 128 x 128 leave
-// room for a second workgroup and do better (2048 x 4096 -> 4096 36 us against 39).
+// tile a CU, 29 to 31 us, the library 41): 22 us of stages, the rest the launch, the first
+// loads and the stores.  Calls of it back to back gain 32 stages in 24.6 us, 2.8 POP/s again,
+// and as much with all loads taken from one tile, so that memory is not what they wait
+// for; on half of the CUs, with power to spare, a stage takes .55 us in place of .77.
+// Smaller products wait for their stages' loads: a third and a fourth buffer take a 64 x
+// 128 stage from .51 to .23 us and a 128 x 128 one from .61 to .48; where CUs hold several
+// tiles, two buffers of 128 x 128 leave room for a second workgroup and do better (2048 x
+// 4096 -> 4096 36 us against 39).
 // Measured and not kept: a workgroup that takes its tiles one after another, the next
 // one's first loads under the last products (4096 x 4096 -> 11008 176 us against 163: the
-// loop over tiles left no registers); four wavefronts of 128 x 128 (1638 against 1449).
+// loop over tiles left no registers); four wavefronts of 128 x 128 (1614 against 1440) or of
+// 64 x 128 and 128 x 64 (128 x 256 tiles, 2048 x 4096 -> 4096 39 against 36): fewer LDS reads,
+// but a SIMD's only wavefront waits for them.
 template <int NG, int BM, int BN, int WM, int WN>
 struct TileCfg {
     static constexpr int kThreads = 64 * WM * WN;
