@@ -565,6 +565,50 @@ def test_graph_replays_match_eager(op, dev, M):
             assert torch.equal(y, want[k]) and torch.equal(eager, want[k]), (rep, i)
 
 
+def test_graphs_and_threads_at_the_same_time(op, sgq, dev):
+    """Two graphs of products that split K replayed on two streams at once, and eager calls of two host threads: each
+    has partial sums of its own."""
+    import threading
+
+    M, K, N = 90, 14000, 1030
+    assert sgq.load_library().sgq_linear_w8a8_workspace_bytes(M, K, N, 256) > 0
+    qw = op.quantize_int8_channels(_randn(dev, 1, K, N))
+    ts = [op.quantize_int8_tokens(_randn(dev, 2 + i, M, K)) for i in range(2)]
+    want = [op.quantized_matmul_w8a8(t, qw) for t in ts]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(dev) for _ in range(2)]
+    graphs, outs = [], []
+    for s, t in zip(streams, ts):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            outs.append(op.quantized_matmul_w8a8(t, qw))
+        graphs.append(g)
+    for _ in range(5):
+        for y in outs:
+            y.fill_(float("nan"))
+        torch.cuda.synchronize()
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, w) for y, w in zip(outs, want))
+    got = [[], []]
+
+    def work(i):
+        with torch.cuda.stream(streams[i]):
+            for _ in range(10):
+                got[i].append(op.quantized_matmul_w8a8(ts[i], qw))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert len(got[i]) == 10 and all(torch.equal(y, want[i]) for y in got[i])
+
+
 def test_other_stream(op, dev):
     D, H, M = 512, 1024, 64
     _, _, mlp = _mlp(op, dev, D, H, torch.float32)
