@@ -388,6 +388,13 @@ int64_t sgq_tokens_row_bytes(int64_t K);
 int sgq_quantize_tokens(const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, void* codes, int64_t ldc,
                         float* scales, void* stream);
 
+/* The same for activations on their way through a model: a row with an infinity or a
+ * NaN has a scale of NaN (as behind the norm below), so that it stays one.  Under
+ * sgq_quantize_tokens a NaN loses the maximum: a row of NaN becomes codes of 127 at the
+ * smallest scale, and -inf reads back as +inf. */
+int sgq_quantize_tokens_keep_nan(const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, void* codes, int64_t ldc,
+                                 float* scales, void* stream);
+
 /* The same of an RMSNorm's output: h = x + residual, rounded to the type, and
  *   rms_norm(h) = h * g / sqrt(sum(h^2) / K + eps)
  * row by row, g [K] fp32.  residual NULL: h is x, and the argument h must be NULL;

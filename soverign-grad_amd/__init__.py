@@ -80,6 +80,7 @@ SIGNATURES = {
     "sgq_embedding": (_int, [_vp, _i64, _vp, _i64, _i64, _vp, _vp]),
     "sgq_tokens_row_bytes": (_i64, [_i64]),
     "sgq_quantize_tokens": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
+    "sgq_quantize_tokens_keep_nan": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
     "sgq_rms_norm_tokens": (_int, [_vp, _int, _i64, _vp, _i64, _vp, _i64, _vp, ctypes.c_float, _i64, _i64, _vp, _i64,
                                    _vp, _vp]),
     "sgq_dequantize_tokens": (_int, [_vp, _i64, _vp, _i64, _i64, _vp, _int, _i64, _vp]),

@@ -370,6 +370,21 @@ int linear_int4(const char* fn, const float* x, int64_t M, int64_t K, int64_t N,
     return ok();
 }
 
+int quantize_tokens(const char* fn, const void* x, int dtype, int64_t ldx, bool keep_nan, int64_t M, int64_t K, void* codes,
+                    int64_t ldc, float* scales, void* stream) {
+    int st = check_w8a8_shape(fn, M, K);
+    if (st != SGQ_OK) return st;
+    if (bad_dtype(dtype)) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: bad dtype", fn);
+    if (M == 0) return ok();
+    if (!scales) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: null scales", fn);
+    if ((st = check_token_codes(fn, codes, ldc, K)) != SGQ_OK) return st;
+    if (K > 0 && (st = check_rows(fn, "x", x, dtype, ldx, K)) != SGQ_OK) return st;
+    SGQ_HIP(launch_tokens(x, (DType)dtype, ldx, nullptr, 0, nullptr, 0, nullptr, 0.0f, keep_nan, M, K, codes, ldc, scales,
+                          (hipStream_t)stream),
+            "tokens");
+    return ok();
+}
+
 // Workspace of such a product on `cus` compute units (0: the current device's).
 int64_t w8a8_ws_bytes(int ng, int64_t M, int64_t K, int64_t N, int cus) {
     if (bad_dims(M, K) || bad_dims(K, N) || bad_dims(M, N) || K > kMaxTokenK || cus < 0) return -1;
@@ -1034,18 +1049,12 @@ int64_t sgq_channels_workspace_bytes(int64_t K, int64_t N) {
 
 int sgq_quantize_tokens(const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, void* codes, int64_t ldc,
                         float* scales, void* stream) {
-    const char* fn = "sgq_quantize_tokens";
-    int st = check_w8a8_shape(fn, M, K);
-    if (st != SGQ_OK) return st;
-    if (bad_dtype(dtype)) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: bad dtype", fn);
-    if (M == 0) return ok();
-    if (!scales) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: null scales", fn);
-    if ((st = check_token_codes(fn, codes, ldc, K)) != SGQ_OK) return st;
-    if (K > 0 && (st = check_rows(fn, "x", x, dtype, ldx, K)) != SGQ_OK) return st;
-    SGQ_HIP(launch_tokens(x, (DType)dtype, ldx, nullptr, 0, nullptr, 0, nullptr, 0.0f, M, K, codes, ldc, scales,
-                          (hipStream_t)stream),
-            "tokens");
-    return ok();
+    return quantize_tokens("sgq_quantize_tokens", x, dtype, ldx, false, M, K, codes, ldc, scales, stream);
+}
+
+int sgq_quantize_tokens_keep_nan(const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, void* codes, int64_t ldc,
+                                 float* scales, void* stream) {
+    return quantize_tokens("sgq_quantize_tokens_keep_nan", x, dtype, ldx, true, M, K, codes, ldc, scales, stream);
 }
 
 int sgq_rms_norm_tokens(const void* x, int dtype, int64_t ldx, const void* residual, int64_t ldr, void* h, int64_t ldh,
@@ -1067,7 +1076,7 @@ int sgq_rms_norm_tokens(const void* x, int dtype, int64_t ldx, const void* resid
     } else if (h) {
         return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: h without a residual", fn);
     }
-    SGQ_HIP(launch_tokens(x, (DType)dtype, ldx, residual, ldr, h, ldh, g, eps, M, K, codes, ldc, scales,
+    SGQ_HIP(launch_tokens(x, (DType)dtype, ldx, residual, ldr, h, ldh, g, eps, false, M, K, codes, ldc, scales,
                           (hipStream_t)stream),
             "tokens");
     return ok();

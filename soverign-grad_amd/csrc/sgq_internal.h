@@ -513,10 +513,11 @@ hipError_t launch_attention_decode(const float* q, const float* knew, const floa
 
 // ---- 8-bit tokens and their products (sgq_tokens.hip, sgq_w8a8.hip) ------
 // Rows of x [M, K] as codes and scales.  g (optional): of the RMSNorm of h = x + r
-// (r optional; h is then written); without g the rows of x themselves.
+// (r optional; h is then written); without g the rows of x themselves (keep_nan: a row
+// that is not finite has a scale of NaN, as it has behind the norm).
 hipError_t launch_tokens(const void* x, DType t, int64_t ldx, const void* r, int64_t ldr, void* h, int64_t ldh,
-                         const float* g, float eps, int64_t M, int64_t K, void* codes, int64_t ldc, float* scales,
-                         hipStream_t s);
+                         const float* g, float eps, bool keep_nan, int64_t M, int64_t K, void* codes, int64_t ldc,
+                         float* scales, hipStream_t s);
 hipError_t launch_tokens_values(const void* codes, int64_t ldc, const float* scales, int64_t M, int64_t K, void* out,
                                 DType t, int64_t ldo, hipStream_t s);
 // Weights [K, N] with a scale per column.  top: N floats of workspace; qdata and

@@ -10,6 +10,11 @@
 // positive factor of the whole row: it cancels out of n / max|n|, so the codes are
 // taken from u (m = max(max|u|, 1e-8 / rstd)) and do not depend on the order of
 // the sum; rstd only enters the scale, m * rstd / 127.
+// Rows that are not finite: behind the norm the sum of squares carries them into the
+// scale.  Without it the rule is the weights' (NaN never wins the maximum), which would
+// turn the hidden row of NaN of an MLP into small finite tokens; KEEP sums v * 0, zero
+// or, of an infinity or a NaN, a NaN, beside the maximum and adds it to the scale (2048 x
+// 11008 fp32 20.9 us against 20.8 without, bf16 14.7 against 14.5).
 // Nothing in this file may be contracted into FMAs but the sum of squares.
 #include "sgq_internal.h"
 
@@ -66,8 +71,9 @@ __device__ __forceinline__ void row_reduce(float& ss, float& m, float (*red)[16]
     }
 }
 
-// Scale and inverse of a row from its sum of squares and its maximum.
-template <bool NORM>
+// Scale of a row, and m as the codes take it, from its sum of squares (KEEP: of v * 0)
+// and its maximum.
+template <bool NORM, bool KEEP>
 __device__ __forceinline__ float row_scale(float ss, float& m, float K, float eps) {
     if constexpr (NORM) {
         const float rstd = 1.0f / sqrtf(ss / K + eps);
@@ -75,13 +81,13 @@ __device__ __forceinline__ float row_scale(float ss, float& m, float K, float ep
         return m * rstd / 127.0f;
     } else {
         m = fmaxf(m, 1e-8f);
-        return m / 127.0f;
+        return KEEP ? m / 127.0f + ss : m / 127.0f;
     }
 }
 
 // NT threads a row (a wavefront of several in a workgroup, or a workgroup), C
 // chunks of eight elements a thread: the row stays in registers.
-template <typename T, bool NORM, bool RES, int NT, int C>
+template <typename T, bool NORM, bool RES, bool KEEP, int NT, int C>
 __global__ __launch_bounds__(NT < kBlock ? kBlock : NT) void k_tokens_row(const TokensArgs a) {
     __shared__ float red[2][16];
     constexpr int kRows = NT < kBlock ? kBlock / NT : 1;
@@ -137,6 +143,7 @@ __global__ __launch_bounds__(NT < kBlock ? kBlock : NT) void k_tokens_row(const 
 #pragma unroll
             for (int e = 0; e < kV; ++e) {
                 float v = (float)xv[i][e];
+                if constexpr (KEEP) ss = fmaf(v, 0.0f, ss);
                 if constexpr (NORM) {
                     ss = fmaf(v, v, ss);
                     v = v * gv[i][e];
@@ -146,7 +153,7 @@ __global__ __launch_bounds__(NT < kBlock ? kBlock : NT) void k_tokens_row(const 
             }
         }
         row_reduce<NT>(ss, m, red);
-        const float scale = row_scale<NORM>(ss, m, (float)K, a.eps), inv = 127.0f / m;
+        const float scale = row_scale<NORM, KEEP>(ss, m, (float)K, a.eps), inv = 127.0f / m;
         if (t == 0) a.scales[row] = scale;
         signed char* c = a.codes + row * a.ldc;
 #pragma unroll
@@ -164,7 +171,7 @@ __global__ __launch_bounds__(NT < kBlock ? kBlock : NT) void k_tokens_row(const 
 // from 16384 on: x, the residual, g and u of four chunks do not fit the 128 registers
 // that sixteen wavefronts leave a thread.
 constexpr int kLoopBlock = 1024;
-template <typename T, bool NORM, bool RES>
+template <typename T, bool NORM, bool RES, bool KEEP>
 __global__ __launch_bounds__(kLoopBlock) void k_tokens_loop(const TokensArgs a) {
     __shared__ float red[2][16];
     for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
@@ -180,6 +187,7 @@ __global__ __launch_bounds__(kLoopBlock) void k_tokens_loop(const TokensArgs a) 
                 h[k] = t;
                 v = (float)t;
             }
+            if constexpr (KEEP) ss = fmaf(v, 0.0f, ss);
             if constexpr (NORM) {
                 ss = fmaf(v, v, ss);
                 v = v * a.g[k];
@@ -187,7 +195,7 @@ __global__ __launch_bounds__(kLoopBlock) void k_tokens_loop(const TokensArgs a) 
             m = fmaxf(m, fabsf(v));
         }
         row_reduce<kLoopBlock>(ss, m, red);
-        const float scale = row_scale<NORM>(ss, m, (float)a.K, a.eps), inv = 127.0f / m;
+        const float scale = row_scale<NORM, KEEP>(ss, m, (float)a.K, a.eps), inv = 127.0f / m;
         if (threadIdx.x == 0) a.scales[row] = scale;
         const T* src = RES ? h : x;  // each thread reads what it wrote
 #pragma unroll 4
@@ -231,53 +239,53 @@ constexpr int64_t kMaxRowGroups = (int64_t)1 << 20;  // workgroups of a launch (
 // 7.0 / 7.9; 512 of two against 256 of four, 8192 x 8192 84 / 87, 16 x 8192 3.9 / 4.3.  HBM bounds
 // them from there: 2048 x 4096 11.3 us, 5.2 TB/s, 2048 x 11008 fp32 tokens 20.7, 5.4 TB/s (a large
 // copy reaches 5.1); a few rows are one row's latency.
-template <typename T, bool NORM, bool RES>
+template <typename T, bool NORM, bool RES, bool KEEP>
 hipError_t launch_rows(const TokensArgs& a, hipStream_t s) {
     const auto grid = [&](int rows) { return (unsigned)(ceil_div(a.M, rows) < kMaxRowGroups ? ceil_div(a.M, rows) : kMaxRowGroups); };
     const int64_t q = a.Kpad / kV;
     if (q <= 64)
-        k_tokens_row<T, NORM, RES, 64, 1><<<grid(4), kBlock, 0, s>>>(a);
+        k_tokens_row<T, NORM, RES, KEEP, 64, 1><<<grid(4), kBlock, 0, s>>>(a);
     else if (q <= 128)
-        k_tokens_row<T, NORM, RES, 64, 2><<<grid(4), kBlock, 0, s>>>(a);
+        k_tokens_row<T, NORM, RES, KEEP, 64, 2><<<grid(4), kBlock, 0, s>>>(a);
     else if (q <= 256)
-        k_tokens_row<T, NORM, RES, 256, 1><<<grid(1), 256, 0, s>>>(a);
+        k_tokens_row<T, NORM, RES, KEEP, 256, 1><<<grid(1), 256, 0, s>>>(a);
     else if (q <= 512)
-        k_tokens_row<T, NORM, RES, 256, 2><<<grid(1), 256, 0, s>>>(a);
+        k_tokens_row<T, NORM, RES, KEEP, 256, 2><<<grid(1), 256, 0, s>>>(a);
     else if (q <= 768)
-        k_tokens_row<T, NORM, RES, 256, 3><<<grid(1), 256, 0, s>>>(a);
+        k_tokens_row<T, NORM, RES, KEEP, 256, 3><<<grid(1), 256, 0, s>>>(a);
     else if (q <= 1024)
-        k_tokens_row<T, NORM, RES, 512, 2><<<grid(1), 512, 0, s>>>(a);
+        k_tokens_row<T, NORM, RES, KEEP, 512, 2><<<grid(1), 512, 0, s>>>(a);
     else if (q <= 2048)
-        k_tokens_row<T, NORM, RES, 512, 4><<<grid(1), 512, 0, s>>>(a);
+        k_tokens_row<T, NORM, RES, KEEP, 512, 4><<<grid(1), 512, 0, s>>>(a);
     else if constexpr (!NORM) {
         if (q <= 4096)
-            k_tokens_row<T, NORM, RES, 1024, 4><<<grid(1), 1024, 0, s>>>(a);
+            k_tokens_row<T, NORM, RES, KEEP, 1024, 4><<<grid(1), 1024, 0, s>>>(a);
         else
-            k_tokens_loop<T, NORM, RES><<<grid(1), kLoopBlock, 0, s>>>(a);
+            k_tokens_loop<T, NORM, RES, KEEP><<<grid(1), kLoopBlock, 0, s>>>(a);
     } else {
-        k_tokens_loop<T, NORM, RES><<<grid(1), kLoopBlock, 0, s>>>(a);
+        k_tokens_loop<T, NORM, RES, KEEP><<<grid(1), kLoopBlock, 0, s>>>(a);
     }
     return hipGetLastError();
 }
 
 template <typename T>
-hipError_t launch_t(const TokensArgs& a, hipStream_t s) {
-    if (!a.g) return launch_rows<T, false, false>(a, s);
-    return a.r ? launch_rows<T, true, true>(a, s) : launch_rows<T, true, false>(a, s);
+hipError_t launch_t(const TokensArgs& a, bool keep, hipStream_t s) {
+    if (!a.g) return keep ? launch_rows<T, false, false, true>(a, s) : launch_rows<T, false, false, false>(a, s);
+    return a.r ? launch_rows<T, true, true, false>(a, s) : launch_rows<T, true, false, false>(a, s);
 }
 
 }  // namespace
 
 hipError_t launch_tokens(const void* x, DType t, int64_t ldx, const void* r, int64_t ldr, void* h, int64_t ldh,
-                         const float* g, float eps, int64_t M, int64_t K, void* codes, int64_t ldc, float* scales,
-                         hipStream_t s) {
+                         const float* g, float eps, bool keep_nan, int64_t M, int64_t K, void* codes, int64_t ldc,
+                         float* scales, hipStream_t s) {
     TokensArgs a{};
     a.x = x, a.r = r, a.h = h, a.g = g, a.eps = eps;
     a.ldx = ldx, a.ldr = ldr, a.ldh = ldh, a.ldc = ldc;
     a.M = M, a.K = K, a.Kpad = K > 0 ? round_up(K, kTokenPadK) : kTokenPadK;
     a.codes = (signed char*)codes, a.scales = scales;
-    return t == DType::f32 ? launch_t<float>(a, s)
-                           : (t == DType::bf16 ? launch_t<__bf16>(a, s) : launch_t<_Float16>(a, s));
+    return t == DType::f32 ? launch_t<float>(a, keep_nan, s)
+                           : (t == DType::bf16 ? launch_t<__bf16>(a, keep_nan, s) : launch_t<_Float16>(a, keep_nan, s));
 }
 
 hipError_t launch_tokens_values(const void* codes, int64_t ldc, const float* scales, int64_t M, int64_t K, void* out,

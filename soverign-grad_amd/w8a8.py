@@ -4,7 +4,7 @@ Activations become int8 tokens (a scale per row), weights int8 channels (a scale
 per output column of W [K, N]), and products of the two run on the int8 matrix
 cores, exact until the scales are applied (inference only: nothing here has a gradient):
 
-    quantize_int8_tokens(x)                        x as tokens
+    quantize_int8_tokens(x)                        x as tokens (keep_nan: rows that are not finite stay so)
     rms_norm_int8_tokens(x, weight)                rms_norm(x) as tokens
     add_rms_norm_int8_tokens(x, residual, weight)  h = x + residual, and rms_norm(h) as tokens
     dequantize_int8_tokens(t)                      their values
@@ -147,12 +147,18 @@ def _output(out: Optional[torch.Tensor], M: int, N: int, dtype: torch.dtype, dev
     return out
 
 
-def quantize_int8_tokens(x: torch.Tensor) -> TokensInt8:
-    """The rows of x (all dimensions but the last taken together) as int8 tokens."""
+def quantize_int8_tokens(x: torch.Tensor, keep_nan: bool = False) -> TokensInt8:
+    """The rows of x (all dimensions but the last taken together) as int8 tokens.  By
+    itself this is quantize_int8's rule, where a NaN loses the maximum: a row of NaN
+    becomes small finite values.  keep_nan: a row with a NaN or an infinity has a scale
+    of NaN, as it has behind the norms, and every product of it is NaN; what a model
+    computes on the way (an MLP's hidden values) wants this."""
     x = _rows(x, "x")
     M, K = x.shape
     t = _new_tokens(M, K, x.device)
-    _call(x.device, load_library().sgq_quantize_tokens, x.data_ptr(), _dtype(x.dtype), _ld(x), M, K,
+    lib = load_library()
+    fn = lib.sgq_quantize_tokens_keep_nan if keep_nan else lib.sgq_quantize_tokens
+    _call(x.device, fn, x.data_ptr(), _dtype(x.dtype), _ld(x), M, K,
           t.codes.data_ptr(), _row_bytes(K), t.scales.data_ptr())
     return t
 
@@ -347,7 +353,9 @@ class QuantizedMLPInt8:
       h   = x + residual
       out = down(silu(gate(n)) * up(n)),  n = rms_norm(h, norm)
 
-    forward() returns (out, h); the next layer adds the two in its own norm."""
+    forward() returns (out, h); the next layer adds the two in its own norm.  Where a
+    row of h is not finite, its squares pass fp32 or its hidden values pass the type,
+    the row of out is NaN."""
 
     def __init__(self, gate: ChannelsInt8, up: ChannelsInt8, down: ChannelsInt8, norm: torch.Tensor,
                  eps: float = 1e-5):
@@ -367,7 +375,7 @@ class QuantizedMLPInt8:
         else:
             t, h = add_rms_norm_int8_tokens(x, residual, self.norm, self.eps)
         a = quantized_swiglu_w8a8(t, self.gate, self.up, dtype=x.dtype)
-        return quantized_matmul_w8a8(quantize_int8_tokens(a), self.down, dtype=x.dtype).reshape(x.shape), h
+        return quantized_matmul_w8a8(quantize_int8_tokens(a, keep_nan=True), self.down, dtype=x.dtype).reshape(x.shape), h
 
 
 __all__ = ["TokensInt8", "ChannelsInt8", "quantize_int8_tokens", "rms_norm_int8_tokens", "add_rms_norm_int8_tokens",
