@@ -441,8 +441,8 @@ int sgq_linear_w8a8(const void* codes, int64_t ldc, const float* x_scales, int64
                     const void* packed, const float* w_scales, const float* bias, void* y, int dtype, int64_t ldy,
                     void* workspace, int64_t workspace_bytes, void* stream);
 
-/* h = silu(gate) * up of two such products (as sgq_swiglu_int8), in fp32 until it
- * is rounded to the type. */
+/* h = silu(gate) * up of two such products (silu as in sgq_swiglu_int8, to a few
+ * roundings of fp32 for every gate), in fp32 until it is rounded to the type. */
 int64_t sgq_swiglu_w8a8_workspace_bytes(int64_t M, int64_t K, int64_t N, int compute_units);
 int sgq_swiglu_w8a8(const void* codes, int64_t ldc, const float* x_scales, int64_t M, int64_t K, int64_t N,
                     const void* packed_gate, const float* scales_gate, const float* bias_gate, const void* packed_up,
