@@ -85,6 +85,10 @@ __device__ __forceinline__ float row_scale(float ss, float& m, float K, float ep
     }
 }
 
+// 127 / m, at most the largest float: without eps the norm of a row of zeros has m = 0, and
+// an infinite factor would leave no zeros past K (nor the signs of values below 2^-126).
+__device__ __forceinline__ float row_inv(float m) { return fminf(127.0f / m, 3.40282347e38f); }
+
 // NT threads a row (a wavefront of several in a workgroup, or a workgroup), C
 // chunks of eight elements a thread: the row stays in registers.
 template <typename T, bool NORM, bool RES, bool KEEP, int NT, int C>
@@ -153,7 +157,7 @@ __global__ __launch_bounds__(NT < kBlock ? kBlock : NT) void k_tokens_row(const 
             }
         }
         row_reduce<NT>(ss, m, red);
-        const float scale = row_scale<NORM, KEEP>(ss, m, (float)K, a.eps), inv = 127.0f / m;
+        const float scale = row_scale<NORM, KEEP>(ss, m, (float)K, a.eps), inv = row_inv(m);
         if (t == 0) a.scales[row] = scale;
         signed char* c = a.codes + row * a.ldc;
 #pragma unroll
@@ -195,7 +199,7 @@ __global__ __launch_bounds__(kLoopBlock) void k_tokens_loop(const TokensArgs a) 
             m = fmaxf(m, fabsf(v));
         }
         row_reduce<kLoopBlock>(ss, m, red);
-        const float scale = row_scale<NORM, KEEP>(ss, m, (float)a.K, a.eps), inv = 127.0f / m;
+        const float scale = row_scale<NORM, KEEP>(ss, m, (float)a.K, a.eps), inv = row_inv(m);
         if (threadIdx.x == 0) a.scales[row] = scale;
         const T* src = RES ? h : x;  // each thread reads what it wrote
 #pragma unroll 4

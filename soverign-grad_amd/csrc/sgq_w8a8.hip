@@ -164,7 +164,7 @@ __device__ __forceinline__ void store4(T* row, int64_t n, int64_t N, floatx4 v) 
 // or is subnormal before the last step, down to the gates (-104) where silu leaves fp32.
 // n's limits: from 43 on 2^f counts for nothing, below -160 the result is zero.  f takes g
 // itself, so that 2^f carries infinities and a NaN.  The exponential and the reciprocal
-// are the hardware's, each within a step.  Error over a million gates in each of twelve ranges of
+// are the hardware's, each within a step.  Error over a million gates in each of eleven ranges of
 // [-92, 100], in units of 2^-24: 0.9 rms, 3.3 at most (expf and a division: 0.7 and 2.5, but
 // zero from -88.7 on; g * -log2 e rounded into the exponential: 8 rms at -20, 32 at -85, zero
 // from -87.3 on).  A 256 x 256 tile takes 64 of these a lane: 4096 x 4096 -> 11008 gated 320
