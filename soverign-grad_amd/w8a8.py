@@ -222,6 +222,8 @@ def _weight2d(w: torch.Tensor) -> torch.Tensor:
         raise ValueError("sgq: expected a device tensor")
     if w.dim() != 2:
         raise ValueError("a weight of channels must be [K, N]")
+    if w.is_complex():
+        raise ValueError("a weight of channels cannot be complex")
     return w.to(torch.float32).contiguous()
 
 
@@ -247,7 +249,10 @@ def quantize_int8_channels(w: torch.Tensor) -> ChannelsInt8:
 def pack_int8_channels(codes: torch.Tensor, scales: torch.Tensor) -> ChannelsInt8:
     """From codes [K, N] (whole numbers in [-128, 127], of any type) and scales [N], as a
     checkpoint holds them.  Waits for the stream, to say whether the codes are such."""
-    codes = _weight2d(codes)
+    given, codes = codes, _weight2d(codes)
+    if given.dtype is torch.float64:
+        # What only fp32 takes for a whole number is none.
+        codes = torch.where(codes == given, codes, float("nan")).contiguous()
     K, N = codes.shape
     qw, ws = _new_channels(K, N, _vector(scales, N, codes.device, "scales").reshape(-1).clone())
     _call(codes.device, load_library().sgq_pack_channels, codes.data_ptr(), K, N, qw.packed.data_ptr(), ws.data_ptr(),
