@@ -247,8 +247,14 @@ def quantize_int8_channels(w: torch.Tensor) -> ChannelsInt8:
 
 
 def pack_int8_channels(codes: torch.Tensor, scales: torch.Tensor) -> ChannelsInt8:
-    """From codes [K, N] (whole numbers in [-128, 127], of any type) and scales [N], as a
-    checkpoint holds them.  Waits for the stream, to say whether the codes are such."""
+    """From codes [K, N] (whole numbers in [-128, 127], of any real type) and scales [N], as
+    a checkpoint holds them.  Waits for the stream, to say whether the codes are such.
+
+    Of a QuantizedTensor q with one scale (quantize_int8, per tensor):
+    pack_int8_channels(unpack_codes(q), q.scales.expand(N)).  One per channel cannot come
+    along: it has a scale for each row of W [K, N], which would have to multiply the terms
+    of a sum that is in integers here; such a weight is quantized again, by
+    quantize_int8_channels(dequantize_int8(q))."""
     given, codes = codes, _weight2d(codes)
     if given.dtype is torch.float64:
         # What only fp32 takes for a whole number is none.
