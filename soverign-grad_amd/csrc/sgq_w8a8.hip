@@ -162,24 +162,23 @@ __device__ __forceinline__ void store4(T* row, int64_t n, int64_t N, floatx4 v) 
 //   silu(g) = g / (1 + e^-g) = 2^n * g / (2^n + 2^f):
 // the exponential's argument keeps its bits however large g is, and nothing overflows
 // or is subnormal before the last step, down to the gates (-104) where silu leaves fp32.
-// n's limits: from 43 on 2^f counts for nothing, below -160 the result is zero.  f takes g
-// itself, so that 2^f carries infinities and a NaN.  The exponential and the reciprocal
-// are the hardware's, each within a step.  Error over a million gates in each of eleven ranges of
-// [-92, 100], in units of 2^-24: 0.9 rms, 3.3 at most (expf and a division: 0.7 and 2.5, but
-// zero from -88.7 on; g * -log2 e rounded into the exponential: 8 rms at -20, 32 at -85, zero
-// from -87.3 on).  A 256 x 256 tile takes 64 of these a lane: 4096 x 4096 -> 11008 gated 320
-// us, 512 x 2048 -> 5632 18.4 (expf and a division 332 and 18.9, the rounded product 311
-// and 18.0).
+// n's limits: from 43 on 2^f counts for nothing, and 2^-149 is the smallest number (f,
+// which takes g itself, has what is left, and by it 2^f carries infinities and a NaN).
+// The exponential and the reciprocal are the hardware's, each within a step.  Error over
+// a million gates in each of eleven ranges of [-92, 100], in units of 2^-24: 0.9 rms, 3.3
+// at most (expf and a division: 0.7 and 2.5, but zero from -88.7 on; g * -log2 e rounded
+// into the exponential: 8 rms at -20, 32 at -85, zero from -87.3 on).  A 256 x 256 tile
+// takes 64 of these a lane: 4096 x 4096 -> 11008 gated 319 us, 512 x 2048 -> 5632 17.7 (the
+// rounded product 312 and 17.3; expf and a division 332 and 18.9).
 __device__ __forceinline__ floatx4 silu_mul4(floatx4 g, floatx4 u) {
     constexpr float kLog2e = 1.44269502f, kLog2eRest = 1.92596299e-8f;  // their sum is log2 e to 48 bits
     floatx4 v;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-        const float n = rintf(__builtin_amdgcn_fmed3f(g[r] * kLog2e, -160.0f, 43.0f));
+        const float n = rintf(__builtin_amdgcn_fmed3f(g[r] * kLog2e, -149.0f, 43.0f));
         const float f = fmaf(g[r], -kLog2eRest, fmaf(g[r], -kLog2e, n));
-        const int k = (int)n;
-        const float d = __builtin_ldexpf(1.0f, k) + __builtin_amdgcn_exp2f(f);
-        v[r] = __builtin_ldexpf(g[r] * __builtin_amdgcn_rcpf(d), k) * u[r];
+        const float s = __builtin_ldexpf(1.0f, (int)n);
+        v[r] = g[r] * __builtin_amdgcn_rcpf(s + __builtin_amdgcn_exp2f(f)) * s * u[r];
     }
     return v;
 }
