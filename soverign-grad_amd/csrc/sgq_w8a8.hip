@@ -47,8 +47,11 @@ __global__ __launch_bounds__(kWG) void k_channels_top(const float* __restrict__ 
     }
 }
 
-// HBM bounds the two passes over w: packing 4096 x 4096 fp32 codes takes 22 us, 8192 x
-// 28672 360 us (3.3 TB/s).
+// Their bytes bound them: quantizing 4096 x 11008 takes 76 us (w read twice, the second
+// time partly from the caches: 5.3 TB/s, a large copy reaches 5.1), 8192 x 28672 500 us
+// (4.2 TB/s), unpacking 34 and 215 us (6.6 and 5.5 TB/s).  Packing fp32 codes of 8192 x
+// 28672 takes 358 us with the wait for the flag (3.3 TB/s) and was left there: a weight is
+// packed once.
 //
 // Codes of a kTileK x kTileN tile: FROM_CODES reads fp32 codes (validated into
 // *bad), else w with the columns' maxima in top; through LDS into the layout.
@@ -211,8 +214,17 @@ __device__ __forceinline__ floatx4 load4(const float* v, int64_t n, int64_t N) {
 // come from HBM).
 template <int NG, typename T, int MB, int C, int NW>
 __global__ __launch_bounds__(64 * NW) void k_w8a8_few(const W8A8Args a, int mblocks, int xlog) {
-    constexpr int B = MB * C * NG;                     // 16 x 16 blocks of sums
-    constexpr int U = B >= 8 ? 1 : (B >= 4 ? 2 : 4);   // steps whose loads are in flight together
+    constexpr int B = MB * C * NG;  // 16 x 16 blocks of sums
+    // Steps whose loads are in flight together.  Measured with 1 / 2 / 3 / 4 (us, bf16,
+    // weights from HBM), one weight and the gated two:
+    //   16 x 16, 16 x 4096 -> 11008   13.0 / 13.8 / 14.0 / 12.3   21.0 / 19.4 / 20.0 / 19.2
+    //   32 x 16, 32 x 4096 -> 4096     8.2 /  8.1 /  8.8 /  7.9   10.8 / 11.1 / 11.8 / 10.9
+    //   32 x 32, 48 x 4096 -> 4096     8.2 /  8.4 /  9.0 /  8.2   13.0 / 13.4 / 15.0 / 14.6
+    //   64 x 32, 128 x 4096 -> 4096   12.9 / 13.4 / 14.2 / 13.4   18.1 / 17.4 / 21.3 / 22.3
+    // One block of sums gains; from four on more of them gain little or lose, so it is not
+    // single latencies that those forms wait for: their workgroups read tokens and weights
+    // of 100 MB in all through the L2s in the last line, at 8 TB/s.
+    constexpr int U = B >= 8 ? 1 : (B >= 4 ? 2 : 4);
     __shared__ i32x4 red[NW][B][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lr = lane & 15, g = lane >> 4;
@@ -731,9 +743,9 @@ int64_t w8a8_plan_bytes(const W8A8Plan& p, int ng, int64_t M, int64_t K, int64_t
 // 128 / 128 x 128 with two buffers / with four / 128 x 256 / 256 x 256): 333 x 2043 -> 5001 9.6 /
 // 13.8 / 12.7 / 15.6 / 24.6, 1024 x 4096 -> 4096 23.4 / 24.4 / 20.2 / 23.7 / 38, 2048 x 4096 -> 4096
 // 44 / 36 / 39 / 31 / 40, 4096 x 4096 -> 4096 86 / 69 / 75 / 61 / 54; 128 x 11008 -> 4096 on 64 x
-// 128 without a split 26.4, with two 19.2.  The forms for few tokens read a weight once
-// for each of their row blocks: 48 x 4096 -> 4096 9.8 on 64 x 32 against 11.2, but 48 x
-// 14336 -> 28672 132 against 73.
+// 128 (from HBM) without a split 40, with two 27, with four, its plan, 21, with eight 24.
+// The forms for few tokens read a weight once for each of their row blocks: 48 x 4096 ->
+// 4096 9.8 on 64 x 32 against 11.2, but 48 x 14336 -> 28672 132 against 73.
 W8A8Plan w8a8_plan(int ng, int64_t M, int64_t K, int64_t N, int64_t cus) {
     W8A8Plan best;
     if (K == 0) return best;
