@@ -403,7 +403,8 @@ int sgq_quantize_tokens_keep_nan(const void* x, int dtype, int64_t ldx, int64_t 
  * The codes are those of u = fp32(h * g) with m = max(max|u|, 1e-8 / rstd), rstd =
  * 1 / sqrt(...): the norm's factor is common to a row and changes none of them.
  * scale = m * rstd / 127.  A row with an infinity or a NaN, or whose sum of squares
- * passes fp32's largest value, or of zeros where eps is 0, has a scale of NaN. */
+ * passes fp32's largest value, or of zeros where eps is 0, has a scale of NaN.
+ * Without columns (K == 0) nothing is written. */
 int sgq_rms_norm_tokens(const void* x, int dtype, int64_t ldx, const void* residual, int64_t ldr, void* h, int64_t ldh,
                         const float* g, float eps, int64_t M, int64_t K, void* codes, int64_t ldc, float* scales,
                         void* stream);

@@ -265,9 +265,10 @@ bool rows_clash(const void* h, int64_t ldh, const void* x, int64_t ldx, int64_t 
 }
 int check_token_codes(const char* fn, const void* codes, int64_t ldc, int64_t K) {
     if (!codes || !aligned16(codes)) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: codes must be 16-byte aligned", fn);
-    if (ldc % 16 != 0 || ldc < round_up(K, kTokenPadK))
+    const int64_t row = sgq_tokens_row_bytes(K);
+    if (ldc % 16 != 0 || ldc < row)
         return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: rows of codes need a multiple of 16 bytes, at least %lld", fn,
-                    (long long)round_up(K, kTokenPadK));
+                    (long long)row);
     if (ldc > kMaxTokenStride)
         return fail(SGQ_ERR_UNSUPPORTED, "%s: rows of codes more than %lld bytes apart", fn, (long long)kMaxTokenStride);
     return SGQ_OK;
