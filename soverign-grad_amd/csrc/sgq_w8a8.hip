@@ -251,8 +251,9 @@ __global__ __launch_bounds__(64 * NW) void k_w8a8_few(const W8A8Args a, int mblo
         i32x4 x[U][MB], w[U][NG * C];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            // Past the last step and the last column block: zeros.  What a buffer checks is the
-            // lane's offset alone, so the column block is in it.
+            // Past the last step and the last column block: zeros.  The column block is in the
+            // lane's offset, which a buffer's check is sure to count (on this card it counts the
+            // scalar offset too).
             const int k = st + u * NW;
             const int wo = k < steps ? lane * 16 : kOobOff;
 #pragma unroll
