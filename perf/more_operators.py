@@ -204,7 +204,8 @@ def prepare(case, seed):
     s = {"case": c, "dtype": dtype, "lengths": lengths, "starts": starts, "table": table}
     s["k_cache"] = _normal(gen, pool, page, KV, d).to(dtype)
     s["v_cache"] = _normal(gen, pool, page, KV, d).to(dtype)
-    if own:
+    if own:  # a serving program makes them once, the batch for each step of all layers
+        s["kv"] = attention().PagedKV(s["k_cache"], s["v_cache"])
         s["batch"] = attention().SequenceBatch(table, _ints([n for _, n in lengths]), _ints(starts),
                                                max_len=max(n for _, n in lengths), max_new=c["new"])
     if c["kind"] == "append":
@@ -295,12 +296,11 @@ def run(state):
         return _plain_append(s) if c["kind"] == "append" else _plain_attend(s)
     op = attention()
     if c["kind"] == "append":
-        q = op.norm_rope_append(s["q"], s["k"], s["v"], s["k_cache"], s["v_cache"], s["batch"], freqs=s["freqs"],
-                                q_norm=s["q_norm"], k_norm=s["k_norm"], eps=EPS, interleaved=c["interleaved"])
+        q = op.norm_rope_append(s["q"], s["k"], s["v"], s["kv"], s["batch"], freqs=s["freqs"], q_norm=s["q_norm"],
+                                k_norm=s["k_norm"], eps=EPS, interleaved=c["interleaved"])
         return {"q": q, "k": s["k_cache"], "v": s["v_cache"]}
-    return op.paged_attention(s["q"], s["k_cache"], s["v_cache"], s["batch"], softcap=c["softcap"],
-                              alibi_slopes=s["slopes"], window=c["window"], prefix=s["prefix"],
-                              first_key=s["first_key"])
+    return op.paged_attention(s["q"], s["kv"], s["batch"], softcap=c["softcap"], alibi_slopes=s["slopes"],
+                              window=c["window"], prefix=s["prefix"], first_key=s["first_key"])
 
 
 # ---- what a pass cannot do without -----------------------------------------
