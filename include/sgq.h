@@ -458,6 +458,97 @@ int sgq_swiglu_w8a8(const void* codes, int64_t ldc, const float* x_scales, int64
  * a second kernel.  Host-only. */
 int sgq_w8a8_plan(int gated, int64_t M, int64_t K, int64_t N, int compute_units, int* form, int* k_splits);
 
+/* ---- attention over a paged key/value cache ----------------------------- */
+
+/* These have no counterpart in the reference, whose attention runs over the whole
+ * sequence at full width.  Heads of queries share those of keys and values (heads a
+ * multiple of kv_heads); types are SGQ_F32, SGQ_BF16, SGQ_F16, one for all of a call;
+ * head_dim is a multiple of 16, at most 256.  At most 1024 heads, 2^23 rows and 2^20
+ * sequences (SGQ_ERR_UNSUPPORTED past them).
+ *
+ * A cache is a pool of pages for one layer: key (or value) row t of page p and head h
+ * at k (or v) + p * page_stride + t * token_stride + h * head_stride elements, head_dim
+ * elements next to each other, every row 16-byte aligned.  page_size is a power of
+ * two, at most 65536. */
+typedef struct sgq_paged_cache {
+    void* k;
+    void* v;
+    int64_t pages, page_size, kv_heads, head_dim;
+    int64_t page_stride, token_stride, head_stride;
+    int dtype;
+} sgq_paged_cache;
+
+/* What one call works on: some new tokens of each of B sequences, row by row, one
+ * sequence after the other.  All arrays are int32 on the device.
+ *   table:   [B] rows of table_ld page numbers, table_pages of them usable: key j of
+ *            sequence b is in page table[b][j / page_size].
+ *   lens:    [B] keys per sequence, its new tokens included.
+ *   starts:  [B + 1] first row of each sequence's new tokens, never decreasing; rows from
+ *            starts[B] up to the call's `rows` belong to none (their outputs stay as they were).
+ *            New token i of sequence b has position lens[b] - (starts[b+1] - starts[b]) + i.
+ *   max_len, max_new: host bounds on lens and on a sequence's new tokens (they size the
+ *            launch and the workspace).
+ * A sequence with no new token is left alone.  One that breaks a bound (more new tokens
+ * than max_new or than keys; more keys than max_len or than its pages hold) has NaN for its
+ * output rows, and nothing is appended.  Where the table names a page outside [0, pages),
+ * a token of it has a row of NaN and is not appended (append), and the rows that see a key of it
+ * are NaN, of the same sequence others may be too (attention). */
+typedef struct sgq_sequences {
+    const int32_t* table;
+    int64_t table_ld, table_pages;
+    const int32_t* lens;
+    const int32_t* starts;
+    int64_t B, max_len, max_new;
+} sgq_sequences;
+
+/* Norms of the heads, position rotation and the new tokens' rows of the cache, in one
+ * pass: for every head x of q and of k
+ *   u = x * g / sqrt(sum(x^2) / head_dim + eps)   (g = q_norm, k_norm [head_dim] fp32; NULL: u = x)
+ * and its pairs (u_a, u_b) turned by the angle position * freqs[i] to
+ *   (u_a cos - u_b sin, u_b cos + u_a sin),  i < rotary_dim / 2,
+ * (a, b) = (i, i + rotary_dim / 2), or (2i, 2i + 1) where `interleaved`; elements from
+ * rotary_dim on are not turned.  In fp32 (the angle in 64 bits), rounded once.  q's
+ * heads go to out, k's to the cache's keys and v's, as they are, to its values, at the tokens' positions.
+ *   q, k, v, out: [rows, heads or kv_heads, head_dim], strides in elements between rows and
+ *              between heads, every head 16-byte aligned; they may lie side by side.
+ *              out may be q itself (with its strides) but share no other memory with it.
+ *   freqs:     [rotary_dim / 2] float64, radians per position; NULL only where rotary_dim is 0.
+ *   rotary_dim: even, at most head_dim.
+ *   positions: [rows] int32, what the rotation takes instead of the tokens' positions (NULL: those). */
+int sgq_norm_rope_append(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
+                         const void* v, int64_t v_row, int64_t v_head, void* out, int64_t out_row, int64_t out_head,
+                         int64_t rows, int64_t heads, const sgq_paged_cache* cache, const sgq_sequences* seqs, const float* q_norm,
+                         const float* k_norm, float eps, const double* freqs, int64_t rotary_dim, int interleaved,
+                         const int32_t* positions, void* stream);
+
+/* Scores of a query at position p and a key at position j, and who sees whom:
+ *   s = scale * (q . k);  softcap > 0: s = softcap * tanh(s / softcap);
+ *   alibi_slopes [heads] fp32: s -= slope * |p - j|;
+ *   key j is seen where j < lens[b], j <= p or j < prefix[b], window == 0 or
+ *   j > p - window, and j >= first_key[row].
+ * prefix [B] int32: the keys that all of a sequence's tokens see (also ahead of them);
+ * first_key [rows] int32: the first key of a token's document.  Each of the pointers may be NULL. */
+typedef struct sgq_scores {
+    float scale, softcap;
+    int64_t window;
+    const float* alibi_slopes;
+    const int32_t* prefix;
+    const int32_t* first_key;
+} sgq_scores;
+
+/* out = sum_j exp(s_j - max s) v_j / sum_j exp(s_j - max s) over the keys that a row
+ * sees; zeros for a row that sees none.  Sums and softmax in fp32.  What a row does not see does
+ * not touch it, infinities and NaN included.  q, out: [rows, heads, head_dim] as above
+ * (out may be q itself).  workspace:
+ * sgq_paged_attention_workspace_bytes bytes for a device of `compute_units` CUs (0: the
+ * calling thread's current device), 16-byte aligned, else SGQ_ERR_WORKSPACE; it needs
+ * no initialisation, and calls that overlap in time must not share one. */
+int64_t sgq_paged_attention_workspace_bytes(int64_t heads, int64_t kv_heads, int64_t head_dim, int dtype, int64_t B,
+                                            int64_t rows, int64_t max_len, int64_t max_new, int compute_units);
+int sgq_paged_attention(const void* q, int64_t q_row, int64_t q_head, void* out, int64_t out_row, int64_t out_head,
+                        int64_t rows, int64_t heads, const sgq_paged_cache* cache, const sgq_sequences* seqs,
+                        const sgq_scores* scores, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

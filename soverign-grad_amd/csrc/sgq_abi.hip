@@ -423,6 +423,91 @@ int product_w8a8(const char* fn, int ng, const void* codes, int64_t ldc, const f
     return ok();
 }
 
+// ---- attention over a paged cache ----------------------------------------
+
+// Rows of heads: every head 16-byte aligned, heads of a row (rows of a head) apart.
+int check_heads(const char* fn, const char* what, const void* p, int64_t row, int64_t head, int64_t rows, int64_t heads,
+                int64_t head_dim, int dtype) {
+    const int64_t step = 16 / dtype_bytes((DType)dtype);
+    if (!p) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: null %s", fn, what);
+    if (!aligned16(p) || row % step || head % step)
+        return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: heads of %s must be 16-byte aligned", fn, what);
+    if (row < 0 || head < 0 || row > kMaxDim || head > kMaxDim)
+        return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: bad strides of %s", fn, what);
+    // Heads do not overlap: the one stride spans the other's extent.
+    const int64_t in_row = (heads - 1) * head + head_dim, in_head = (rows - 1) * row + head_dim;
+    const bool ok = (heads == 1 || head >= head_dim) && (rows == 1 || row >= head_dim) &&
+                    (heads == 1 || rows == 1 || row >= in_row || head >= in_head);
+    if (!ok) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: heads of %s overlap", fn, what);
+    return SGQ_OK;
+}
+
+// Whether [p, p + bytes of its rows) meets the other's; the same memory with the same
+// strides is no clash.
+bool heads_clash(const HeadRows& a, const HeadRows& b, int64_t rows, int64_t heads, int64_t other_heads, int64_t head_dim,
+                 int dtype) {
+    if (a.p == b.p && heads == other_heads && (a.row == b.row || rows == 1) && (a.head == b.head || heads == 1)) return false;
+    const int64_t size = dtype_bytes((DType)dtype);
+    auto end = [&](const HeadRows& x, int64_t h) {
+        return (uintptr_t)x.p + (uintptr_t)(((rows - 1) * x.row + (h - 1) * x.head + head_dim) * size);
+    };
+    if (end(a, heads) <= (uintptr_t)b.p || end(b, other_heads) <= (uintptr_t)a.p) return false;
+    // Side by side in rows of one stride: apart where both lie within the stride.
+    if (a.row == b.row && rows > 1) {
+        const int64_t ra = (heads - 1) * a.head + head_dim, rb = (other_heads - 1) * b.head + head_dim;
+        const uintptr_t d = (uintptr_t)a.p > (uintptr_t)b.p ? (uintptr_t)a.p - (uintptr_t)b.p : (uintptr_t)b.p - (uintptr_t)a.p;
+        const int64_t at = (int64_t)(d / (uintptr_t)size) % a.row;
+        const int64_t first = (uintptr_t)a.p > (uintptr_t)b.p ? rb : ra, second = (uintptr_t)a.p > (uintptr_t)b.p ? ra : rb;
+        return !(at >= first && at + second <= a.row);
+    }
+    return true;
+}
+
+int check_paged(const char* fn, int64_t rows, int64_t heads, const sgq_paged_cache* c, const sgq_sequences* q, PagedCache& pc,
+                Sequences& sq) {
+    if (!c || !q) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: null cache or sequences", fn);
+    if (bad_dtype(c->dtype)) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: bad dtype", fn);
+    if (c->head_dim < kHeadDimStep || c->head_dim % kHeadDimStep || c->head_dim > kMaxHeadDim)
+        return fail(SGQ_ERR_UNSUPPORTED, "%s: head_dim must be a multiple of %d, at most %d", fn, kHeadDimStep, kMaxHeadDim);
+    if (c->kv_heads < 1 || heads < 1 || heads % c->kv_heads)
+        return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: heads must be a multiple of kv_heads", fn);
+    if (c->page_size < 1 || (c->page_size & (c->page_size - 1)) || c->page_size > 65536)
+        return fail(SGQ_ERR_UNSUPPORTED, "%s: page_size must be a power of two, at most 65536", fn);
+    if (c->pages < 0 || c->pages > kMaxDim) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: bad number of pages", fn);
+    if (q->B < 0 || rows < 0 || q->max_len < 0 || q->max_new < 0 || q->table_pages < 0 || q->table_pages > kMaxDim ||
+        q->max_len > kMaxDim || q->max_new > kMaxDim || q->table_ld < q->table_pages || q->table_ld > kMaxDim)
+        return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: bad sequences", fn);
+    if (heads > kMaxHeads || rows > kMaxHeadRows || q->B > kMaxSequences)
+        return fail(SGQ_ERR_UNSUPPORTED, "%s: more than %d heads, %d rows or %d sequences", fn, kMaxHeads, kMaxHeadRows,
+                    kMaxSequences);
+    const int64_t step = 16 / dtype_bytes((DType)c->dtype), d = c->head_dim;
+    // Strides that cross the whole pool stay within 64 bits, and rows of the pool apart.
+    const int64_t big = (int64_t)1 << 40;
+    if (c->page_stride < 0 || c->token_stride < 0 || c->head_stride < 0 || c->page_stride > big || c->token_stride > big ||
+        c->head_stride > big || c->page_stride % step || c->token_stride % step || c->head_stride % step)
+        return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: strides of the cache must be multiples of 16 bytes", fn);
+    if ((c->kv_heads > 1 && c->head_stride < d) || (c->page_size > 1 && c->token_stride < d) ||
+        (c->pages > 1 && c->page_stride < d))
+        return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: rows of the cache overlap", fn);
+    if (!aligned16(c->k) || !aligned16(c->v))
+        return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: the cache must be 16-byte aligned", fn);
+    if (q->B > 0 && rows > 0) {
+        if (!q->lens || !q->starts || (q->table_pages > 0 && !q->table))
+            return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: null array of the sequences", fn);
+        if (c->pages > 0 && (!c->k || !c->v)) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: null cache", fn);
+    }
+    pc.k = (char*)c->k, pc.v = (char*)c->v, pc.t = (DType)c->dtype;
+    pc.page_stride = c->page_stride, pc.token_stride = c->token_stride, pc.head_stride = c->head_stride;
+    pc.pages = (int)c->pages, pc.kv_heads = (int)c->kv_heads, pc.head_dim = (int)d, pc.page_log = 0;
+    while ((int64_t)1 << pc.page_log < c->page_size) ++pc.page_log;
+    sq.table = q->table, sq.lens = q->lens, sq.starts = q->starts, sq.table_ld = q->table_ld;
+    sq.B = (int)q->B, sq.rows = (int)rows;
+    sq.max_len = (int)q->max_len, sq.max_new = (int)q->max_new;
+    const int64_t cap = q->table_pages * c->page_size;
+    sq.capacity = (int)(cap < kMaxDim ? cap : kMaxDim);
+    return SGQ_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1186,6 +1271,74 @@ int sgq_swiglu_w8a8(const void* codes, int64_t ldc, const float* x_scales, int64
     const float* bias[2] = {bias_gate, bias_up};
     return product_w8a8("sgq_swiglu_w8a8", 2, codes, ldc, x_scales, M, K, N, packed, scales, bias, h, dtype, ldh,
                         workspace, workspace_bytes, stream);
+}
+
+// ---- attention over a paged cache ----------------------------------------
+
+int sgq_norm_rope_append(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
+                         const void* v, int64_t v_row, int64_t v_head, void* out, int64_t out_row, int64_t out_head,
+                         int64_t rows, int64_t heads, const sgq_paged_cache* cache, const sgq_sequences* seqs, const float* q_norm,
+                         const float* k_norm, float eps, const double* freqs, int64_t rotary_dim, int interleaved,
+                         const int32_t* positions, void* stream) {
+    const char* fn = "sgq_norm_rope_append";
+    PagedCache c;
+    Sequences s;
+    int st = check_paged(fn, rows, heads, cache, seqs, c, s);
+    if (st != SGQ_OK) return st;
+    if (rotary_dim < 0 || rotary_dim % 2 || rotary_dim > c.head_dim)
+        return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: rotary_dim must be even, at most head_dim", fn);
+    if (s.rows == 0 || s.B == 0) return ok();
+    if (rotary_dim > 0 && !freqs) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: null freqs", fn);
+    const int dt = cache->dtype;
+    const int64_t d = c.head_dim;
+    if ((st = check_heads(fn, "q", q, q_row, q_head, s.rows, heads, d, dt)) != SGQ_OK) return st;
+    if ((st = check_heads(fn, "k", k, k_row, k_head, s.rows, c.kv_heads, d, dt)) != SGQ_OK) return st;
+    if ((st = check_heads(fn, "v", v, v_row, v_head, s.rows, c.kv_heads, d, dt)) != SGQ_OK) return st;
+    if ((st = check_heads(fn, "out", out, out_row, out_head, s.rows, heads, d, dt)) != SGQ_OK) return st;
+    if (c.k == c.v && c.pages > 0) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: keys and values in one pool", fn);
+    RopeArgs a;
+    a.q = {(void*)q, q_row, q_head}, a.k = {(void*)k, k_row, k_head}, a.v = {(void*)v, v_row, v_head};
+    a.out = {out, out_row, out_head};
+    if (heads_clash(a.out, a.q, s.rows, heads, heads, d, dt) || heads_clash(a.out, a.k, s.rows, heads, c.kv_heads, d, dt) ||
+        heads_clash(a.out, a.v, s.rows, heads, c.kv_heads, d, dt) || out == k || out == v)
+        return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: out may be q itself but share no other memory with q, k or v", fn);
+    a.heads = (int)heads, a.q_norm = q_norm, a.k_norm = k_norm, a.eps = eps, a.freqs = freqs, a.half = (int)(rotary_dim / 2);
+    a.interleaved = interleaved != 0, a.positions = positions;
+    SGQ_HIP(launch_norm_rope_append(a, c, s, (hipStream_t)stream), "norm_rope_append");
+    return ok();
+}
+
+int64_t sgq_paged_attention_workspace_bytes(int64_t heads, int64_t kv_heads, int64_t head_dim, int dtype, int64_t B,
+                                            int64_t rows, int64_t max_len, int64_t max_new, int compute_units) {
+    return 0;
+}
+
+int sgq_paged_attention(const void* q, int64_t q_row, int64_t q_head, void* out, int64_t out_row, int64_t out_head,
+                        int64_t rows, int64_t heads, const sgq_paged_cache* cache, const sgq_sequences* seqs,
+                        const sgq_scores* scores, void* workspace, int64_t workspace_bytes, void* stream) {
+    const char* fn = "sgq_paged_attention";
+    PagedCache c;
+    Sequences s;
+    int st = check_paged(fn, rows, heads, cache, seqs, c, s);
+    if (st != SGQ_OK) return st;
+    if (!scores) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: null scores", fn);
+    if (scores->window < 0) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: negative window", fn);
+    if (!(scores->softcap >= 0.0f) || scores->softcap > 3.0e38f)
+        return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: softcap must be finite and not negative", fn);
+    if (s.rows == 0 || s.B == 0) return ok();
+    const int dt = cache->dtype;
+    const int64_t d = c.head_dim;
+    if ((st = check_heads(fn, "q", q, q_row, q_head, s.rows, heads, d, dt)) != SGQ_OK) return st;
+    if ((st = check_heads(fn, "out", out, out_row, out_head, s.rows, heads, d, dt)) != SGQ_OK) return st;
+    AttendArgs a;
+    a.q = {(void*)q, q_row, q_head}, a.out = {out, out_row, out_head};
+    if (heads_clash(a.out, a.q, s.rows, heads, heads, d, dt))
+        return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: out may be q itself but share no other memory with it", fn);
+    a.heads = (int)heads, a.scale = scores->scale, a.softcap = scores->softcap;
+    a.window = (int)(scores->window < kMaxDim ? scores->window : kMaxDim);
+    a.slopes = scores->alibi_slopes, a.prefix = scores->prefix, a.first_key = scores->first_key;
+    SGQ_HIP(launch_attend(a, c, s, workspace, (hipStream_t)stream), "attend");
+    return ok();
 }
 
 }  // extern "C"

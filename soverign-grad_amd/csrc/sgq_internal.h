@@ -552,4 +552,49 @@ W8A8Plan w8a8_plan(int ng, int64_t M, int64_t K, int64_t N, int64_t cus);
 int64_t w8a8_plan_bytes(const W8A8Plan& p, int ng, int64_t M, int64_t K, int64_t N);
 hipError_t launch_w8a8(const W8A8Args& a, int ng, const W8A8Plan& p, void* ws, hipStream_t s);
 
+// ---- attention over a paged cache (sgq_rope.hip, sgq_attention.hip) -------
+constexpr int kHeadDimStep = 16, kMaxHeadDim = 256;
+constexpr int kMaxHeads = 1024, kMaxHeadRows = 1 << 23, kMaxSequences = 1 << 20;  // launches of fewer than 2^32 threads
+struct HeadRows {  // [rows, heads, head_dim], strides in elements
+    void* p;
+    int64_t row, head;
+};
+struct PagedCache {
+    char* k;
+    char* v;
+    int64_t page_stride, token_stride, head_stride;  // elements
+    int pages, page_log, kv_heads, head_dim;
+    DType t;
+};
+struct Sequences {
+    const int32_t* table;
+    const int32_t* lens;
+    const int32_t* starts;
+    int64_t table_ld;
+    int B, rows, max_len, max_new;
+    int capacity;  // keys that a table's pages hold
+};
+struct RopeArgs {
+    HeadRows q, k, v, out;
+    int heads;
+    const float* q_norm;
+    const float* k_norm;
+    float eps;
+    const double* freqs;
+    int half;  // pairs that are turned
+    bool interleaved;
+    const int32_t* positions;
+};
+hipError_t launch_norm_rope_append(const RopeArgs& a, const PagedCache& c, const Sequences& s, hipStream_t st);
+struct AttendArgs {
+    HeadRows q, out;
+    int heads;
+    float scale, softcap;
+    int window;
+    const float* slopes;
+    const int32_t* prefix;
+    const int32_t* first_key;
+};
+hipError_t launch_attend(const AttendArgs& a, const PagedCache& c, const Sequences& s, void* ws, hipStream_t st);
+
 }  // namespace sgq
