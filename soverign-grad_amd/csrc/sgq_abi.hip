@@ -463,6 +463,13 @@ bool heads_clash(const HeadRows& a, const HeadRows& b, int64_t rows, int64_t hea
     return true;
 }
 
+bool bad_attention(int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t B, int64_t rows, int64_t max_len,
+                   int64_t max_new) {
+    return kv_heads < 1 || heads < 1 || heads > kMaxHeads || heads % kv_heads || head_dim < kHeadDimStep ||
+           head_dim % kHeadDimStep || head_dim > kMaxHeadDim || B < 0 || B > kMaxSequences || rows < 0 ||
+           rows > kMaxHeadRows || max_len < 0 || max_len > kMaxDim || max_new < 0 || max_new > kMaxDim;
+}
+
 int check_paged(const char* fn, int64_t rows, int64_t heads, const sgq_paged_cache* c, const sgq_sequences* q, PagedCache& pc,
                 Sequences& sq) {
     if (!c || !q) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: null cache or sequences", fn);
@@ -1310,7 +1317,10 @@ int sgq_norm_rope_append(const void* q, int64_t q_row, int64_t q_head, const voi
 
 int64_t sgq_paged_attention_workspace_bytes(int64_t heads, int64_t kv_heads, int64_t head_dim, int dtype, int64_t B,
                                             int64_t rows, int64_t max_len, int64_t max_new, int compute_units) {
-    return 0;
+    if (bad_dtype(dtype) || bad_attention(heads, kv_heads, head_dim, B, rows, max_len, max_new) || compute_units < 0) return -1;
+    if (B == 0 || rows == 0) return 0;
+    const AttendShape q = {heads, kv_heads, head_dim, B, rows, max_len, max_new, (DType)dtype};
+    return attend_plan_bytes(attend_plan(q, compute_units > 0 ? compute_units : device_cus(nullptr)), q);
 }
 
 int sgq_paged_attention(const void* q, int64_t q_row, int64_t q_head, void* out, int64_t out_row, int64_t out_head,
@@ -1323,6 +1333,8 @@ int sgq_paged_attention(const void* q, int64_t q_row, int64_t q_head, void* out,
     if (st != SGQ_OK) return st;
     if (!scores) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: null scores", fn);
     if (scores->window < 0) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: negative window", fn);
+    if (!(scores->scale >= -3.0e38f && scores->scale <= 3.0e38f))
+        return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: scale must be finite", fn);
     if (!(scores->softcap >= 0.0f) || scores->softcap > 3.0e38f)
         return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: softcap must be finite and not negative", fn);
     if (s.rows == 0 || s.B == 0) return ok();
@@ -1337,7 +1349,14 @@ int sgq_paged_attention(const void* q, int64_t q_row, int64_t q_head, void* out,
     a.heads = (int)heads, a.scale = scores->scale, a.softcap = scores->softcap;
     a.window = (int)(scores->window < kMaxDim ? scores->window : kMaxDim);
     a.slopes = scores->alibi_slopes, a.prefix = scores->prefix, a.first_key = scores->first_key;
-    SGQ_HIP(launch_attend(a, c, s, workspace, (hipStream_t)stream), "attend");
+    const AttendShape shape = {heads, c.kv_heads, d, s.B, s.rows, s.max_len, s.max_new, c.t};
+    const AttendPlan p = attend_plan(shape, device_cus((hipStream_t)stream));
+    if (p.workgroups * 256 >= (int64_t)1 << 32 || (p.splits > 1 && (int64_t)s.rows * heads * 256 >= (int64_t)1 << 32))
+        return fail(SGQ_ERR_UNSUPPORTED, "%s: too many rows for one call", fn);
+    const int64_t need = attend_plan_bytes(p, shape);
+    if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+        return fail(SGQ_ERR_WORKSPACE, "%s: workspace needs %lld bytes, 16-byte aligned", fn, (long long)need);
+    SGQ_HIP(launch_attend(a, c, s, p, workspace, (hipStream_t)stream), "attend");
     return ok();
 }
 

@@ -1,85 +1,831 @@
-// sgq_attention.hip -- attention of new tokens over a paged key/value cache.
+// sgq_attention.hip -- attention of new tokens over a paged key/value cache, for gfx950.
 //
 // Mathematics.  Row i of a sequence (position p) sees the keys of one interval [lo, hi)
 // (causal, window, document start, prefix); with s_j its scores
 //   out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),  m = max_j s_j,
 // in one pass over the keys with a running maximum: when it grows from m to m', what
-// was summed is multiplied by exp(m - m').  All of it in fp32.
+// was summed is multiplied by exp(m - m').  Ranges of keys that different workgroups (or
+// wavefronts) took are joined the same way.  Scores, softmax and sums are fp32; in
+// 16-bit types a weight is rounded to the type before its product with v, for the matrix
+// instruction takes it so (half a step of each weight, while the sum of weights keeps them
+// unrounded); fp32 stays fp32 throughout.
+//
+// Matrix layout.  A wavefront owns 32 rows (a row: a new token and one of the heads that
+// share a kv head, heads next to each other) and computes transposed: S^T = K Q^T and O^T =
+// V^T P^T with 32 x 32 products.  Column = row of the batch = lane & 31, so a row's
+// maximum, sum and factor are one register of a lane, and the only exchange is with lane ^ 32,
+// which has the other half of the keys.  The result registers of S^T are, in order, the
+// B operand of the second product, if the k slots of that product are the keys in the order
+// that the registers hold them: lane half h has keys 8 a + 4 h + 0..3 of each 32, and the A
+// operand V^T is read in the same order.
+//   16 bits: 32x32x16; K rows as 16-byte LDS reads, V^T by transposing 8-byte LDS reads
+//   (four keys of a column a lane).
+//   fp32: 32x32x2; a 16-byte read of K serves four products; V^T a float a lane.
+// Keys and values go from their pages to LDS directly (a lane's address is its row's page),
+// the 16-byte chunks of a row permuted so that all reads are free of conflicts.
 #include "sgq_paged.h"
+
+#include <algorithm>
 
 namespace sgq {
 namespace {
 
 constexpr float kLog2e = 1.44269504f;
 
-// The keys [lo, hi) that a row sees.
-__device__ __forceinline__ void row_keys(const AttendArgs& a, const SeqRows& r, int b, int row, int& lo, int& hi) {
-    const int p = r.position(row);
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(1))) const void global_void;
+
+// Sixteen bytes that a lane without a row of its own reads: zeros.
+__device__ const uint32_t g_zeros[4] = {0, 0, 0, 0};
+
+template <typename T>
+struct Mat;
+template <>
+struct Mat<__bf16> {
+    typedef b16x8 Frag;
+    static constexpr int kStep = 16;  // head elements of a fragment, both lane halves together
+    static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+};
+template <>
+struct Mat<_Float16> {
+    typedef h16x8 Frag;
+    static constexpr int kStep = 16;
+    static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+};
+template <>
+struct Mat<float> {
+    typedef f32x4 Frag;
+    static constexpr int kStep = 8;
+    static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+        return c;
+    }
+};
+
+constexpr int pow2_from(int v) {
+    int p = 1;
+    while (p < v) p *= 2;
+    return p;
+}
+
+// A tile of keys (or values) in LDS: rows of kRow bytes, chunk c of row r at position c ^ mix(r).
+template <typename T, int DP>
+struct TileRows {
+    static constexpr int kRow = pow2_from(DP * (int)sizeof(T));
+    static constexpr int kChunks = kRow / 16;
+    // 16 bits: sixteen neighbouring rows have their chunk c in sixteen places of 256 bytes (K),
+    // four neighbouring rows their 64 bytes in four places (V).  fp32: sixteen rows likewise,
+    // rows four apart their 128 bytes in two places.
+    static __device__ __forceinline__ int mix(int r) {
+        if constexpr (sizeof(T) == 4) return ((r & 4) << 1) | ((r & 3) << 1) | ((r >> 3) & 1);
+        if constexpr (kChunks == 8) return ((r & 2) << 1) | ((r >> 2) & 3);
+        return ((r & 3) << 2) | ((r >> 2) & 3);
+    }
+};
+
+// The keys [lo, hi) that a row at position p sees.
+__device__ __forceinline__ void row_keys(const AttendArgs& a, const SeqRows& r, int b, int row, int p, int& lo, int& hi) {
     lo = a.first_key ? max(a.first_key[row], 0) : 0;
     if (a.window > 0) lo = max(lo, p - a.window + 1);
     hi = p + 1;
     if (a.prefix) hi = max(hi, min(a.prefix[b], r.len));
 }
 
-// A wavefront per row and head, a key at a time.
+__device__ __forceinline__ float other_half(float v, bool take_max) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    const float x = __uint_as_float(r[0]), y = __uint_as_float(r[1]);
+    return take_max ? fmaxf(x, y) : x + y;
+}
+
+__device__ __forceinline__ int wave_min(int v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
+    return v;
+}
+__device__ __forceinline__ int wave_max(int v) { return -wave_min(-v); }
+
+// How scores become weights, the same for all of a launch.
+struct Score {
+    float c;         // exponent of 2 per raw score (without a cap)
+    float in, out;   // cap: 2^ of out * tanh(in * raw)
+    bool negate;     // scale < 0: the queries are negated instead
+    bool capped;
+    __device__ __forceinline__ explicit Score(const AttendArgs& a) {
+        negate = a.scale < 0.0f;
+        capped = a.softcap > 0.0f;
+        in = capped ? fabsf(a.scale) / a.softcap : 0.0f;
+        out = a.softcap * kLog2e;
+        // Never zero: a hidden score is -inf, and has to stay that.
+        c = fmaxf(fabsf(a.scale) * kLog2e, 1.17549435e-38f);
+    }
+};
+
+// A wavefront's 32 rows on tiles of 32 NK keys.
+template <typename T, int DP, int NK>
+struct Rows {
+    typedef Mat<T> M;
+    typedef typename M::Frag Frag;
+    typedef TileRows<T, DP> Tile;
+    static constexpr int kFrags = DP / M::kStep, kCols = DP / 32;
+
+    Frag q[kFrags];
+    f32x16 o[kCols];
+    float m, l;            // maximum of the scores (as c multiplies them), this half's sum of weights
+    int lo, hi, pos;       // the row's keys and position
+    float slope;           // times log2 e
+    int max_lo, min_hi, min_lo, max_hi;  // over the wavefront's rows
+
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < kCols; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
+        m = -INFINITY, l = 0.0f;
+    }
+    // Elements kStep i + (kStep / 2) half + 0 .. of the row's query, zeros from d on.
+    __device__ __forceinline__ void load(const T* p, int d, bool negate) {
+        const int h = (threadIdx.x & 63) >> 5;
+#pragma unroll
+        for (int i = 0; i < kFrags; ++i) {
+            const int e = i * M::kStep + h * (M::kStep / 2);
+            Frag f = {};
+            if (e < d) f = *(const Frag*)(p + e);
+            q[i] = negate ? -f : f;
+        }
+    }
+    __device__ __forceinline__ void bounds() {
+        max_lo = wave_max(lo), min_hi = wave_min(hi);
+        min_lo = wave_min(lo), max_hi = wave_max(hi);
+    }
+
+    // Keys k0 .. k0 + 32 NK - 1 in the tiles ks and vs.  careful: values that are not finite touch
+    // only the rows that see them.
+    template <bool CAREFUL>
+    __device__ __forceinline__ void step(const char* ks, const char* vs, int k0, const Score& sc) {
+        const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
+        f32x16 s[NK];
+        {
+            const int x = (h ^ Tile::mix(n)) << 4;  // chunk 2 i + h of row n (mix has the period of 16 rows)
+            const char* row = ks + n * Tile::kRow;
+#pragma unroll
+            for (int t = 0; t < NK; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[t][e] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kFrags; ++i)
+#pragma unroll
+                for (int t = 0; t < NK; ++t)
+                    s[t] = M::mma(*(const Frag*)(row + t * 32 * Tile::kRow + ((i * 32) ^ x)), q[i], s[t]);
+        }
+        // Key of register e of tile t: k0 + 32 t + 8 (e / 4) + 4 h + e % 4.
+        const int kb = k0 + 4 * h;
+        float c = sc.c;
+        if (sc.capped || slope != 0.0f) {
+            c = 1.0f;
+#pragma unroll
+            for (int t = 0; t < NK; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    float v = s[t][e];
+                    if (sc.capped) {
+                        if constexpr (sizeof(T) == 4) {
+                            v = sc.out * tanhf(v * sc.in);
+                        } else {
+                            // tanh x = 1 - 2 / (1 + e^2x): off by some 2^-23, which a 16-bit weight does not see.
+                            const float u = __builtin_amdgcn_exp2f(v * (2.0f * kLog2e * sc.in));
+                            v = fmaf(sc.out * -2.0f, __builtin_amdgcn_rcpf(1.0f + u), sc.out);
+                        }
+                    } else {
+                        v *= sc.c;
+                    }
+                    const int away = pos - (kb + 32 * t + 8 * (e / 4) + e % 4);
+                    s[t][e] = fmaf(-slope, (float)abs(away), v);
+                }
+        }
+        const bool part = k0 < max_lo || k0 + 32 * NK > min_hi;  // some row does not see some key
+        if (part) {
+            const unsigned width = (unsigned)max(hi - lo, 0);
+#pragma unroll
+            for (int t = 0; t < NK; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if ((unsigned)(kb + 32 * t + 8 * (e / 4) + e % 4 - lo) >= width) s[t][e] = -INFINITY;
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int t = 0; t < NK; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) top = fmaxf(top, s[t][e]);
+        top = other_half(top, true);
+        // The factor of what was summed is due only where a maximum grew by more than 2^8: until
+        // then weights are up to 2^8 and sums as exact as before.
+        if (__any((top - m) * c > 8.0f)) {
+            const float now = fmaxf(m, top);
+            const float w = __builtin_amdgcn_exp2f((m - (now == -INFINITY ? 0.0f : now)) * c);
+            m = now;
+            l *= w;
+#pragma unroll
+            for (int i = 0; i < kCols; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[i][e] *= w;
+        }
+        const float base = m == -INFINITY ? 0.0f : -m * c;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int t = 0; t < NK; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                s[t][e] = __builtin_amdgcn_exp2f(fmaf(s[t][e], c, base));
+                sum[e & 3] += s[t][e];
+            }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if (CAREFUL && part)
+            values<true>(vs, s);
+        else
+            values<false>(vs, s);
+    }
+
+    // O^T += V^T P^T.
+    template <bool CAREFUL>
+    __device__ __forceinline__ void values(const char* vs, const f32x16 (&s)[NK]) {
+        const int lane = threadIdx.x & 63, h = lane >> 5;
+        if constexpr (sizeof(T) == 2) {
+            // A 16-lane group reads four keys of sixteen columns, a lane eight bytes of them.
+            const int i = lane & 15, r0 = 4 * h + (i >> 2);
+            const int x = ((2 * ((lane >> 4) & 1) + ((i >> 1) & 1)) ^ Tile::mix(r0)) << 4;
+            const char* row = vs + r0 * Tile::kRow + 8 * (i & 1);
+            // mix of a row eight further: two chunks on where rows hold sixteen chunks or more, for
+            // eight it is (r >> 2) & 3 likewise.
+            constexpr int kNext = 2 << 4;
+#pragma unroll
+            for (int t = 0; t < NK; ++t)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    Frag p;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) p[e] = (T)s[t][8 * u + e];
+#pragma unroll
+                    for (int cidx = 0; cidx < kCols; ++cidx) {
+                        const char* at = row + (t * 32 + u * 16) * Tile::kRow;
+                        const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + ((cidx * 64) ^ x)));
+                        const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (lds_s16x4*)(at + 8 * Tile::kRow + ((cidx * 64) ^ x ^ kNext)));
+                        const Frag v = __builtin_bit_cast(Frag, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+                        product<CAREFUL>(o[cidx], v, p);
+                    }
+                }
+        } else {
+            const int n = lane & 31;
+#pragma unroll
+            for (int t = 0; t < NK; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int r = t * 32 + 8 * (e / 4) + 4 * h + e % 4;
+                    const char* row = vs + r * Tile::kRow + 4 * (n & 3);
+                    const int x = ((n >> 2) ^ Tile::mix(r)) << 4;
+#pragma unroll
+                    for (int cidx = 0; cidx < kCols; ++cidx)
+                        product<CAREFUL>(o[cidx], *(const float*)(row + ((cidx * 128) ^ x)), s[t][e]);
+                }
+        }
+    }
+    static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) { return M::mma(a, b, c); }
+    static __device__ __forceinline__ f32x16 mma(float a, float b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ float each(float v, float (*f)(float)) { return f(v); }
+    static __device__ __forceinline__ Frag each(Frag v, float (*f)(float)) {
+        Frag r;
+#pragma unroll
+        for (int e = 0; e < (int)(sizeof(Frag) / sizeof(T)); ++e) r[e] = (T)f((float)v[e]);
+        return r;
+    }
+    // CAREFUL: 0 * infinity is NaN, so values that are not finite take no part in the product; the weights
+    // that rows give them are summed apart, and where that is not zero the column becomes what it has to.
+    template <bool CAREFUL, typename A>
+    static __device__ __forceinline__ void product(f32x16& acc, A v, A p) {
+        if constexpr (!CAREFUL) {
+            acc = mma(v, p, acc);
+        } else {
+            acc = mma(each(v, [](float x) { return isfinite(x) ? x : 0.0f; }), p, acc);
+            const f32x16 none = {};
+            const f32x16 up = mma(each(v, [](float x) { return x == INFINITY ? 1.0f : 0.0f; }), p, none);
+            const f32x16 down = mma(each(v, [](float x) { return x == -INFINITY ? 1.0f : 0.0f; }), p, none);
+            const f32x16 nan = mma(each(v, [](float x) { return x != x ? 1.0f : 0.0f; }), p, none);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                if (up[e] > 0.0f) acc[e] += INFINITY;
+                if (down[e] > 0.0f) acc[e] -= INFINITY;
+                if (nan[e] > 0.0f) acc[e] = NAN;
+            }
+        }
+    }
+    // Whether a column below d of the row is not finite.
+    __device__ __forceinline__ bool not_finite(int d) const {
+        const int h = (threadIdx.x & 63) >> 5;
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < kCols; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                if (32 * i + 8 * (e / 4) + 4 * h < d) bad = bad || !isfinite(o[i][e]);
+        return bad;
+    }
+    // The row's columns times w, as T, 16 bytes a store.
+    __device__ __forceinline__ void store(T* out, int d, float w) const {
+        const int h = (threadIdx.x & 63) >> 5;
+        if constexpr (sizeof(T) == 4) {
+            store_f32(out, d, w);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kCols; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; e += 8) {
+                    typedef T T4 __attribute__((ext_vector_type(4)));
+                    typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+                    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+                    T4 a, b;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) a[j] = (T)(o[i][e + j] * w), b[j] = (T)(o[i][e + 4 + j] * w);
+                    const u32x2 ua = __builtin_bit_cast(u32x2, a), ub = __builtin_bit_cast(u32x2, b);
+                    // Columns 0-3 | 4-7 and 8-11 | 12-15 of the halves: the lower lane takes 0-7, the upper 8-15.
+                    const auto x = __builtin_amdgcn_permlane32_swap(ua[0], ub[0], false, false);
+                    const auto y = __builtin_amdgcn_permlane32_swap(ua[1], ub[1], false, false);
+                    const int col = 32 * i + 2 * e + 8 * h;
+                    if (out && col < d) *(u32x4*)(out + col) = u32x4{x[0], y[0], x[1], y[1]};
+                }
+        }
+    }
+    // As fp32 (out null: no store, but all lanes come along).
+    __device__ __forceinline__ void store_f32(float* out, int d, float w) const {
+        const int h = (threadIdx.x & 63) >> 5;
+#pragma unroll
+        for (int i = 0; i < kCols; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int col = 32 * i + 2 * e + 4 * h;
+                if (out && col < d)
+                    *(f32x4*)(out + col) = f32x4{o[i][e] * w, o[i][e + 1] * w, o[i][e + 2] * w, o[i][e + 3] * w};
+            }
+    }
+};
+
+// Loads tiles of KEYS keys and their values: 16 bytes a lane, straight to LDS.  THREADS
+// threads (whole wavefronts) share a tile.  The pages of a tile are looked up ahead (pages), used by load.
+template <typename T, int DP, int KEYS, int THREADS>
+struct Loader {
+    typedef TileRows<T, DP> Tile;
+    static constexpr int kLoads = KEYS * Tile::kChunks / THREADS;  // of keys, and of values, a lane
+    static constexpr int kRowsApart = THREADS / Tile::kChunks;     // rows between a lane's loads
+    static constexpr int kBytes = KEYS * Tile::kRow;
+    static_assert(THREADS % Tile::kChunks == 0 && KEYS * Tile::kChunks % THREADS == 0, "");
+
+    const PagedCache* c;
+    const int32_t* table;
+    int64_t k_base, v_less_k;
+    int row;        // of the lane's first load
+    int chunk_off;  // bytes; negative: past the head
+    int page[kLoads];
+    bool bad = false;
+
+    __device__ __forceinline__ Loader(const PagedCache& cache, const int32_t* t, int kvh, int thread) {
+        c = &cache, table = t;
+        k_base = (int64_t)cache.k + (int64_t)kvh * cache.head_stride * (int)sizeof(T);
+        v_less_k = (int64_t)cache.v - (int64_t)cache.k;
+        row = thread / Tile::kChunks;
+    }
+    __device__ __forceinline__ int key(int i, int k0, int end) const { return min(k0 + row + i * kRowsApart, end - 1); }
+    // Pages of the keys from k0 on; keys from `end` on are the one before it.
+    __device__ __forceinline__ void pages(int k0, int end) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) page[i] = table[key(i, k0, end) >> c->page_log];
+    }
+    __device__ __forceinline__ void load(char* ks, char* vs, int k0, int end, int thread) {
+        const int mask = (1 << c->page_log) - 1;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int r = row + i * kRowsApart;
+            const int chunk = (thread & (Tile::kChunks - 1)) ^ Tile::mix(r);
+            const bool named = (unsigned)page[i] < (unsigned)c->pages;
+            bad = bad || !named;
+            const bool on = named && chunk * Chunk<T>::N < c->head_dim;
+            const int64_t off = ((int64_t)page[i] * c->page_stride + (int64_t)(key(i, k0, end) & mask) * c->token_stride) *
+                                    (int)sizeof(T) + chunk * 16;
+            const int64_t ka = on ? k_base + off : (int64_t)g_zeros;
+            const int64_t va = on ? k_base + v_less_k + off : (int64_t)g_zeros;
+            const int at = ((thread & ~63) + i * THREADS) * 16;  // a wavefront's loads fall side by side
+            __builtin_amdgcn_global_load_lds((global_void*)ka, (lds_void*)(ks + at), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((global_void*)va, (lds_void*)(vs + at), 16, 0, 0);
+        }
+    }
+};
+
+// Where a launch's partial results lie: for (row, head) r and split s, fp32 columns at
+// o[(r * splits + s) * d ..] and (maximum, sum) at ml[r * splits + s].  The maximum is of exponents of 2.
+struct Parts {
+    float* o;
+    float2* ml;
+    int splits;
+};
+
+// A split's share of the keys [lo, hi): whole steps of `step` keys.
+__device__ __forceinline__ void split_range(int lo, int hi, int split, int splits, int step, int& k0, int& k1) {
+    const int steps = (max(hi - lo, 0) + step - 1) / step;
+    const int per = (steps + splits - 1) / splits;
+    k0 = min(lo + split * per * step, hi);
+    k1 = min(k0 + per * step, hi);
+}
+
+// The end of a wavefront's rows: out (one split) or a partial result.  on: the lane's row exists.
+template <typename T, int DP, int NK>
+__device__ __forceinline__ void finish(const Rows<T, DP, NK>& w, const AttendArgs& a, const Parts& parts, float c, int split,
+                                       int d, int row, int head, bool on, bool bad) {
+    float l = other_half(w.l, false);
+    if (bad) l = NAN;
+    if (parts.splits == 1) {
+        T* out = on ? (T*)a.out.p + (int64_t)row * a.out.row + (int64_t)head * a.out.head : nullptr;
+        w.store(out, d, l == 0.0f ? 0.0f : 1.0f / l);
+    } else {
+        const int64_t r = ((int64_t)row * a.heads + head) * parts.splits + split;
+        if (on && (threadIdx.x & 63) < 32) parts.ml[r] = make_float2(w.m * c, l);
+        w.store_f32(on && l != 0.0f ? parts.o + r * d : nullptr, d, 1.0f);
+    }
+}
+
+// What a workgroup of a sequence that breaks a bound does: NaN for rows [first, end).
 template <typename T>
-__global__ __launch_bounds__(256) void k_attend_rows(const AttendArgs a, const PagedCache c, const Sequences s) {
-    const int row = blockIdx.x, h = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (h >= a.heads) return;
+__device__ __forceinline__ void poison(const AttendArgs& a, const Parts& parts, int d, int first, int end, int h0, int heads,
+                                       int split) {
+    const int per = heads * d;
+    for (int64_t i = threadIdx.x; i < (int64_t)(end - first) * per; i += blockDim.x) {
+        const int row = first + (int)(i / per), e = (int)(i % per), h = h0 + e / d;
+        if (parts.splits == 1)
+            ((T*)a.out.p)[(int64_t)row * a.out.row + (int64_t)h * a.out.head + e % d] = (T)NAN;
+        else if (e % d == 0)
+            parts.ml[((int64_t)row * a.heads + h) * parts.splits + split] = make_float2(-INFINITY, NAN);
+    }
+}
+
+constexpr int kTileRows = 32;  // of a wavefront
+
+// ---- tiles of rows ----------------------------------------------------------
+
+// A workgroup of NW wavefronts takes 32 NW rows of one sequence and kv head, which share tiles of
+// 32 NK keys in two buffers: while one is worked on, the next loads.
+template <typename T, int DP, int NW, int NK, bool CAREFUL>
+__device__ __forceinline__ bool tile_pass(Rows<T, DP, NK>& w, Loader<T, DP, 32 * NK, 64 * NW>& ld, const Score& sc, char* lds,
+                                          int k0, int k1) {
+    typedef Loader<T, DP, 32 * NK, 64 * NW> L;
+    constexpr int kKeys = 32 * NK;
+    w.clear();
+    bool any_part = false;
+    ld.pages(k0, k1);
+    ld.load(lds, lds + L::kBytes, k0, k1, threadIdx.x);
+    if (k0 + kKeys < k1) ld.pages(k0 + kKeys, k1);
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    int buf = 0;
+#pragma unroll 1
+    for (int k = k0; k < k1; k += kKeys, buf ^= 1) {
+        char* cur = lds + buf * 2 * L::kBytes;
+        char* nxt = lds + (buf ^ 1) * 2 * L::kBytes;
+        if (k + kKeys < k1) {
+            ld.load(nxt, nxt + L::kBytes, k + kKeys, k1, threadIdx.x);
+            if (k + 2 * kKeys < k1) ld.pages(k + 2 * kKeys, k1);
+        }
+        if (k < w.max_hi && k + kKeys > w.min_lo) {
+            any_part = any_part || k < w.max_lo || k + kKeys > w.min_hi;
+            w.template step<CAREFUL>(cur, cur + L::kBytes, k, sc);
+        }
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    }
+    return any_part;
+}
+
+template <typename T, int DP, int NW, int NK>
+__global__ __launch_bounds__(64 * NW, DP * sizeof(T) <= 256 ? 2 : 1) void k_attend_tiles(const AttendArgs a, const PagedCache c, const Sequences s,
+                                                          const Parts parts) {
+    typedef Loader<T, DP, 32 * NK, 64 * NW> L;
+    constexpr int kRows = kTileRows * NW;
+    __shared__ __align__(16) char lds[4 * L::kBytes];
+    __shared__ int range[2][NW];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = a.heads / c.kv_heads;
+    const int kvh = blockIdx.x % c.kv_heads, split = blockIdx.x / c.kv_heads % parts.splits;
+
+    // The sequence and the tile of it that this workgroup is: tiles in order of the sequences.
+    int want = blockIdx.x / (c.kv_heads * parts.splits), b = -1, tile = 0, tiles = 0;
+    for (int i0 = 0; i0 < s.B; i0 += 64) {
+        int n = 0;
+        if (i0 + lane < s.B) {
+            const SeqRows r = seq_rows(s, i0 + lane);
+            n = (int)(((int64_t)min(r.n, s.max_new) * g + kRows - 1) / kRows);
+        }
+        int upto = n;
+#pragma unroll
+        for (int o = 1; o < 64; o *= 2) {
+            const int v = __shfl_up(upto, o, 64);
+            if (lane >= o) upto += v;
+        }
+        const unsigned long long past = __ballot(upto > want);
+        if (past) {
+            const int at = __ffsll(past) - 1;
+            b = i0 + at;
+            tiles = __shfl(n, at, 64);
+            tile = want - (__shfl(upto, at, 64) - tiles);
+            break;
+        }
+        want -= __shfl(upto, 63, 64);
+    }
+    if (b < 0) return;
+    const SeqRows r = seq_rows(s, b);
+    if (!r.ok) {
+        const int per = (r.n + tiles - 1) / tiles;
+        poison<T>(a, parts, c.head_dim, r.row0 + min(r.n, tile * per), r.row0 + min(r.n, (tile + 1) * per), kvh * g, g, split);
+        return;
+    }
+    tile = tiles - 1 - tile;  // the longest rows first
+
+    const Score sc(a);
+    Rows<T, DP, NK> w;
+    const int64_t first = (int64_t)tile * kRows + wave * kTileRows + (lane & 31), last = (int64_t)r.n * g - 1;
+    const bool on = first <= last;
+    const int item = (int)min(first, last);
+    const int row = r.row0 + item / g, head = kvh * g + item % g;
+    w.pos = r.position(row);
+    row_keys(a, r, b, row, w.pos, w.lo, w.hi);
+    w.slope = a.slopes ? a.slopes[head] * kLog2e : 0.0f;
+    w.load((const T*)a.q.p + (int64_t)row * a.q.row + (int64_t)head * a.q.head, c.head_dim, sc.negate);
+    w.bounds();
+    if (lane == 0) range[0][wave] = w.min_lo, range[1][wave] = w.max_hi;
+    __syncthreads();
+    int lo = range[0][0], hi = range[1][0];
+#pragma unroll
+    for (int i = 1; i < NW; ++i) lo = min(lo, range[0][i]), hi = max(hi, range[1][i]);
+    lo = __builtin_amdgcn_readfirstlane(lo), hi = __builtin_amdgcn_readfirstlane(hi);
+    int k0, k1;
+    split_range(lo, hi, split, parts.splits, 32 * NK, k0, k1);
+
+    L ld(c, s.table + b * s.table_ld, kvh, threadIdx.x);
+    if (k0 < k1) {
+        const bool part = tile_pass<T, DP, NW, NK, false>(w, ld, sc, lds, k0, k1);
+        if (__syncthreads_or(part && on && w.not_finite(c.head_dim)))
+            tile_pass<T, DP, NW, NK, true>(w, ld, sc, lds, k0, k1);
+    } else {
+        w.clear();
+    }
+    const bool bad = __syncthreads_or(ld.bad);
+    const float unit = sc.capped || a.slopes ? 1.0f : sc.c;
+    finish(w, a, parts, unit, split, c.head_dim, row, head, on, bad);
+}
+
+// ---- few rows ----------------------------------------------------------------
+
+// Up to 32 rows of a sequence and kv head (single tokens and a few more): the NW wavefronts of a workgroup
+// have tiles of 32 keys of their own, in two buffers each, and are joined at the end.
+template <typename T, int DP, int NW, bool CAREFUL>
+__device__ __forceinline__ bool few_pass(Rows<T, DP, 1>& w, Loader<T, DP, 32, 64>& ld, const Score& sc, char* lds, int k0,
+                                         int k1) {
+    typedef Loader<T, DP, 32, 64> L;
+    const int lane = threadIdx.x & 63;
+    w.clear();
+    if (k0 >= k1) return false;
+    bool any_part = false;
+    ld.pages(k0, k1);
+    ld.load(lds, lds + L::kBytes, k0, k1, lane);
+    if (k0 + 32 * NW < k1) ld.pages(k0 + 32 * NW, k1);
+    int buf = 0;
+#pragma unroll 1
+    for (int k = k0; k < k1; k += 32 * NW, buf ^= 1) {
+        char* cur = lds + buf * 2 * L::kBytes;
+        char* nxt = lds + (buf ^ 1) * 2 * L::kBytes;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (k + 32 * NW < k1) {
+            ld.load(nxt, nxt + L::kBytes, k + 32 * NW, k1, lane);
+            if (k + 64 * NW < k1) ld.pages(k + 64 * NW, k1);
+        }
+        any_part = any_part || k < w.max_lo || k + 32 > w.min_hi;
+        w.template step<CAREFUL>(cur, cur + L::kBytes, k, sc);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    return any_part;
+}
+
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(64 * NW) void k_attend_few(const AttendArgs a, const PagedCache c, const Sequences s,
+                                                        const Parts parts) {
+    typedef Loader<T, DP, 32, 64> L;
+    static_assert(L::kBytes * 4 >= 32 * DP * 4, "a wavefront's buffers hold its result");
+    __shared__ __align__(16) char lds[NW][4 * L::kBytes];
+    __shared__ float ml[2][NW][32];
+    __shared__ int wrong[NW];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = a.heads / c.kv_heads, d = c.head_dim;
+    const int kvh = blockIdx.x % c.kv_heads, rest = blockIdx.x / c.kv_heads;
+    const int split = rest % parts.splits, b = rest / parts.splits;
+    const SeqRows r = seq_rows(s, b);
+    if (r.n == 0) return;
+    if (!r.ok) {
+        poison<T>(a, parts, d, r.row0, r.row0 + r.n, kvh * g, g, split);
+        return;
+    }
+    const Score sc(a);
+    Rows<T, DP, 1> w;
+    const int rows = r.n * g, item = min(lane & 31, rows - 1);
+    const int row = r.row0 + item / g, head = kvh * g + item % g;
+    const bool on = (lane & 31) < rows;
+    w.pos = r.position(row);
+    row_keys(a, r, b, row, w.pos, w.lo, w.hi);
+    w.slope = a.slopes ? a.slopes[head] * kLog2e : 0.0f;
+    w.load((const T*)a.q.p + (int64_t)row * a.q.row + (int64_t)head * a.q.head, d, sc.negate);
+    w.bounds();
+    int k0, k1;
+    split_range(__builtin_amdgcn_readfirstlane(w.min_lo), __builtin_amdgcn_readfirstlane(w.max_hi), split, parts.splits, 32 * NW,
+                k0, k1);
+    L ld(c, s.table + b * s.table_ld, kvh, lane);
+    k0 += 32 * wave;
+    const bool part = few_pass<T, DP, NW, false>(w, ld, sc, lds[wave], k0, k1);
+    if (__any(part && w.not_finite(d))) few_pass<T, DP, NW, true>(w, ld, sc, lds[wave], k0, k1);
+    const float unit = sc.capped || a.slopes ? 1.0f : sc.c;
+    if constexpr (NW == 1) {
+        finish(w, a, parts, unit, split, d, row, head, on, __any(ld.bad));
+    } else {
+        const float l = other_half(w.l, false);
+        const bool bad = __any(ld.bad);
+        if (lane < 32) ml[0][wave][lane] = w.m * unit, ml[1][wave][lane] = l;
+        if (lane == 0) wrong[wave] = bad;
+        float* mine = (float*)lds[wave];
+        w.store_f32(on ? mine + (lane & 31) * DP : nullptr, d, 1.0f);
+        __syncthreads();
+        bool any_bad = false;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) any_bad = any_bad || wrong[i];
+        // Four columns of a row a thread.
+        const int quads = d / 4;
+        for (int i = threadIdx.x; i < rows * quads; i += 64 * NW) {
+            const int q = i / quads, col = 4 * (i % quads);
+            float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+            for (int v = 0; v < NW; ++v) top = fmaxf(top, ml[0][v][q]);
+            f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int v = 0; v < NW; ++v) {
+                const float lv = ml[1][v][q];
+                if (lv == 0.0f) continue;  // nothing seen, its maximum -inf
+                const float f = __builtin_amdgcn_exp2f(ml[0][v][q] - (top == -INFINITY ? 0.0f : top));
+                sum = fmaf(lv, f, sum);
+                const f32x4 x = *(const f32x4*)((const float*)lds[v] + q * DP + col);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], f, o[e]);
+            }
+            if (any_bad) sum = NAN;
+            const int rw = r.row0 + q / g, hd = kvh * g + q % g;
+            if (parts.splits == 1) {
+                T* out = (T*)a.out.p + (int64_t)rw * a.out.row + (int64_t)hd * a.out.head + col;
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                typedef T T4 __attribute__((ext_vector_type(4)));
+                T4 y;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = (T)(o[e] * inv);
+                *(T4*)out = y;
+            } else {
+                const int64_t at = ((int64_t)rw * a.heads + hd) * parts.splits + split;
+                if (sum != 0.0f) *(f32x4*)(parts.o + at * d + col) = o;
+                if (col == 0) parts.ml[at] = make_float2(top, sum);
+            }
+        }
+    }
+}
+
+// ---- the splits of a row joined ------------------------------------------------
+
+// A workgroup per row and head: its threads take four columns and a share of the splits each.
+template <typename T>
+__global__ __launch_bounds__(256) void k_attend_join(const AttendArgs a, int d, const Sequences s, const Parts parts) {
+    __shared__ f32x4 red[256];
+    __shared__ float total[256];
+    const int row = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
     const int b = seq_of_row(s, row);
     if (b >= s.B) return;
     const SeqRows r = seq_rows(s, b);
-    const bool inside = row >= r.row0 && row < r.row0 + r.n;
-    if (!inside && r.ok) return;
-    const int d = c.head_dim, kvh = h / (a.heads / c.kv_heads);
-    const T* q = (const T*)a.q.p + (int64_t)row * a.q.row + (int64_t)h * a.q.head;
-    T* out = (T*)a.out.p + (int64_t)row * a.out.row + (int64_t)h * a.out.head;
-    float x[4], o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < 4; ++i) x[i] = lane + 64 * i < d ? (float)q[lane + 64 * i] : 0.0f;
-    float m = -INFINITY, l = 0.0f;
-    bool ok = r.ok;
-    if (ok) {
-        int lo, hi;
-        row_keys(a, r, b, row, lo, hi);
-        const float slope = a.slopes ? a.slopes[h] : 0.0f;
-        for (int j = lo; j < hi; ++j) {
-            const int64_t off = key_offset(c, s.table + b * s.table_ld, j);
-            if (off < 0) {
-                ok = false;
-                break;
-            }
-            const T* k = (const T*)c.k + off + kvh * c.head_stride;
-            const T* v = (const T*)c.v + off + kvh * c.head_stride;
-            float sc = 0.0f;
-            for (int i = 0; i < 4; ++i)
-                if (lane + 64 * i < d) sc = fmaf(x[i], (float)k[lane + 64 * i], sc);
-            for (int t = 32; t > 0; t >>= 1) sc += __shfl_xor(sc, t, 64);
-            sc *= a.scale;
-            if (a.softcap > 0.0f) sc = a.softcap * tanhf(sc / a.softcap);
-            sc -= slope * fabsf((float)(r.position(row) - j));
-            const float mn = fmaxf(m, sc);
-            const float base = mn == -INFINITY ? 0.0f : mn;
-            const float w = expf(m - base), e = sc != sc ? sc : expf(sc - base);
-            l = l * w + e;
-            for (int i = 0; i < 4; ++i)
-                if (lane + 64 * i < d) o[i] = o[i] * w + e * (float)v[lane + 64 * i];
-            m = mn;
+    if (row < r.row0 || row >= r.row0 + r.n) return;
+    const int64_t at = (int64_t)blockIdx.x * parts.splits;
+    float top = -INFINITY;
+    for (int i = threadIdx.x & 63; i < parts.splits; i += 64) top = fmaxf(top, parts.ml[at + i].x);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    if (top == -INFINITY) top = 0.0f;
+    const int quads = d / 4, groups = 256 / quads, grp = threadIdx.x / quads, col = 4 * (threadIdx.x % quads);
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    float sum = 0.0f;
+    if (grp < groups)
+        for (int i = grp; i < parts.splits; i += groups) {
+            const float2 v = parts.ml[at + i];
+            if (v.y == 0.0f) continue;
+            const float f = __builtin_amdgcn_exp2f(v.x - top);
+            sum = fmaf(v.y, f, sum);
+            if (v.y != v.y) continue;  // NaN; the columns may not have been written
+            const f32x4 x = *(const f32x4*)(parts.o + (at + i) * d + col);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], f, o[e]);
         }
+    red[threadIdx.x] = o, total[threadIdx.x] = sum;
+    __syncthreads();
+    if (threadIdx.x >= quads) return;
+    for (int i = 1; i < groups; ++i) {
+        o += red[threadIdx.x + i * quads];
+        sum += total[threadIdx.x + i * quads];
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    for (int i = 0; i < 4; ++i)
-        if (lane + 64 * i < d) out[lane + 64 * i] = ok ? (T)(o[i] * inv) : (T)NAN;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    T4 y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = (T)(o[e] * inv);
+    *(T4*)((T*)a.out.p + (int64_t)row * a.out.row + (int64_t)head * a.out.head + col) = y;
+}
+
+constexpr int kTileWaves = 4;
+
+// Wavefronts of k_attend_few whose buffers (two of 32 keys and values each) fit 128 KiB.
+constexpr int few_waves(int row_bytes) { return row_bytes <= 256 ? 4 : 1024 / row_bytes; }
+
+template <typename T, int DP>
+void start(const AttendArgs& a, const PagedCache& c, const Sequences& s, const AttendPlan& p, const Parts& parts,
+           hipStream_t st) {
+    constexpr int kRow = TileRows<T, DP>::kRow;
+    if (p.few) {
+        constexpr int NW = few_waves(kRow);
+        k_attend_few<T, DP, NW><<<(unsigned)((int64_t)s.B * c.kv_heads * p.splits), 64 * NW, 0, st>>>(a, c, s, parts);
+    } else {
+        constexpr int NK = kRow <= 256 ? 2 : 1;
+        k_attend_tiles<T, DP, kTileWaves, NK>
+            <<<(unsigned)(p.tiles * c.kv_heads * p.splits), 64 * kTileWaves, 0, st>>>(a, c, s, parts);
+    }
+    if (p.splits > 1)
+        k_attend_join<T><<<(unsigned)((int64_t)s.rows * a.heads), 256, 0, st>>>(a, c.head_dim, s, parts);
+}
+
+template <typename T>
+void start(const AttendArgs& a, const PagedCache& c, const Sequences& s, const AttendPlan& p, const Parts& parts,
+           hipStream_t st) {
+    const int d = c.head_dim;
+    if (d <= 64) start<T, 64>(a, c, s, p, parts, st);
+    else if (d <= 96) start<T, 96>(a, c, s, p, parts, st);
+    else if (d <= 128) start<T, 128>(a, c, s, p, parts, st);
+    else if (d <= 192) start<T, 192>(a, c, s, p, parts, st);
+    else start<T, 256>(a, c, s, p, parts, st);
 }
 
 }  // namespace
 
-hipError_t launch_attend(const AttendArgs& a, const PagedCache& c, const Sequences& s, void* ws, hipStream_t st) {
+AttendPlan attend_plan(const AttendShape& q, int64_t cus) {
+    AttendPlan p;
+    const int64_t g = q.heads / q.kv_heads;
+    p.few = q.max_new * g <= kTileRows;
+    const int64_t len = std::max<int64_t>(q.max_len, 1);
+    int64_t wgs, step;
+    if (p.few) {
+        p.tiles = 0;
+        wgs = q.B * q.kv_heads;
+        step = 128;
+        // Eight workgroups a compute unit.
+        p.splits = (int)std::max<int64_t>(1, std::min(ceil_div(8 * cus, wgs), ceil_div(len, step)));
+    } else {
+        const int64_t rows = kTileRows * kTileWaves;
+        p.tiles = std::min(q.rows * g / rows + q.B, q.B * ceil_div(q.max_new * g, rows));
+        wgs = p.tiles * q.kv_heads;
+        step = 512;
+        p.splits = (int)std::max<int64_t>(1, std::min(2 * cus / wgs, ceil_div(len, step)));
+    }
+    p.workgroups = wgs * p.splits;
+    return p;
+}
+
+int64_t attend_plan_bytes(const AttendPlan& p, const AttendShape& q) {
+    if (p.splits == 1) return 0;
+    return q.rows * q.heads * p.splits * (q.head_dim * 4 + 8);
+}
+
+hipError_t launch_attend(const AttendArgs& a, const PagedCache& c, const Sequences& s, const AttendPlan& p, void* ws,
+                         hipStream_t st) {
     if (s.rows <= 0 || s.B <= 0) return hipSuccess;
-    const dim3 grid((unsigned)s.rows, (unsigned)ceil_div(a.heads, 4));
+    const int64_t n = (int64_t)s.rows * a.heads * p.splits;
+    const Parts parts = {(float*)ws, (float2*)((float*)ws + n * c.head_dim), p.splits};
     switch (c.t) {
-        case DType::f32: k_attend_rows<float><<<grid, 256, 0, st>>>(a, c, s); break;
-        case DType::bf16: k_attend_rows<__bf16><<<grid, 256, 0, st>>>(a, c, s); break;
-        case DType::f16: k_attend_rows<_Float16><<<grid, 256, 0, st>>>(a, c, s); break;
+        case DType::f32: start<float>(a, c, s, p, parts, st); break;
+        case DType::bf16: start<__bf16>(a, c, s, p, parts, st); break;
+        case DType::f16: start<_Float16>(a, c, s, p, parts, st); break;
     }
     return hipGetLastError();
 }

@@ -595,6 +595,20 @@ struct AttendArgs {
     const int32_t* prefix;
     const int32_t* first_key;
 };
-hipError_t launch_attend(const AttendArgs& a, const PagedCache& c, const Sequences& s, void* ws, hipStream_t st);
+struct AttendShape {
+    int64_t heads, kv_heads, head_dim, B, rows, max_len, max_new;
+    DType t;
+};
+// few: a workgroup has all rows of a sequence and kv head (at most 32), else `tiles` tiles of
+// rows at most; splits: workgroups that share the keys of those, joined by a second kernel.
+struct AttendPlan {
+    bool few;
+    int64_t tiles, workgroups;
+    int splits;
+};
+AttendPlan attend_plan(const AttendShape& q, int64_t cus);
+int64_t attend_plan_bytes(const AttendPlan& p, const AttendShape& q);
+hipError_t launch_attend(const AttendArgs& a, const PagedCache& c, const Sequences& s, const AttendPlan& p, void* ws,
+                         hipStream_t st);
 
 }  // namespace sgq
