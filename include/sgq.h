@@ -469,7 +469,7 @@ int sgq_w8a8_plan(int gated, int64_t M, int64_t K, int64_t N, int compute_units,
  * A cache is a pool of pages for one layer: key (or value) row t of page p and head h
  * at k (or v) + p * page_stride + t * token_stride + h * head_stride elements, head_dim
  * elements next to each other, every row 16-byte aligned.  page_size is a power of
- * two, at most 65536. */
+ * two from 8 to 65536; page_stride and page_size * token_stride are less than 4 GiB. */
 typedef struct sgq_paged_cache {
     void* k;
     void* v;

@@ -52,7 +52,7 @@ class _Scores(ctypes.Structure):
 
 class PagedKV:
     """A layer's pool of pages: k and v [pages, page, kv_heads, head_dim], alike in shape,
-    strides and type; page a power of two, head_dim a multiple of 16 up to 256, heads next to
+    strides and type; page a power of two from 8 on, head_dim a multiple of 16 up to 256, heads next to
     each other in any order of the first three dimensions (views of [pages, kv_heads, page, head_dim] will do)."""
 
     __slots__ = ("k", "v", "_struct", "_at")
@@ -63,8 +63,8 @@ class PagedKV:
         if v.shape != k.shape or v.dtype != k.dtype or v.device != k.device or v.stride() != k.stride():
             raise ValueError("k and v must be alike in shape, strides, type and device")
         pages, page, heads, d = k.shape
-        if page < 1 or page & (page - 1) or page > 65536:
-            raise ValueError("a page's rows must be a power of two, at most 65536")
+        if page < 8 or page & (page - 1) or page > 65536:
+            raise ValueError("a page's rows must be a power of two from 8 to 65536")
         if d < 16 or d % 16 or d > 256:
             raise ValueError("head_dim must be a multiple of 16, at most 256")
         if heads < 1:

@@ -478,8 +478,8 @@ int check_paged(const char* fn, int64_t rows, int64_t heads, const sgq_paged_cac
         return fail(SGQ_ERR_UNSUPPORTED, "%s: head_dim must be a multiple of %d, at most %d", fn, kHeadDimStep, kMaxHeadDim);
     if (c->kv_heads < 1 || heads < 1 || heads % c->kv_heads)
         return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: heads must be a multiple of kv_heads", fn);
-    if (c->page_size < 1 || (c->page_size & (c->page_size - 1)) || c->page_size > 65536)
-        return fail(SGQ_ERR_UNSUPPORTED, "%s: page_size must be a power of two, at most 65536", fn);
+    if (c->page_size < kMinPage || (c->page_size & (c->page_size - 1)) || c->page_size > kMaxPage)
+        return fail(SGQ_ERR_UNSUPPORTED, "%s: page_size must be a power of two from %d to %d", fn, kMinPage, kMaxPage);
     if (c->pages < 0 || c->pages > kMaxDim) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: bad number of pages", fn);
     if (q->B < 0 || rows < 0 || q->max_len < 0 || q->max_new < 0 || q->table_pages < 0 || q->table_pages > kMaxDim ||
         q->max_len > kMaxDim || q->max_new > kMaxDim || q->table_ld < q->table_pages || q->table_ld > kMaxDim)
@@ -488,11 +488,13 @@ int check_paged(const char* fn, int64_t rows, int64_t heads, const sgq_paged_cac
         return fail(SGQ_ERR_UNSUPPORTED, "%s: more than %d heads, %d rows or %d sequences", fn, kMaxHeads, kMaxHeadRows,
                     kMaxSequences);
     const int64_t step = 16 / dtype_bytes((DType)c->dtype), d = c->head_dim;
-    // Strides that cross the whole pool stay within 64 bits, and rows of the pool apart.
-    const int64_t big = (int64_t)1 << 40;
-    if (c->page_stride < 0 || c->token_stride < 0 || c->head_stride < 0 || c->page_stride > big || c->token_stride > big ||
-        c->head_stride > big || c->page_stride % step || c->token_stride % step || c->head_stride % step)
+    if (c->page_stride < 0 || c->token_stride < 0 || c->head_stride < 0 || c->page_stride % step || c->token_stride % step ||
+        c->head_stride % step)
         return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: strides of the cache must be multiples of 16 bytes", fn);
+    // The kernels multiply page and row numbers by 32-bit strides to 64-bit offsets.
+    const int64_t most = (((int64_t)1 << 32) - 1) / dtype_bytes((DType)c->dtype);
+    if (c->page_stride > most || c->token_stride > most / c->page_size || c->head_stride > ((int64_t)1 << 40))
+        return fail(SGQ_ERR_UNSUPPORTED, "%s: pages, or rows of a page, of the cache 4 GiB apart", fn);
     if ((c->kv_heads > 1 && c->head_stride < d) || (c->page_size > 1 && c->token_stride < d) ||
         (c->pages > 1 && c->page_stride < d))
         return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: rows of the cache overlap", fn);
@@ -505,13 +507,14 @@ int check_paged(const char* fn, int64_t rows, int64_t heads, const sgq_paged_cac
     }
     pc.k = (char*)c->k, pc.v = (char*)c->v, pc.t = (DType)c->dtype;
     pc.page_stride = c->page_stride, pc.token_stride = c->token_stride, pc.head_stride = c->head_stride;
+    pc.page_bytes = (uint32_t)(c->page_stride * dtype_bytes(pc.t)), pc.token_bytes = (uint32_t)(c->token_stride * dtype_bytes(pc.t));
     pc.pages = (int)c->pages, pc.kv_heads = (int)c->kv_heads, pc.head_dim = (int)d, pc.page_log = 0;
     while ((int64_t)1 << pc.page_log < c->page_size) ++pc.page_log;
     sq.table = q->table, sq.lens = q->lens, sq.starts = q->starts, sq.table_ld = q->table_ld;
     sq.B = (int)q->B, sq.rows = (int)rows;
     sq.max_len = (int)q->max_len, sq.max_new = (int)q->max_new;
     const int64_t cap = q->table_pages * c->page_size;
-    sq.capacity = (int)(cap < kMaxDim ? cap : kMaxDim);
+    sq.capacity = c->pages == 0 ? 0 : (int)(cap < kMaxDim ? cap : kMaxDim);
     return SGQ_OK;
 }
 
@@ -1351,7 +1354,7 @@ int sgq_paged_attention(const void* q, int64_t q_row, int64_t q_head, void* out,
     a.slopes = scores->alibi_slopes, a.prefix = scores->prefix, a.first_key = scores->first_key;
     const AttendShape shape = {heads, c.kv_heads, d, s.B, s.rows, s.max_len, s.max_new, c.t};
     const AttendPlan p = attend_plan(shape, device_cus((hipStream_t)stream));
-    if (p.workgroups * 256 >= (int64_t)1 << 32 || (p.splits > 1 && (int64_t)s.rows * heads * 256 >= (int64_t)1 << 32))
+    if (p.workgroups * 512 >= (int64_t)1 << 32 || (p.splits > 1 && (int64_t)s.rows * heads * 256 >= (int64_t)1 << 32))
         return fail(SGQ_ERR_UNSUPPORTED, "%s: too many rows for one call", fn);
     const int64_t need = attend_plan_bytes(p, shape);
     if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))

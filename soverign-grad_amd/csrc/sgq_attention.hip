@@ -26,6 +26,7 @@
 #include "sgq_paged.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace sgq {
 namespace {
@@ -121,10 +122,11 @@ struct Score {
     float c;         // exponent of 2 per raw score (without a cap)
     float in, out;   // cap: 2^ of out * tanh(in * raw)
     bool negate;     // scale < 0: the queries are negated instead
-    bool capped;
+    bool capped, sloped;
     __device__ __forceinline__ explicit Score(const AttendArgs& a) {
         negate = a.scale < 0.0f;
         capped = a.softcap > 0.0f;
+        sloped = a.slopes != nullptr;
         in = capped ? fabsf(a.scale) / a.softcap : 0.0f;
         out = a.softcap * kLog2e;
         // Never zero: a hidden score is -inf, and has to stay that.
@@ -142,6 +144,8 @@ struct Rows {
 
     Frag q[kFrags];
     f32x16 o[kCols];
+    f32x16 s[NK];  // scores of a tile
+    std::conditional_t<sizeof(T) == 4, f32x16, Frag> p[sizeof(T) == 4 ? NK : 2 * NK];  // weights of a tile
     float m, l;            // maximum of the scores (as c multiplies them), this half's sum of weights
     int lo, hi, pos;       // the row's keys and position
     float slope;           // times log2 e
@@ -160,62 +164,51 @@ struct Rows {
 #pragma unroll
         for (int i = 0; i < kFrags; ++i) {
             const int e = i * M::kStep + h * (M::kStep / 2);
-            Frag f = {};
-            if (e < d) f = *(const Frag*)(p + e);
-            q[i] = negate ? -f : f;
+            const Frag f = *(const Frag*)(p + min(e, d - M::kStep / 2)), none = {};
+            q[i] = e < d ? (negate ? -f : f) : none;
         }
     }
     __device__ __forceinline__ void bounds() {
-        max_lo = wave_max(lo), min_hi = wave_min(hi);
-        min_lo = wave_min(lo), max_hi = wave_max(hi);
+        max_lo = __builtin_amdgcn_readfirstlane(wave_max(lo)), min_hi = __builtin_amdgcn_readfirstlane(wave_min(hi));
+        min_lo = __builtin_amdgcn_readfirstlane(wave_min(lo)), max_hi = __builtin_amdgcn_readfirstlane(wave_max(hi));
     }
 
-    // Keys k0 .. k0 + 32 NK - 1 in the tiles ks and vs.  careful: values that are not finite touch
-    // only the rows that see them.
-    template <bool CAREFUL>
-    __device__ __forceinline__ void step(const char* ks, const char* vs, int k0, const Score& sc) {
-        const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
-        f32x16 s[NK];
-        {
-            const int x = (h ^ Tile::mix(n)) << 4;  // chunk 2 i + h of row n (mix has the period of 16 rows)
-            const char* row = ks + n * Tile::kRow;
-#pragma unroll
-            for (int t = 0; t < NK; ++t)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) s[t][e] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < kFrags; ++i)
-#pragma unroll
-                for (int t = 0; t < NK; ++t)
-                    s[t] = M::mma(*(const Frag*)(row + t * 32 * Tile::kRow + ((i * 32) ^ x)), q[i], s[t]);
-        }
+    // Whether some row does not see some key of the tile at k0.
+    __device__ __forceinline__ bool part(int k0) const { return k0 < max_lo || k0 + 32 * NK > min_hi; }
+
+    // Scores of the keys from k0 on to weights, the sum and, where the maximum grows, the factor of what was summed.
+    __device__ __forceinline__ void softmax(int k0, const Score& sc) {
+        const int h = (threadIdx.x & 63) >> 5;
         // Key of register e of tile t: k0 + 32 t + 8 (e / 4) + 4 h + e % 4.
         const int kb = k0 + 4 * h;
         float c = sc.c;
-        if (sc.capped || slope != 0.0f) {
-            c = 1.0f;
+        if (sc.capped || sc.sloped) c = 1.0f;
+        if (sc.capped) {
 #pragma unroll
             for (int t = 0; t < NK; ++t)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    float v = s[t][e];
-                    if (sc.capped) {
-                        if constexpr (sizeof(T) == 4) {
-                            v = sc.out * tanhf(v * sc.in);
-                        } else {
-                            // tanh x = 1 - 2 / (1 + e^2x): off by some 2^-23, which a 16-bit weight does not see.
-                            const float u = __builtin_amdgcn_exp2f(v * (2.0f * kLog2e * sc.in));
-                            v = fmaf(sc.out * -2.0f, __builtin_amdgcn_rcpf(1.0f + u), sc.out);
-                        }
+                    if constexpr (sizeof(T) == 4) {
+                        s[t][e] = sc.out * tanhf(s[t][e] * sc.in);
                     } else {
-                        v *= sc.c;
+                        // tanh x = 1 - 2 / (1 + e^2x): off by some 2^-23, which a 16-bit weight does not see.
+                        const float u = __builtin_amdgcn_exp2f(s[t][e] * (2.0f * kLog2e * sc.in));
+                        s[t][e] = fmaf(sc.out * -2.0f, __builtin_amdgcn_rcpf(1.0f + u), sc.out);
                     }
-                    const int away = pos - (kb + 32 * t + 8 * (e / 4) + e % 4);
-                    s[t][e] = fmaf(-slope, (float)abs(away), v);
                 }
+        } else if (sc.sloped) {
+#pragma unroll
+            for (int t = 0; t < NK; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[t][e] *= sc.c;
         }
-        const bool part = k0 < max_lo || k0 + 32 * NK > min_hi;  // some row does not see some key
-        if (part) {
+        if (sc.sloped)
+#pragma unroll
+            for (int t = 0; t < NK; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    s[t][e] = fmaf(-slope, (float)abs(pos - (kb + 32 * t + 8 * (e / 4) + e % 4)), s[t][e]);
+        if (part(k0)) {
             const unsigned width = (unsigned)max(hi - lo, 0);
 #pragma unroll
             for (int t = 0; t < NK; ++t)
@@ -247,44 +240,69 @@ struct Rows {
         for (int t = 0; t < NK; ++t)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                s[t][e] = __builtin_amdgcn_exp2f(fmaf(s[t][e], c, base));
-                sum[e & 3] += s[t][e];
+                const float w = __builtin_amdgcn_exp2f(fmaf(s[t][e], c, base));
+                sum[e & 3] += w;
+                if constexpr (sizeof(T) == 4)
+                    p[t][e] = w;
+                else
+                    p[2 * t + e / 8][e % 8] = (T)w;
             }
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        if (CAREFUL && part)
-            values<true>(vs, s);
-        else
-            values<false>(vs, s);
     }
 
-    // O^T += V^T P^T.
-    template <bool CAREFUL>
-    __device__ __forceinline__ void values(const char* vs, const f32x16 (&s)[NK]) {
+    // S^T of the keys in the tile at ks.  The LDS reads of four products are issued ahead of the four before
+    // them; left alone, the compiler reads for each product as it comes and waits.  beside(g): what is issued
+    // beside the g-th four.
+    static constexpr int kScoreGroups = (kFrags * NK + 3) / 4;
+    template <typename F>
+    __device__ __forceinline__ void scores(const char* ks, F beside) {
+        const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
+        const int x = (h ^ Tile::mix(n)) << 4;  // chunk 2 i + h of row n (mix has the period of 16 rows)
+        const char* const row = ks + n * Tile::kRow;
+#pragma unroll
+        for (int t = 0; t < NK; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[t][e] = 0.0f;
+        constexpr int N = kFrags * NK, G = 4;
+        auto read = [&](int j) { return *(const Frag*)(row + j % NK * 32 * Tile::kRow + ((j / NK * 32) ^ x)); };
+        Frag f[2][G];
+#pragma unroll
+        for (int j = 0; j < G; ++j) f[0][j] = read(j);
+#pragma unroll
+        for (int g = 0; g < (N + G - 1) / G; ++g) {
+#pragma unroll
+            for (int j = 0; j < G; ++j)
+                if ((g + 1) * G + j < N) f[(g + 1) & 1][j] = read((g + 1) * G + j);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 0; j < G; ++j) {
+                const int i = g * G + j;
+                if (i < N) s[i % NK] = M::mma(f[g & 1][j], q[i / NK], s[i % NK]);
+            }
+            beside(g);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+
+    // O^T += V^T P^T with the values in the tile at vs.
+    __device__ __forceinline__ void values(const char* vs) {
         const int lane = threadIdx.x & 63, h = lane >> 5;
         if constexpr (sizeof(T) == 2) {
             // A 16-lane group reads four keys of sixteen columns, a lane eight bytes of them.
             const int i = lane & 15, r0 = 4 * h + (i >> 2);
             const int x = ((2 * ((lane >> 4) & 1) + ((i >> 1) & 1)) ^ Tile::mix(r0)) << 4;
-            const char* row = vs + r0 * Tile::kRow + 8 * (i & 1);
-            // mix of a row eight further: two chunks on where rows hold sixteen chunks or more, for
-            // eight it is (r >> 2) & 3 likewise.
-            constexpr int kNext = 2 << 4;
+            const char* const row = vs + r0 * Tile::kRow + 8 * (i & 1);
+            constexpr int kNext = 2 << 4;  // how mix moves a chunk in a row eight further
 #pragma unroll
-            for (int t = 0; t < NK; ++t)
+            for (int u = 0; u < 2 * NK; ++u)
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    Frag p;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) p[e] = (T)s[t][8 * u + e];
-#pragma unroll
-                    for (int cidx = 0; cidx < kCols; ++cidx) {
-                        const char* at = row + (t * 32 + u * 16) * Tile::kRow;
-                        const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + ((cidx * 64) ^ x)));
-                        const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (lds_s16x4*)(at + 8 * Tile::kRow + ((cidx * 64) ^ x ^ kNext)));
-                        const Frag v = __builtin_bit_cast(Frag, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
-                        product<CAREFUL>(o[cidx], v, p);
-                    }
+                for (int cidx = 0; cidx < kCols; ++cidx) {
+                    const char* const at = row + u * 16 * Tile::kRow;
+                    const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + ((cidx * 64) ^ x)));
+                    const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (lds_s16x4*)(at + 8 * Tile::kRow + ((cidx * 64) ^ x ^ kNext)));
+                    const Frag v = __builtin_bit_cast(Frag, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+                    o[cidx] = M::mma(v, p[u], o[cidx]);
                 }
         } else {
             const int n = lane & 31;
@@ -297,43 +315,13 @@ struct Rows {
                     const int x = ((n >> 2) ^ Tile::mix(r)) << 4;
 #pragma unroll
                     for (int cidx = 0; cidx < kCols; ++cidx)
-                        product<CAREFUL>(o[cidx], *(const float*)(row + ((cidx * 128) ^ x)), s[t][e]);
+                        o[cidx] = __builtin_amdgcn_mfma_f32_32x32x2f32(*(const float*)(row + ((cidx * 128) ^ x)), p[t][e],
+                                                                       o[cidx], 0, 0, 0);
                 }
         }
     }
-    static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) { return M::mma(a, b, c); }
-    static __device__ __forceinline__ f32x16 mma(float a, float b, f32x16 c) {
-        return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
-    }
-    static __device__ __forceinline__ float each(float v, float (*f)(float)) { return f(v); }
-    static __device__ __forceinline__ Frag each(Frag v, float (*f)(float)) {
-        Frag r;
-#pragma unroll
-        for (int e = 0; e < (int)(sizeof(Frag) / sizeof(T)); ++e) r[e] = (T)f((float)v[e]);
-        return r;
-    }
-    // CAREFUL: 0 * infinity is NaN, so values that are not finite take no part in the product; the weights
-    // that rows give them are summed apart, and where that is not zero the column becomes what it has to.
-    template <bool CAREFUL, typename A>
-    static __device__ __forceinline__ void product(f32x16& acc, A v, A p) {
-        if constexpr (!CAREFUL) {
-            acc = mma(v, p, acc);
-        } else {
-            acc = mma(each(v, [](float x) { return isfinite(x) ? x : 0.0f; }), p, acc);
-            const f32x16 none = {};
-            const f32x16 up = mma(each(v, [](float x) { return x == INFINITY ? 1.0f : 0.0f; }), p, none);
-            const f32x16 down = mma(each(v, [](float x) { return x == -INFINITY ? 1.0f : 0.0f; }), p, none);
-            const f32x16 nan = mma(each(v, [](float x) { return x != x ? 1.0f : 0.0f; }), p, none);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                if (up[e] > 0.0f) acc[e] += INFINITY;
-                if (down[e] > 0.0f) acc[e] -= INFINITY;
-                if (nan[e] > 0.0f) acc[e] = NAN;
-            }
-        }
-    }
-    // Whether a column below d of the row is not finite.
-    __device__ __forceinline__ bool not_finite(int d) const {
+    // Whether a column below d of the row is not finite, though its sum of weights is.
+    __device__ __forceinline__ bool not_finite(int d, float sum) const {
         const int h = (threadIdx.x & 63) >> 5;
         bool bad = false;
 #pragma unroll
@@ -341,7 +329,7 @@ struct Rows {
 #pragma unroll
             for (int e = 0; e < 16; ++e)
                 if (32 * i + 8 * (e / 4) + 4 * h < d) bad = bad || !isfinite(o[i][e]);
-        return bad;
+        return bad && sum == sum;
     }
     // The row's columns times w, as T, 16 bytes a store.
     __device__ __forceinline__ void store(T* out, int d, float w) const {
@@ -382,54 +370,96 @@ struct Rows {
     }
 };
 
-// Loads tiles of KEYS keys and their values: 16 bytes a lane, straight to LDS.  THREADS
-// threads (whole wavefronts) share a tile.  The pages of a tile are looked up ahead (pages), used by load.
+// 16 bytes a lane to LDS, a wavefront's next to each other from `lds` on: from p, or from base + off.  Written
+// out, because the compiler waits for such a load of its own before the next LDS read, whatever either is
+// of; here the waits are the kernels'.  The load has no register of its own to be overwritten, and the
+// compiler's count of loads in flight, which misses it, only makes its waits longer.
+__device__ __forceinline__ void load_lds(uint64_t p, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory", "m0");
+}
+__device__ __forceinline__ void load_lds(uint64_t base, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base)
+                 : "memory", "m0");
+}
+__device__ __forceinline__ uint32_t lds_address(const char* p) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
+}
+
+// Loads tiles of KEYS keys or their values: 16 bytes a lane, straight to LDS.  THREADS threads (whole
+// wavefronts) share a tile.  A wavefront's load is kGroup neighbouring rows, at most eight, which are all of one
+// page (pages have eight at least, tiles begin at multiples of kGroup): the page, looked up ahead by one lane a
+// load, and the address are scalar, and a lane's offset is the same for every tile.  With a page and an address
+// of each lane's own, a tile of 64 keys of 128 in bf16 took 80 vector instructions more.
 template <typename T, int DP, int KEYS, int THREADS>
 struct Loader {
     typedef TileRows<T, DP> Tile;
-    static constexpr int kLoads = KEYS * Tile::kChunks / THREADS;  // of keys, and of values, a lane
+    static constexpr int kLoads = KEYS * Tile::kChunks / THREADS;  // of a lane
     static constexpr int kRowsApart = THREADS / Tile::kChunks;     // rows between a lane's loads
+    static constexpr int kGroup = 64 / Tile::kChunks;
     static constexpr int kBytes = KEYS * Tile::kRow;
-    static_assert(THREADS % Tile::kChunks == 0 && KEYS * Tile::kChunks % THREADS == 0, "");
+    static_assert(THREADS % 64 == 0 && 64 % Tile::kChunks == 0 && KEYS * Tile::kChunks % THREADS == 0 && kLoads <= 64, "");
 
     const PagedCache* c;
     const int32_t* table;
-    int64_t k_base, v_less_k;
-    int row;        // of the lane's first load
-    int chunk_off;  // bytes; negative: past the head
-    int page[kLoads];
-    bool bad = false;
+    uint64_t k_base, v_base;
+    int first, row, chunk[kRowsApart % 16 ? kLoads : 1];  // first row of the wavefront's first load; the lane's in it
+    uint32_t lds;                                         // of the wavefront's first load, from a tile's begin
+    unsigned top_page = 0;
+
+    // Pages of a tile's loads, lane i that of load i.
+    struct Pages {
+        unsigned of;
+    };
 
     __device__ __forceinline__ Loader(const PagedCache& cache, const int32_t* t, int kvh, int thread) {
         c = &cache, table = t;
-        k_base = (int64_t)cache.k + (int64_t)kvh * cache.head_stride * (int)sizeof(T);
-        v_less_k = (int64_t)cache.v - (int64_t)cache.k;
-        row = thread / Tile::kChunks;
-    }
-    __device__ __forceinline__ int key(int i, int k0, int end) const { return min(k0 + row + i * kRowsApart, end - 1); }
-    // Pages of the keys from k0 on; keys from `end` on are the one before it.
-    __device__ __forceinline__ void pages(int k0, int end) {
+        const uint64_t head = (uint64_t)kvh * cache.head_stride * sizeof(T);
+        k_base = (uint64_t)cache.k + head, v_base = (uint64_t)cache.v + head;
+        const int wave = __builtin_amdgcn_readfirstlane(thread >> 6), lane = thread & 63;
+        first = wave * kGroup, row = lane / Tile::kChunks;
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) page[i] = table[key(i, k0, end) >> c->page_log];
+        for (int i = 0; i < (int)(sizeof(chunk) / 4); ++i)
+            chunk[i] = (lane & (Tile::kChunks - 1)) ^ Tile::mix(first + row + i * kRowsApart);
+        lds = wave * 1024;
     }
-    __device__ __forceinline__ void load(char* ks, char* vs, int k0, int end, int thread) {
-        const int mask = (1 << c->page_log) - 1;
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int r = row + i * kRowsApart;
-            const int chunk = (thread & (Tile::kChunks - 1)) ^ Tile::mix(r);
-            const bool named = (unsigned)page[i] < (unsigned)c->pages;
-            bad = bad || !named;
-            const bool on = named && chunk * Chunk<T>::N < c->head_dim;
-            const int64_t off = ((int64_t)page[i] * c->page_stride + (int64_t)(key(i, k0, end) & mask) * c->token_stride) *
-                                    (int)sizeof(T) + chunk * 16;
-            const int64_t ka = on ? k_base + off : (int64_t)g_zeros;
-            const int64_t va = on ? k_base + v_less_k + off : (int64_t)g_zeros;
-            const int at = ((thread & ~63) + i * THREADS) * 16;  // a wavefront's loads fall side by side
-            __builtin_amdgcn_global_load_lds((global_void*)ka, (lds_void*)(ks + at), 16, 0, 0);
-            __builtin_amdgcn_global_load_lds((global_void*)va, (lds_void*)(vs + at), 16, 0, 0);
+    // Where tiles of keys from lo on may begin.
+    static __device__ __forceinline__ int begin(int lo) { return lo & ~(kGroup - 1); }
+    // A page that is not in the pool was named (by any lane so far; its last page was read instead).
+    __device__ __forceinline__ bool bad() const { return top_page >= (unsigned)c->pages; }
+    // Pages of the keys from k0 on; from `end` on they are those of the key before it.
+    __device__ __forceinline__ Pages pages(int k0, int end) const {
+        Pages p;
+        const int key = min(k0 + first + min((int)(threadIdx.x & 63), kLoads - 1) * kRowsApart, end - 1);
+        p.of = *(const unsigned*)((const char*)table + 4u * (unsigned)(key >> c->page_log));
+        return p;
+    }
+    // Load i of the keys and of the values from k0 on (from `end` on those of the one before it), to the tiles at LDS
+    // addresses ks and vs.
+    __device__ __forceinline__ void load(uint32_t ks, uint32_t vs, int k0, int end, const Pages& p, int i) {
+        const int key = min(k0 + first + i * kRowsApart, (end - 1) & ~(kGroup - 1));
+        const unsigned page = __builtin_amdgcn_readlane(p.of, i);
+        top_page = max(top_page, page);
+        const uint64_t at = (uint64_t)min(page, (unsigned)c->pages - 1) * c->page_bytes +
+                            (unsigned)(key & ((1 << c->page_log) - 1)) * c->token_bytes;
+        const uint32_t to = lds + i * THREADS * 16;
+        const int ch = chunk[kRowsApart % 16 ? i : 0];
+        const uint32_t off = (uint32_t)min(row, end - 1 - key) * c->token_bytes + ch * 16;
+        if (DP != c->head_dim) {
+            const bool on = ch * Chunk<T>::N < c->head_dim;
+            load_lds(on ? k_base + at + off : (uint64_t)g_zeros, ks + to);
+            load_lds(on ? v_base + at + off : (uint64_t)g_zeros, vs + to);
+        } else {
+            load_lds(k_base + at, off, ks + to);
+            load_lds(v_base + at, off, vs + to);
         }
     }
+    // All of them.  Where the pages have come is said first: the compiler does not count the loads here.
+    __device__ __forceinline__ void load(uint32_t ks, uint32_t vs, int k0, int end, Pages& p) {
+        arrived(p);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) load(ks, vs, k0, end, p, i);
+    }
+    static __device__ __forceinline__ void arrived(Pages& p) { asm volatile("" : "+v"(p.of)); }
 };
 
 // Where a launch's partial results lie: for (row, head) r and split s, fp32 columns at
@@ -464,6 +494,56 @@ __device__ __forceinline__ void finish(const Rows<T, DP, NK>& w, const AttendArg
     }
 }
 
+// One row by a whole wavefront, key by key, over the keys [lo, hi) alone, as finish() leaves it.  In a tile whose
+// keys some rows do not see, a weight of 0 times an infinity or a NaN among the values would be a NaN for those
+// rows: where such a tile's row came out not finite it is done again here, with what it sees.
+template <typename T>
+__device__ __forceinline__ void row_alone(const AttendArgs& a, const PagedCache& c, const int32_t* table, const Parts& parts,
+                                          int split, int row, int head, int pos, int lo, int hi) {
+    const int lane = threadIdx.x & 63, d = c.head_dim;
+    const int64_t kv = (int64_t)(head / (a.heads / c.kv_heads)) * c.head_stride;
+    const T* q = (const T*)a.q.p + (int64_t)row * a.q.row + (int64_t)head * a.q.head;
+    const float slope = a.slopes ? a.slopes[head] : 0.0f;
+    float x[kMaxHeadDim / 64], o[kMaxHeadDim / 64], m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kMaxHeadDim / 64; ++i) x[i] = lane + 64 * i < d ? (float)q[lane + 64 * i] : 0.0f, o[i] = 0.0f;
+    for (int j = lo; j < hi && l == l; ++j) {  // a sum of NaN stays one
+        const int64_t off = key_offset(c, table, j);
+        if (off < 0) break;  // the caller has seen that
+        const T* k = (const T*)c.k + off + kv;
+        const T* v = (const T*)c.v + off + kv;
+        float s = 0.0f, y[kMaxHeadDim / 64];
+#pragma unroll
+        for (int i = 0; i < kMaxHeadDim / 64; ++i) {
+            const bool on = lane + 64 * i < d;
+            s = fmaf(x[i], on ? (float)k[lane + 64 * i] : 0.0f, s);
+            y[i] = on ? (float)v[lane + 64 * i] : 0.0f;
+        }
+#pragma unroll
+        for (int t = 32; t > 0; t >>= 1) s += __shfl_xor(s, t, 64);
+        s *= a.scale;
+        if (a.softcap > 0.0f) s = a.softcap * tanhf(s / a.softcap);
+        s = fmaf(-slope, (float)abs(pos - j), s);
+        const float now = fmaxf(m, s), base = now == -INFINITY ? 0.0f : now;
+        const float w = expf(m - base), e = expf(s - base);
+        l = fmaf(l, w, e), m = now;
+#pragma unroll
+        for (int i = 0; i < kMaxHeadDim / 64; ++i) o[i] = fmaf(o[i], w, e * y[i]);
+    }
+    const int64_t at = ((int64_t)row * a.heads + head) * parts.splits + split;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int i = 0; i < kMaxHeadDim / 64; ++i) {
+        const int col = lane + 64 * i;
+        if (col >= d) continue;
+        if (parts.splits == 1)
+            ((T*)a.out.p)[(int64_t)row * a.out.row + (int64_t)head * a.out.head + col] = (T)(o[i] * inv);
+        else
+            parts.o[at * d + col] = o[i];
+    }
+    if (parts.splits > 1 && lane == 0) parts.ml[at] = make_float2(m * kLog2e, l);
+}
+
 // What a workgroup of a sequence that breaks a bound does: NaN for rows [first, end).
 template <typename T>
 __device__ __forceinline__ void poison(const AttendArgs& a, const Parts& parts, int d, int first, int end, int h0, int heads,
@@ -482,39 +562,51 @@ constexpr int kTileRows = 32;  // of a wavefront
 
 // ---- tiles of rows ----------------------------------------------------------
 
+// Ends a phase: nothing is scheduled across it.
+__device__ __forceinline__ void phase_end() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+__device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 // A workgroup of NW wavefronts takes 32 NW rows of one sequence and kv head, which share tiles of
 // 32 NK keys in two buffers: while one is worked on, the next loads.
-template <typename T, int DP, int NW, int NK, bool CAREFUL>
-__device__ __forceinline__ bool tile_pass(Rows<T, DP, NK>& w, Loader<T, DP, 32 * NK, 64 * NW>& ld, const Score& sc, char* lds,
+template <typename T, int DP, int NW, int NK>
+__device__ __forceinline__ void tile_pass(Rows<T, DP, NK>& w, Loader<T, DP, 32 * NK, 64 * NW>& ld, const Score& sc, char* lds,
                                           int k0, int k1) {
     typedef Loader<T, DP, 32 * NK, 64 * NW> L;
-    constexpr int kKeys = 32 * NK;
-    w.clear();
-    bool any_part = false;
-    ld.pages(k0, k1);
-    ld.load(lds, lds + L::kBytes, k0, k1, threadIdx.x);
-    if (k0 + kKeys < k1) ld.pages(k0 + kKeys, k1);
-    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-    int buf = 0;
+    constexpr int kKeys = 32 * NK, B = L::kBytes;
+    const uint32_t at = __builtin_amdgcn_readfirstlane(lds_address(lds));  // keys, values; keys, values
+    typename L::Pages p = ld.pages(k0, k1);
+    ld.load(at, at + B, k0, k1, p);
+    p = ld.pages(k0 + kKeys, k1);
+    loads_done();
+    phase_end();
+    int odd = 0;
 #pragma unroll 1
-    for (int k = k0; k < k1; k += kKeys, buf ^= 1) {
-        char* cur = lds + buf * 2 * L::kBytes;
-        char* nxt = lds + (buf ^ 1) * 2 * L::kBytes;
-        if (k + kKeys < k1) {
-            ld.load(nxt, nxt + L::kBytes, k + kKeys, k1, threadIdx.x);
-            if (k + 2 * kKeys < k1) ld.pages(k + 2 * kKeys, k1);
-        }
-        if (k < w.max_hi && k + kKeys > w.min_lo) {
-            any_part = any_part || k < w.max_lo || k + kKeys > w.min_hi;
-            w.template step<CAREFUL>(cur, cur + L::kBytes, k, sc);
-        }
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    for (int k = k0; k < k1; k += kKeys, odd ^= 1) {
+        const char* const cur = lds + odd * 2 * B;
+        const uint32_t next = at + (odd ^ 1) * 2 * B;
+        L::arrived(p);
+        // The next tile's loads beside the products of the scores, which leave the scalar unit idle (after the last
+        // tile too, then of its last rows: a branch here would part the products).
+        constexpr int NG = Rows<T, DP, NK>::kScoreGroups;
+        w.scores(cur, [&](int g) {
+#pragma unroll
+            for (int i = 0; i < L::kLoads; ++i)
+                if (i * NG / L::kLoads == g) ld.load(next, next + B, k + kKeys, k1, p, i);
+        });
+        p = ld.pages(k + 2 * kKeys, k1);
+        w.softmax(k, sc);
+        w.values(cur + B);
+        loads_done();
+        phase_end();
     }
-    return any_part;
 }
 
 template <typename T, int DP, int NW, int NK>
-__global__ __launch_bounds__(64 * NW, DP * sizeof(T) <= 256 ? 2 : 1) void k_attend_tiles(const AttendArgs a, const PagedCache c, const Sequences s,
+__global__ __launch_bounds__(64 * NW, NW == 8 || DP * sizeof(T) <= 256 ? 2 : 1) void k_attend_tiles(const AttendArgs a, const PagedCache c, const Sequences s,
                                                           const Parts parts) {
     typedef Loader<T, DP, 32 * NK, 64 * NW> L;
     constexpr int kRows = kTileRows * NW;
@@ -575,48 +667,54 @@ __global__ __launch_bounds__(64 * NW, DP * sizeof(T) <= 256 ? 2 : 1) void k_atte
     for (int i = 1; i < NW; ++i) lo = min(lo, range[0][i]), hi = max(hi, range[1][i]);
     lo = __builtin_amdgcn_readfirstlane(lo), hi = __builtin_amdgcn_readfirstlane(hi);
     int k0, k1;
-    split_range(lo, hi, split, parts.splits, 32 * NK, k0, k1);
-
     L ld(c, s.table + b * s.table_ld, kvh, threadIdx.x);
-    if (k0 < k1) {
-        const bool part = tile_pass<T, DP, NW, NK, false>(w, ld, sc, lds, k0, k1);
-        if (__syncthreads_or(part && on && w.not_finite(c.head_dim)))
-            tile_pass<T, DP, NW, NK, true>(w, ld, sc, lds, k0, k1);
-    } else {
-        w.clear();
+    split_range(ld.begin(lo), hi, split, parts.splits, 32 * NK, k0, k1);
+    w.clear();
+    if (k0 < k1) tile_pass<T, DP, NW, NK>(w, ld, sc, lds, k0, k1);
+    const bool part = k0 < w.max_lo || k0 + round_up(k1 - k0, 32 * NK) > w.min_hi;
+    const bool bad = __syncthreads_or(ld.bad());
+    const float unit = sc.capped || sc.sloped ? 1.0f : sc.c;
+    const bool again = part && !bad && on && w.not_finite(c.head_dim, other_half(w.l, false));
+    unsigned long long todo = __ballot(again);
+    todo = (todo | todo >> 32) & 0xffffffffull;
+    finish(w, a, parts, unit, split, c.head_dim, row, head, on && !(todo >> (lane & 31) & 1), bad);
+    for (; todo; todo &= todo - 1) {
+        const int i = __ffsll(todo) - 1;
+        row_alone<T>(a, c, ld.table, parts, split, __shfl(row, i, 64), __shfl(head, i, 64), __shfl(w.pos, i, 64),
+                     max(__shfl(w.lo, i, 64), k0), min(__shfl(w.hi, i, 64), k1));
     }
-    const bool bad = __syncthreads_or(ld.bad);
-    const float unit = sc.capped || a.slopes ? 1.0f : sc.c;
-    finish(w, a, parts, unit, split, c.head_dim, row, head, on, bad);
 }
 
 // ---- few rows ----------------------------------------------------------------
 
 // Up to 32 rows of a sequence and kv head (single tokens and a few more): the NW wavefronts of a workgroup
 // have tiles of 32 keys of their own, in two buffers each, and are joined at the end.
-template <typename T, int DP, int NW, bool CAREFUL>
+template <typename T, int DP, int NW>
 __device__ __forceinline__ bool few_pass(Rows<T, DP, 1>& w, Loader<T, DP, 32, 64>& ld, const Score& sc, char* lds, int k0,
                                          int k1) {
     typedef Loader<T, DP, 32, 64> L;
-    const int lane = threadIdx.x & 63;
+    constexpr int B = L::kBytes, kStep = 32 * NW;
+    const uint32_t at = __builtin_amdgcn_readfirstlane(lds_address(lds));  // keys, values; keys, values
     w.clear();
     if (k0 >= k1) return false;
     bool any_part = false;
-    ld.pages(k0, k1);
-    ld.load(lds, lds + L::kBytes, k0, k1, lane);
-    if (k0 + 32 * NW < k1) ld.pages(k0 + 32 * NW, k1);
-    int buf = 0;
+    typename L::Pages p = ld.pages(k0, k1);
+    ld.load(at, at + B, k0, k1, p);
+    p = ld.pages(k0 + kStep, k1);
+    int odd = 0;
 #pragma unroll 1
-    for (int k = k0; k < k1; k += 32 * NW, buf ^= 1) {
-        char* cur = lds + buf * 2 * L::kBytes;
-        char* nxt = lds + (buf ^ 1) * 2 * L::kBytes;
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        if (k + 32 * NW < k1) {
-            ld.load(nxt, nxt + L::kBytes, k + 32 * NW, k1, lane);
-            if (k + 64 * NW < k1) ld.pages(k + 64 * NW, k1);
+    for (int k = k0; k < k1; k += kStep, odd ^= 1) {
+        loads_done();
+        if (k + kStep < k1) {
+            const uint32_t next = at + (odd ^ 1) * 2 * B;
+            ld.load(next, next + B, k + kStep, k1, p);
         }
-        any_part = any_part || k < w.max_lo || k + 32 > w.min_hi;
-        w.template step<CAREFUL>(cur, cur + L::kBytes, k, sc);
+        p = ld.pages(k + 2 * kStep, k1);
+        any_part = any_part || w.part(k);
+        const char* cur = lds + odd * 2 * B;
+        w.scores(cur, [](int) {});
+        w.softmax(k, sc);
+        w.values(cur + B);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
     return any_part;
@@ -630,6 +728,7 @@ __global__ __launch_bounds__(64 * NW) void k_attend_few(const AttendArgs a, cons
     __shared__ __align__(16) char lds[NW][4 * L::kBytes];
     __shared__ float ml[2][NW][32];
     __shared__ int wrong[NW];
+    __shared__ unsigned again[NW];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = a.heads / c.kv_heads, d = c.head_dim;
     const int kvh = blockIdx.x % c.kv_heads, rest = blockIdx.x / c.kv_heads;
@@ -651,30 +750,35 @@ __global__ __launch_bounds__(64 * NW) void k_attend_few(const AttendArgs a, cons
     w.load((const T*)a.q.p + (int64_t)row * a.q.row + (int64_t)head * a.q.head, d, sc.negate);
     w.bounds();
     int k0, k1;
-    split_range(__builtin_amdgcn_readfirstlane(w.min_lo), __builtin_amdgcn_readfirstlane(w.max_hi), split, parts.splits, 32 * NW,
-                k0, k1);
     L ld(c, s.table + b * s.table_ld, kvh, lane);
-    k0 += 32 * wave;
-    const bool part = few_pass<T, DP, NW, false>(w, ld, sc, lds[wave], k0, k1);
-    if (__any(part && w.not_finite(d))) few_pass<T, DP, NW, true>(w, ld, sc, lds[wave], k0, k1);
-    const float unit = sc.capped || a.slopes ? 1.0f : sc.c;
+    split_range(ld.begin(w.min_lo), w.max_hi, split, parts.splits, 32 * NW, k0, k1);
+    const bool part = few_pass<T, DP, NW>(w, ld, sc, lds[wave], k0 + 32 * wave, k1);
+    const float unit = sc.capped || sc.sloped ? 1.0f : sc.c;
+    const float l = other_half(w.l, false);
+    unsigned long long todo = __ballot(part && on && w.not_finite(d, l));
+    todo = (todo | todo >> 32) & 0xffffffffull;
     if constexpr (NW == 1) {
-        finish(w, a, parts, unit, split, d, row, head, on, __any(ld.bad));
+        const bool bad = __any(ld.bad());
+        if (bad) todo = 0;
+        finish(w, a, parts, unit, split, d, row, head, on && !(todo >> (lane & 31) & 1), bad);
     } else {
-        const float l = other_half(w.l, false);
-        const bool bad = __any(ld.bad);
         if (lane < 32) ml[0][wave][lane] = w.m * unit, ml[1][wave][lane] = l;
-        if (lane == 0) wrong[wave] = bad;
+        if (lane == 0) wrong[wave] = ld.bad(), again[wave] = (unsigned)todo;
         float* mine = (float*)lds[wave];
         w.store_f32(on ? mine + (lane & 31) * DP : nullptr, d, 1.0f);
         __syncthreads();
         bool any_bad = false;
 #pragma unroll
         for (int i = 0; i < NW; ++i) any_bad = any_bad || wrong[i];
+        todo = 0;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) todo |= again[i];
+        if (any_bad) todo = 0;
         // Four columns of a row a thread.
         const int quads = d / 4;
         for (int i = threadIdx.x; i < rows * quads; i += 64 * NW) {
             const int q = i / quads, col = 4 * (i % quads);
+            if (todo >> q & 1) continue;
             float top = -INFINITY, sum = 0.0f;
 #pragma unroll
             for (int v = 0; v < NW; ++v) top = fmaxf(top, ml[0][v][q]);
@@ -705,6 +809,12 @@ __global__ __launch_bounds__(64 * NW) void k_attend_few(const AttendArgs a, cons
                 if (col == 0) parts.ml[at] = make_float2(top, sum);
             }
         }
+    }
+    for (int n = 0; todo; todo &= todo - 1, ++n) {
+        if (n % NW != wave) continue;
+        const int i = __ffsll(todo) - 1;
+        row_alone<T>(a, c, ld.table, parts, split, __shfl(row, i, 64), __shfl(head, i, 64), __shfl(w.pos, i, 64),
+                     max(__shfl(w.lo, i, 64), k0), min(__shfl(w.hi, i, 64), k1));
     }
 }
 
@@ -755,7 +865,8 @@ __global__ __launch_bounds__(256) void k_attend_join(const AttendArgs a, int d, 
     *(T4*)((T*)a.out.p + (int64_t)row * a.out.row + (int64_t)head * a.out.head + col) = y;
 }
 
-constexpr int kTileWaves = 4;
+// Wavefronts of k_attend_tiles: eight where two of them fit a SIMD's registers.
+constexpr int tile_waves(DType t, int64_t head_dim) { return 4; }
 
 // Wavefronts of k_attend_few whose buffers (two of 32 keys and values each) fit 128 KiB.
 constexpr int few_waves(int row_bytes) { return row_bytes <= 256 ? 4 : 1024 / row_bytes; }
@@ -769,8 +880,9 @@ void start(const AttendArgs& a, const PagedCache& c, const Sequences& s, const A
         k_attend_few<T, DP, NW><<<(unsigned)((int64_t)s.B * c.kv_heads * p.splits), 64 * NW, 0, st>>>(a, c, s, parts);
     } else {
         constexpr int NK = kRow <= 256 ? 2 : 1;
-        k_attend_tiles<T, DP, kTileWaves, NK>
-            <<<(unsigned)(p.tiles * c.kv_heads * p.splits), 64 * kTileWaves, 0, st>>>(a, c, s, parts);
+        constexpr int NW = tile_waves(sizeof(T) == 4 ? DType::f32 : DType::bf16, DP);
+        k_attend_tiles<T, DP, NW, NK>
+            <<<(unsigned)(p.tiles * c.kv_heads * p.splits), 64 * NW, 0, st>>>(a, c, s, parts);
     }
     if (p.splits > 1)
         k_attend_join<T><<<(unsigned)((int64_t)s.rows * a.heads), 256, 0, st>>>(a, c.head_dim, s, parts);
@@ -802,7 +914,7 @@ AttendPlan attend_plan(const AttendShape& q, int64_t cus) {
         // Eight workgroups a compute unit.
         p.splits = (int)std::max<int64_t>(1, std::min(ceil_div(8 * cus, wgs), ceil_div(len, step)));
     } else {
-        const int64_t rows = kTileRows * kTileWaves;
+        const int64_t rows = kTileRows * tile_waves(q.t, q.head_dim);
         p.tiles = std::min(q.rows * g / rows + q.B, q.B * ceil_div(q.max_new * g, rows));
         wgs = p.tiles * q.kv_heads;
         step = 512;

@@ -553,7 +553,7 @@ int64_t w8a8_plan_bytes(const W8A8Plan& p, int ng, int64_t M, int64_t K, int64_t
 hipError_t launch_w8a8(const W8A8Args& a, int ng, const W8A8Plan& p, void* ws, hipStream_t s);
 
 // ---- attention over a paged cache (sgq_rope.hip, sgq_attention.hip) -------
-constexpr int kHeadDimStep = 16, kMaxHeadDim = 256;
+constexpr int kHeadDimStep = 16, kMaxHeadDim = 256, kMinPage = 8, kMaxPage = 65536;
 constexpr int kMaxHeads = 1024, kMaxHeadRows = 1 << 23, kMaxSequences = 1 << 20;  // launches of fewer than 2^32 threads
 struct HeadRows {  // [rows, heads, head_dim], strides in elements
     void* p;
@@ -563,6 +563,7 @@ struct PagedCache {
     char* k;
     char* v;
     int64_t page_stride, token_stride, head_stride;  // elements
+    uint32_t page_bytes, token_bytes;                // the first two in bytes
     int pages, page_log, kv_heads, head_dim;
     DType t;
 };

@@ -52,11 +52,11 @@ def _append(op, lib, cache={}, seqs={}, q=4 * P, q_row=512, q_head=64, k=4 * P +
 SHARED = [
     (INVALID, dict(cache=dict(dtype=3))), (UNSUPPORTED, dict(cache=dict(head_dim=40))), (UNSUPPORTED, dict(cache=dict(head_dim=272))),
     (UNSUPPORTED, dict(cache=dict(head_dim=0))), (UNSUPPORTED, dict(cache=dict(page_size=12))),
-    (UNSUPPORTED, dict(cache=dict(page_size=1 << 17))), (UNSUPPORTED, dict(cache=dict(page_size=0))),
+    (UNSUPPORTED, dict(cache=dict(page_size=1 << 17))), (UNSUPPORTED, dict(cache=dict(page_size=0))), (UNSUPPORTED, dict(cache=dict(page_size=4))),
     (INVALID, dict(cache=dict(kv_heads=0))), (INVALID, dict(cache=dict(kv_heads=3, head_stride=64))), (INVALID, dict(cache=dict(pages=-1))),
     (INVALID, dict(cache=dict(token_stride=60))), (INVALID, dict(cache=dict(token_stride=56))),
     (INVALID, dict(cache=dict(head_stride=-64))), (INVALID, dict(cache=dict(page_stride=0))),
-    (INVALID, dict(cache=dict(page_stride=1 << 41))), (INVALID, dict(cache=dict(k=P + 8))), (INVALID, dict(cache=dict(v=None))),
+    (UNSUPPORTED, dict(cache=dict(page_stride=1 << 31))), (UNSUPPORTED, dict(cache=dict(token_stride=1 << 31))), (UNSUPPORTED, dict(cache=dict(head_stride=1 << 41))), (INVALID, dict(cache=dict(k=P + 8))), (INVALID, dict(cache=dict(v=None))),
     (INVALID, dict(seqs=dict(B=-1))), (INVALID, dict(seqs=dict(max_len=-1))), (INVALID, dict(seqs=dict(max_new=-1))),
     (INVALID, dict(seqs=dict(table_ld=3))), (INVALID, dict(seqs=dict(table=None))), (INVALID, dict(seqs=dict(lens=None))),
     (INVALID, dict(seqs=dict(starts=None))), (UNSUPPORTED, dict(seqs=dict(B=(1 << 20) + 1))),

@@ -151,13 +151,13 @@ SHAPES = [  # sequences (new, keys), page, heads, kv_heads, head_dim
     ([(1, 1)], 16, 1, 1, 64),
     ([(1, 2), (1, 1), (1, 33)], 16, 4, 2, 128),
     ([(1, 1000), (1, 64), (1, 65), (1, 63), (1, 513)], 16, 8, 2, 128),
-    ([(1, 300)] * 3, 1, 16, 16, 64),
+    ([(1, 300)] * 3, 8, 16, 16, 64),
     ([(2, 100), (0, 50), (3, 3), (0, 0), (4, 200)], 32, 8, 1, 128),
     ([(5, 5), (1, 700), (17, 40), (32, 32)], 8, 8, 2, 80),
     ([(33, 90), (31, 31)], 64, 2, 2, 16),
     ([(130, 130), (1, 400), (63, 200)], 16, 6, 3, 96),
     ([(257, 300), (127, 127)], 128, 4, 2, 128),
-    ([(100, 333)], 4, 14, 2, 112),
+    ([(100, 333)], 8, 14, 2, 112),
     ([(70, 150), (1, 150)], 16, 4, 4, 192),
     ([(40, 260), (129, 129), (1, 90)], 32, 4, 1, 256),
     ([(500, 1100)], 256, 8, 8, 64),
@@ -357,7 +357,7 @@ def test_norm_rope_append(op, dev, shape, interleaved, dtype):
     H, KV, d, rot = ROPES[shape]
     seqs = [(1, 1), (7, 40), (0, 12), (1, 17), (64, 64), (3, 100003)] if shape == 1 else [(1, 1), (7, 40), (0, 12), (33, 49)]
     hole = 3.0
-    page = 1 << shape % 6
+    page = 8 << shape % 6
     b = Batch(op, dev, seqs, page, KV, d, dtype, hole=hole, head_major=shape % 2 == 0, pad=2)
     before = b.k.clone(), b.v.clone()
     qkv = _randn(dev, shape, b.rows, H + 2 * KV, d).to(dtype)
@@ -389,13 +389,13 @@ def test_norm_rope_append(op, dev, shape, interleaved, dtype):
 
 
 def test_one_norm_of_two(op, dev):
-    b = Batch(op, dev, [(5, 9)], 4, 2, 64, torch.float32)
+    b = Batch(op, dev, [(5, 9)], 8, 2, 64, torch.float32)
     q, k, v = (_randn(dev, i, 5, 2, 64) for i in range(3))
     g = 1 + 0.1 * _randn(dev, 9, 64)
     y = op.norm_rope_append(q, k, v, b.kv, b.batch, k_norm=g)
     assert torch.equal(y, q)
     pos = torch.arange(4, 9, device=dev)
-    where = b.table[0, pos // 4].long(), pos % 4
+    where = b.table[0, pos // 8].long(), pos % 8
     _close(b.k[where], *_turned(k, g, 1e-5, None, pos, False), 64, torch.float32)
 
 
