@@ -331,6 +331,22 @@ struct Rows {
                 if (32 * i + 8 * (e / 4) + 4 * h < d) bad = bad || !isfinite(o[i][e]);
         return bad && sum == sum;
     }
+    // Values v of a key that are not finite, to the rows that see it.
+    __device__ __forceinline__ void add_not_finite(const T* v, int key, int d) {
+        const int h = (threadIdx.x & 63) >> 5;
+        const bool sees = key >= lo && key < hi;
+#pragma unroll
+        for (int i = 0; i < kCols; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                typedef T T4 __attribute__((ext_vector_type(4)));
+                const int col = 32 * i + 2 * e + 4 * h;
+                const T4 x = *(const T4*)(v + min(col, d - 4));
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (sees && col < d && !isfinite((float)x[j])) o[i][e + j] += (float)x[j];
+            }
+    }
     // The row's columns times w, as T, 16 bytes a store.
     __device__ __forceinline__ void store(T* out, int d, float w) const {
         const int h = (threadIdx.x & 63) >> 5;
@@ -462,6 +478,40 @@ struct Loader {
     static __device__ __forceinline__ void arrived(Pages& p) { asm volatile("" : "+v"(p.of)); }
 };
 
+// A weight of 0 times an infinity or a NaN is a NaN: values that are not finite touch rows that do not see them,
+// in tiles whose keys some rows see and some do not.  Where a row's result is not finite after such a tile, the
+// wavefront (workgroup) goes over its keys again with such values taken out of those tiles (clean_values), and adds them to
+// the rows that see them at the end (add_values).  THREADS threads, all of which come along.
+template <typename T, int BYTES, int THREADS>
+__device__ __forceinline__ void clean_values(char* tile, int thread) {
+    typedef typename Chunk<T>::type Vec;
+    for (int i = thread * 16; i < BYTES; i += THREADS * 16) {
+        Vec v = *(const Vec*)(tile + i);
+#pragma unroll
+        for (int e = 0; e < Chunk<T>::N; ++e) v[e] = isfinite((float)v[e]) ? v[e] : (T)0.0f;
+        *(Vec*)(tile + i) = v;
+    }
+}
+template <typename T, int DP, int NK>
+__device__ __forceinline__ void add_values(Rows<T, DP, NK>& w, const PagedCache& c, const int32_t* table, int kvh, int k0, int k1,
+                                           int step, int max_lo, int min_hi) {
+    const int lane = threadIdx.x & 63, d = c.head_dim;
+#pragma unroll 1
+    for (int k = k0; k < k1; k += step) {
+        if (k >= max_lo && k + 32 * NK <= min_hi) continue;
+#pragma unroll 1
+        for (int key = k; key < min(k + 32 * NK, k1); ++key) {
+            const int64_t off = key_offset(c, table, key);
+            if (off < 0) continue;  // the result is NaN anyway
+            const T* v = (const T*)c.v + off + (int64_t)kvh * c.head_stride;
+            bool bad = false;
+#pragma unroll
+            for (int i = 0; i < kMaxHeadDim / 64; ++i) bad = bad || !isfinite((float)v[min(lane + 64 * i, d - 1)]);
+            if (__any(bad)) w.add_not_finite(v, key, d);
+        }
+    }
+}
+
 // Where a launch's partial results lie: for (row, head) r and split s, fp32 columns at
 // o[(r * splits + s) * d ..] and (maximum, sum) at ml[r * splits + s].  The maximum is of exponents of 2.
 struct Parts {
@@ -494,56 +544,6 @@ __device__ __forceinline__ void finish(const Rows<T, DP, NK>& w, const AttendArg
     }
 }
 
-// One row by a whole wavefront, key by key, over the keys [lo, hi) alone, as finish() leaves it.  In a tile whose
-// keys some rows do not see, a weight of 0 times an infinity or a NaN among the values would be a NaN for those
-// rows: where such a tile's row came out not finite it is done again here, with what it sees.
-template <typename T>
-__device__ __forceinline__ void row_alone(const AttendArgs& a, const PagedCache& c, const int32_t* table, const Parts& parts,
-                                          int split, int row, int head, int pos, int lo, int hi) {
-    const int lane = threadIdx.x & 63, d = c.head_dim;
-    const int64_t kv = (int64_t)(head / (a.heads / c.kv_heads)) * c.head_stride;
-    const T* q = (const T*)a.q.p + (int64_t)row * a.q.row + (int64_t)head * a.q.head;
-    const float slope = a.slopes ? a.slopes[head] : 0.0f;
-    float x[kMaxHeadDim / 64], o[kMaxHeadDim / 64], m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kMaxHeadDim / 64; ++i) x[i] = lane + 64 * i < d ? (float)q[lane + 64 * i] : 0.0f, o[i] = 0.0f;
-    for (int j = lo; j < hi && l == l; ++j) {  // a sum of NaN stays one
-        const int64_t off = key_offset(c, table, j);
-        if (off < 0) break;  // the caller has seen that
-        const T* k = (const T*)c.k + off + kv;
-        const T* v = (const T*)c.v + off + kv;
-        float s = 0.0f, y[kMaxHeadDim / 64];
-#pragma unroll
-        for (int i = 0; i < kMaxHeadDim / 64; ++i) {
-            const bool on = lane + 64 * i < d;
-            s = fmaf(x[i], on ? (float)k[lane + 64 * i] : 0.0f, s);
-            y[i] = on ? (float)v[lane + 64 * i] : 0.0f;
-        }
-#pragma unroll
-        for (int t = 32; t > 0; t >>= 1) s += __shfl_xor(s, t, 64);
-        s *= a.scale;
-        if (a.softcap > 0.0f) s = a.softcap * tanhf(s / a.softcap);
-        s = fmaf(-slope, (float)abs(pos - j), s);
-        const float now = fmaxf(m, s), base = now == -INFINITY ? 0.0f : now;
-        const float w = expf(m - base), e = expf(s - base);
-        l = fmaf(l, w, e), m = now;
-#pragma unroll
-        for (int i = 0; i < kMaxHeadDim / 64; ++i) o[i] = fmaf(o[i], w, e * y[i]);
-    }
-    const int64_t at = ((int64_t)row * a.heads + head) * parts.splits + split;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-    for (int i = 0; i < kMaxHeadDim / 64; ++i) {
-        const int col = lane + 64 * i;
-        if (col >= d) continue;
-        if (parts.splits == 1)
-            ((T*)a.out.p)[(int64_t)row * a.out.row + (int64_t)head * a.out.head + col] = (T)(o[i] * inv);
-        else
-            parts.o[at * d + col] = o[i];
-    }
-    if (parts.splits > 1 && lane == 0) parts.ml[at] = make_float2(m * kLog2e, l);
-}
-
 // What a workgroup of a sequence that breaks a bound does: NaN for rows [first, end).
 template <typename T>
 __device__ __forceinline__ void poison(const AttendArgs& a, const Parts& parts, int d, int first, int end, int h0, int heads,
@@ -572,9 +572,9 @@ __device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)"
 
 // A workgroup of NW wavefronts takes 32 NW rows of one sequence and kv head, which share tiles of
 // 32 NK keys in two buffers: while one is worked on, the next loads.
-template <typename T, int DP, int NW, int NK>
+template <typename T, int DP, int NW, int NK, bool CLEAN>
 __device__ __forceinline__ void tile_pass(Rows<T, DP, NK>& w, Loader<T, DP, 32 * NK, 64 * NW>& ld, const Score& sc, char* lds,
-                                          int k0, int k1) {
+                                          int k0, int k1, int max_lo, int min_hi) {
     typedef Loader<T, DP, 32 * NK, 64 * NW> L;
     constexpr int kKeys = 32 * NK, B = L::kBytes;
     const uint32_t at = __builtin_amdgcn_readfirstlane(lds_address(lds));  // keys, values; keys, values
@@ -586,7 +586,11 @@ __device__ __forceinline__ void tile_pass(Rows<T, DP, NK>& w, Loader<T, DP, 32 *
     int odd = 0;
 #pragma unroll 1
     for (int k = k0; k < k1; k += kKeys, odd ^= 1) {
-        const char* const cur = lds + odd * 2 * B;
+        char* const cur = lds + odd * 2 * B;
+        if (CLEAN && (k < max_lo || k + kKeys > min_hi)) {
+            clean_values<T, B, 64 * NW>(cur + B, threadIdx.x);
+            phase_end();
+        }
         const uint32_t next = at + (odd ^ 1) * 2 * B;
         L::arrived(p);
         // The next tile's loads beside the products of the scores, which leave the scalar unit idle (after the last
@@ -606,12 +610,12 @@ __device__ __forceinline__ void tile_pass(Rows<T, DP, NK>& w, Loader<T, DP, 32 *
 }
 
 template <typename T, int DP, int NW, int NK>
-__global__ __launch_bounds__(64 * NW, NW == 8 || DP * sizeof(T) <= 256 ? 2 : 1) void k_attend_tiles(const AttendArgs a, const PagedCache c, const Sequences s,
+__global__ __launch_bounds__(64 * NW, DP * sizeof(T) <= 256 ? 2 : 1) void k_attend_tiles(const AttendArgs a, const PagedCache c, const Sequences s,
                                                           const Parts parts) {
     typedef Loader<T, DP, 32 * NK, 64 * NW> L;
     constexpr int kRows = kTileRows * NW;
     __shared__ __align__(16) char lds[4 * L::kBytes];
-    __shared__ int range[2][NW];
+    __shared__ int range[4][NW];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = a.heads / c.kv_heads;
     const int kvh = blockIdx.x % c.kv_heads, split = blockIdx.x / c.kv_heads % parts.splits;
@@ -660,36 +664,37 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || DP * sizeof(T) <= 256 ? 2 : 1) 
     w.slope = a.slopes ? a.slopes[head] * kLog2e : 0.0f;
     w.load((const T*)a.q.p + (int64_t)row * a.q.row + (int64_t)head * a.q.head, c.head_dim, sc.negate);
     w.bounds();
-    if (lane == 0) range[0][wave] = w.min_lo, range[1][wave] = w.max_hi;
+    if (lane == 0) range[0][wave] = w.min_lo, range[1][wave] = w.max_hi, range[2][wave] = w.max_lo, range[3][wave] = w.min_hi;
     __syncthreads();
-    int lo = range[0][0], hi = range[1][0];
+    int lo = range[0][0], hi = range[1][0], max_lo = range[2][0], min_hi = range[3][0];
 #pragma unroll
-    for (int i = 1; i < NW; ++i) lo = min(lo, range[0][i]), hi = max(hi, range[1][i]);
+    for (int i = 1; i < NW; ++i) {
+        lo = min(lo, range[0][i]), hi = max(hi, range[1][i]);
+        max_lo = max(max_lo, range[2][i]), min_hi = min(min_hi, range[3][i]);
+    }
     lo = __builtin_amdgcn_readfirstlane(lo), hi = __builtin_amdgcn_readfirstlane(hi);
+    max_lo = __builtin_amdgcn_readfirstlane(max_lo), min_hi = __builtin_amdgcn_readfirstlane(min_hi);
     int k0, k1;
     L ld(c, s.table + b * s.table_ld, kvh, threadIdx.x);
     split_range(ld.begin(lo), hi, split, parts.splits, 32 * NK, k0, k1);
     w.clear();
-    if (k0 < k1) tile_pass<T, DP, NW, NK>(w, ld, sc, lds, k0, k1);
-    const bool part = k0 < w.max_lo || k0 + round_up(k1 - k0, 32 * NK) > w.min_hi;
+    if (k0 < k1) tile_pass<T, DP, NW, NK, false>(w, ld, sc, lds, k0, k1, max_lo, min_hi);
     const bool bad = __syncthreads_or(ld.bad());
-    const float unit = sc.capped || sc.sloped ? 1.0f : sc.c;
-    const bool again = part && !bad && on && w.not_finite(c.head_dim, other_half(w.l, false));
-    unsigned long long todo = __ballot(again);
-    todo = (todo | todo >> 32) & 0xffffffffull;
-    finish(w, a, parts, unit, split, c.head_dim, row, head, on && !(todo >> (lane & 31) & 1), bad);
-    for (; todo; todo &= todo - 1) {
-        const int i = __ffsll(todo) - 1;
-        row_alone<T>(a, c, ld.table, parts, split, __shfl(row, i, 64), __shfl(head, i, 64), __shfl(w.pos, i, 64),
-                     max(__shfl(w.lo, i, 64), k0), min(__shfl(w.hi, i, 64), k1));
+    const bool part = k0 < k1 && (k0 < max_lo || k0 + round_up(k1 - k0, 32 * NK) > min_hi);
+    if (!bad && __builtin_expect(__syncthreads_or(part && on && w.not_finite(c.head_dim, other_half(w.l, false))), 0)) {
+        w.clear();
+        tile_pass<T, DP, NW, NK, true>(w, ld, sc, lds, k0, k1, max_lo, min_hi);
+        add_values(w, c, ld.table, kvh, k0, k1, 32 * NK, max_lo, min_hi);
     }
+    const float unit = sc.capped || sc.sloped ? 1.0f : sc.c;
+    finish(w, a, parts, unit, split, c.head_dim, row, head, on, bad);
 }
 
 // ---- few rows ----------------------------------------------------------------
 
 // Up to 32 rows of a sequence and kv head (single tokens and a few more): the NW wavefronts of a workgroup
 // have tiles of 32 keys of their own, in two buffers each, and are joined at the end.
-template <typename T, int DP, int NW>
+template <typename T, int DP, int NW, bool CLEAN>
 __device__ __forceinline__ bool few_pass(Rows<T, DP, 1>& w, Loader<T, DP, 32, 64>& ld, const Score& sc, char* lds, int k0,
                                          int k1) {
     typedef Loader<T, DP, 32, 64> L;
@@ -711,7 +716,8 @@ __device__ __forceinline__ bool few_pass(Rows<T, DP, 1>& w, Loader<T, DP, 32, 64
         }
         p = ld.pages(k + 2 * kStep, k1);
         any_part = any_part || w.part(k);
-        const char* cur = lds + odd * 2 * B;
+        char* const cur = lds + odd * 2 * B;
+        if (CLEAN && w.part(k)) clean_values<T, B, 64>(cur + B, threadIdx.x & 63);
         w.scores(cur, [](int) {});
         w.softmax(k, sc);
         w.values(cur + B);
@@ -728,7 +734,6 @@ __global__ __launch_bounds__(64 * NW) void k_attend_few(const AttendArgs a, cons
     __shared__ __align__(16) char lds[NW][4 * L::kBytes];
     __shared__ float ml[2][NW][32];
     __shared__ int wrong[NW];
-    __shared__ unsigned again[NW];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = a.heads / c.kv_heads, d = c.head_dim;
     const int kvh = blockIdx.x % c.kv_heads, rest = blockIdx.x / c.kv_heads;
@@ -752,33 +757,30 @@ __global__ __launch_bounds__(64 * NW) void k_attend_few(const AttendArgs a, cons
     int k0, k1;
     L ld(c, s.table + b * s.table_ld, kvh, lane);
     split_range(ld.begin(w.min_lo), w.max_hi, split, parts.splits, 32 * NW, k0, k1);
-    const bool part = few_pass<T, DP, NW>(w, ld, sc, lds[wave], k0 + 32 * wave, k1);
+    const bool part = few_pass<T, DP, NW, false>(w, ld, sc, lds[wave], k0 + 32 * wave, k1);
+    float l = other_half(w.l, false);
+    if (__builtin_expect(__any(part && on && w.not_finite(d, l)), 0)) {
+        few_pass<T, DP, NW, true>(w, ld, sc, lds[wave], k0 + 32 * wave, k1);
+        l = other_half(w.l, false);
+        add_values(w, c, ld.table, kvh, k0 + 32 * wave, k1, 32 * NW, w.max_lo, w.min_hi);
+    }
     const float unit = sc.capped || sc.sloped ? 1.0f : sc.c;
-    const float l = other_half(w.l, false);
-    unsigned long long todo = __ballot(part && on && w.not_finite(d, l));
-    todo = (todo | todo >> 32) & 0xffffffffull;
+    const bool bad = __any(ld.bad());
     if constexpr (NW == 1) {
-        const bool bad = __any(ld.bad());
-        if (bad) todo = 0;
-        finish(w, a, parts, unit, split, d, row, head, on && !(todo >> (lane & 31) & 1), bad);
+        finish(w, a, parts, unit, split, d, row, head, on, bad);
     } else {
         if (lane < 32) ml[0][wave][lane] = w.m * unit, ml[1][wave][lane] = l;
-        if (lane == 0) wrong[wave] = ld.bad(), again[wave] = (unsigned)todo;
+        if (lane == 0) wrong[wave] = bad;
         float* mine = (float*)lds[wave];
         w.store_f32(on ? mine + (lane & 31) * DP : nullptr, d, 1.0f);
         __syncthreads();
         bool any_bad = false;
 #pragma unroll
         for (int i = 0; i < NW; ++i) any_bad = any_bad || wrong[i];
-        todo = 0;
-#pragma unroll
-        for (int i = 0; i < NW; ++i) todo |= again[i];
-        if (any_bad) todo = 0;
         // Four columns of a row a thread.
         const int quads = d / 4;
         for (int i = threadIdx.x; i < rows * quads; i += 64 * NW) {
             const int q = i / quads, col = 4 * (i % quads);
-            if (todo >> q & 1) continue;
             float top = -INFINITY, sum = 0.0f;
 #pragma unroll
             for (int v = 0; v < NW; ++v) top = fmaxf(top, ml[0][v][q]);
@@ -809,12 +811,6 @@ __global__ __launch_bounds__(64 * NW) void k_attend_few(const AttendArgs a, cons
                 if (col == 0) parts.ml[at] = make_float2(top, sum);
             }
         }
-    }
-    for (int n = 0; todo; todo &= todo - 1, ++n) {
-        if (n % NW != wave) continue;
-        const int i = __ffsll(todo) - 1;
-        row_alone<T>(a, c, ld.table, parts, split, __shfl(row, i, 64), __shfl(head, i, 64), __shfl(w.pos, i, 64),
-                     max(__shfl(w.lo, i, 64), k0), min(__shfl(w.hi, i, 64), k1));
     }
 }
 
@@ -865,8 +861,7 @@ __global__ __launch_bounds__(256) void k_attend_join(const AttendArgs a, int d, 
     *(T4*)((T*)a.out.p + (int64_t)row * a.out.row + (int64_t)head * a.out.head + col) = y;
 }
 
-// Wavefronts of k_attend_tiles: eight where two of them fit a SIMD's registers.
-constexpr int tile_waves(DType t, int64_t head_dim) { return 4; }
+constexpr int kTileWaves = 4;
 
 // Wavefronts of k_attend_few whose buffers (two of 32 keys and values each) fit 128 KiB.
 constexpr int few_waves(int row_bytes) { return row_bytes <= 256 ? 4 : 1024 / row_bytes; }
@@ -880,9 +875,8 @@ void start(const AttendArgs& a, const PagedCache& c, const Sequences& s, const A
         k_attend_few<T, DP, NW><<<(unsigned)((int64_t)s.B * c.kv_heads * p.splits), 64 * NW, 0, st>>>(a, c, s, parts);
     } else {
         constexpr int NK = kRow <= 256 ? 2 : 1;
-        constexpr int NW = tile_waves(sizeof(T) == 4 ? DType::f32 : DType::bf16, DP);
-        k_attend_tiles<T, DP, NW, NK>
-            <<<(unsigned)(p.tiles * c.kv_heads * p.splits), 64 * NW, 0, st>>>(a, c, s, parts);
+        k_attend_tiles<T, DP, kTileWaves, NK>
+            <<<(unsigned)(p.tiles * c.kv_heads * p.splits), 64 * kTileWaves, 0, st>>>(a, c, s, parts);
     }
     if (p.splits > 1)
         k_attend_join<T><<<(unsigned)((int64_t)s.rows * a.heads), 256, 0, st>>>(a, c.head_dim, s, parts);
@@ -914,7 +908,7 @@ AttendPlan attend_plan(const AttendShape& q, int64_t cus) {
         // Eight workgroups a compute unit.
         p.splits = (int)std::max<int64_t>(1, std::min(ceil_div(8 * cus, wgs), ceil_div(len, step)));
     } else {
-        const int64_t rows = kTileRows * tile_waves(q.t, q.head_dim);
+        const int64_t rows = kTileRows * kTileWaves;
         p.tiles = std::min(q.rows * g / rows + q.B, q.B * ceil_div(q.max_new * g, rows));
         wgs = p.tiles * q.kv_heads;
         step = 512;
