@@ -544,7 +544,8 @@ typedef struct sgq_scores {
  * calling thread's current device), 16-byte aligned, else SGQ_ERR_WORKSPACE; it needs
  * no initialisation, and calls that overlap in time must not share one. */
 int64_t sgq_paged_attention_workspace_bytes(int64_t heads, int64_t kv_heads, int64_t head_dim, int dtype, int64_t B,
-                                            int64_t rows, int64_t max_len, int64_t max_new, int compute_units);
+                                            int64_t rows, int64_t max_len, int64_t max_new, int64_t window,
+                                            int compute_units);
 int sgq_paged_attention(const void* q, int64_t q_row, int64_t q_head, void* out, int64_t out_row, int64_t out_head,
                         int64_t rows, int64_t heads, const sgq_paged_cache* cache, const sgq_sequences* seqs,
                         const sgq_scores* scores, void* workspace, int64_t workspace_bytes, void* stream);

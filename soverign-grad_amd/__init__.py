@@ -97,7 +97,7 @@ SIGNATURES = {
                                _i64, _vp]),
     "sgq_norm_rope_append": (_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _vp,
                                     _vp, _vp, _vp, ctypes.c_float, _vp, _i64, _int, _vp, _vp]),
-    "sgq_paged_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _int, _i64, _i64, _i64, _i64, _int]),
+    "sgq_paged_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _int, _i64, _i64, _i64, _i64, _i64, _int]),
     "sgq_paged_attention": (_int, [_vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp]),
     "sgq_w8a8_plan": (_int, [_int, _i64, _i64, _i64, _int, ctypes.POINTER(_int), ctypes.POINTER(_int)]),
 }

@@ -216,10 +216,10 @@ def norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv: Page
     return out
 
 
-def _attention_workspace(kv: PagedKV, batch: SequenceBatch, T: int, H: int, dev: torch.device):
+def _attention_workspace(kv: PagedKV, batch: SequenceBatch, T: int, H: int, window: int, dev: torch.device):
     """A workspace of its own for each call: what a graph captures stays the graph's."""
     s = kv._struct
-    args = (H, s.kv_heads, s.head_dim, s.dtype, batch._struct.B, T, batch.max_len, batch.max_new, 0)
+    args = (H, s.kv_heads, s.head_dim, s.dtype, batch._struct.B, T, batch.max_len, batch.max_new, window, 0)
     query = load_library().sgq_paged_attention_workspace_bytes
     if dev.index == _current_device():
         need = query(*args)
@@ -261,7 +261,7 @@ def paged_attention(q: torch.Tensor, kv: PagedKV, batch: SequenceBatch, scale: O
     how = _Scores(1.0 / math.sqrt(d) if scale is None else scale, softcap, window,
                   None if slopes is None else slopes.data_ptr(), None if prefix is None else prefix.data_ptr(),
                   None if first is None else first.data_ptr())
-    ws, need = _attention_workspace(kv, batch, T, H, dev)
+    ws, need = _attention_workspace(kv, batch, T, H, window, dev)
     _call(dev, load_library().sgq_paged_attention, q.data_ptr(), q_row, q_head, out.data_ptr(), o_row, o_head, T, H,
           kv._at, batch._at, ctypes.addressof(how), None if ws is None else ws.data_ptr(), need)
     return out

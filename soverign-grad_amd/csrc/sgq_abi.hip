@@ -1319,10 +1319,12 @@ int sgq_norm_rope_append(const void* q, int64_t q_row, int64_t q_head, const voi
 }
 
 int64_t sgq_paged_attention_workspace_bytes(int64_t heads, int64_t kv_heads, int64_t head_dim, int dtype, int64_t B,
-                                            int64_t rows, int64_t max_len, int64_t max_new, int compute_units) {
-    if (bad_dtype(dtype) || bad_attention(heads, kv_heads, head_dim, B, rows, max_len, max_new) || compute_units < 0) return -1;
+                                            int64_t rows, int64_t max_len, int64_t max_new, int64_t window,
+                                            int compute_units) {
+    if (bad_dtype(dtype) || bad_attention(heads, kv_heads, head_dim, B, rows, max_len, max_new) || window < 0 ||
+        compute_units < 0) return -1;
     if (B == 0 || rows == 0) return 0;
-    const AttendShape q = {heads, kv_heads, head_dim, B, rows, max_len, max_new, (DType)dtype};
+    const AttendShape q = {heads, kv_heads, head_dim, B, rows, max_len, max_new, window < kMaxDim ? window : kMaxDim, (DType)dtype};
     return attend_plan_bytes(attend_plan(q, compute_units > 0 ? compute_units : device_cus(nullptr)), q);
 }
 
@@ -1352,7 +1354,7 @@ int sgq_paged_attention(const void* q, int64_t q_row, int64_t q_head, void* out,
     a.heads = (int)heads, a.scale = scores->scale, a.softcap = scores->softcap;
     a.window = (int)(scores->window < kMaxDim ? scores->window : kMaxDim);
     a.slopes = scores->alibi_slopes, a.prefix = scores->prefix, a.first_key = scores->first_key;
-    const AttendShape shape = {heads, c.kv_heads, d, s.B, s.rows, s.max_len, s.max_new, c.t};
+    const AttendShape shape = {heads, c.kv_heads, d, s.B, s.rows, s.max_len, s.max_new, a.window, c.t};
     const AttendPlan p = attend_plan(shape, device_cus((hipStream_t)stream));
     if (p.workgroups * 512 >= (int64_t)1 << 32 || (p.splits > 1 && (int64_t)s.rows * heads * 256 >= (int64_t)1 << 32))
         return fail(SGQ_ERR_UNSUPPORTED, "%s: too many rows for one call", fn);

@@ -253,7 +253,9 @@ struct Rows {
     // S^T of the keys in the tile at ks.  The LDS reads of four products are issued ahead of the four before
     // them; left alone, the compiler reads for each product as it comes and waits.  beside(g): what is issued
     // beside the g-th four.
-    static constexpr int kScoreGroups = (kFrags * NK + 3) / 4;
+    // (One ahead of one for the widest heads in 16 bits, which leave few registers: 1024 rows of 16 heads of 256, a window of
+    // 4096 keys 123 us, with two 127, with four 160.)
+    static constexpr int kAhead = DP == 256 && sizeof(T) == 2 ? 1 : 4, kScoreGroups = (kFrags * NK + kAhead - 1) / kAhead;
     template <typename F>
     __device__ __forceinline__ void scores(const char* ks, F beside) {
         const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
@@ -263,7 +265,7 @@ struct Rows {
         for (int t = 0; t < NK; ++t)
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[t][e] = 0.0f;
-        constexpr int N = kFrags * NK, G = 4;
+        constexpr int N = kFrags * NK, G = kAhead;
         auto read = [&](int j) { return *(const Frag*)(row + j % NK * 32 * Tile::kRow + ((j / NK * 32) ^ x)); };
         Frag f[2][G];
 #pragma unroll
@@ -559,6 +561,7 @@ __device__ __forceinline__ void poison(const AttendArgs& a, const Parts& parts, 
 }
 
 constexpr int kTileRows = 32;  // of a wavefront
+constexpr int kJoinSplits = 256, kWaveSplits = 16;
 
 // ---- tiles of rows ----------------------------------------------------------
 
@@ -610,7 +613,7 @@ __device__ __forceinline__ void tile_pass(Rows<T, DP, NK>& w, Loader<T, DP, 32 *
 }
 
 template <typename T, int DP, int NW, int NK>
-__global__ __launch_bounds__(64 * NW, DP * sizeof(T) <= 256 ? 2 : 1) void k_attend_tiles(const AttendArgs a, const PagedCache c, const Sequences s,
+__global__ __launch_bounds__(64 * NW, DP * sizeof(T) <= 512 ? 2 : 1) void k_attend_tiles(const AttendArgs a, const PagedCache c, const Sequences s,
                                                           const Parts parts) {
     typedef Loader<T, DP, 32 * NK, 64 * NW> L;
     constexpr int kRows = kTileRows * NW;
@@ -816,43 +819,65 @@ __global__ __launch_bounds__(64 * NW) void k_attend_few(const AttendArgs a, cons
 
 // ---- the splits of a row joined ------------------------------------------------
 
-// A workgroup per row and head: its threads take four columns and a share of the splits each.
-template <typename T>
+// W wavefronts per row and head (a workgroup has four): the factors of the splits first, to LDS, then four columns and a
+// share of the splits a thread, whose loads are independent.
+template <typename T, int W>
 __global__ __launch_bounds__(256) void k_attend_join(const AttendArgs a, int d, const Sequences s, const Parts parts) {
+    constexpr int kThreads = 64 * W, kItems = 4 / W, kSplits = W == 4 ? kJoinSplits : kWaveSplits;
+    __shared__ float factor[kItems][kSplits];
     __shared__ f32x4 red[256];
-    __shared__ float total[256];
-    const int row = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
+    __shared__ float part[2][4];
+    const int own = threadIdx.x / kThreads, t = threadIdx.x % kThreads;
+    const int item = min((int)blockIdx.x * kItems + own, s.rows * a.heads - 1);  // the last again: the same result
+    const int row = item / a.heads, head = item % a.heads;
     const int b = seq_of_row(s, row);
-    if (b >= s.B) return;
-    const SeqRows r = seq_rows(s, b);
-    if (row < r.row0 || row >= r.row0 + r.n) return;
-    const int64_t at = (int64_t)blockIdx.x * parts.splits;
-    float top = -INFINITY;
-    for (int i = threadIdx.x & 63; i < parts.splits; i += 64) top = fmaxf(top, parts.ml[at + i].x);
+    bool on = b < s.B;
+    if (on) {
+        const SeqRows r = seq_rows(s, b);
+        on = row >= r.row0 && row < r.row0 + r.n;
+    }
+    const int64_t at = (int64_t)item * parts.splits;
+    const float2 v = on && t < parts.splits ? parts.ml[at + t] : make_float2(-INFINITY, 0.0f);
+    float top = v.x;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-    if (top == -INFINITY) top = 0.0f;
-    const int quads = d / 4, groups = 256 / quads, grp = threadIdx.x / quads, col = 4 * (threadIdx.x % quads);
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    float sum = 0.0f;
-    if (grp < groups)
-        for (int i = grp; i < parts.splits; i += groups) {
-            const float2 v = parts.ml[at + i];
-            if (v.y == 0.0f) continue;
-            const float f = __builtin_amdgcn_exp2f(v.x - top);
-            sum = fmaf(v.y, f, sum);
-            if (v.y != v.y) continue;  // NaN; the columns may not have been written
-            const f32x4 x = *(const f32x4*)(parts.o + (at + i) * d + col);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], f, o[e]);
-        }
-    red[threadIdx.x] = o, total[threadIdx.x] = sum;
-    __syncthreads();
-    if (threadIdx.x >= quads) return;
-    for (int i = 1; i < groups; ++i) {
-        o += red[threadIdx.x + i * quads];
-        sum += total[threadIdx.x + i * quads];
+    if constexpr (W == 4) {
+        if ((t & 63) == 0) part[0][t >> 6] = top;
+        __syncthreads();
+        top = fmaxf(fmaxf(part[0][0], part[0][1]), fmaxf(part[0][2], part[0][3]));
     }
+    const float f = v.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(v.x - (top == -INFINITY ? 0.0f : top));
+    float sum = v.y == 0.0f ? 0.0f : v.y * f;
+    if (t < kSplits) factor[own][t] = v.y == v.y ? f : 0.0f;  // a sum of NaN: its columns may not have been written
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    if constexpr (W == 4)
+        if ((t & 63) == 0) part[1][t >> 6] = sum;
+    __syncthreads();
+    if constexpr (W == 4) sum = (part[1][0] + part[1][1]) + (part[1][2] + part[1][3]);
+    const int quads = d / 4, groups = kThreads / quads, grp = t / quads, col = 4 * (t % quads);
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    if (on && grp < groups) {
+        constexpr int U = 8;
+        for (int i0 = grp; i0 < parts.splits; i0 += U * groups) {
+            f32x4 x[U];
+            float w[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int i = i0 + u * groups;
+                w[u] = i < parts.splits ? factor[own][i] : 0.0f;
+                x[u] = w[u] != 0.0f ? *(const f32x4*)(parts.o + (at + i) * d + col) : f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = fmaf(x[u][e], w[u], o[e]);
+        }
+    }
+    red[threadIdx.x] = o;
+    __syncthreads();
+    if (!on || t >= quads) return;
+    for (int i = 1; i < groups; ++i) o += red[threadIdx.x + i * quads];
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     typedef T T4 __attribute__((ext_vector_type(4)));
     T4 y;
@@ -878,8 +903,11 @@ void start(const AttendArgs& a, const PagedCache& c, const Sequences& s, const A
         k_attend_tiles<T, DP, kTileWaves, NK>
             <<<(unsigned)(p.tiles * c.kv_heads * p.splits), 64 * kTileWaves, 0, st>>>(a, c, s, parts);
     }
-    if (p.splits > 1)
-        k_attend_join<T><<<(unsigned)((int64_t)s.rows * a.heads), 256, 0, st>>>(a, c.head_dim, s, parts);
+    const int64_t items = (int64_t)s.rows * a.heads;
+    if (p.splits > kWaveSplits)
+        k_attend_join<T, 4><<<(unsigned)items, 256, 0, st>>>(a, c.head_dim, s, parts);
+    else if (p.splits > 1)
+        k_attend_join<T, 1><<<(unsigned)ceil_div(items, 4), 256, 0, st>>>(a, c.head_dim, s, parts);
 }
 
 template <typename T>
@@ -895,24 +923,42 @@ void start(const AttendArgs& a, const PagedCache& c, const Sequences& s, const A
 
 }  // namespace
 
+// Splits share the keys of too few workgroups for the device.  Few rows: four workgroups a compute unit, of at least 128
+// keys (fp32: 256), so that sequences of different lengths come out even; a sequence by itself two, for its splits are
+// alike and each costs its beginning (us, two / four / eight a unit: 131072 keys of one sequence 115 / 122 / 140, 64
+// sequences of up to 8192 240 / 221 / 221).  Tiles: the number, a power of two, of the least time by a model of the launch.
 AttendPlan attend_plan(const AttendShape& q, int64_t cus) {
     AttendPlan p;
-    const int64_t g = q.heads / q.kv_heads;
+    const int64_t g = q.heads / q.kv_heads, len = std::max<int64_t>(q.max_len, 1);
+    const bool f32 = q.t == DType::f32;
     p.few = q.max_new * g <= kTileRows;
-    const int64_t len = std::max<int64_t>(q.max_len, 1);
-    int64_t wgs, step;
+    p.splits = 1;
+    int64_t wgs;
     if (p.few) {
         p.tiles = 0;
         wgs = q.B * q.kv_heads;
-        step = 128;
-        // Eight workgroups a compute unit.
-        p.splits = (int)std::max<int64_t>(1, std::min(ceil_div(8 * cus, wgs), ceil_div(len, step)));
+        p.splits = (int)std::max<int64_t>(1, std::min({ceil_div((q.B == 1 ? 2 : 4) * cus, wgs), ceil_div(len, f32 ? 256 : 128),
+                                                       (int64_t)kJoinSplits}));
     } else {
         const int64_t rows = kTileRows * kTileWaves;
         p.tiles = std::min(q.rows * g / rows + q.B, q.B * ceil_div(q.max_new * g, rows));
         wgs = p.tiles * q.kv_heads;
-        step = 512;
-        p.splits = (int)std::max<int64_t>(1, std::min(2 * cus / wgs, ceil_div(len, step)));
+        // us that a workgroup takes for 64 keys where it shares a compute unit with others (their number times this
+        // each), and by itself, as measured at head sizes of 64, 128 and 256; joining: the partial sums there and back.
+        const double width = (double)round_up(q.head_dim, 32) / 128;
+        const double step = f32 ? 7.3 * width : (width <= 1 ? 0.35 + 0.7 * width : 1.05 + 2.4 * (width - 1));
+        const double alone = (f32 ? 1.5 : 1.4) * step;
+        const int64_t seen = q.window > 0 ? std::min(len, q.window + rows / g) : len;
+        const double longest = ceil_div(seen, 64);
+        const double mean = q.window > 0 ? longest : std::max(1.0, longest - (double)q.max_new / 128);
+        double best = 0;
+        for (int S = 1; S <= kWaveSplits && (S == 1 || S * 128 <= seen); S *= 2) {
+            const double rounds = (double)ceil_div(wgs * S, cus);
+            const double work = rounds <= 1 ? alone * longest / S : std::max(step * rounds * mean / S, 2 * step * longest / S);
+            const double join = S == 1 ? 0 : 4 + (double)(q.rows * q.heads) * (S * q.head_dim * 8 + 256) / 3.5e6;
+            const double t = work + 1.5 * std::max(rounds, 2.0) + join;
+            if (S == 1 || t < best) best = t, p.splits = S;
+        }
     }
     p.workgroups = wgs * p.splits;
     return p;

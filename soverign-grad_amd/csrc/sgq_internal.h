@@ -597,7 +597,7 @@ struct AttendArgs {
     const int32_t* first_key;
 };
 struct AttendShape {
-    int64_t heads, kv_heads, head_dim, B, rows, max_len, max_new;
+    int64_t heads, kv_heads, head_dim, B, rows, max_len, max_new, window;
     DType t;
 };
 // few: a workgroup has all rows of a sequence and kv head (at most 32), else `tiles` tiles of
