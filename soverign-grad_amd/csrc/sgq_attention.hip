@@ -23,6 +23,7 @@
 //   fp32: 32x32x2; a 16-byte read of K serves four products; V^T a float a lane.
 // Keys and values go from their pages to LDS directly (a lane's address is its row's page),
 // the 16-byte chunks of a row permuted so that all reads are free of conflicts.
+#include "sgq_lanes.h"
 #include "sgq_paged.h"
 
 #include <algorithm>
@@ -462,7 +463,7 @@ struct Loader {
         const uint32_t to = lds + i * THREADS * 16;
         const int ch = chunk[kRowsApart % 16 ? i : 0];
         const uint32_t off = (uint32_t)min(row, end - 1 - key) * c->token_bytes + ch * 16;
-        if (DP != c->head_dim) {
+        if (Tile::kChunks * Chunk<T>::N != c->head_dim) {
             const bool on = ch * Chunk<T>::N < c->head_dim;
             load_lds(on ? k_base + at + off : (uint64_t)g_zeros, ks + to);
             load_lds(on ? v_base + at + off : (uint64_t)g_zeros, vs + to);
@@ -557,6 +558,42 @@ __device__ __forceinline__ void poison(const AttendArgs& a, const Parts& parts, 
             ((T*)a.out.p)[(int64_t)row * a.out.row + (int64_t)h * a.out.head + e % d] = (T)NAN;
         else if (e % d == 0)
             parts.ml[((int64_t)row * a.heads + h) * parts.splits + split] = make_float2(-INFINITY, NAN);
+    }
+}
+
+// Four columns (the i-th such) of the rows that the wavefronts of a workgroup have parts of: their maxima (exponents of
+// 2), sums and columns, joined and left as finish() does.
+template <typename T, int NW, typename M, typename L, typename C>
+__device__ __forceinline__ void join_waves(const AttendArgs& a, const Parts& parts, const SeqRows& r, int kvh, int g, int split,
+                                           int d, int i, bool bad, M max_of, L sum_of, C cols_of) {
+    const int quads = d / 4, q = i / quads, col = 4 * (i % quads);
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int v = 0; v < NW; ++v) top = fmaxf(top, max_of(v, q));
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int v = 0; v < NW; ++v) {
+        const float l = sum_of(v, q);
+        if (l == 0.0f) continue;  // nothing seen, its maximum -inf
+        const float f = __builtin_amdgcn_exp2f(max_of(v, q) - (top == -INFINITY ? 0.0f : top));
+        sum = fmaf(l, f, sum);
+        const f32x4 x = *(const f32x4*)(cols_of(v, q) + col);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], f, o[e]);
+    }
+    if (bad) sum = NAN;
+    const int row = r.row0 + q / g, head = kvh * g + q % g;
+    if (parts.splits == 1) {
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        T4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = (T)(o[e] * inv);
+        *(T4*)((T*)a.out.p + (int64_t)row * a.out.row + (int64_t)head * a.out.head + col) = y;
+    } else {
+        const int64_t at = ((int64_t)row * a.heads + head) * parts.splits + split;
+        if (sum != 0.0f) *(f32x4*)(parts.o + at * d + col) = o;
+        if (col == 0) parts.ml[at] = make_float2(top, sum);
     }
 }
 
@@ -780,41 +817,162 @@ __global__ __launch_bounds__(64 * NW) void k_attend_few(const AttendArgs a, cons
         bool any_bad = false;
 #pragma unroll
         for (int i = 0; i < NW; ++i) any_bad = any_bad || wrong[i];
-        // Four columns of a row a thread.
-        const int quads = d / 4;
-        for (int i = threadIdx.x; i < rows * quads; i += 64 * NW) {
-            const int q = i / quads, col = 4 * (i % quads);
-            float top = -INFINITY, sum = 0.0f;
+        for (int i = threadIdx.x; i < rows * (d / 4); i += 64 * NW)
+            join_waves<T, NW>(a, parts, r, kvh, g, split, d, i, any_bad, [&](int v, int q) { return ml[0][v][q]; },
+                              [&](int v, int q) { return ml[1][v][q]; },
+                              [&](int v, int q) { return (const float*)lds[v] + q * DP; });
+    }
+}
+
+// ---- few rows in fp32 -----------------------------------------------------------
+
+// Up to eight rows in fp32, whose 32-row products on the matrix cores would be mostly idle: a wavefront has the columns
+// across its lanes (NV each) and takes eight keys at a time, keys and values straight from their page (pages have eight
+// rows at least) and the next eight's loads in flight.  Scores of eight keys are summed over the lanes together,
+// each lane ending with one key's, so that eight keys take one exponential; a weight goes to all lanes as a scalar.
+// HBM bounds it: 8 sequences of 512 keys, 16 heads of 128, 67 MB.
+template <int NV, int R, int NW>
+__global__ __launch_bounds__(64 * NW) void k_attend_lanes(const AttendArgs a, const PagedCache c, const Sequences s,
+                                                          const Parts parts) {
+    constexpr int U = kMinPage;
+    typedef float Vec __attribute__((ext_vector_type(NV), aligned(NV == 4 ? 16 : 4 * NV)));
+    __shared__ __align__(16) float cols[NW][R][64 * NV];
+    __shared__ float ml[2][NW][R];
+    __shared__ int wrong[NW];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = a.heads / c.kv_heads, d = c.head_dim;
+    const int kvh = blockIdx.x % c.kv_heads, rest = blockIdx.x / c.kv_heads;
+    const int split = rest % parts.splits, b = rest / parts.splits;
+    const SeqRows r = seq_rows(s, b);
+    if (r.n == 0) return;
+    if (!r.ok) {
+        poison<float>(a, parts, d, r.row0, r.row0 + r.n, kvh * g, g, split);
+        return;
+    }
+    const int rows = r.n * g, col = lane * NV;
+    const bool on = col < d;
+    float q[R][NV], o[R][NV], m[R], l[R], slope[R];
+    int lo[R], hi[R], pos[R], first = 0x7fffffff, end = 0, max_lo = 0, min_hi = 0x7fffffff;
 #pragma unroll
-            for (int v = 0; v < NW; ++v) top = fmaxf(top, ml[0][v][q]);
-            f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < R; ++i) {
+        const int item = min(i, rows - 1), row = r.row0 + item / g, head = kvh * g + item % g;
+        pos[i] = r.position(row);
+        row_keys(a, r, b, row, pos[i], lo[i], hi[i]);
+        lo[i] = __builtin_amdgcn_readfirstlane(lo[i]), hi[i] = __builtin_amdgcn_readfirstlane(hi[i]);
+        slope[i] = a.slopes ? a.slopes[head] * kLog2e : 0.0f;
+        const Vec x = *(const Vec*)((const float*)a.q.p + (int64_t)row * a.q.row + (int64_t)head * a.q.head + min(col, d - NV));
 #pragma unroll
-            for (int v = 0; v < NW; ++v) {
-                const float lv = ml[1][v][q];
-                if (lv == 0.0f) continue;  // nothing seen, its maximum -inf
-                const float f = __builtin_amdgcn_exp2f(ml[0][v][q] - (top == -INFINITY ? 0.0f : top));
-                sum = fmaf(lv, f, sum);
-                const f32x4 x = *(const f32x4*)((const float*)lds[v] + q * DP + col);
+        for (int e = 0; e < NV; ++e) q[i][e] = on ? x[e] : 0.0f, o[i][e] = 0.0f;
+        m[i] = -INFINITY, l[i] = 0.0f;
+        first = min(first, lo[i]), end = max(end, hi[i]);
+        max_lo = max(max_lo, lo[i]), min_hi = min(min_hi, hi[i]);
+    }
+    int k0, k1;
+    split_range(first & ~(U - 1), end, split, parts.splits, U * NW, k0, k1);
+    const int32_t* const table = s.table + b * s.table_ld;
+    const float* const kp = (const float*)c.k + (int64_t)kvh * c.head_stride + min(col, d - NV);
+    const float* const vp = (const float*)c.v + (int64_t)kvh * c.head_stride + min(col, d - NV);
+    const int last = k1 - 1, mask = (1 << c.page_log) - 1;
+    const bool narrow = d < 64 * NV, sloped = a.slopes != nullptr, capped = a.softcap > 0.0f;
+    const float unit = a.scale * kLog2e, in = capped ? a.scale / a.softcap : 0.0f, out_cap = a.softcap * kLog2e;
+    unsigned top_page = 0;
+
+    auto row_top = [&](float v) {  // over the lanes of the eight keys
+        v = fmaxf(v, __shfl_xor(v, 32, 64));
+        v = fmaxf(v, __shfl_xor(v, 16, 64));
+        return fmaxf(v, __shfl_xor(v, 1, 64));
+    };
+    auto page_of = [&](int k) { return (unsigned)table[min(k, last) >> c.page_log]; };
+    auto load = [&](int k, unsigned page, Vec (&kx)[U], Vec (&vx)[U]) {
+        top_page = max(top_page, page);
+        const int64_t at = (int64_t)min(page, (unsigned)c.pages - 1) * c.page_stride;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], f, o[e]);
+        for (int u = 0; u < U; ++u) {
+            const int64_t off = at + (int64_t)(min(k + u, last) & mask) * c.token_stride;
+            kx[u] = __builtin_nontemporal_load((const Vec*)(kp + off));
+            vx[u] = __builtin_nontemporal_load((const Vec*)(vp + off));
+        }
+    };
+    auto take = [&](int k, Vec (&kx)[U], Vec (&vx)[U]) {
+        if (narrow && !on)
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < NV; ++e) kx[u][e] = 0.0f;
+        const bool part = k < max_lo || k + U > min_hi;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            float x[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                x[u] = q[i][0] * kx[u][0];
+#pragma unroll
+                for (int e = 1; e < NV; ++e) x[u] = fmaf(q[i][e], kx[u][e], x[u]);
             }
-            if (any_bad) sum = NAN;
-            const int rw = r.row0 + q / g, hd = kvh * g + q % g;
-            if (parts.splits == 1) {
-                T* out = (T*)a.out.p + (int64_t)rw * a.out.row + (int64_t)hd * a.out.head + col;
-                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                typedef T T4 __attribute__((ext_vector_type(4)));
-                T4 y;
+            int mine = 0;
+            lane_reduce<U, 0>(x, lane, mine);
+            const int key = k + mine;
+            float v = x[0];
+            v = capped ? out_cap * tanhf(v * in) : v * unit;
+            if (sloped) v = fmaf(-slope[i], (float)abs(pos[i] - key), v);
+            if (part && (key < lo[i] || key >= hi[i])) v = -INFINITY;
+            if (__any(v - m[i] > 8.0f)) {
+                const float now = fmaxf(m[i], row_top(v));
+                const float w = __builtin_amdgcn_exp2f(m[i] - (now == -INFINITY ? 0.0f : now));
+                m[i] = now, l[i] *= w;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] = (T)(o[e] * inv);
-                *(T4*)out = y;
-            } else {
-                const int64_t at = ((int64_t)rw * a.heads + hd) * parts.splits + split;
-                if (sum != 0.0f) *(f32x4*)(parts.o + at * d + col) = o;
-                if (col == 0) parts.ml[at] = make_float2(top, sum);
+                for (int e = 0; e < NV; ++e) o[i][e] *= w;
+            }
+            const float p = __builtin_amdgcn_exp2f(v - (m[i] == -INFINITY ? 0.0f : m[i]));
+            l[i] += p;  // each key's in the lanes that have it
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(p), (u & 4) * 8 + (u & 2) * 8 + (u & 1)));
+                const bool seen = !part || (k + u >= lo[i] && k + u < hi[i]);
+#pragma unroll
+                for (int e = 0; e < NV; ++e)
+                    o[i][e] = seen ? fmaf(w, vx[u][e], o[i][e]) : o[i][e];  // what is not seen may be anything
             }
         }
+    };
+    int k = k0 + U * wave;
+    constexpr int step = U * NW;
+    if (k < k1) {
+        Vec ka[U], va[U], kb[U], vb[U];
+        unsigned page = page_of(k), next = page_of(k + step);
+        load(k, page, ka, va);
+#pragma unroll 1
+        for (;;) {
+            page = page_of(k + 2 * step);
+            load(k + step, next, kb, vb);
+            take(k, ka, va);
+            if ((k += step) >= k1) break;
+            next = page_of(k + 2 * step);
+            load(k + step, page, ka, va);
+            take(k, kb, vb);
+            if ((k += step) >= k1) break;
+        }
     }
+    // A key's weight is in eight lanes of a wavefront's sum.
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+#pragma unroll
+        for (int t = 32; t > 0; t >>= 1) l[i] += __shfl_xor(l[i], t, 64);
+        l[i] *= 0.125f;
+        if (lane == 0) ml[0][wave][i] = m[i], ml[1][wave][i] = l[i];
+        Vec x;
+#pragma unroll
+        for (int e = 0; e < NV; ++e) x[e] = o[i][e];
+        *(Vec*)&cols[wave][i][col] = x;
+    }
+    if (lane == 0) wrong[wave] = top_page >= (unsigned)c.pages;
+    __syncthreads();
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) bad = bad || wrong[i];
+    for (int i = threadIdx.x; i < rows * (d / 4); i += 64 * NW)
+        join_waves<float, NW>(a, parts, r, kvh, g, split, d, i, bad, [&](int w, int q) { return ml[0][w][q]; },
+                              [&](int w, int q) { return ml[1][w][q]; }, [&](int w, int q) { return (const float*)cols[w][q]; });
 }
 
 // ---- the splits of a row joined ------------------------------------------------
@@ -891,11 +1049,26 @@ constexpr int kTileWaves = 4;
 // Wavefronts of k_attend_few whose buffers (two of 32 keys and values each) fit 128 KiB.
 constexpr int few_waves(int row_bytes) { return row_bytes <= 256 ? 4 : 1024 / row_bytes; }
 
+constexpr int kLaneRows = 8, kLaneWaves = 4;
+
+template <int NV>
+void start_lanes(const AttendArgs& a, const PagedCache& c, const Sequences& s, const AttendPlan& p, const Parts& parts,
+                 hipStream_t st) {
+    const unsigned wgs = (unsigned)((int64_t)s.B * c.kv_heads * p.splits);
+    const int rows = s.max_new * (a.heads / c.kv_heads);
+    if (rows <= 1) k_attend_lanes<NV, 1, kLaneWaves><<<wgs, 64 * kLaneWaves, 0, st>>>(a, c, s, parts);
+    else if (rows <= 2) k_attend_lanes<NV, 2, kLaneWaves><<<wgs, 64 * kLaneWaves, 0, st>>>(a, c, s, parts);
+    else if (rows <= 4) k_attend_lanes<NV, 4, kLaneWaves><<<wgs, 64 * kLaneWaves, 0, st>>>(a, c, s, parts);
+    else k_attend_lanes<NV, 8, kLaneWaves><<<wgs, 64 * kLaneWaves, 0, st>>>(a, c, s, parts);
+}
+
 template <typename T, int DP>
 void start(const AttendArgs& a, const PagedCache& c, const Sequences& s, const AttendPlan& p, const Parts& parts,
            hipStream_t st) {
     constexpr int kRow = TileRows<T, DP>::kRow;
-    if (p.few) {
+    if (p.lanes) {
+        start_lanes<(DP <= 64 ? 1 : DP <= 128 ? 2 : 4)>(a, c, s, p, parts, st);
+    } else if (p.few) {
         constexpr int NW = few_waves(kRow);
         k_attend_few<T, DP, NW><<<(unsigned)((int64_t)s.B * c.kv_heads * p.splits), 64 * NW, 0, st>>>(a, c, s, parts);
     } else {
@@ -932,12 +1105,13 @@ AttendPlan attend_plan(const AttendShape& q, int64_t cus) {
     const int64_t g = q.heads / q.kv_heads, len = std::max<int64_t>(q.max_len, 1);
     const bool f32 = q.t == DType::f32;
     p.few = q.max_new * g <= kTileRows;
+    p.lanes = f32 && q.max_new * g <= kLaneRows;
     p.splits = 1;
     int64_t wgs;
     if (p.few) {
         p.tiles = 0;
         wgs = q.B * q.kv_heads;
-        p.splits = (int)std::max<int64_t>(1, std::min({ceil_div((q.B == 1 ? 2 : 4) * cus, wgs), ceil_div(len, f32 ? 256 : 128),
+        p.splits = (int)std::max<int64_t>(1, std::min({ceil_div((q.B == 1 ? 2 : 4) * cus, wgs), ceil_div(len, f32 && !p.lanes ? 256 : 128),
                                                        (int64_t)kJoinSplits}));
     } else {
         const int64_t rows = kTileRows * kTileWaves;
