@@ -521,6 +521,7 @@ struct Parts {
     float* o;
     float2* ml;
     int splits;
+    int fold;  // tiles of a sequence in falling order, before the others in rising order
 };
 
 // A split's share of the keys [lo, hi): whole steps of `step` keys.
@@ -691,7 +692,9 @@ __global__ __launch_bounds__(64 * NW, DP * sizeof(T) <= 512 ? 2 : 1) void k_atte
         poison<T>(a, parts, c.head_dim, r.row0 + min(r.n, tile * per), r.row0 + min(r.n, (tile + 1) * per), kvh * g, g, split);
         return;
     }
-    tile = tiles - 1 - tile;  // the longest rows first
+    // The longest rows first.  Where all workgroups are resident, two a compute unit: the ones that come second to a unit
+    // the other way round, so that the shortest share with the longest (a prompt of 2048 tokens, 32 on 8 heads of 128).
+    tile = tile < parts.fold ? tiles - 1 - tile : tile - parts.fold;
 
     const Score sc(a);
     Rows<T, DP, NK> w;
@@ -826,11 +829,12 @@ __global__ __launch_bounds__(64 * NW) void k_attend_few(const AttendArgs a, cons
 
 // ---- few rows in fp32 -----------------------------------------------------------
 
-// Up to eight rows in fp32, whose 32-row products on the matrix cores would be mostly idle: a wavefront has the columns
+// Up to four rows in fp32, of whose 32-row products on the matrix cores little would be used: a wavefront has the columns
 // across its lanes (NV each) and takes eight keys at a time, keys and values straight from their page (pages have eight
 // rows at least) and the next eight's loads in flight.  Scores of eight keys are summed over the lanes together,
 // each lane ending with one key's, so that eight keys take one exponential; a weight goes to all lanes as a scalar.
-// HBM bounds it: 8 sequences of 512 keys, 16 heads of 128, 67 MB.
+// HBM bounds it (us, k_attend_few in brackets: 32 sequences of 1024 keys, 16 heads of 128, 537 MB 85 [222]; 8 of 512
+// 18.3 [37]; four rows, 8 of 2048, 32 on 8 heads 41 [67]; with eight rows it would lose, 51 [39] at a head size of 64).
 template <int NV, int R, int NW>
 __global__ __launch_bounds__(64 * NW) void k_attend_lanes(const AttendArgs a, const PagedCache c, const Sequences s,
                                                           const Parts parts) {
@@ -1049,7 +1053,7 @@ constexpr int kTileWaves = 4;
 // Wavefronts of k_attend_few whose buffers (two of 32 keys and values each) fit 128 KiB.
 constexpr int few_waves(int row_bytes) { return row_bytes <= 256 ? 4 : 1024 / row_bytes; }
 
-constexpr int kLaneRows = 8, kLaneWaves = 4;
+constexpr int kLaneRows = 4, kLaneWaves = 4;
 
 template <int NV>
 void start_lanes(const AttendArgs& a, const PagedCache& c, const Sequences& s, const AttendPlan& p, const Parts& parts,
@@ -1058,8 +1062,7 @@ void start_lanes(const AttendArgs& a, const PagedCache& c, const Sequences& s, c
     const int rows = s.max_new * (a.heads / c.kv_heads);
     if (rows <= 1) k_attend_lanes<NV, 1, kLaneWaves><<<wgs, 64 * kLaneWaves, 0, st>>>(a, c, s, parts);
     else if (rows <= 2) k_attend_lanes<NV, 2, kLaneWaves><<<wgs, 64 * kLaneWaves, 0, st>>>(a, c, s, parts);
-    else if (rows <= 4) k_attend_lanes<NV, 4, kLaneWaves><<<wgs, 64 * kLaneWaves, 0, st>>>(a, c, s, parts);
-    else k_attend_lanes<NV, 8, kLaneWaves><<<wgs, 64 * kLaneWaves, 0, st>>>(a, c, s, parts);
+    else k_attend_lanes<NV, 4, kLaneWaves><<<wgs, 64 * kLaneWaves, 0, st>>>(a, c, s, parts);
 }
 
 template <typename T, int DP>
@@ -1135,6 +1138,7 @@ AttendPlan attend_plan(const AttendShape& q, int64_t cus) {
         }
     }
     p.workgroups = wgs * p.splits;
+    p.fold = q.B == 1 && p.workgroups <= 2 * cus ? (int)std::max<int64_t>(1, cus / (q.kv_heads * p.splits)) : 1 << 30;
     return p;
 }
 
@@ -1147,7 +1151,7 @@ hipError_t launch_attend(const AttendArgs& a, const PagedCache& c, const Sequenc
                          hipStream_t st) {
     if (s.rows <= 0 || s.B <= 0) return hipSuccess;
     const int64_t n = (int64_t)s.rows * a.heads * p.splits;
-    const Parts parts = {(float*)ws, (float2*)((float*)ws + n * c.head_dim), p.splits};
+    const Parts parts = {(float*)ws, (float2*)((float*)ws + n * c.head_dim), p.splits, p.fold};
     switch (c.t) {
         case DType::f32: start<float>(a, c, s, p, parts, st); break;
         case DType::bf16: start<__bf16>(a, c, s, p, parts, st); break;

@@ -605,7 +605,7 @@ struct AttendShape {
 struct AttendPlan {
     bool few, lanes;
     int64_t tiles, workgroups;
-    int splits;
+    int splits, fold;
 };
 AttendPlan attend_plan(const AttendShape& q, int64_t cus);
 int64_t attend_plan_bytes(const AttendPlan& p, const AttendShape& q);
