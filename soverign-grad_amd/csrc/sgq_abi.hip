@@ -467,7 +467,7 @@ bool bad_attention(int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t B,
                    int64_t max_new) {
     return kv_heads < 1 || heads < 1 || heads > kMaxHeads || heads % kv_heads || head_dim < kHeadDimStep ||
            head_dim % kHeadDimStep || head_dim > kMaxHeadDim || B < 0 || B > kMaxSequences || rows < 0 ||
-           rows > kMaxHeadRows || max_len < 0 || max_len > kMaxDim || max_new < 0 || max_new > kMaxDim;
+           rows > kMaxHeadRows || rows * heads > kMaxDim || max_len < 0 || max_len > kMaxDim || max_new < 0 || max_new > kMaxDim;
 }
 
 int check_paged(const char* fn, int64_t rows, int64_t heads, const sgq_paged_cache* c, const sgq_sequences* q, PagedCache& pc,
@@ -484,9 +484,9 @@ int check_paged(const char* fn, int64_t rows, int64_t heads, const sgq_paged_cac
     if (q->B < 0 || rows < 0 || q->max_len < 0 || q->max_new < 0 || q->table_pages < 0 || q->table_pages > kMaxDim ||
         q->max_len > kMaxDim || q->max_new > kMaxDim || q->table_ld < q->table_pages || q->table_ld > kMaxDim)
         return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: bad sequences", fn);
-    if (heads > kMaxHeads || rows > kMaxHeadRows || q->B > kMaxSequences)
-        return fail(SGQ_ERR_UNSUPPORTED, "%s: more than %d heads, %d rows or %d sequences", fn, kMaxHeads, kMaxHeadRows,
-                    kMaxSequences);
+    if (heads > kMaxHeads || rows > kMaxHeadRows || q->B > kMaxSequences || rows * heads > kMaxDim)
+        return fail(SGQ_ERR_UNSUPPORTED, "%s: more than %d heads, %d rows, 2^30 heads of rows or %d sequences", fn, kMaxHeads,
+                    kMaxHeadRows, kMaxSequences);
     const int64_t step = 16 / dtype_bytes((DType)c->dtype), d = c->head_dim;
     if (c->page_stride < 0 || c->token_stride < 0 || c->head_stride < 0 || c->page_stride % step || c->token_stride % step ||
         c->head_stride % step)

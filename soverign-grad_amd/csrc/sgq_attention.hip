@@ -128,7 +128,7 @@ struct Score {
         negate = a.scale < 0.0f;
         capped = a.softcap > 0.0f;
         sloped = a.slopes != nullptr;
-        in = capped ? fabsf(a.scale) / a.softcap : 0.0f;
+        in = capped ? fminf(fabsf(a.scale) / a.softcap, 1.0e30f) : 0.0f;  // times 0 has to be 0
         out = a.softcap * kLog2e;
         // Never zero: a hidden score is -inf, and has to stay that.
         c = fmaxf(fabsf(a.scale) * kLog2e, 1.17549435e-38f);
@@ -878,7 +878,7 @@ __global__ __launch_bounds__(64 * NW) void k_attend_lanes(const AttendArgs a, co
     const float* const vp = (const float*)c.v + (int64_t)kvh * c.head_stride + min(col, d - NV);
     const int last = k1 - 1, mask = (1 << c.page_log) - 1;
     const bool narrow = d < 64 * NV, sloped = a.slopes != nullptr, capped = a.softcap > 0.0f;
-    const float unit = a.scale * kLog2e, in = capped ? a.scale / a.softcap : 0.0f, out_cap = a.softcap * kLog2e;
+    const float unit = a.scale * kLog2e, in = capped ? __builtin_amdgcn_fmed3f(a.scale / a.softcap, -1.0e30f, 1.0e30f) : 0.0f, out_cap = a.softcap * kLog2e;
     unsigned top_page = 0;
 
     auto row_top = [&](float v) {  // over the lanes of the eight keys

@@ -61,7 +61,7 @@ SHARED = [
     (INVALID, dict(seqs=dict(table_ld=3))), (INVALID, dict(seqs=dict(table=None))), (INVALID, dict(seqs=dict(lens=None))),
     (INVALID, dict(seqs=dict(starts=None))), (UNSUPPORTED, dict(seqs=dict(B=(1 << 20) + 1))),
     (UNSUPPORTED, dict(rows=(1 << 23) + 1)), (INVALID, dict(rows=-1)), (INVALID, dict(heads=3)), (INVALID, dict(heads=0)),
-    (UNSUPPORTED, dict(heads=1026)), (INVALID, dict(q=None)), (INVALID, dict(q=4 * P + 2)), (INVALID, dict(out=None)),
+    (UNSUPPORTED, dict(heads=1026)), (UNSUPPORTED, dict(heads=512, rows=1 << 22)), (INVALID, dict(q=None)), (INVALID, dict(q=4 * P + 2)), (INVALID, dict(out=None)),
     (INVALID, dict(out=8 * P + 4)), (INVALID, dict(o_row=252)), (INVALID, dict(o_row=192)), (INVALID, dict(q_row=-512)),
     (INVALID, dict(q_head=32)), (INVALID, dict(q_row=1 << 31)),
 ]
@@ -111,3 +111,33 @@ def test_python_refuses_what_is_not_on_the_device(op):
             op.rotary_frequencies(dim, device="cpu")
     f = op.rotary_frequencies(8, 10000.0, device="cpu")
     assert f.dtype == torch.float64 and torch.allclose(f, torch.tensor([1, 0.1, 0.01, 0.001], dtype=torch.float64), rtol=1e-15)
+
+
+def test_workspace(op, lib):
+    """What a call needs it says beforehand, for a device of any size, and refuses to run without."""
+    fn = lib.sgq_paged_attention_workspace_bytes
+    seen = 0
+    for cus in (1, 32, 256, 304):
+        for heads, kv in ((1, 1), (32, 8), (16, 16), (28, 4)):
+            for d in (16, 64, 80, 128, 192, 256):
+                for dtype in (0, 1, 2):
+                    for B, rows, length, new in ((1, 1, 1, 1), (1, 1, 131072, 1), (64, 64, 8192, 1), (1, 2048, 2048, 2048), (5, 100, 900, 33)):
+                        for window in (0, 100):
+                            need = fn(heads, kv, d, dtype, B, rows, length, new, window, cus)
+                            per = rows * heads * (4 * d + 8)
+                            assert need == 0 or need % per == 0 and 2 <= need // per <= 256
+                            seen += need > 0
+    assert seen > 100
+    for bad in ((0, 1, 64, 0, 1, 1, 1, 1, 0, 0), (3, 2, 64, 0, 1, 1, 1, 1, 0, 0), (2, 2, 60, 0, 1, 1, 1, 1, 0, 0), (2, 2, 64, 3, 1, 1, 1, 1, 0, 0),
+                (2, 2, 64, 0, -1, 1, 1, 1, 0, 0), (2, 2, 64, 0, 1, -1, 1, 1, 0, 0), (2, 2, 64, 0, 1, 1, -1, 1, 0, 0),
+                (2, 2, 64, 0, 1, 1, 1, -1, 0, 0), (2, 2, 64, 0, 1, 1, 1, 1, -1, 0), (2, 2, 64, 0, 1, 1, 1, 1, 0, -1)):
+        assert fn(*bad) == -1, bad
+    assert fn(2, 2, 64, 0, 0, 5, 1, 1, 0, 0) == 0 and fn(2, 2, 64, 0, 5, 0, 1, 1, 0, 0) == 0
+    # One sequence of many keys is shared out: no workspace, too small a one, one at an odd address.
+    long = dict(seqs=dict(B=1, max_len=60000, table_ld=4096, table_pages=4096, max_new=1), rows=1)
+    need = fn(4, 2, 64, 1, 1, 1, 60000, 1, 0, 0)
+    assert need > 0
+    for ws, nws in ((None, need), (P, need - 1), (P + 8, need)):
+        assert _attend(op, lib, ws=ws, nws=nws, **long) == WORKSPACE
+    for scale in (float("inf"), float("nan")):
+        assert _attend(op, lib, scores=dict(scale=scale)) == INVALID

@@ -226,13 +226,13 @@ def test_masks(op, dev, mask, dtype, chunks):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
-@pytest.mark.parametrize("seqs", [[(90, 250), (40, 40)], [(4, 250), (2, 40)]])
+@pytest.mark.parametrize("seqs", [[(90, 250), (40, 40)], [(4, 250), (2, 40)], [(2, 250), (1, 40)]])
 def test_not_finite_in_places_that_rows_do_not_see(op, dev, dtype, value, seqs):
     """A value or a key that is not finite reaches the rows that see it and no other."""
     H, KV, d = 4, 2, 128
     b = Batch(op, dev, seqs, 16, KV, d, dtype)
     n, length = seqs[0]
-    for where, key in ((b.values, length - n // 2), (b.values, 100), (b.keys, length - n // 2 + 1)):
+    for where, key in ((b.values, length - n // 2), (b.values, 100), (b.keys, min(length - n // 2 + 1, length - 1))):
         where[0][key, 1, 5] = value
     for where, pool in ((b.keys, b.k), (b.values, b.v)):
         j = torch.arange(length, device=dev)
@@ -249,6 +249,34 @@ def test_not_finite_in_places_that_rows_do_not_see(op, dev, dtype, value, seqs):
     clean = seen_by_none.all(-1, keepdim=True).expand_as(y)
     yy = torch.where(clean, y.double(), ref[0])
     _check(yy, ref, b, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("new", [1, 60])
+def test_not_finite_values_that_all_rows_see(op, dev, dtype, new):
+    """An infinity among values makes that column infinite, of both signs or a NaN makes it a NaN."""
+    b = Batch(op, dev, [(new, 300)], 16, 1, 64, dtype)
+    v = b.values[0]
+    v[7, 0, 1], v[7, 0, 2], v[90, 0, 2], v[30, 0, 3] = float("inf"), float("inf"), float("-inf"), float("nan")
+    v[200, 0, 4] = float("-inf")
+    j = torch.arange(300, device=dev)
+    b.v[b.table[0, j // 16].long(), j % 16] = v
+    q = _randn(dev, 3, new, 2, 64).to(dtype)
+    y = op.paged_attention(q, b.kv, b.batch).float()
+    assert bool((y[..., 1] == float("inf")).all()) and bool(y[..., 2].isnan().all()) and bool(y[..., 3].isnan().all())
+    assert bool((y[..., 4] == float("-inf")).all())
+    rest = [0] + list(range(5, 64))
+    assert bool(torch.isfinite(y[..., rest]).all())
+    out, A, ds, n = _reference(b, q)
+    _check(torch.where(torch.isfinite(out), y.double(), out), (out, A, ds, n), b, dtype)
+
+
+def test_a_tiny_cap(op, dev):
+    b = Batch(op, dev, [(3, 40), (40, 40)], 16, 2, 64, torch.float32)
+    q = _randn(dev, 3, b.rows, 4, 64)
+    q[0] = 0
+    y = op.paged_attention(q, b.kv, b.batch, softcap=1e-38)
+    _check(y, _reference(b, q, softcap=1e-38), b, torch.float32)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
