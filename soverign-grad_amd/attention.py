@@ -55,7 +55,7 @@ class PagedKV:
     strides and type; page a power of two from 8 on, head_dim a multiple of 16 up to 256, heads next to
     each other in any order of the first three dimensions (views of [pages, kv_heads, page, head_dim] will do)."""
 
-    __slots__ = ("k", "v", "_struct", "_at")
+    __slots__ = ("k", "v", "dtype", "device", "kv_heads", "head_dim", "_step", "_struct", "_at")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor):
         if not k.is_cuda or k.dim() != 4:
@@ -76,7 +76,8 @@ class PagedKV:
             raise ValueError("every head of a page must be 16-byte aligned and contiguous")
         if k.numel() and k.data_ptr() == v.data_ptr():
             raise ValueError("k and v must have memory of their own")
-        self.k, self.v = k, v
+        self.k, self.v, self.dtype, self.device = k, v, k.dtype, k.device
+        self.kv_heads, self.head_dim, self._step = heads, d, step
         self._struct = _PagedCache(k.data_ptr(), v.data_ptr(), pages, page, heads, d, *strides, _dtype(k.dtype))
         self._at = ctypes.addressof(self._struct)
 
@@ -113,7 +114,7 @@ class SequenceBatch:
     pool, has NaN for its outputs.  The tensors are read when a call runs: a captured graph takes
     what they hold at its replay."""
 
-    __slots__ = ("table", "lens", "starts", "max_len", "max_new", "_struct", "_at")
+    __slots__ = ("table", "lens", "starts", "max_len", "max_new", "device", "_struct", "_at")
 
     def __init__(self, table: torch.Tensor, lens: torch.Tensor, starts: torch.Tensor, max_len: int, max_new: int):
         if not table.is_cuda or table.dim() != 2 or table.dtype is not torch.int32:
@@ -128,6 +129,7 @@ class SequenceBatch:
         if not 0 <= max_len <= 2**30 or not 0 <= max_new <= 2**30:
             raise ValueError("max_len and max_new must be from 0 to 2^30")
         self.table, self.lens, self.starts, self.max_len, self.max_new = table, lens, starts, max_len, max_new
+        self.device = table.device
         self._struct = _Sequences(table.data_ptr(), table.stride(0) if B > 1 else max(pages, 1), pages, lens.data_ptr(),
                                   starts.data_ptr(), B, max_len, max_new)
         self._at = ctypes.addressof(self._struct)
@@ -141,32 +143,46 @@ def rotary_frequencies(dim: int, base: float = 10000.0, device="cuda") -> torch.
     return (float(base) ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)).to(device)
 
 
-def _heads(x: torch.Tensor, name: str, heads: Optional[int], kv: PagedKV, copy: bool = True):
-    """x [rows, heads, head_dim], its row and its head stride; a copy where heads are not
+def _heads(x: torch.Tensor, name: str, rows: int, heads: int, kv: PagedKV, copy: bool = True):
+    """x [rows, heads, head_dim], its address, its row and its head stride; a copy where heads are not
     16-byte aligned."""
-    if x.dim() != 3 or x.shape[2] != kv.k.shape[3] or (heads is not None and x.shape[1] != heads):
-        raise ValueError(f"{name} must be [rows, {'heads' if heads is None else heads}, {kv.k.shape[3]}]")
-    if x.dtype != kv.k.dtype or x.device != kv.k.device:
+    d = kv.head_dim
+    if x.shape != (rows, heads, d):
+        raise ValueError(f"{name} must be [{rows}, {heads}, {d}]")
+    if x.dtype is not kv.dtype or x.device != kv.device:
         raise ValueError(f"{name} must have the cache's type and device")
-    T, H, d = x.shape
-    row, head, one = x.stride()
-    if H == 1:
-        head = d
-    if T == 1:
-        row = max(H * head, d)
-    step = 16 // x.element_size()
-    if (one != 1 or row % step or head % step or x.data_ptr() % 16 or head < d or row < d
-            or (row < (H - 1) * head + d and head < (T - 1) * row + d)) and x.numel():
-        if not copy:
-            raise ValueError(f"heads of {name} must be contiguous and 16-byte aligned, and not overlap")
-        x = x.clone(memory_format=torch.contiguous_format)
-        row, head = H * d, d
-    return x, row, head
+    at = x.data_ptr()
+    if x.is_contiguous():
+        if at % 16 == 0:
+            return x, at, heads * d, d
+    else:
+        row, head, one = x.stride()
+        if heads == 1:
+            head = d
+        if rows == 1:
+            row = heads * head
+        step = kv._step
+        if (one == 1 and row % step == 0 and head % step == 0 and at % 16 == 0 and head >= d and row >= d
+                and (row >= (heads - 1) * head + d or head >= (rows - 1) * row + d)):
+            return x, at, row, head
+    if not copy:
+        raise ValueError(f"heads of {name} must be contiguous and 16-byte aligned, and not overlap")
+    x = x.clone(memory_format=torch.contiguous_format)
+    return x, x.data_ptr(), heads * d, d
+
+
+def _queries(q: torch.Tensor, kv: PagedKV):
+    if q.dim() != 3:
+        raise ValueError(f"q must be [rows, heads, {kv.head_dim}]")
+    rows, heads, _ = q.shape
+    if heads == 0 or heads % kv.kv_heads:
+        raise ValueError(f"heads of q must be a multiple of {kv.kv_heads}")
+    return rows, heads, _heads(q, "q", rows, heads, kv)
 
 
 def _same_device(kv: PagedKV, batch: SequenceBatch) -> torch.device:
-    dev = kv.k.device
-    if batch.table.device != dev:
+    dev = kv.device
+    if batch.device != dev:
         raise ValueError(f"the batch must be on {dev}")
     return dev
 
@@ -184,21 +200,15 @@ def norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv: Page
     interleaved, the elements behind 2 * pairs stay.  positions [rows]: what the rotation takes
     instead of the tokens' own positions.  q, k and v may be parts of one projection's rows; out may be q."""
     dev = _same_device(kv, batch)
-    q, q_row, q_head = _heads(q, "q", None, kv)
-    T, H, d = q.shape
-    KV = kv.k.shape[2]
-    if H == 0 or H % KV:
-        raise ValueError(f"heads of q must be a multiple of {KV}")
-    k, k_row, k_head = _heads(k, "k", KV, kv)
-    v, v_row, v_head = _heads(v, "v", KV, kv)
-    if k.shape[0] != T or v.shape[0] != T:
-        raise ValueError("q, k and v must have the same rows")
+    d, KV = kv.head_dim, kv.kv_heads
+    T, H, (q, q_at, q_row, q_head) = _queries(q, kv)
+    k, k_at, k_row, k_head = _heads(k, "k", T, KV, kv)
+    v, v_at, v_row, v_head = _heads(v, "v", T, KV, kv)
     if out is None:
-        out, o_row, o_head = torch.empty(T, H, d, dtype=q.dtype, device=dev), H * d, d
+        out = torch.empty(T, H, d, dtype=kv.dtype, device=dev)
+        o_at, o_row, o_head = out.data_ptr(), H * d, d
     else:
-        if out.shape[0] != T:
-            raise ValueError("out must be alike q")
-        out, o_row, o_head = _heads(out, "out", H, kv, copy=False)
+        out, o_at, o_row, o_head = _heads(out, "out", T, H, kv, copy=False)
     half = 0
     if freqs is not None:
         half = freqs.numel()
@@ -209,8 +219,8 @@ def norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv: Page
     g = None if q_norm is None else _vector(q_norm, d, dev, "q_norm")
     gk = None if k_norm is None else _vector(k_norm, d, dev, "k_norm")
     pos = None if positions is None else _int32(positions, T, dev, "positions")
-    _call(dev, load_library().sgq_norm_rope_append, q.data_ptr(), q_row, q_head, k.data_ptr(), k_row, k_head,
-          v.data_ptr(), v_row, v_head, out.data_ptr(), o_row, o_head, T, H, kv._at, batch._at,
+    _call(dev, load_library().sgq_norm_rope_append, q_at, q_row, q_head, k_at, k_row, k_head, v_at, v_row, v_head, o_at,
+          o_row, o_head, T, H, kv._at, batch._at,
           None if g is None else g.data_ptr(), None if gk is None else gk.data_ptr(), eps,
           freqs.data_ptr() if half else None, 2 * half, interleaved, None if pos is None else pos.data_ptr())
     return out
@@ -242,17 +252,13 @@ def paged_attention(q: torch.Tensor, kv: PagedKV, batch: SequenceBatch, scale: O
     (window > 0) and j >= first_key[row] ([rows], its document's first).  A row that sees
     none is zeros.  out may be q."""
     dev = _same_device(kv, batch)
-    q, q_row, q_head = _heads(q, "q", None, kv)
-    T, H, d = q.shape
-    KV = kv.k.shape[2]
-    if H == 0 or H % KV:
-        raise ValueError(f"heads of q must be a multiple of {KV}")
+    d = kv.head_dim
+    T, H, (q, q_at, q_row, q_head) = _queries(q, kv)
     if out is None:
-        out, o_row, o_head = torch.empty(T, H, d, dtype=q.dtype, device=dev), H * d, d
+        out = torch.empty(T, H, d, dtype=kv.dtype, device=dev)
+        o_at, o_row, o_head = out.data_ptr(), H * d, d
     else:
-        if out.shape[0] != T:
-            raise ValueError("out must be alike q")
-        out, o_row, o_head = _heads(out, "out", H, kv, copy=False)
+        out, o_at, o_row, o_head = _heads(out, "out", T, H, kv, copy=False)
     if window < 0:
         raise ValueError("window must not be negative")
     slopes = None if alibi_slopes is None else _vector(alibi_slopes, H, dev, "alibi_slopes")
@@ -262,8 +268,8 @@ def paged_attention(q: torch.Tensor, kv: PagedKV, batch: SequenceBatch, scale: O
                   None if slopes is None else slopes.data_ptr(), None if prefix is None else prefix.data_ptr(),
                   None if first is None else first.data_ptr())
     ws, need = _attention_workspace(kv, batch, T, H, window, dev)
-    _call(dev, load_library().sgq_paged_attention, q.data_ptr(), q_row, q_head, out.data_ptr(), o_row, o_head, T, H,
-          kv._at, batch._at, ctypes.addressof(how), None if ws is None else ws.data_ptr(), need)
+    _call(dev, load_library().sgq_paged_attention, q_at, q_row, q_head, o_at, o_row, o_head, T, H, kv._at, batch._at,
+          ctypes.addressof(how), None if ws is None else ws.data_ptr(), need)
     return out
 
 

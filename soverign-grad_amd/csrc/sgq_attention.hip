@@ -21,8 +21,12 @@
 //   16 bits: 32x32x16; K rows as 16-byte LDS reads, V^T by transposing 8-byte LDS reads
 //   (four keys of a column a lane).
 //   fp32: 32x32x2; a 16-byte read of K serves four products; V^T a float a lane.
-// Keys and values go from their pages to LDS directly (a lane's address is its row's page),
-// the 16-byte chunks of a row permuted so that all reads are free of conflicts.
+// Keys and values go from their pages to LDS directly, the 16-byte chunks of a row permuted so
+// that all reads are free of conflicts (counted: none).
+//
+// Forms.  Up to 32 rows of a sequence and kv head (single tokens, and a few): k_attend_few, or
+// k_attend_lanes for up to four in fp32; more: k_attend_tiles.  Where their workgroups are too
+// few for the device the keys are split, and k_attend_join joins the splits.
 #include "sgq_lanes.h"
 #include "sgq_paged.h"
 
@@ -39,10 +43,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-typedef __attribute__((address_space(3))) void lds_void;
-typedef __attribute__((address_space(1))) const void global_void;
 
 // Sixteen bytes that a lane without a row of its own reads: zeros.
 __device__ const uint32_t g_zeros[4] = {0, 0, 0, 0};
@@ -612,7 +613,13 @@ __device__ __forceinline__ void phase_end() {
 __device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // A workgroup of NW wavefronts takes 32 NW rows of one sequence and kv head, which share tiles of
-// 32 NK keys in two buffers: while one is worked on, the next loads.
+// 32 NK keys in two buffers: while one is worked on, the next loads.  Two workgroups share a compute unit (64 KiB of LDS
+// each, up to 256 registers a lane), and while the one has the matrix cores the other has the vector unit: a wavefront's 64
+// keys of 128 in bf16 are 32 products of 32 cycles, 32 exponentials of 16 and some 180 vector instructions of 4, so that neither
+// unit can be busy all the time.  4 prompts of 8192 tokens, 64 on 8 heads of 128 in bf16: 4.22 ms, 1040 TFLOP/s, matrix
+// cores 53% and vector unit 55% busy at 1.9 GHz (a large library product: 1094 TFLOP/s); without the loads 3.8.  A prompt of 2048, 32 heads: 52 us,
+// the longest tile's 32 steps one after another.  Measured and not kept: eight wavefronts, half of them a phase behind the other
+// half and barriers between products and softmax (4.8 ms against 4.4: barriers cost more than the units' overlap gave).
 template <typename T, int DP, int NW, int NK, bool CLEAN>
 __device__ __forceinline__ void tile_pass(Rows<T, DP, NK>& w, Loader<T, DP, 32 * NK, 64 * NW>& ld, const Score& sc, char* lds,
                                           int k0, int k1, int max_lo, int min_hi) {
@@ -736,7 +743,8 @@ __global__ __launch_bounds__(64 * NW, DP * sizeof(T) <= 512 ? 2 : 1) void k_atte
 // ---- few rows ----------------------------------------------------------------
 
 // Up to 32 rows of a sequence and kv head (single tokens and a few more): the NW wavefronts of a workgroup
-// have tiles of 32 keys of their own, in two buffers each, and are joined at the end.
+// have tiles of 32 keys of their own, in two buffers each, and are joined at the end.  The cache's bytes bound it: 64 sequences of up
+// to 8192 keys, 32 on 8 heads of 128 in bf16, 1.05 GB in 218 us, 4.8 TB/s; one of 131072 537 MB in 109 us with its join, 4.9.
 template <typename T, int DP, int NW, bool CLEAN>
 __device__ __forceinline__ bool few_pass(Rows<T, DP, 1>& w, Loader<T, DP, 32, 64>& ld, const Score& sc, char* lds, int k0,
                                          int k1) {
@@ -982,7 +990,8 @@ __global__ __launch_bounds__(64 * NW) void k_attend_lanes(const AttendArgs a, co
 // ---- the splits of a row joined ------------------------------------------------
 
 // W wavefronts per row and head (a workgroup has four): the factors of the splits first, to LDS, then four columns and a
-// share of the splits a thread, whose loads are independent.
+// share of the splits a thread, whose loads are independent (64 splits of 32 heads 4 us; one thread's loads one after
+// another took 30 for 256 splits).  About 3.5 TB/s where there are many rows.
 template <typename T, int W>
 __global__ __launch_bounds__(256) void k_attend_join(const AttendArgs a, int d, const Sequences s, const Parts parts) {
     constexpr int kThreads = 64 * W, kItems = 4 / W, kSplits = W == 4 ? kJoinSplits : kWaveSplits;

