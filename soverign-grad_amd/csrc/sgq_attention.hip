@@ -143,6 +143,9 @@ struct Rows {
     typedef typename M::Frag Frag;
     typedef TileRows<T, DP> Tile;
     static constexpr int kFrags = DP / M::kStep, kCols = DP / 32;
+    // Weights and their sum are 2^kLift times what they are: in fp16, which has steps of 2^-24 only below 2^-14, those of many
+    // keys beside a large one would be off together (4095 of e^-14.5: 5%).  The largest is 2^15.
+    static constexpr float kLift = std::is_same_v<T, _Float16> ? 7.0f : 0.0f;
 
     Frag q[kFrags];
     f32x16 o[kCols];
@@ -236,7 +239,7 @@ struct Rows {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) o[i][e] *= w;
         }
-        const float base = m == -INFINITY ? 0.0f : -m * c;
+        const float base = m == -INFINITY ? 0.0f : fmaf(-m, c, kLift);
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int t = 0; t < NK; ++t)
