@@ -1356,8 +1356,8 @@ int sgq_paged_attention(const void* q, int64_t q_row, int64_t q_head, void* out,
     a.slopes = scores->alibi_slopes, a.prefix = scores->prefix, a.first_key = scores->first_key;
     const AttendShape shape = {heads, c.kv_heads, d, s.B, s.rows, s.max_len, s.max_new, a.window, c.t};
     const AttendPlan p = attend_plan(shape, device_cus((hipStream_t)stream));
-    if (p.workgroups * 512 >= (int64_t)1 << 32 || (p.splits > 1 && (int64_t)s.rows * heads * 256 >= (int64_t)1 << 32))
-        return fail(SGQ_ERR_UNSUPPORTED, "%s: too many rows for one call", fn);
+    if (p.workgroups * 256 >= (int64_t)1 << 32)
+        return fail(SGQ_ERR_UNSUPPORTED, "%s: too many sequences for one call", fn);
     const int64_t need = attend_plan_bytes(p, shape);
     if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
         return fail(SGQ_ERR_WORKSPACE, "%s: workspace needs %lld bytes, 16-byte aligned", fn, (long long)need);

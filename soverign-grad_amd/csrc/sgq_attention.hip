@@ -1111,6 +1111,8 @@ void start(const AttendArgs& a, const PagedCache& c, const Sequences& s, const A
 
 }  // namespace
 
+static int64_t attend_split_bytes(const AttendShape& q) { return q.rows * q.heads * (q.head_dim * 4 + 8); }
+
 // Splits share the keys of too few workgroups for the device.  Few rows: four workgroups a compute unit, of at least 128
 // keys (fp32: 256), so that sequences of different lengths come out even; a sequence by itself two, for its splits are
 // alike and each costs its beginning (us, two / four / eight a unit: 131072 keys of one sequence 115 / 122 / 140, 64
@@ -1122,12 +1124,15 @@ AttendPlan attend_plan(const AttendShape& q, int64_t cus) {
     p.few = q.max_new * g <= kTileRows;
     p.lanes = f32 && q.max_new * g <= kLaneRows;
     p.splits = 1;
+    // Rows behind the last sequence have their places among the partial results too: 1 GiB of those at most, which only a
+    // call padded to many times its tokens would need.
+    const int64_t most = std::max<int64_t>(1, ((int64_t)1 << 30) / attend_split_bytes(q));
     int64_t wgs;
     if (p.few) {
         p.tiles = 0;
         wgs = q.B * q.kv_heads;
         p.splits = (int)std::max<int64_t>(1, std::min({ceil_div((q.B == 1 ? 2 : 4) * cus, wgs), ceil_div(len, f32 && !p.lanes ? 256 : 128),
-                                                       (int64_t)kJoinSplits}));
+                                                       (int64_t)kJoinSplits, most}));
     } else {
         const int64_t rows = kTileRows * kTileWaves;
         p.tiles = std::min(q.rows * g / rows + q.B, q.B * ceil_div(q.max_new * g, rows));
@@ -1141,7 +1146,7 @@ AttendPlan attend_plan(const AttendShape& q, int64_t cus) {
         const double longest = ceil_div(seen, 64);
         const double mean = q.window > 0 ? longest : std::max(1.0, longest - (double)q.max_new / 128);
         double best = 0;
-        for (int S = 1; S <= kWaveSplits && (S == 1 || S * 128 <= seen); S *= 2) {
+        for (int S = 1; S <= std::min<int64_t>(kWaveSplits, most) && (S == 1 || S * 128 <= seen); S *= 2) {
             const double rounds = (double)ceil_div(wgs * S, cus);
             const double work = rounds <= 1 ? alone * longest / S : std::max(step * rounds * mean / S, 2 * step * longest / S);
             const double join = S == 1 ? 0 : 4 + (double)(q.rows * q.heads) * (S * q.head_dim * 8 + 256) / 3.5e6;
@@ -1156,7 +1161,7 @@ AttendPlan attend_plan(const AttendShape& q, int64_t cus) {
 
 int64_t attend_plan_bytes(const AttendPlan& p, const AttendShape& q) {
     if (p.splits == 1) return 0;
-    return q.rows * q.heads * p.splits * (q.head_dim * 4 + 8);
+    return attend_split_bytes(q) * p.splits;
 }
 
 hipError_t launch_attend(const AttendArgs& a, const PagedCache& c, const Sequences& s, const AttendPlan& p, void* ws,

@@ -128,6 +128,10 @@ def test_workspace(op, lib):
                             assert need == 0 or need % per == 0 and 2 <= need // per <= 256
                             seen += need > 0
     assert seen > 100
+    # Rows behind the last sequence: a gibibyte at most, however many.
+    for heads, d, new in ((1, 16, 1), (32, 128, 1), (8, 256, 4), (32, 128, 100), (1024, 16, 1)):
+        for rows in (1, 1000, 30000, 2**30 // 1024):
+            assert fn(heads, 1, d, 1, 1, rows, 131072, new, 0, 0) <= 2**30
     for bad in ((0, 1, 64, 0, 1, 1, 1, 1, 0, 0), (3, 2, 64, 0, 1, 1, 1, 1, 0, 0), (2, 2, 60, 0, 1, 1, 1, 1, 0, 0), (2, 2, 64, 3, 1, 1, 1, 1, 0, 0),
                 (2, 2, 64, 0, -1, 1, 1, 1, 0, 0), (2, 2, 64, 0, 1, -1, 1, 1, 0, 0), (2, 2, 64, 0, 1, 1, -1, 1, 0, 0),
                 (2, 2, 64, 0, 1, 1, 1, -1, 0, 0), (2, 2, 64, 0, 1, 1, 1, 1, -1, 0), (2, 2, 64, 0, 1, 1, 1, 1, 0, -1)):

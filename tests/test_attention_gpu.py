@@ -612,6 +612,18 @@ def test_a_cache_past_32_bits(op, dev):
         assert torch.equal(k[table[0].long()], small_k) and torch.equal(v[table[0].long()], small_v)
 
 
+def test_few_tokens_in_a_batch_padded_to_many(op, dev):
+    """One token of one long sequence among 2^21 rows of 8 heads: its row is right, the others stay."""
+    dtype, rows = torch.float16, 2**21
+    b = Batch(op, dev, [(1, 3000)], 16, 8, 16, dtype, pad=rows - 1)
+    q = torch.zeros(rows, 8, 16, dtype=dtype, device=dev)
+    q[0] = _randn(dev, 3, 8, 16)
+    out = torch.full_like(q, 7)
+    op.paged_attention(q, b.kv, b.batch, out=out)
+    assert bool((out[1:] == 7).all())
+    _check(out[:1], _reference(b, q[:1]), b, dtype)
+
+
 def test_heads_that_are_not_aligned_are_copied(op, dev):
     b = Batch(op, dev, [(4, 50)], 16, 2, 64, torch.float16)
     flat = _randn(dev, 1, 4 * 4 * 64 + 1).half()
