@@ -523,7 +523,8 @@ int sgq_norm_rope_append(const void* q, int64_t q_row, int64_t q_head, const voi
                          const int32_t* positions, void* stream);
 
 /* Scores of a query at position p and a key at position j, and who sees whom:
- *   s = scale * (q . k);  softcap > 0: s = softcap * tanh(s / softcap);
+ *   s = scale * (q . k);  softcap > 0: s = softcap * tanh(s / softcap) (|scale| and softcap
+ *   1e30 at most, softcap 1024 at most in 16-bit types: 0 is none);
  *   alibi_slopes [heads] fp32: s -= slope * |p - j|;
  *   key j is seen where j < lens[b], j <= p or j < prefix[b], window == 0 or
  *   j > p - window, and j >= first_key[row].

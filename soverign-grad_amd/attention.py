@@ -246,7 +246,8 @@ def paged_attention(q: torch.Tensor, kv: PagedKV, batch: SequenceBatch, scale: O
     """Attention of the new tokens q [rows, heads, head_dim] over their sequences' keys and values,
     the new ones included (norm_rope_append has put them there).
 
-    Scores s = scale * q . k (scale: 1 / sqrt(head_dim) by itself); softcap > 0: softcap * tanh(s / softcap);
+    Scores s = scale * q . k (scale: 1 / sqrt(head_dim) by itself); softcap > 0: softcap * tanh(s / softcap)
+    (0: none; 1024 at most in 16-bit types);
     alibi_slopes [heads]: then less slope * distance of the positions.  A token at position p sees the
     keys j <= p and those below prefix[b] ([B]; also ahead of it), of them those with j > p - window
     (window > 0) and j >= first_key[row] ([rows], its document's first).  A row that sees

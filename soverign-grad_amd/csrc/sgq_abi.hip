@@ -1338,10 +1338,12 @@ int sgq_paged_attention(const void* q, int64_t q_row, int64_t q_head, void* out,
     if (st != SGQ_OK) return st;
     if (!scores) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: null scores", fn);
     if (scores->window < 0) return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: negative window", fn);
-    if (!(scores->scale >= -3.0e38f && scores->scale <= 3.0e38f))
-        return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: scale must be finite", fn);
-    if (!(scores->softcap >= 0.0f) || scores->softcap > 3.0e38f)
-        return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: softcap must be finite and not negative", fn);
+    if (!(scores->scale >= -1.0e30f && scores->scale <= 1.0e30f))
+        return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: scale must be within 1e30 of zero", fn);
+    if (!(scores->softcap >= 0.0f) || scores->softcap > 1.0e30f)
+        return fail(SGQ_ERR_INVALID_ARGUMENT, "%s: softcap must be from 0 to 1e30", fn);
+    if (scores->softcap > 1024.0f && c.t != DType::f32)
+        return fail(SGQ_ERR_UNSUPPORTED, "%s: softcap past 1024 in 16 bits", fn);
     if (s.rows == 0 || s.B == 0) return ok();
     const int dt = cache->dtype;
     const int64_t d = c.head_dim;

@@ -196,7 +196,9 @@ struct Rows {
                     if constexpr (sizeof(T) == 4) {
                         s[t][e] = sc.out * tanhf(s[t][e] * sc.in);
                     } else {
-                        // tanh x = 1 - 2 / (1 + e^2x): off by some 2^-23, which a 16-bit weight does not see.
+                        // tanh x = 1 - 2 / (1 + e^2x): off by some 2^-23 of the cap, which is 1024 at most here, and a
+                        // 16-bit weight does not see it.  (With a series for the small x of
+                        // wider caps 4 prompts of 8192 tokens, without a cap, took 4.49 ms instead of 4.22.)
                         const float u = __builtin_amdgcn_exp2f(s[t][e] * (2.0f * kLog2e * sc.in));
                         s[t][e] = fmaf(sc.out * -2.0f, __builtin_amdgcn_rcpf(1.0f + u), sc.out);
                     }

@@ -76,8 +76,10 @@ def test_refused_by_both(op, lib, case):
 
 def test_refused_by_attention(op, lib):
     for kw in (dict(scores=dict(window=-1)), dict(scores=dict(softcap=-1.0)), dict(scores=dict(softcap=float("inf"))),
+               dict(scores=dict(softcap=3e38)), dict(scores=dict(scale=3e38)), dict(scores=dict(scale=-3e38)),
                dict(scores=dict(softcap=float("nan"))), dict(out=4 * P + 128), dict(out=4 * P, o_row=320), dict(out=4 * P + 256)):
         assert _attend(op, lib, **kw) == INVALID, kw
+    assert _attend(op, lib, scores=dict(softcap=1025.0)) == UNSUPPORTED
     c, s = _cache(op), _seqs(op)
     assert lib.sgq_paged_attention(P, 256, 64, 2 * P, 256, 64, 5, 4, ctypes.addressof(c), ctypes.addressof(s), None, None, 0,
                                    None) == INVALID

@@ -279,6 +279,27 @@ def test_a_tiny_cap(op, dev):
     _check(y, _reference(b, q, softcap=1e-38), b, torch.float32)
 
 
+@pytest.mark.parametrize("cap", [1024.0, 1e6, 1e30])
+def test_a_wide_cap(op, dev, cap):
+    """A cap that leaves the scores nearly as they are: each off by 2^-20 of itself at most in fp32 (of the cap, steps of
+    2^-23 would be seen), which with (d + 8) >= 72 U of a score twice the uncapped bound covers."""
+    dtype = torch.float32
+    b = Batch(op, dev, [(3, 40), (70, 130), (1, 50)], 16, 2, 64, dtype)
+    q = _randn(dev, 3, b.rows, 4, 64) * 8
+    out, A, _, n = _reference(b, q, softcap=cap)
+    ds = _reference(b, q)[2]
+    _check(op.paged_attention(q, b.kv, b.batch, softcap=cap), (out, A, 2 * ds, n), b, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:])
+def test_the_widest_cap_in_16_bits(op, dev, dtype):
+    b = Batch(op, dev, [(3, 40), (70, 130), (1, 50)], 16, 2, 64, dtype)
+    q = (_randn(dev, 3, b.rows, 4, 64) * 8).to(dtype)
+    _check(op.paged_attention(q, b.kv, b.batch, softcap=1024.0), _reference(b, q, softcap=1024.0), b, dtype)
+    with pytest.raises(Exception, match="softcap past 1024"):
+        op.paged_attention(q, b.kv, b.batch, softcap=1025.0)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_a_row_of_not_finite_queries(op, dev, dtype):
     b = Batch(op, dev, [(70, 200), (1, 100)], 16, 2, 64, dtype)
