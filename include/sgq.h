@@ -489,6 +489,7 @@ typedef struct sgq_paged_cache {
  *            New token i of sequence b has position lens[b] - (starts[b+1] - starts[b]) + i.
  *   max_len, max_new: host bounds on lens and on a sequence's new tokens (they size the
  *            launch and the workspace).
+ * Sequences may share pages of keys that are not new; where two new tokens have one place, it holds either's.
  * A sequence with no new token is left alone.  One that breaks a bound (more new tokens
  * than max_new or than keys; more keys than max_len or than its pages hold) has NaN for its
  * output rows, and nothing is appended.  Where the table names a page outside [0, pages),

@@ -111,7 +111,8 @@ class SequenceBatch:
     New token i of n stands at position lens - n + i.  max_len and max_new bound lens and
     n from the host, which does not see them; they size launches and workspaces, so a bound
     near the truth is the better one.  A sequence that breaks a bound, or whose pages are not in the
-    pool, has NaN for its outputs.  The tensors are read when a call runs: a captured graph takes
+    pool, has NaN for its outputs.  Sequences may share pages of keys that are not new (where two new
+    tokens have one place, it holds either's).  The tensors are read when a call runs: a captured graph takes
     what they hold at its replay."""
 
     __slots__ = ("table", "lens", "starts", "max_len", "max_new", "device", "_struct", "_at")

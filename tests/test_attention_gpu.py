@@ -450,6 +450,29 @@ def test_norm_rope_append(op, dev, shape, interleaved, dtype):
     assert torch.equal(y[:T], out[:T])
 
 
+@pytest.mark.parametrize("count", [64, 65, 130, 4200])
+def test_append_of_many_sequences(op, dev, count):
+    """A token finds its sequence among many, some without tokens."""
+    dtype = torch.float32
+    new = [(7 * i) % 3 for i in range(count)]
+    table = torch.arange(count, dtype=torch.int32, device=dev)[:, None]
+    starts = [0]
+    for n in new:
+        starts.append(starts[-1] + n)
+    rows = starts[-1] + 3
+    kv = op.PagedKV(*(torch.full((count, 8, 1, 16), 5, dtype=dtype, device=dev) for _ in range(2)))
+    batch = op.SequenceBatch(table, _i32(dev, [6] * count), _i32(dev, starts), 8, 2)
+    q, k, v = _randn(dev, 1, rows, 2, 16), _randn(dev, 2, rows, 1, 16), _randn(dev, 3, rows, 1, 16)
+    out = torch.full_like(q, 7)
+    op.norm_rope_append(q, k, v, kv, batch, out=out)
+    assert torch.equal(out[: rows - 3], q[: rows - 3]) and bool((out[rows - 3 :] == 7).all())
+    want = torch.full_like(kv.k, 5), torch.full_like(kv.v, 5)
+    seq = torch.repeat_interleave(torch.arange(count), torch.tensor(new)).to(dev)
+    at = torch.cat([torch.arange(6 - n, 6) for n in new]).to(dev)
+    want[0][seq, at], want[1][seq, at] = k[: rows - 3], v[: rows - 3]
+    assert torch.equal(kv.k, want[0]) and torch.equal(kv.v, want[1])
+
+
 def test_one_norm_of_two(op, dev):
     b = Batch(op, dev, [(5, 9)], 8, 2, 64, torch.float32)
     q, k, v = (_randn(dev, i, 5, 2, 64) for i in range(3))
