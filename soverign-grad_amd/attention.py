@@ -96,6 +96,8 @@ def _int32(t: torch.Tensor, n: int, dev: torch.device, name: str) -> torch.Tenso
     if t.dtype is not torch.int32:
         if t.is_floating_point() or t.is_complex() or t.dtype is torch.bool:
             raise ValueError(f"{name} must be whole numbers")
+        if t.dtype is torch.int64:  # a limit past 32 bits is one past every key, and does not wrap
+            t = t.clamp(-(2**31), 2**31 - 1)
         t = t.to(torch.int32)
     return t if t.is_contiguous() else t.contiguous()
 

@@ -115,6 +115,12 @@ def test_python_refuses_what_is_not_on_the_device(op):
     assert f.dtype == torch.float64 and torch.allclose(f, torch.tensor([1, 0.1, 0.01, 0.001], dtype=torch.float64), rtol=1e-15)
 
 
+def test_limits_in_64_bits_do_not_wrap(op):
+    t = torch.tensor([2**40, -(2**40), 2**31, 5])
+    got = op._int32(t, 4, t.device, "prefix")
+    assert got.dtype is torch.int32 and got.tolist() == [2**31 - 1, -(2**31), 2**31 - 1, 5]
+
+
 def test_workspace(op, lib):
     """What a call needs it says beforehand, for a device of any size, and refuses to run without."""
     fn = lib.sgq_paged_attention_workspace_bytes

@@ -668,6 +668,18 @@ def test_few_tokens_in_a_batch_padded_to_many(op, dev):
     _check(out[:1], _reference(b, q[:1]), b, dtype)
 
 
+def test_limits_past_32_bits(op, dev):
+    """A prefix or a first key in 64 bits that 32 do not hold is past (or before) every key."""
+    b = Batch(op, dev, [(4, 50), (1, 30)], 16, 2, 64, torch.float16)
+    q = _randn(dev, 1, 5, 4, 64).half()
+    for far, near in ((2**63 - 1, 50), (2**32 + 3, 50), (2**31, 50), (-(2**32) + 7, 0), (-(2**63), 0)):
+        got = op.paged_attention(q, b.kv, b.batch, prefix=torch.tensor([far, far], device=dev))
+        assert torch.equal(got, op.paged_attention(q, b.kv, b.batch, prefix=_i32(dev, [near, near])))
+        got = op.paged_attention(q, b.kv, b.batch, first_key=torch.full((5,), far, device=dev))
+        assert torch.equal(got, op.paged_attention(q, b.kv, b.batch, first_key=_i32(dev, [near] * 5)))
+    assert bool((op.paged_attention(q, b.kv, b.batch, first_key=torch.full((5,), 2**40, device=dev)) == 0).all())
+
+
 def test_heads_that_are_not_aligned_are_copied(op, dev):
     b = Batch(op, dev, [(4, 50)], 16, 2, 64, torch.float16)
     flat = _randn(dev, 1, 4 * 4 * 64 + 1).half()
