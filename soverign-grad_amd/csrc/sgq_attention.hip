@@ -621,7 +621,7 @@ __device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)"
 // 32 NK keys in two buffers: while one is worked on, the next loads.  Two workgroups share a compute unit (64 KiB of LDS
 // each, up to 256 registers a lane), and while the one has the matrix cores the other has the vector unit: a wavefront's 64
 // keys of 128 in bf16 are 32 products of 32 cycles, 32 exponentials of 16 and some 180 vector instructions of 4, so that neither
-// unit can be busy all the time.  4 prompts of 8192 tokens, 64 on 8 heads of 128 in bf16: 4.22 ms, 1040 TFLOP/s, matrix
+// unit can be busy all the time.  4 prompts of 8192 tokens, 64 on 8 heads of 128 in bf16: 4.22 to 4.46 ms, 986 to 1040 TFLOP/s, matrix
 // cores 53% and vector unit 55% busy at 1.9 GHz (a large library product: 1094 TFLOP/s); without the loads 3.8.  A prompt of 2048, 32 heads: 52 us,
 // the longest tile's 32 steps one after another.  Measured and not kept: eight wavefronts, half of them a phase behind the other
 // half and barriers between products and softmax (4.8 ms against 4.4: barriers cost more than the units' overlap gave).
