@@ -254,7 +254,8 @@ def paged_attention(q: torch.Tensor, kv: PagedKV, batch: SequenceBatch, scale: O
     alibi_slopes [heads]: then less slope * distance of the positions.  A token at position p sees the
     keys j <= p and those below prefix[b] ([B]; also ahead of it), of them those with j > p - window
     (window > 0) and j >= first_key[row] ([rows], its document's first).  A row that sees
-    none is zeros.  out may be q."""
+    none is zeros.  A value seen that is not finite makes its column so (NaN, or that infinity), whatever its
+    weight.  out may be q."""
     dev = _same_device(kv, batch)
     d = kv.head_dim
     T, H, (q, q_at, q_row, q_head) = _queries(q, kv)

@@ -329,16 +329,15 @@ struct Rows {
                 }
         }
     }
-    // Whether a column below d of the row is not finite, though its sum of weights is.
-    __device__ __forceinline__ bool not_finite(int d, float sum) const {
-        const int h = (threadIdx.x & 63) >> 5;
-        bool bad = false;
+    // Whether a column of the row is not finite (those from d on are zeros), though its sum of weights is: then a sum of zeros
+    // times the columns is a NaN.  (An instruction a column; asking each whether it is finite took 2 us of 106.)
+    __device__ __forceinline__ bool not_finite(float sum) const {
+        float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < kCols; ++i)
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-                if (32 * i + 8 * (e / 4) + 4 * h < d) bad = bad || !isfinite(o[i][e]);
-        return bad && sum == sum;
+            for (int e = 0; e < 16; ++e) z[e & 3] = fmaf(o[i][e], 0.0f, z[e & 3]);
+        return (z[0] + z[1]) + (z[2] + z[3]) != 0.0f && sum == sum;
     }
     // Values v of a key that are not finite, to the rows that see it.
     __device__ __forceinline__ void add_not_finite(const T* v, int key, int d) {
@@ -487,38 +486,62 @@ struct Loader {
     static __device__ __forceinline__ void arrived(Pages& p) { asm volatile("" : "+v"(p.of)); }
 };
 
-// A weight of 0 times an infinity or a NaN is a NaN: values that are not finite touch rows that do not see them,
-// in tiles whose keys some rows see and some do not.  Where a row's result is not finite after such a tile, the
-// wavefront (workgroup) goes over its keys again with such values taken out of those tiles (clean_values), and adds them to
-// the rows that see them at the end (add_values).  THREADS threads, all of which come along.
+// A weight of 0 times an infinity or a NaN is a NaN: values that are not finite touch rows that do not see them, and an
+// infinity that a row sees with a weight below fp32's range (exactly, it is positive) becomes a NaN.  Where a row's
+// result is not finite, the wavefront (workgroup) goes over its keys again with such values taken out of the tiles
+// (clean_values), and adds them, as they are, to the rows that see them at the end (add_values, of the tiles that had some: bit i of
+// `found` is for tiles i, i + 64, ..).  THREADS threads, all of which come along.
 template <typename T, int BYTES, int THREADS>
-__device__ __forceinline__ void clean_values(char* tile, int thread) {
+__device__ __forceinline__ bool clean_values(char* tile, int thread) {
     typedef typename Chunk<T>::type Vec;
+    bool found = false;
     for (int i = thread * 16; i < BYTES; i += THREADS * 16) {
         Vec v = *(const Vec*)(tile + i);
 #pragma unroll
-        for (int e = 0; e < Chunk<T>::N; ++e) v[e] = isfinite((float)v[e]) ? v[e] : (T)0.0f;
+        for (int e = 0; e < Chunk<T>::N; ++e) {
+            const bool ok = isfinite((float)v[e]);
+            v[e] = ok ? v[e] : (T)0.0f;
+            found = found || !ok;
+        }
         *(Vec*)(tile + i) = v;
     }
+    return found;
 }
 template <typename T, int DP, int NK>
 __device__ __forceinline__ void add_values(Rows<T, DP, NK>& w, const PagedCache& c, const int32_t* table, int kvh, int k0, int k1,
-                                           int step, int max_lo, int min_hi) {
+                                           int step, uint64_t found) {
+    constexpr int U = 8;  // keys whose loads are in flight together
     const int lane = threadIdx.x & 63, d = c.head_dim;
+    int tile = 0;
 #pragma unroll 1
-    for (int k = k0; k < k1; k += step) {
-        if (k >= max_lo && k + 32 * NK <= min_hi) continue;
+    for (int k = k0; k < k1; k += step, ++tile) {
+        if (!(found >> (tile & 63) & 1)) continue;
+        const int end = min(k + 32 * NK, k1);
 #pragma unroll 1
-        for (int key = k; key < min(k + 32 * NK, k1); ++key) {
-            const int64_t off = key_offset(c, table, key);
-            if (off < 0) continue;  // the result is NaN anyway
-            const T* v = (const T*)c.v + off + (int64_t)kvh * c.head_stride;
-            bool bad = false;
+        for (int first = k; first < end; first += U) {
+            // (Of a page that is not in the pool the pool's first rows: the result is NaN anyway.)
+            auto values = [&](int key) {
+                return (const T*)c.v + max(key_offset(c, table, min(key, end - 1)), (int64_t)0) + (int64_t)kvh * c.head_stride;
+            };
+            unsigned bad = 0;
 #pragma unroll
-            for (int i = 0; i < kMaxHeadDim / 64; ++i) bad = bad || !isfinite((float)v[min(lane + 64 * i, d - 1)]);
-            if (__any(bad)) w.add_not_finite(v, key, d);
+            for (int u = 0; u < U; ++u) {
+                const T* v = values(first + u);
+#pragma unroll
+                for (int i = 0; i < kMaxHeadDim / 64; ++i) bad |= (unsigned)!isfinite((float)v[min(lane + 64 * i, d - 1)]) << u;
+            }
+#pragma unroll 1
+            for (int u = 0; u < U && first + u < end; ++u)
+                if (__any(bad >> u & 1)) w.add_not_finite(values(first + u), first + u, d);
         }
     }
+}
+
+// What a part with a factor below fp32's range adds to a join, with a factor of 1: what is not finite, as it is.
+__device__ __forceinline__ f32x4 rest_of(f32x4 x) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = isfinite(x[e]) ? 0.0f : x[e];
+    return x;
 }
 
 // Where a launch's partial results lie: for (row, head) r and split s, fp32 columns at
@@ -582,9 +605,10 @@ __device__ __forceinline__ void join_waves(const AttendArgs& a, const Parts& par
     for (int v = 0; v < NW; ++v) {
         const float l = sum_of(v, q);
         if (l == 0.0f) continue;  // nothing seen, its maximum -inf
-        const float f = __builtin_amdgcn_exp2f(max_of(v, q) - (top == -INFINITY ? 0.0f : top));
+        float f = __builtin_amdgcn_exp2f(max_of(v, q) - (top == -INFINITY ? 0.0f : top));
         sum = fmaf(l, f, sum);
-        const f32x4 x = *(const f32x4*)(cols_of(v, q) + col);
+        f32x4 x = *(const f32x4*)(cols_of(v, q) + col);
+        if (f == 0.0f) x = rest_of(x), f = 1.0f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], f, o[e]);
     }
@@ -626,8 +650,8 @@ __device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)"
 // the longest tile's 32 steps one after another.  Measured and not kept: eight wavefronts, half of them a phase behind the other
 // half and barriers between products and softmax (4.8 ms against 4.4: barriers cost more than the units' overlap gave).
 template <typename T, int DP, int NW, int NK, bool CLEAN>
-__device__ __forceinline__ void tile_pass(Rows<T, DP, NK>& w, Loader<T, DP, 32 * NK, 64 * NW>& ld, const Score& sc, char* lds,
-                                          int k0, int k1, int max_lo, int min_hi) {
+__device__ __forceinline__ uint64_t tile_pass(Rows<T, DP, NK>& w, Loader<T, DP, 32 * NK, 64 * NW>& ld, const Score& sc, char* lds,
+                                              int k0, int k1) {
     typedef Loader<T, DP, 32 * NK, 64 * NW> L;
     constexpr int kKeys = 32 * NK, B = L::kBytes;
     const uint32_t at = __builtin_amdgcn_readfirstlane(lds_address(lds));  // keys, values; keys, values
@@ -637,11 +661,12 @@ __device__ __forceinline__ void tile_pass(Rows<T, DP, NK>& w, Loader<T, DP, 32 *
     loads_done();
     phase_end();
     int odd = 0;
+    uint64_t found = 0;
 #pragma unroll 1
     for (int k = k0; k < k1; k += kKeys, odd ^= 1) {
         char* const cur = lds + odd * 2 * B;
-        if (CLEAN && (k < max_lo || k + kKeys > min_hi)) {
-            clean_values<T, B, 64 * NW>(cur + B, threadIdx.x);
+        if constexpr (CLEAN) {
+            if (__syncthreads_or(clean_values<T, B, 64 * NW>(cur + B, threadIdx.x))) found |= 1ull << ((k - k0) / kKeys & 63);
             phase_end();
         }
         const uint32_t next = at + (odd ^ 1) * 2 * B;
@@ -660,6 +685,7 @@ __device__ __forceinline__ void tile_pass(Rows<T, DP, NK>& w, Loader<T, DP, 32 *
         loads_done();
         phase_end();
     }
+    return found;
 }
 
 template <typename T, int DP, int NW, int NK>
@@ -668,7 +694,7 @@ __global__ __launch_bounds__(64 * NW, DP * sizeof(T) <= 512 ? 2 : 1) void k_atte
     typedef Loader<T, DP, 32 * NK, 64 * NW> L;
     constexpr int kRows = kTileRows * NW;
     __shared__ __align__(16) char lds[4 * L::kBytes];
-    __shared__ int range[4][NW];
+    __shared__ int range[2][NW];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = a.heads / c.kv_heads;
     const int kvh = blockIdx.x % c.kv_heads, split = blockIdx.x / c.kv_heads % parts.splits;
@@ -719,27 +745,22 @@ __global__ __launch_bounds__(64 * NW, DP * sizeof(T) <= 512 ? 2 : 1) void k_atte
     w.slope = a.slopes ? a.slopes[head] * kLog2e : 0.0f;
     w.load((const T*)a.q.p + (int64_t)row * a.q.row + (int64_t)head * a.q.head, c.head_dim, sc.negate);
     w.bounds();
-    if (lane == 0) range[0][wave] = w.min_lo, range[1][wave] = w.max_hi, range[2][wave] = w.max_lo, range[3][wave] = w.min_hi;
+    if (lane == 0) range[0][wave] = w.min_lo, range[1][wave] = w.max_hi;
     __syncthreads();
-    int lo = range[0][0], hi = range[1][0], max_lo = range[2][0], min_hi = range[3][0];
+    int lo = range[0][0], hi = range[1][0];
 #pragma unroll
-    for (int i = 1; i < NW; ++i) {
-        lo = min(lo, range[0][i]), hi = max(hi, range[1][i]);
-        max_lo = max(max_lo, range[2][i]), min_hi = min(min_hi, range[3][i]);
-    }
+    for (int i = 1; i < NW; ++i) lo = min(lo, range[0][i]), hi = max(hi, range[1][i]);
     lo = __builtin_amdgcn_readfirstlane(lo), hi = __builtin_amdgcn_readfirstlane(hi);
-    max_lo = __builtin_amdgcn_readfirstlane(max_lo), min_hi = __builtin_amdgcn_readfirstlane(min_hi);
     int k0, k1;
     L ld(c, s.table + b * s.table_ld, kvh, threadIdx.x);
     split_range(ld.begin(lo), hi, split, parts.splits, 32 * NK, k0, k1);
     w.clear();
-    if (k0 < k1) tile_pass<T, DP, NW, NK, false>(w, ld, sc, lds, k0, k1, max_lo, min_hi);
+    if (k0 < k1) tile_pass<T, DP, NW, NK, false>(w, ld, sc, lds, k0, k1);
     const bool bad = __syncthreads_or(ld.bad());
-    const bool part = k0 < k1 && (k0 < max_lo || k0 + round_up(k1 - k0, 32 * NK) > min_hi);
-    if (!bad && __builtin_expect(__syncthreads_or(part && on && w.not_finite(c.head_dim, other_half(w.l, false))), 0)) {
+    if (!bad && __builtin_expect(__syncthreads_or(k0 < k1 && on && w.not_finite(other_half(w.l, false))), 0)) {
         w.clear();
-        tile_pass<T, DP, NW, NK, true>(w, ld, sc, lds, k0, k1, max_lo, min_hi);
-        add_values(w, c, ld.table, kvh, k0, k1, 32 * NK, max_lo, min_hi);
+        const uint64_t found = tile_pass<T, DP, NW, NK, true>(w, ld, sc, lds, k0, k1);
+        add_values(w, c, ld.table, kvh, k0, k1, 32 * NK, found);
     }
     const float unit = sc.capped || sc.sloped ? 1.0f : sc.c;
     finish(w, a, parts, unit, split, c.head_dim, row, head, on, bad);
@@ -751,14 +772,14 @@ __global__ __launch_bounds__(64 * NW, DP * sizeof(T) <= 512 ? 2 : 1) void k_atte
 // have tiles of 32 keys of their own, in two buffers each, and are joined at the end.  The cache's bytes bound it: 64 sequences of up
 // to 8192 keys, 32 on 8 heads of 128 in bf16, 1.05 GB in 218 us, 4.8 TB/s; one of 131072 537 MB in 109 us with its join, 4.9.
 template <typename T, int DP, int NW, bool CLEAN>
-__device__ __forceinline__ bool few_pass(Rows<T, DP, 1>& w, Loader<T, DP, 32, 64>& ld, const Score& sc, char* lds, int k0,
-                                         int k1) {
+__device__ __forceinline__ uint64_t few_pass(Rows<T, DP, 1>& w, Loader<T, DP, 32, 64>& ld, const Score& sc, char* lds, int k0,
+                                             int k1) {
     typedef Loader<T, DP, 32, 64> L;
     constexpr int B = L::kBytes, kStep = 32 * NW;
     const uint32_t at = __builtin_amdgcn_readfirstlane(lds_address(lds));  // keys, values; keys, values
     w.clear();
-    if (k0 >= k1) return false;
-    bool any_part = false;
+    if (k0 >= k1) return 0;
+    uint64_t found = 0;
     typename L::Pages p = ld.pages(k0, k1);
     ld.load(at, at + B, k0, k1, p);
     p = ld.pages(k0 + kStep, k1);
@@ -771,15 +792,15 @@ __device__ __forceinline__ bool few_pass(Rows<T, DP, 1>& w, Loader<T, DP, 32, 64
             ld.load(next, next + B, k + kStep, k1, p);
         }
         p = ld.pages(k + 2 * kStep, k1);
-        any_part = any_part || w.part(k);
         char* const cur = lds + odd * 2 * B;
-        if (CLEAN && w.part(k)) clean_values<T, B, 64>(cur + B, threadIdx.x & 63);
+        if constexpr (CLEAN)
+            if (__any(clean_values<T, B, 64>(cur + B, threadIdx.x & 63))) found |= 1ull << ((k - k0) / kStep & 63);
         w.scores(cur, [](int) {});
         w.softmax(k, sc);
         w.values(cur + B);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
-    return any_part;
+    return found;
 }
 
 template <typename T, int DP, int NW>
@@ -813,12 +834,12 @@ __global__ __launch_bounds__(64 * NW) void k_attend_few(const AttendArgs a, cons
     int k0, k1;
     L ld(c, s.table + b * s.table_ld, kvh, lane);
     split_range(ld.begin(w.min_lo), w.max_hi, split, parts.splits, 32 * NW, k0, k1);
-    const bool part = few_pass<T, DP, NW, false>(w, ld, sc, lds[wave], k0 + 32 * wave, k1);
+    few_pass<T, DP, NW, false>(w, ld, sc, lds[wave], k0 + 32 * wave, k1);
     float l = other_half(w.l, false);
-    if (__builtin_expect(__any(part && on && w.not_finite(d, l)), 0)) {
-        few_pass<T, DP, NW, true>(w, ld, sc, lds[wave], k0 + 32 * wave, k1);
+    if (__builtin_expect(__any(on && w.not_finite(l)), 0)) {
+        const uint64_t found = few_pass<T, DP, NW, true>(w, ld, sc, lds[wave], k0 + 32 * wave, k1);
         l = other_half(w.l, false);
-        add_values(w, c, ld.table, kvh, k0 + 32 * wave, k1, 32 * NW, w.max_lo, w.min_hi);
+        add_values(w, c, ld.table, kvh, k0 + 32 * wave, k1, 32 * NW, found);
     }
     const float unit = sc.capped || sc.sloped ? 1.0f : sc.c;
     const bool bad = __any(ld.bad());
@@ -910,7 +931,8 @@ __global__ __launch_bounds__(64 * NW) void k_attend_lanes(const AttendArgs a, co
             vx[u] = __builtin_nontemporal_load((const Vec*)(vp + off));
         }
     };
-    auto take = [&](int k, Vec (&kx)[U], Vec (&vx)[U]) {
+    float extra[R][NV];  // what is not finite among the values seen
+    auto take = [&](auto clean, int k, Vec (&kx)[U], Vec (&vx)[U]) {
         if (narrow && !on)
 #pragma unroll
             for (int u = 0; u < U; ++u)
@@ -947,8 +969,11 @@ __global__ __launch_bounds__(64 * NW) void k_attend_lanes(const AttendArgs a, co
                 const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(p), (u & 4) * 8 + (u & 2) * 8 + (u & 1)));
                 const bool seen = !part || (k + u >= lo[i] && k + u < hi[i]);
 #pragma unroll
-                for (int e = 0; e < NV; ++e)
-                    o[i][e] = seen ? fmaf(w, vx[u][e], o[i][e]) : o[i][e];  // what is not seen may be anything
+                for (int e = 0; e < NV; ++e) {
+                    const bool in_sum = seen && (!clean() || isfinite(vx[u][e]));
+                    if (clean() && seen && !in_sum) extra[i][e] += vx[u][e];
+                    o[i][e] = in_sum ? fmaf(w, vx[u][e], o[i][e]) : o[i][e];  // what is not seen may be anything
+                }
             }
         }
     };
@@ -962,13 +987,37 @@ __global__ __launch_bounds__(64 * NW) void k_attend_lanes(const AttendArgs a, co
         for (;;) {
             page = page_of(k + 2 * step);
             load(k + step, next, kb, vb);
-            take(k, ka, va);
+            take(std::false_type{}, k, ka, va);
             if ((k += step) >= k1) break;
             next = page_of(k + 2 * step);
             load(k + step, page, ka, va);
-            take(k, kb, vb);
+            take(std::false_type{}, k, kb, vb);
             if ((k += step) >= k1) break;
         }
+    }
+    // A weight below fp32's range is 0 and makes a NaN of an infinity: again without them, and they as they are at the end.
+    bool not_finite = false;
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int e = 0; e < NV; ++e) not_finite = not_finite || !isfinite(o[i][e]);
+    if (__builtin_expect(__any(not_finite), 0)) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            m[i] = -INFINITY, l[i] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < NV; ++e) o[i][e] = extra[i][e] = 0.0f;
+        }
+#pragma unroll 1
+        for (k = k0 + U * wave; k < k1; k += step) {
+            Vec kx[U], vx[U];
+            load(k, page_of(k), kx, vx);
+            take(std::true_type{}, k, kx, vx);
+        }
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int e = 0; e < NV; ++e) o[i][e] += extra[i][e];
     }
     // A key's weight is in eight lanes of a wavefront's sum.
 #pragma unroll
@@ -1024,7 +1073,8 @@ __global__ __launch_bounds__(256) void k_attend_join(const AttendArgs a, int d, 
     }
     const float f = v.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(v.x - (top == -INFINITY ? 0.0f : top));
     float sum = v.y == 0.0f ? 0.0f : v.y * f;
-    if (t < kSplits) factor[own][t] = v.y == v.y ? f : 0.0f;  // a sum of NaN: its columns may not have been written
+    // Columns have been written where something was seen; beside a sum of NaN they may not have been, and need not.
+    if (t < kSplits) factor[own][t] = v.y != 0.0f && v.y == v.y ? f : -1.0f;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
     if constexpr (W == 4)
@@ -1041,9 +1091,12 @@ __global__ __launch_bounds__(256) void k_attend_join(const AttendArgs a, int d, 
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int i = i0 + u * groups;
-                w[u] = i < parts.splits ? factor[own][i] : 0.0f;
-                x[u] = w[u] != 0.0f ? *(const f32x4*)(parts.o + (at + i) * d + col) : f32x4{0.f, 0.f, 0.f, 0.f};
+                w[u] = i < parts.splits ? factor[own][i] : -1.0f;
+                x[u] = w[u] >= 0.0f ? *(const f32x4*)(parts.o + (at + i) * d + col) : f32x4{0.f, 0.f, 0.f, 0.f};
             }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (w[u] == 0.0f) x[u] = rest_of(x[u]), w[u] = 1.0f;
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll

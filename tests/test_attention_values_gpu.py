@@ -1,0 +1,106 @@
+"""Values and scores at the ends of the types' ranges, in every form of attention over a paged cache.
+
+Exact weights are positive, however small: a NaN among the values that a row sees makes that column of
+the row NaN, an infinity that infinity, infinities of both signs NaN.  It may not depend on whether fp32
+has the weight, or on how a call's keys are shared out.  Tolerances of finite columns are those of
+test_attention_gpu.
+"""
+import math
+
+import pytest
+import torch
+
+from test_attention_gpu import TYPES, Batch, _check, _i32, _randn, _reference
+
+pytestmark = pytest.mark.gpu
+
+INF, NAN = float("inf"), float("nan")
+
+
+@pytest.fixture(scope="module")
+def op(sgq):
+    import soverign_grad_amd.attention as attention
+
+    return attention
+
+
+def _put(b, seq=0):
+    """The sequence's values (and keys) into their pages again."""
+    n = b.seqs[seq][1]
+    j = torch.arange(n, device=b.dev)
+    at = b.table[seq, j // b.page].long(), j % b.page
+    b.k[at], b.v[at] = b.keys[seq], b.values[seq]
+
+
+def _expect(b, y, q, bad, dtype, **how):
+    """bad: {column: what it is} for every row; the other columns against 64 bits."""
+    for col, want in bad.items():
+        got = y[..., col].float()
+        ok = got.isnan() if math.isnan(want) else got == want
+        assert bool(ok.all()), f"column {col}: {got.flatten()[~ok.flatten()][:4].tolist()} for {want}"
+    for v in b.values:
+        v.copy_(torch.where(torch.isfinite(v), v, 0))
+    out, A, ds, n = _reference(b, q, **how)
+    hit = torch.zeros(y.shape[-1], dtype=torch.bool, device=y.device)
+    hit[list(bad)] = True
+    _check(torch.where(hit, out, y.double()), (out, A, ds, n), b, dtype)
+
+
+# (new, keys): lanes or few rows, few rows in fp32 too, tiles; keys in one piece and shared out.
+SEQS = [(1, 90), (1, 4000), (6, 90), (6, 4000), (40, 90), (40, 4000), (150, 700)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("seq", SEQS)
+@pytest.mark.parametrize("where", ["bias", "low", "early"])
+def test_seen_values_that_are_not_finite_whatever_their_weight(op, dev, seq, dtype, where):
+    """Keys whose weights are far below fp32's range, by a bias, by their scores, or by a maximum that comes
+    later: at the beginning, in the middle, in the last page that all rows see."""
+    new, n = seq
+    d, last = 64, n - new
+    b = Batch(op, dev, [seq], 16, 1, d, dtype)
+    q = _randn(dev, 3, new, 2, d).to(dtype)
+    b.keys[0][..., 0], q[..., 0] = 0, 8
+    keys = {0: (1, INF), last // 2: (2, -INF), max(last - 1, 0): (3, NAN)}
+    how = dict(scale=1.0)
+    if where == "bias":  # 50 keys from every row, e^-700
+        how["alibi_slopes"] = torch.full((2,), 14.0, device=dev)
+        keys = {k: c for k, c in keys.items() if k <= n - new - 50}
+    else:
+        b.keys[0][..., 1:] = 0
+        for k in list(keys) + [1]:
+            b.keys[0][k, :, 0] = -40 if where == "low" else 0
+        if where == "early":
+            b.keys[0][last, :, 0] = 40  # all rows see it
+    keys[1] = (4, INF)
+    b.values[0][1, 0, 5] = INF
+    for k, (col, value) in keys.items():
+        b.values[0][k, 0, col] = value
+    b.values[0][max(k for k in keys if k != 1), 0, 5] = -INF
+    _put(b)
+    bad = {col: value for col, value in keys.values()}
+    bad[5] = NAN
+    y = op.paged_attention(q, b.kv, b.batch, **how)
+    _expect(b, y, q, bad, dtype, **how)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("new", [1, 6, 40])
+def test_they_do_not_reach_rows_that_do_not_see_them(op, dev, dtype, new):
+    """Weights below fp32's range again, and half of the rows begin behind the key."""
+    n, d = 4000, 64
+    b = Batch(op, dev, [(new, n), (2, 50)], 16, 1, d, dtype)
+    q = _randn(dev, 3, b.rows, 4, d).to(dtype)
+    how = dict(alibi_slopes=torch.full((4,), 0.25, device=dev))
+    b.values[0][500, 0, 7] = INF
+    _put(b)
+    first = [0 if i % 2 == 0 else 501 for i in range(b.rows)]
+    how["first_key"] = _i32(dev, first)
+    y = op.paged_attention(q, b.kv, b.batch, **how)
+    sees = torch.tensor([f == 0 for f in first], device=dev)
+    sees[new:] = False
+    assert bool((y[sees][..., 7] == INF).all())
+    b.values[0][500, 0, 7] = 0
+    out, A, ds, cnt = _reference(b, q, **how)
+    hit = sees[:, None, None] & (torch.arange(d, device=dev) == 7)
+    _check(torch.where(hit, out, y.double()), (out, A, ds, cnt), b, dtype)
