@@ -37,6 +37,7 @@ namespace sgq {
 namespace {
 
 constexpr float kLog2e = 1.44269504f;
+constexpr float kGrowth = 8.0f;  // a running maximum is raised where a score's weight passes 2^kGrowth
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -143,9 +144,11 @@ struct Rows {
     typedef typename M::Frag Frag;
     typedef TileRows<T, DP> Tile;
     static constexpr int kFrags = DP / M::kStep, kCols = DP / 32;
-    // Weights and their sum are 2^kLift times what they are: in fp16, which has steps of 2^-24 only below 2^-14, those of many
-    // keys beside a large one would be off together (4095 of e^-14.5: 5%).  The largest is 2^15.
-    static constexpr float kLift = std::is_same_v<T, _Float16> ? 7.0f : 0.0f;
+    // Weights and their sum are 2^kLift times what they are, which without it is 2^8 at most (softmax() says why).  With 2^-8
+    // they are 1 at most, so that a sum of large values passes fp32's range no sooner than with a maximum that is raised at once.
+    // In fp16, which has steps of 2^-24 only below 2^-14, those of many keys beside a large one would be off
+    // together (4095 of e^-14.5: 5%); its values are 2^16 at most, and the weights go up to 2^15.
+    static constexpr float kLift = std::is_same_v<T, _Float16> ? 7.0f : -kGrowth;
 
     Frag q[kFrags];
     f32x16 o[kCols];
@@ -230,8 +233,8 @@ struct Rows {
             for (int e = 0; e < 16; ++e) top = fmaxf(top, s[t][e]);
         top = other_half(top, true);
         // The factor of what was summed is due only where a maximum grew by more than 2^8: until
-        // then weights are up to 2^8 and sums as exact as before.
-        if (__any((top - m) * c > 8.0f)) {
+        // then weights are up to 2^8 (times 2^kLift) and sums as exact as before.
+        if (__any((top - m) * c > kGrowth)) {
             const float now = fmaxf(m, top);
             const float w = __builtin_amdgcn_exp2f((m - (now == -INFINITY ? 0.0f : now)) * c);
             m = now;
@@ -955,14 +958,14 @@ __global__ __launch_bounds__(64 * NW) void k_attend_lanes(const AttendArgs a, co
             v = capped ? out_cap * tanhf(v * in) : v * unit;
             if (sloped) v = fmaf(-slope[i], (float)abs(pos[i] - key), v);
             if (part && (key < lo[i] || key >= hi[i])) v = -INFINITY;
-            if (__any(v - m[i] > 8.0f)) {
+            if (__any(v - m[i] > kGrowth)) {
                 const float now = fmaxf(m[i], row_top(v));
                 const float w = __builtin_amdgcn_exp2f(m[i] - (now == -INFINITY ? 0.0f : now));
                 m[i] = now, l[i] *= w;
 #pragma unroll
                 for (int e = 0; e < NV; ++e) o[i][e] *= w;
             }
-            const float p = __builtin_amdgcn_exp2f(v - (m[i] == -INFINITY ? 0.0f : m[i]));
+            const float p = __builtin_amdgcn_exp2f(v - (m[i] == -INFINITY ? 0.0f : m[i]) - kGrowth);  // 1 at most
             l[i] += p;  // each key's in the lanes that have it
 #pragma unroll
             for (int u = 0; u < U; ++u) {

@@ -104,3 +104,24 @@ def test_they_do_not_reach_rows_that_do_not_see_them(op, dev, dtype, new):
     out, A, ds, cnt = _reference(b, q, **how)
     hit = sees[:, None, None] & (torch.arange(d, device=dev) == 7)
     _check(torch.where(hit, out, y.double()), (out, A, ds, cnt), b, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES[:2])
+@pytest.mark.parametrize("seq", SEQS + [(1, 131072), (6, 131072)])
+def test_large_values_under_a_maximum_that_grows(op, dev, seq, dtype):
+    """Values of 2^123 whose weights, of 1 at most, sum to less than 4: the sums stay within fp32, also where the largest
+    score comes after one that is 5 (2^7.2) less."""
+    new, n = seq
+    b = Batch(op, dev, [seq], 16, 1, 64, dtype)
+    top = 128 if n > 300 else n - new  # a later tile, of the same wavefront where keys are many
+    k = b.keys[0]
+    k.zero_()
+    k[..., 0] = -20
+    k[0, :, 0], k[top, :, 0] = -0.625, 0  # scores of -160, -5, 0
+    b.values[0].copy_(b.values[0].sign() * 2.0**123)
+    _put(b)
+    q = torch.zeros(new, 2, 64, dtype=dtype, device=dev)
+    q[..., 0] = 8
+    y = op.paged_attention(q, b.kv, b.batch, scale=1.0)
+    assert bool(torch.isfinite(y).all())
+    _check(y, _reference(b, q, scale=1.0), b, dtype)
