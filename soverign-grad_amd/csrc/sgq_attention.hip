@@ -244,7 +244,18 @@ struct Rows {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) o[i][e] *= w;
         }
-        const float base = m == -INFINITY ? 0.0f : fmaf(-m, c, kLift);
+        // exp2(s c - m c) with m c rounded has one instruction for the exponent.  What is lost of m c, 2^-24 of it, is the same
+        // for all keys under one maximum, but from 2^28 on it takes weights past the type's range: scores past 2^12 have
+        // the maximum taken off first.
+        float base = m == -INFINITY ? 0.0f : fmaf(-m, c, kLift);
+        if (__builtin_expect(__any(fabsf(base) > 4096.0f), 0)) {
+            const float off = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+            for (int t = 0; t < NK; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[t][e] -= off;
+            base = kLift;
+        }
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int t = 0; t < NK; ++t)

@@ -125,3 +125,25 @@ def test_large_values_under_a_maximum_that_grows(op, dev, seq, dtype):
     y = op.paged_attention(q, b.kv, b.batch, scale=1.0)
     assert bool(torch.isfinite(y).all())
     _check(y, _reference(b, q, scale=1.0), b, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("seq", SEQS)
+@pytest.mark.parametrize("bias", [False, True])
+def test_scores_of_many_digits(op, dev, seq, dtype, bias):
+    """Scores of up to 2^33 (fp16) and 2^50, whose differences fp32 still has: the largest takes it all, and its value comes out
+    as it is."""
+    new, n = seq
+    big = 2.0**15 if dtype is torch.float16 else 2.0**23
+    b = Batch(op, dev, [seq], 16, 1, 64, dtype)
+    top = (n - new) // 2
+    b.keys[0].copy_(b.keys[0].sign() * big)
+    b.keys[0][top] = big
+    q = (0.5 + _randn(dev, 3, new, 2, 1).abs().clamp(max=3) / 4) * big  # up to 1.25 of it
+    q = q.expand(-1, -1, 64).contiguous().to(dtype)
+    _put(b)
+    # The next score is at least two of 64 terms below.
+    assert int((b.keys[0] > 0).sum(-1).kthvalue(n - 1, 0).values) <= 62
+    how = dict(alibi_slopes=torch.full((2,), 0.5, device=dev)) if bias else {}
+    y = op.paged_attention(q, b.kv, b.batch, **how)
+    assert torch.equal(y, b.values[0][top].expand_as(y))
