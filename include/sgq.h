@@ -484,8 +484,8 @@ typedef struct sgq_paged_cache {
  *   table:   [B] rows of table_ld page numbers, table_pages of them usable: key j of
  *            sequence b is in page table[b][j / page_size].
  *   lens:    [B] keys per sequence, its new tokens included.
- *   starts:  [B + 1] first row of each sequence's new tokens, never decreasing; rows from
- *            starts[B] up to the call's `rows` belong to none (their outputs stay as they were).
+ *   starts:  [B + 1] first row of each sequence's new tokens, never decreasing; rows before starts[0] and
+ *            from starts[B] up to the call's `rows` belong to none (their outputs stay as they were).
  *            New token i of sequence b has position lens[b] - (starts[b+1] - starts[b]) + i.
  *   max_len, max_new: host bounds on lens and on a sequence's new tokens (they size the
  *            launch and the workspace).

@@ -107,8 +107,8 @@ class SequenceBatch:
 
       table [B, pages]  page of key j of sequence b: table[b, j // page]
       lens [B]          keys of a sequence, its new tokens included
-      starts [B + 1]    first row of a sequence's new tokens; rows from starts[B] on are
-                        of no sequence and stay as they are
+      starts [B + 1]    first row of a sequence's new tokens; rows before starts[0] and from
+                        starts[B] on are of no sequence and stay as they are
 
     New token i of n stands at position lens - n + i.  max_len and max_new bound lens and
     n from the host, which does not see them; they size launches and workspaces, so a bound

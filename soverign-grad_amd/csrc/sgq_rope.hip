@@ -39,8 +39,7 @@ __global__ __launch_bounds__(kBlock) void k_norm_rope_append(const RopeArgs a, c
     const int b = seq_of_row(s, row);
     if (b >= s.B) return;
     const SeqRows r = seq_rows(s, b);
-    const bool inside = row >= r.row0 && row < r.row0 + r.n;
-    if (!inside && r.ok) return;  // starts that decrease
+    if (row < r.row0 || row >= r.row0 + r.n) return;  // before the first sequence, or starts that decrease
     const int at = r.position(row);
     const int64_t slot = r.ok ? key_offset(c, s.table + b * s.table_ld, at) : -1;
     const bool ok = slot >= 0;
