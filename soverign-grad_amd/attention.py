@@ -50,10 +50,27 @@ class _Scores(ctypes.Structure):
                 ("alibi_slopes", ctypes.c_void_p), ("prefix", ctypes.c_void_p), ("first_key", ctypes.c_void_p)]
 
 
-class PagedKV:
+class _Held:
+    """An object whose struct holds addresses of its tensors, and so is not changed; a copy of it is made of their copies."""
+
+    __slots__ = ()
+
+    def _hold(self, **values) -> None:
+        for name, value in values.items():
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"{type(self).__name__} keeps addresses of its tensors: make a new one instead of assigning {name}")
+
+    def __delattr__(self, name):
+        self.__setattr__(name, None)
+
+
+class PagedKV(_Held):
     """A layer's pool of pages: k and v [pages, page, kv_heads, head_dim], alike in shape,
     strides and type; page a power of two from 8 on, head_dim a multiple of 16 up to 256, heads next to
-    each other in any order of the first three dimensions (views of [pages, kv_heads, page, head_dim] will do)."""
+    each other in any order of the first three dimensions (views of [pages, kv_heads, page, head_dim] will do).
+    The pool is written in place: assigning an attribute is refused."""
 
     __slots__ = ("k", "v", "dtype", "device", "kv_heads", "head_dim", "_step", "_struct", "_at")
 
@@ -76,10 +93,12 @@ class PagedKV:
             raise ValueError("every head of a page must be 16-byte aligned and contiguous")
         if k.numel() and k.data_ptr() == v.data_ptr():
             raise ValueError("k and v must have memory of their own")
-        self.k, self.v, self.dtype, self.device = k, v, k.dtype, k.device
-        self.kv_heads, self.head_dim, self._step = heads, d, step
-        self._struct = _PagedCache(k.data_ptr(), v.data_ptr(), pages, page, heads, d, *strides, _dtype(k.dtype))
-        self._at = ctypes.addressof(self._struct)
+        struct = _PagedCache(k.data_ptr(), v.data_ptr(), pages, page, heads, d, *strides, _dtype(k.dtype))
+        self._hold(k=k, v=v, dtype=k.dtype, device=k.device, kv_heads=heads, head_dim=d, _step=step, _struct=struct,
+                   _at=ctypes.addressof(struct))
+
+    def __reduce__(self):
+        return PagedKV, (self.k, self.v)
 
     @classmethod
     def empty(cls, pages: int, page: int, kv_heads: int, head_dim: int, dtype: torch.dtype = torch.bfloat16,
@@ -102,7 +121,7 @@ def _int32(t: torch.Tensor, n: int, dev: torch.device, name: str) -> torch.Tenso
     return t if t.is_contiguous() else t.contiguous()
 
 
-class SequenceBatch:
+class SequenceBatch(_Held):
     """The new tokens of B sequences and the pages of all their keys (int32, on the device):
 
       table [B, pages]  page of key j of sequence b: table[b, j // page]
@@ -115,7 +134,7 @@ class SequenceBatch:
     near the truth is the better one.  A sequence that breaks a bound, or whose pages are not in the
     pool, has NaN for its outputs.  Sequences may share pages of keys that are not new (where two new
     tokens have one place, it holds either's).  The tensors are read when a call runs: a captured graph takes
-    what they hold at its replay."""
+    what they hold at its replay.  They are written in place, not exchanged: assigning an attribute is refused."""
 
     __slots__ = ("table", "lens", "starts", "max_len", "max_new", "device", "_struct", "_at")
 
@@ -131,11 +150,13 @@ class SequenceBatch:
         max_len, max_new = int(max_len), int(max_new)
         if not 0 <= max_len <= 2**30 or not 0 <= max_new <= 2**30:
             raise ValueError("max_len and max_new must be from 0 to 2^30")
-        self.table, self.lens, self.starts, self.max_len, self.max_new = table, lens, starts, max_len, max_new
-        self.device = table.device
-        self._struct = _Sequences(table.data_ptr(), table.stride(0) if B > 1 else max(pages, 1), pages, lens.data_ptr(),
-                                  starts.data_ptr(), B, max_len, max_new)
-        self._at = ctypes.addressof(self._struct)
+        struct = _Sequences(table.data_ptr(), table.stride(0) if B > 1 else max(pages, 1), pages, lens.data_ptr(),
+                            starts.data_ptr(), B, max_len, max_new)
+        self._hold(table=table, lens=lens, starts=starts, max_len=max_len, max_new=max_new, device=table.device,
+                   _struct=struct, _at=ctypes.addressof(struct))
+
+    def __reduce__(self):
+        return SequenceBatch, (self.table, self.lens, self.starts, self.max_len, self.max_new)
 
 
 def rotary_frequencies(dim: int, base: float = 10000.0, device="cuda") -> torch.Tensor:
