@@ -113,10 +113,10 @@ def _int32(t: torch.Tensor, n: int, dev: torch.device, name: str) -> torch.Tenso
     if t.numel() != n:
         raise ValueError(f"{name} must have {n} elements")
     if t.dtype is not torch.int32:
-        if t.is_floating_point() or t.is_complex() or t.dtype is torch.bool:
-            raise ValueError(f"{name} must be whole numbers")
-        if t.dtype is torch.int64:  # a limit past 32 bits is one past every key, and does not wrap
-            t = t.clamp(-(2**31), 2**31 - 1)
+        if t.is_floating_point() or t.is_complex() or t.dtype in (torch.bool, torch.uint64):
+            raise ValueError(f"{name} must be whole numbers of at most 64 bits with a sign")
+        if t.dtype in (torch.int64, torch.uint32):  # a limit past 32 bits is one past every key, and does not wrap
+            t = t.to(torch.int64).clamp(-(2**31), 2**31 - 1)
         t = t.to(torch.int32)
     return t if t.is_contiguous() else t.contiguous()
 
@@ -222,7 +222,7 @@ def norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv: Page
     freqs [pairs], float64: pair i of a head is turned by position * freqs[i]
     radians (None: none is); pairs are elements i and i + pairs of a head, or 2i and 2i + 1 where
     interleaved, the elements behind 2 * pairs stay.  positions [rows]: what the rotation takes
-    instead of the tokens' own positions.  q, k and v may be parts of one projection's rows; out may be q."""
+    instead of the tokens' own positions (of 32 bits; what they do not hold is the nearest that they do).  q, k and v may be parts of one projection's rows; out may be q."""
     dev = _same_device(kv, batch)
     d, KV = kv.head_dim, kv.kv_heads
     T, H, (q, q_at, q_row, q_head) = _queries(q, kv)
