@@ -412,12 +412,14 @@ struct Rows {
 // out, because the compiler waits for such a load of its own before the next LDS read, whatever either is
 // of; here the waits are the kernels'.  The load has no register of its own to be overwritten, and the
 // compiler's count of loads in flight, which misses it, only makes its waits longer.
+// (m0 is not among the clobbers: it is reserved, so the compiler would not heed that, and warned of it 4352 times a build.
+// Nothing else in these kernels uses m0.)
 __device__ __forceinline__ void load_lds(uint64_t p, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory");
 }
 __device__ __forceinline__ void load_lds(uint64_t base, uint32_t off, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base)
-                 : "memory", "m0");
+                 : "memory");
 }
 __device__ __forceinline__ uint32_t lds_address(const char* p) {
     return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
