@@ -464,8 +464,8 @@ int sgq_w8a8_plan(int gated, int64_t M, int64_t K, int64_t N, int compute_units,
  * sequence at full width.  Heads of queries share those of keys and values (heads a
  * multiple of kv_heads); types are SGQ_F32, SGQ_BF16, SGQ_F16, one for all of a call;
  * head_dim is a multiple of 16, at most 256.  At most 1024 heads, 2^23 rows, 2^30 heads
- * of rows, 2^20 sequences and (attention) 2^23 of sequences times kv_heads (SGQ_ERR_UNSUPPORTED
- * past them).
+ * of rows and 2^20 sequences (SGQ_ERR_UNSUPPORTED past them, and for attention where a call takes 2^24
+ * workgroups: with 2^24 sequences times kv_heads always, with fewer than 2^23 never).
  *
  * A cache is a pool of pages for one layer: key (or value) row t of page p and head h
  * at k (or v) + p * page_stride + t * token_stride + h * head_stride elements, head_dim

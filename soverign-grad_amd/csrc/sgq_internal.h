@@ -600,7 +600,7 @@ struct AttendShape {
     int64_t heads, kv_heads, head_dim, B, rows, max_len, max_new, window;
     DType t;
 };
-// few: a workgroup has all rows of a sequence and kv head (at most 32; lanes: fp32, at most eight), else `tiles`
+// few: a workgroup has all rows of a sequence and kv head (at most 32; lanes: fp32, at most four), else `tiles`
 // tiles of rows at most; splits: workgroups that share the keys of those, joined by a second kernel.
 struct AttendPlan {
     bool few, lanes;
