@@ -661,10 +661,12 @@ __device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)"
 // 32 NK keys in two buffers: while one is worked on, the next loads.  Two workgroups share a compute unit (64 KiB of LDS
 // each, up to 256 registers a lane), and while the one has the matrix cores the other has the vector unit: a wavefront's 64
 // keys of 128 in bf16 are 32 products of 32 cycles, 32 exponentials of 16 and some 180 vector instructions of 4, so that neither
-// unit can be busy all the time.  4 prompts of 8192 tokens, 64 on 8 heads of 128 in bf16: 4.22 to 4.46 ms, 986 to 1040 TFLOP/s, matrix
+// unit can be busy all the time.  4 prompts of 8192 tokens, 64 on 8 heads of 128 in bf16: 4.17 to 4.46 ms, 986 to 1055 TFLOP/s, matrix
 // cores 53% and vector unit 55% busy at 1.9 GHz (a large library product: 1094 TFLOP/s); without the loads 3.8.  A prompt of 2048, 32 heads: 52 us,
 // the longest tile's 32 steps one after another.  Measured and not kept: eight wavefronts, half of them a phase behind the other
 // half and barriers between products and softmax (4.8 ms against 4.4: barriers cost more than the units' overlap gave).
+// Heads of 256 leave too few registers: 22 spilled in 16 bits (64 bytes of scratch a lane), 35 (140) in fp32, some in the loop; two wavefronts
+// a row's columns, or queries in LDS, would mend that.
 template <typename T, int DP, int NW, int NK, bool CLEAN>
 __device__ __forceinline__ uint64_t tile_pass(Rows<T, DP, NK>& w, Loader<T, DP, 32 * NK, 64 * NW>& ld, const Score& sc, char* lds,
                                               int k0, int k1) {
@@ -787,6 +789,8 @@ __global__ __launch_bounds__(64 * NW, DP * sizeof(T) <= 512 ? 2 : 1) void k_atte
 // Up to 32 rows of a sequence and kv head (single tokens and a few more): the NW wavefronts of a workgroup
 // have tiles of 32 keys of their own, in two buffers each, and are joined at the end.  The cache's bytes bound it: 64 sequences of up
 // to 8192 keys, 32 on 8 heads of 128 in bf16, 1.05 GB in 218 us, 4.8 TB/s; one of 131072 537 MB in 109 us with its join, 4.9.
+// In fp32 the products are made for 32 rows and take longer than the bytes (64 on 8 heads over 8192 keys 38 us, 1.8 TB/s), most at a head size
+// of 256, where one wavefront fits a compute unit and 36 registers are spilled (113 us, 1.2 TB/s).
 template <typename T, int DP, int NW, bool CLEAN>
 __device__ __forceinline__ uint64_t few_pass(Rows<T, DP, 1>& w, Loader<T, DP, 32, 64>& ld, const Score& sc, char* lds, int k0,
                                              int k1) {
