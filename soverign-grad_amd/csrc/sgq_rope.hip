@@ -117,9 +117,12 @@ __global__ __launch_bounds__(kBlock) void k_norm_rope_append(const RopeArgs a, c
         } else if (on && !is_v) {
             if constexpr (P == Pairs::neighbours) {
                 auto two = [&](int e, float p, float q, T& yp, T& yq) {
-                    float2 w = make_float2(1.0f, 0.0f);
-                    if (e < 2 * a.half) w = turn[e / 2];
-                    yp = (T)(p * w.x - q * w.y), yq = (T)(q * w.x + p * w.y);
+                    if (e < 2 * a.half) {  // (else not by an angle of 0: 0 times what is not finite is a NaN)
+                        const float2 w = turn[e / 2];
+                        const float tp = p * w.x - q * w.y, tq = q * w.x + p * w.y;
+                        p = tp, q = tq;
+                    }
+                    yp = (T)p, yq = (T)q;
                 };
 #pragma unroll
                 for (int i = 0; i < N; i += 2) {
@@ -130,9 +133,12 @@ __global__ __launch_bounds__(kBlock) void k_norm_rope_append(const RopeArgs a, c
             } else {
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    float2 w = make_float2(1.0f, 0.0f);
-                    if (t < hc) w = turn[e0 + i];
-                    y0[i] = (T)(u0[i] * w.x - u1[i] * w.y), y1[i] = (T)(u1[i] * w.x + u0[i] * w.y);
+                    float p = u0[i], q = u1[i];
+                    if (t < hc) {
+                        const float2 w = turn[e0 + i];
+                        p = u0[i] * w.x - u1[i] * w.y, q = u1[i] * w.x + u0[i] * w.y;
+                    }
+                    y0[i] = (T)p, y1[i] = (T)q;
                 }
             }
         }
