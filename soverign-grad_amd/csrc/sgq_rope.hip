@@ -84,16 +84,27 @@ __global__ __launch_bounds__(kBlock) void k_norm_rope_append(const RopeArgs a, c
         for (int i = 0; i < N; ++i) u0[i] = (float)x0[i], u1[i] = (float)x1[i];
         const float* g = is_q ? a.q_norm : a.k_norm;
         if (a.q_norm || a.k_norm) {  // the sum by all lanes
-            float ss = 0.0f;
+            auto squares = [&](float unit) {  // of the elements times unit
+                float ss = 0.0f;
 #pragma unroll
-            for (int i = 0; i < N; ++i) ss = fmaf(u0[i], u0[i], ss);
+                for (int i = 0; i < N; ++i) ss = fmaf(u0[i] * unit, u0[i] * unit, ss);
 #pragma unroll
-            for (int i = 0; i < N; ++i) ss = fmaf(u1[i], u1[i], ss);
-            for (int o = 1 << lanes_log >> 1; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+                for (int i = 0; i < N; ++i) ss = fmaf(u1[i] * unit, u1[i] * unit, ss);
+                for (int o = 1 << lanes_log >> 1; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+                return ss;
+            };
+            float ss = squares(1.0f), unit = 1.0f;
+            // Heads whose squares fp32 does not hold have those of 2^-72 or (where eps does not outweigh them) 2^72 times
+            // their elements taken; where one of a wavefront does, all of it comes along.
+            const bool large = ss == INFINITY, small = ss < 0x1p-90f && a.eps < 0x1p-100f;
+            if (__builtin_expect(__any(large || small), 0)) {
+                const float far = large ? 0x1p-72f : 0x1p72f, ss2 = squares(far);
+                if (large || small) ss = ss2, unit = far;
+            }
             if (on && g && !is_v) {
-                const float rstd = 1.0f / sqrtf(ss / (float)d + a.eps);
+                const float rstd = 1.0f / sqrtf(ss / (float)d + a.eps * unit * unit);
 #pragma unroll
-                for (int i = 0; i < N; ++i) u0[i] = u0[i] * rstd * g[e0 + i], u1[i] = u1[i] * rstd * g[e1 + i];
+                for (int i = 0; i < N; ++i) u0[i] = u0[i] * unit * rstd * g[e0 + i], u1[i] = u1[i] * unit * rstd * g[e1 + i];
             }
         }
         Vec y0 = x0, y1 = x1;  // values as they are
