@@ -38,6 +38,9 @@ namespace {
 
 constexpr float kLog2e = 1.44269504f;
 constexpr float kGrowth = 8.0f;  // a running maximum is raised where a score's weight passes 2^kGrowth
+// How much lower (in powers of two) the weights of a row are held where a sum came out not finite: those of 2^30 keys sum to a
+// quarter then, so that no sum of values passes what the largest of them is.
+constexpr float kLower = 32.0f;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -157,6 +160,7 @@ struct Rows {
     float m, l;            // maximum of the scores (as c multiplies them), this half's sum of weights
     int lo, hi, pos;       // the row's keys and position
     float slope;           // times log2 e
+    float lower = 0.0f;    // weights are 2^-lower times what kLift makes them: 0 or kLower
     int max_lo, min_hi, min_lo, max_hi;  // over the wavefront's rows
 
     __device__ __forceinline__ void clear() {
@@ -185,6 +189,8 @@ struct Rows {
     __device__ __forceinline__ bool part(int k0) const { return k0 < max_lo || k0 + 32 * NK > min_hi; }
 
     // Scores of the keys from k0 on to weights, the sum and, where the maximum grows, the factor of what was summed.
+    // LOWER: lower may be other than 0.
+    template <bool LOWER>
     __device__ __forceinline__ void softmax(int k0, const Score& sc) {
         const int h = (threadIdx.x & 63) >> 5;
         // Key of register e of tile t: k0 + 32 t + 8 (e / 4) + 4 h + e % 4.
@@ -247,14 +253,15 @@ struct Rows {
         // exp2(s c - m c) with m c rounded has one instruction for the exponent.  What is lost of m c, 2^-24 of it, is the same
         // for all keys under one maximum, but from 2^28 on it takes weights past the type's range: scores past 2^12 have
         // the maximum taken off first.
-        float base = m == -INFINITY ? 0.0f : fmaf(-m, c, kLift);
+        const float lift = LOWER ? kLift - lower : kLift;
+        float base = m == -INFINITY ? 0.0f : fmaf(-m, c, lift);
         if (__builtin_expect(__any(fabsf(base) > 4096.0f), 0)) {
             const float off = m == -INFINITY ? 0.0f : m;
 #pragma unroll
             for (int t = 0; t < NK; ++t)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[t][e] -= off;
-            base = kLift;
+            base = lift;
         }
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -352,6 +359,12 @@ struct Rows {
 #pragma unroll
             for (int e = 0; e < 16; ++e) z[e & 3] = fmaf(o[i][e], 0.0f, z[e & 3]);
         return (z[0] + z[1]) + (z[2] + z[3]) != 0.0f && sum == sum;
+    }
+    // For another pass: the rows that were not finite have their weights lower (fp16's values cannot pass fp32).
+    __device__ __forceinline__ void again(bool bad) {
+        // A row's columns are in two lanes.
+        if (!std::is_same_v<T, _Float16>) lower = other_half(bad ? 1.0f : 0.0f, true) != 0.0f ? kLower : 0.0f;
+        clear();
     }
     // Values v of a key that are not finite, to the rows that see it.
     __device__ __forceinline__ void add_not_finite(const T* v, int key, int d) {
@@ -503,8 +516,8 @@ struct Loader {
 };
 
 // A weight of 0 times an infinity or a NaN is a NaN: values that are not finite touch rows that do not see them, and an
-// infinity that a row sees with a weight below fp32's range (exactly, it is positive) becomes a NaN.  Where a row's
-// result is not finite, the wavefront (workgroup) goes over its keys again with such values taken out of the tiles
+// infinity that a row sees with a weight below fp32's range (exactly, it is positive) becomes a NaN.  A sum of finite values may
+// also pass fp32 where their mean does not.  Where a row's result is not finite, the wavefront (workgroup) goes over its keys again with such values taken out of the tiles
 // (clean_values), and adds them, as they are, to the rows that see them at the end (add_values, of the tiles that had some: bit i of
 // `found` is for tiles i, i + 64, ..).  THREADS threads, all of which come along.
 template <typename T, int BYTES, int THREADS>
@@ -588,7 +601,7 @@ __device__ __forceinline__ void finish(const Rows<T, DP, NK>& w, const AttendArg
         w.store(out, d, l == 0.0f ? 0.0f : 1.0f / l);
     } else {
         const int64_t r = ((int64_t)row * a.heads + head) * parts.splits + split;
-        if (on && (threadIdx.x & 63) < 32) parts.ml[r] = make_float2(w.m * c, l);
+        if (on && (threadIdx.x & 63) < 32) parts.ml[r] = make_float2(w.m * c + w.lower, l);
         w.store_f32(on && l != 0.0f ? parts.o + r * d : nullptr, d, 1.0f);
     }
 }
@@ -607,6 +620,9 @@ __device__ __forceinline__ void poison(const AttendArgs& a, const Parts& parts, 
     }
 }
 
+// Joined parts have 2^-kRoom times their factors, for 2^kRoom parts at most: their sum passes what one holds no sooner.
+constexpr float kRoom = 2.0f, kSplitRoom = 8.0f;
+
 // Four columns (the i-th such) of the rows that the wavefronts of a workgroup have parts of: their maxima (exponents of
 // 2), sums and columns, joined and left as finish() does.
 template <typename T, int NW, typename M, typename L, typename C>
@@ -615,7 +631,8 @@ __device__ __forceinline__ void join_waves(const AttendArgs& a, const Parts& par
     const int quads = d / 4, q = i / quads, col = 4 * (i % quads);
     float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-    for (int v = 0; v < NW; ++v) top = fmaxf(top, max_of(v, q));
+    for (int v = 0; v < NW; ++v) top = fmaxf(top, max_of(v, q) + kRoom);
+    static_assert(NW <= 1 << (int)kRoom, "");
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int v = 0; v < NW; ++v) {
@@ -698,7 +715,7 @@ __device__ __forceinline__ uint64_t tile_pass(Rows<T, DP, NK>& w, Loader<T, DP, 
                 if (i * NG / L::kLoads == g) ld.load(next, next + B, k + kKeys, k1, p, i);
         });
         p = ld.pages(k + 2 * kKeys, k1);
-        w.softmax(k, sc);
+        w.template softmax<CLEAN>(k, sc);
         w.values(cur + B);
         loads_done();
         phase_end();
@@ -776,7 +793,7 @@ __global__ __launch_bounds__(64 * NW, DP * sizeof(T) <= 512 ? 2 : 1) void k_atte
     if (k0 < k1) tile_pass<T, DP, NW, NK, false>(w, ld, sc, lds, k0, k1);
     const bool bad = __syncthreads_or(ld.bad());
     if (!bad && __builtin_expect(__syncthreads_or(k0 < k1 && on && w.not_finite(other_half(w.l, false))), 0)) {
-        w.clear();
+        w.again(w.not_finite(other_half(w.l, false)));
         const uint64_t found = tile_pass<T, DP, NW, NK, true>(w, ld, sc, lds, k0, k1);
         add_values(w, c, ld.table, kvh, k0, k1, 32 * NK, found);
     }
@@ -797,7 +814,6 @@ __device__ __forceinline__ uint64_t few_pass(Rows<T, DP, 1>& w, Loader<T, DP, 32
     typedef Loader<T, DP, 32, 64> L;
     constexpr int B = L::kBytes, kStep = 32 * NW;
     const uint32_t at = __builtin_amdgcn_readfirstlane(lds_address(lds));  // keys, values; keys, values
-    w.clear();
     if (k0 >= k1) return 0;
     uint64_t found = 0;
     typename L::Pages p = ld.pages(k0, k1);
@@ -816,7 +832,7 @@ __device__ __forceinline__ uint64_t few_pass(Rows<T, DP, 1>& w, Loader<T, DP, 32
         if constexpr (CLEAN)
             if (__any(clean_values<T, B, 64>(cur + B, threadIdx.x & 63))) found |= 1ull << ((k - k0) / kStep & 63);
         w.scores(cur, [](int) {});
-        w.softmax(k, sc);
+        w.template softmax<CLEAN>(k, sc);
         w.values(cur + B);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
@@ -854,9 +870,11 @@ __global__ __launch_bounds__(64 * NW) void k_attend_few(const AttendArgs a, cons
     int k0, k1;
     L ld(c, s.table + b * s.table_ld, kvh, lane);
     split_range(ld.begin(w.min_lo), w.max_hi, split, parts.splits, 32 * NW, k0, k1);
+    w.clear();
     few_pass<T, DP, NW, false>(w, ld, sc, lds[wave], k0 + 32 * wave, k1);
     float l = other_half(w.l, false);
     if (__builtin_expect(__any(on && w.not_finite(l)), 0)) {
+        w.again(w.not_finite(l));
         const uint64_t found = few_pass<T, DP, NW, true>(w, ld, sc, lds[wave], k0 + 32 * wave, k1);
         l = other_half(w.l, false);
         add_values(w, c, ld.table, kvh, k0 + 32 * wave, k1, 32 * NW, found);
@@ -866,7 +884,7 @@ __global__ __launch_bounds__(64 * NW) void k_attend_few(const AttendArgs a, cons
     if constexpr (NW == 1) {
         finish(w, a, parts, unit, split, d, row, head, on, bad);
     } else {
-        if (lane < 32) ml[0][wave][lane] = w.m * unit, ml[1][wave][lane] = l;
+        if (lane < 32) ml[0][wave][lane] = w.m * unit + w.lower, ml[1][wave][lane] = l;
         if (lane == 0) wrong[wave] = bad;
         float* mine = (float*)lds[wave];
         w.store_f32(on ? mine + (lane & 31) * DP : nullptr, d, 1.0f);
@@ -951,7 +969,9 @@ __global__ __launch_bounds__(64 * NW) void k_attend_lanes(const AttendArgs a, co
             vx[u] = __builtin_nontemporal_load((const Vec*)(vp + off));
         }
     };
-    float extra[R][NV];  // what is not finite among the values seen
+    float extra[R][NV], lower[R];  // of a second pass: what is not finite among the values seen, how much lower the weights are
+#pragma unroll
+    for (int i = 0; i < R; ++i) lower[i] = 0.0f;
     auto take = [&](auto clean, int k, Vec (&kx)[U], Vec (&vx)[U]) {
         if (narrow && !on)
 #pragma unroll
@@ -982,7 +1002,7 @@ __global__ __launch_bounds__(64 * NW) void k_attend_lanes(const AttendArgs a, co
 #pragma unroll
                 for (int e = 0; e < NV; ++e) o[i][e] *= w;
             }
-            const float p = __builtin_amdgcn_exp2f(v - (m[i] == -INFINITY ? 0.0f : m[i]) - kGrowth);  // 1 at most
+            const float p = __builtin_amdgcn_exp2f(v - (m[i] == -INFINITY ? 0.0f : m[i]) - (clean() ? kGrowth + lower[i] : kGrowth));  // 1 at most
             l[i] += p;  // each key's in the lanes that have it
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -1016,14 +1036,18 @@ __global__ __launch_bounds__(64 * NW) void k_attend_lanes(const AttendArgs a, co
         }
     }
     // A weight below fp32's range is 0 and makes a NaN of an infinity: again without them, and they as they are at the end.
-    bool not_finite = false;
+    bool wrong_row[R], not_finite = false;
 #pragma unroll
-    for (int i = 0; i < R; ++i)
+    for (int i = 0; i < R; ++i) {
+        bool bad = false;
 #pragma unroll
-        for (int e = 0; e < NV; ++e) not_finite = not_finite || !isfinite(o[i][e]);
-    if (__builtin_expect(__any(not_finite), 0)) {
+        for (int e = 0; e < NV; ++e) bad = bad || !isfinite(o[i][e]);
+        wrong_row[i] = __any(bad), not_finite = not_finite || wrong_row[i];
+    }
+    if (__builtin_expect(not_finite, 0)) {
 #pragma unroll
         for (int i = 0; i < R; ++i) {
+            lower[i] = wrong_row[i] ? kLower : 0.0f;
             m[i] = -INFINITY, l[i] = 0.0f;
 #pragma unroll
             for (int e = 0; e < NV; ++e) o[i][e] = extra[i][e] = 0.0f;
@@ -1045,7 +1069,7 @@ __global__ __launch_bounds__(64 * NW) void k_attend_lanes(const AttendArgs a, co
 #pragma unroll
         for (int t = 32; t > 0; t >>= 1) l[i] += __shfl_xor(l[i], t, 64);
         l[i] *= 0.125f;
-        if (lane == 0) ml[0][wave][i] = m[i], ml[1][wave][i] = l[i];
+        if (lane == 0) ml[0][wave][i] = m[i] + lower[i], ml[1][wave][i] = l[i];
         Vec x;
 #pragma unroll
         for (int e = 0; e < NV; ++e) x[e] = o[i][e];
@@ -1091,7 +1115,8 @@ __global__ __launch_bounds__(256) void k_attend_join(const AttendArgs a, int d, 
         __syncthreads();
         top = fmaxf(fmaxf(part[0][0], part[0][1]), fmaxf(part[0][2], part[0][3]));
     }
-    const float f = v.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(v.x - (top == -INFINITY ? 0.0f : top));
+    static_assert(kSplits <= 1 << (int)kSplitRoom, "");
+    const float f = v.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(v.x - (top == -INFINITY ? 0.0f : top) - kSplitRoom);
     float sum = v.y == 0.0f ? 0.0f : v.y * f;
     // Columns have been written where something was seen; beside a sum of NaN they may not have been, and need not.
     if (t < kSplits) factor[own][t] = v.y != 0.0f && v.y == v.y ? f : -1.0f;

@@ -147,3 +147,36 @@ def test_scores_of_many_digits(op, dev, seq, dtype, bias):
     how = dict(alibi_slopes=torch.full((2,), 0.5, device=dev)) if bias else {}
     y = op.paged_attention(q, b.kv, b.batch, **how)
     assert torch.equal(y, b.values[0][top].expand_as(y))
+
+
+@pytest.mark.parametrize("dtype", TYPES[:2])
+@pytest.mark.parametrize("seq", SEQS + [(1, 131072), (6, 131072)])
+@pytest.mark.parametrize("bias", [False, True])
+def test_means_of_the_largest_values(op, dev, seq, dtype, bias):
+    """Values of 2^127 and more, whose mean fp32 holds and whose sum it does not; beside them columns of ordinary ones."""
+    new, n = seq
+    b = Batch(op, dev, [seq], 16, 1, 64, dtype)
+    v = b.values[0]
+    big = torch.arange(64, device=dev) % 3 != 1
+    v.copy_(torch.where(big, ((1 + v.float().abs().clamp(max=1) / 2) * 2.0**127) * v[0].float().sign(), v.float()))
+    _put(b)
+    q = (_randn(dev, 3, new, 2, 64) / 4).to(dtype)
+    how = dict(alibi_slopes=torch.full((2,), 0.003, device=dev)) if bias else {}
+    y = op.paged_attention(q, b.kv, b.batch, **how)
+    assert bool(torch.isfinite(y).all())
+    _check(y, _reference(b, q, **how), b, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES[:2])
+@pytest.mark.parametrize("new", [1, 6, 40])
+def test_large_values_of_one_part_of_the_keys(op, dev, dtype, new):
+    """Only one workgroup's keys have sums past fp32, and the others' are joined to them."""
+    n = 131072
+    b = Batch(op, dev, [(new, n)], 16, 1, 64, dtype)
+    b.values[0][40000:44000] = 2.0**127
+    b.values[0][40000:44000, :, 3] = 1
+    _put(b)
+    q = (_randn(dev, 3, new, 2, 64) / 4).to(dtype)
+    y = op.paged_attention(q, b.kv, b.batch)
+    assert bool(torch.isfinite(y).all())
+    _check(y, _reference(b, q), b, dtype)
