@@ -110,6 +110,15 @@ __device__ __forceinline__ void row_keys(const AttendArgs& a, const SeqRows& r, 
     if (a.prefix) hi = max(hi, min(a.prefix[b], r.len));
 }
 
+// A row's column as T: its sum over that of the weights (inv: one over it).  A mean is no larger than the largest of the values,
+// but rounded weights, and sums, may take it past the type's range by their last steps.
+template <typename T>
+__device__ __forceinline__ T mean(float sum, float inv) {
+    constexpr float top = std::is_same_v<T, _Float16> ? 65504.0f : std::is_same_v<T, __bf16> ? 0x1.FEp127f : 0x1.FFFFFEp127f;
+    const float x = sum * inv;
+    return (T)(isfinite(sum) && inv == inv ? __builtin_amdgcn_fmed3f(x, -top, top) : x);
+}
+
 __device__ __forceinline__ float other_half(float v, bool take_max) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     const float x = __uint_as_float(r[0]), y = __uint_as_float(r[1]);
@@ -386,7 +395,7 @@ struct Rows {
     __device__ __forceinline__ void store(T* out, int d, float w) const {
         const int h = (threadIdx.x & 63) >> 5;
         if constexpr (sizeof(T) == 4) {
-            store_f32(out, d, w);
+            store_f32(out, d, [&](float x) { return mean<float>(x, w); });
         } else {
 #pragma unroll
             for (int i = 0; i < kCols; ++i)
@@ -397,7 +406,7 @@ struct Rows {
                     typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
                     T4 a, b;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) a[j] = (T)(o[i][e + j] * w), b[j] = (T)(o[i][e + 4 + j] * w);
+                    for (int j = 0; j < 4; ++j) a[j] = mean<T>(o[i][e + j], w), b[j] = mean<T>(o[i][e + 4 + j], w);
                     const u32x2 ua = __builtin_bit_cast(u32x2, a), ub = __builtin_bit_cast(u32x2, b);
                     // Columns 0-3 | 4-7 and 8-11 | 12-15 of the halves: the lower lane takes 0-7, the upper 8-15.
                     const auto x = __builtin_amdgcn_permlane32_swap(ua[0], ub[0], false, false);
@@ -407,8 +416,9 @@ struct Rows {
                 }
         }
     }
-    // As fp32 (out null: no store, but all lanes come along).
-    __device__ __forceinline__ void store_f32(float* out, int d, float w) const {
+    // As fp32, by what(column) (out null: no store, but all lanes come along).
+    template <typename F>
+    __device__ __forceinline__ void store_f32(float* out, int d, F what) const {
         const int h = (threadIdx.x & 63) >> 5;
 #pragma unroll
         for (int i = 0; i < kCols; ++i)
@@ -416,7 +426,7 @@ struct Rows {
             for (int e = 0; e < 16; e += 4) {
                 const int col = 32 * i + 2 * e + 4 * h;
                 if (out && col < d)
-                    *(f32x4*)(out + col) = f32x4{o[i][e] * w, o[i][e + 1] * w, o[i][e + 2] * w, o[i][e + 3] * w};
+                    *(f32x4*)(out + col) = f32x4{what(o[i][e]), what(o[i][e + 1]), what(o[i][e + 2]), what(o[i][e + 3])};
             }
     }
 };
@@ -602,7 +612,7 @@ __device__ __forceinline__ void finish(const Rows<T, DP, NK>& w, const AttendArg
     } else {
         const int64_t r = ((int64_t)row * a.heads + head) * parts.splits + split;
         if (on && (threadIdx.x & 63) < 32) parts.ml[r] = make_float2(w.m * c + w.lower, l);
-        w.store_f32(on && l != 0.0f ? parts.o + r * d : nullptr, d, 1.0f);
+        w.store_f32(on && l != 0.0f ? parts.o + r * d : nullptr, d, [](float x) { return x; });
     }
 }
 
@@ -652,7 +662,7 @@ __device__ __forceinline__ void join_waves(const AttendArgs& a, const Parts& par
         typedef T T4 __attribute__((ext_vector_type(4)));
         T4 y;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = (T)(o[e] * inv);
+        for (int e = 0; e < 4; ++e) y[e] = mean<T>(o[e], inv);
         *(T4*)((T*)a.out.p + (int64_t)row * a.out.row + (int64_t)head * a.out.head + col) = y;
     } else {
         const int64_t at = ((int64_t)row * a.heads + head) * parts.splits + split;
@@ -887,7 +897,7 @@ __global__ __launch_bounds__(64 * NW) void k_attend_few(const AttendArgs a, cons
         if (lane < 32) ml[0][wave][lane] = w.m * unit + w.lower, ml[1][wave][lane] = l;
         if (lane == 0) wrong[wave] = bad;
         float* mine = (float*)lds[wave];
-        w.store_f32(on ? mine + (lane & 31) * DP : nullptr, d, 1.0f);
+        w.store_f32(on ? mine + (lane & 31) * DP : nullptr, d, [](float x) { return x; });
         __syncthreads();
         bool any_bad = false;
 #pragma unroll
@@ -1156,7 +1166,7 @@ __global__ __launch_bounds__(256) void k_attend_join(const AttendArgs a, int d, 
     typedef T T4 __attribute__((ext_vector_type(4)));
     T4 y;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = (T)(o[e] * inv);
+    for (int e = 0; e < 4; ++e) y[e] = mean<T>(o[e], inv);
     *(T4*)((T*)a.out.p + (int64_t)row * a.out.row + (int64_t)head * a.out.head + col) = y;
 }
 

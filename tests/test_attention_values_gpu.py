@@ -180,3 +180,25 @@ def test_large_values_of_one_part_of_the_keys(op, dev, dtype, new):
     y = op.paged_attention(q, b.kv, b.batch)
     assert bool(torch.isfinite(y).all())
     _check(y, _reference(b, q), b, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("new, n", [(1, 3), (3, 5), (1, 2000), (7, 60), (60, 64), (300, 900)])
+@pytest.mark.parametrize("alike", [False, True])
+def test_a_mean_of_the_largest_value_is_no_infinity(op, dev, dtype, new, n, alike):
+    """Columns of one value, the type's largest of either sign: rounded weights may sum to more than their sum, by half a step,
+    and what comes out is that value or less by as much (and the sums' roundings).  alike: all keys but the first are, so that
+    their weights are rounded the same way."""
+    b = Batch(op, dev, [(new, n)] * 4, 16, 1, 64, dtype)
+    top = torch.finfo(dtype).max
+    for i in range(4):
+        b.values[i][..., ::2], b.values[i][..., 1::2] = top, -top
+        if alike:
+            b.keys[i][:], b.keys[i][0] = 0.125, 0.25
+        _put(b, i)
+    q = _randn(dev, 3, b.rows, 8, 64).abs().to(dtype)
+    y = op.paged_attention(q, b.kv, b.batch)
+    assert bool(torch.isfinite(y).all()), int((~torch.isfinite(y)).sum())
+    sign = 1.0 - 2.0 * (torch.arange(64, device=dev) % 2)
+    low = top * (1 - 2 * torch.finfo(dtype).eps - (n + 16) * 2.0**-24)
+    assert float((y.double() * sign).min()) >= low
