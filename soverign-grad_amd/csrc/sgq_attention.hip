@@ -369,27 +369,56 @@ struct Rows {
             for (int e = 0; e < 16; ++e) z[e & 3] = fmaf(o[i][e], 0.0f, z[e & 3]);
         return (z[0] + z[1]) + (z[2] + z[3]) != 0.0f && sum == sum;
     }
-    // For another pass: the rows that were not finite have their weights lower (fp16's values cannot pass fp32).
-    __device__ __forceinline__ void again(bool bad) {
+    // For another pass: rows that were not finite have their weights lower (fp16's values cannot pass fp32).
+    __device__ __forceinline__ void set_lower(bool bad) {
         // A row's columns are in two lanes.
         if (!std::is_same_v<T, _Float16>) lower = other_half(bad ? 1.0f : 0.0f, true) != 0.0f ? kLower : 0.0f;
-        clear();
     }
-    // Values v of a key that are not finite, to the rows that see it.
-    __device__ __forceinline__ void add_not_finite(const T* v, int key, int d) {
-        const int h = (threadIdx.x & 63) >> 5;
-        const bool sees = key >= lo && key < hi;
+    // Which of the row's columns see an infinity of either sign or a NaN among the values, a bit each; of a lane in
+    // LDS, words `step` apart (in registers they would cost every launch some).
+    static constexpr int kWords = (16 * kCols + 31) / 32;
+    struct Marks {
+        uint32_t* at;
+        int step;
+        __device__ __forceinline__ uint32_t& operator()(int kind, int word) const { return at[(kind * kWords + word) * step]; }
+    };
+    static constexpr int kMarks = 3 * kWords;  // of a lane
+    // Those of the tile of codes (code_values) at vs, whose keys are from k0 on, among the others.  The columns and the weights are lost.
+    __device__ __forceinline__ void mark(const char* vs, int k0, const Marks& marks) {
+        const int kb = k0 + 4 * ((threadIdx.x & 63) >> 5);
+        const unsigned width = (unsigned)max(hi - lo, 0);
 #pragma unroll
-        for (int i = 0; i < kCols; ++i)
+        for (int t = 0; t < NK; ++t)
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                typedef T T4 __attribute__((ext_vector_type(4)));
-                const int col = 32 * i + 2 * e + 4 * h;
-                const T4 x = *(const T4*)(v + min(col, d - 4));
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (sees && col < d && !isfinite((float)x[j])) o[i][e + j] += (float)x[j];
+            for (int e = 0; e < 16; ++e) {
+                const float sees = (unsigned)(kb + 32 * t + 8 * (e / 4) + e % 4 - lo) < width ? 1.0f : 0.0f;
+                if constexpr (sizeof(T) == 4)
+                    p[t][e] = sees;
+                else
+                    p[2 * t + e / 8][e % 8] = (T)sees;
             }
+        clear();
+        values(vs);
+#pragma unroll
+        for (int word = 0; word < kWords; ++word) {
+            uint32_t plus = 0, minus = 0, nan = 0;
+#pragma unroll
+            for (int b = 0; b < 32 && 32 * word + b < 16 * kCols; ++b) {
+                const int sum = (int)o[2 * word + b / 16][b % 16];  // how many of each, 64 at most, as digits
+                plus |= (sum & 0x7f ? 1u : 0u) << b, minus |= (sum & 0x3f80 ? 1u : 0u) << b, nan |= (sum >> 14 ? 1u : 0u) << b;
+            }
+            marks(0, word) |= plus, marks(1, word) |= minus, marks(2, word) |= nan;
+        }
+    }
+    __device__ __forceinline__ void add(const Marks& marks) {
+#pragma unroll
+        for (int word = 0; word < kWords; ++word) {
+            const uint32_t plus = marks(0, word), minus = marks(1, word), nan = marks(2, word);
+#pragma unroll
+            for (int b = 0; b < 32 && 32 * word + b < 16 * kCols; ++b)
+                o[2 * word + b / 16][b % 16] += ((plus >> b & 1 ? INFINITY : 0.0f) + (minus >> b & 1 ? -INFINITY : 0.0f)) +
+                                                (nan >> b & 1 ? NAN : 0.0f);
+        }
     }
     // The row's columns times w, as T, 16 bytes a store.
     __device__ __forceinline__ void store(T* out, int d, float w) const {
@@ -525,54 +554,76 @@ struct Loader {
     static __device__ __forceinline__ void arrived(Pages& p) { asm volatile("" : "+v"(p.of)); }
 };
 
+// Ends a phase: nothing is scheduled across it.
+__device__ __forceinline__ void phase_end() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+__device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 // A weight of 0 times an infinity or a NaN is a NaN: values that are not finite touch rows that do not see them, and an
 // infinity that a row sees with a weight below fp32's range (exactly, it is positive) becomes a NaN.  A sum of finite values may
-// also pass fp32 where their mean does not.  Where a row's result is not finite, the wavefront (workgroup) goes over its keys again with such values taken out of the tiles
-// (clean_values), and adds them, as they are, to the rows that see them at the end (add_values, of the tiles that had some: bit i of
-// `found` is for tiles i, i + 64, ..).  THREADS threads, all of which come along.
+// also pass fp32 where their mean does not.  Where a row's result is not finite, the wavefront (workgroup) goes over its
+// keys twice more: which columns see what that is not finite (mark_pass: codes of the values times who sees whom, on the matrix
+// cores), then everything with such values taken out of the tiles (clean_values); what was marked is added at the end.  (Where all
+// values are NaN, 4 prompts of 8192 tokens take 18.7 ms, one token on 131072 keys 0.42; 305 and 3.7 where the marks were found key by
+// key.)  THREADS threads, all of which come along.
 template <typename T, int BYTES, int THREADS>
-__device__ __forceinline__ bool clean_values(char* tile, int thread) {
+__device__ __forceinline__ void clean_values(char* tile, int thread) {
+    typedef typename Chunk<T>::type Vec;
+    for (int i = thread * 16; i < BYTES; i += THREADS * 16) {
+        Vec v = *(const Vec*)(tile + i);
+#pragma unroll
+        for (int e = 0; e < Chunk<T>::N; ++e) v[e] = isfinite((float)v[e]) ? v[e] : (T)0.0f;
+        *(Vec*)(tile + i) = v;
+    }
+}
+// Values as codes: infinities 1 and 2^7, NaN 2^14, others 0, so that sums of 64 of them say how many there are of each.  Whether
+// there were any.
+template <typename T, int BYTES, int THREADS>
+__device__ __forceinline__ bool code_values(char* tile, int thread) {
     typedef typename Chunk<T>::type Vec;
     bool found = false;
     for (int i = thread * 16; i < BYTES; i += THREADS * 16) {
         Vec v = *(const Vec*)(tile + i);
 #pragma unroll
         for (int e = 0; e < Chunk<T>::N; ++e) {
-            const bool ok = isfinite((float)v[e]);
-            v[e] = ok ? v[e] : (T)0.0f;
-            found = found || !ok;
+            const float x = (float)v[e];
+            found = found || !isfinite(x);
+            v[e] = (T)(x == INFINITY ? 1.0f : x == -INFINITY ? 128.0f : x == x ? 0.0f : 16384.0f);
         }
         *(Vec*)(tile + i) = v;
     }
     return found;
 }
-template <typename T, int DP, int NK>
-__device__ __forceinline__ void add_values(Rows<T, DP, NK>& w, const PagedCache& c, const int32_t* table, int kvh, int k0, int k1,
-                                           int step, uint64_t found) {
-    constexpr int U = 8;  // keys whose loads are in flight together
-    const int lane = threadIdx.x & 63, d = c.head_dim;
-    int tile = 0;
-#pragma unroll 1
-    for (int k = k0; k < k1; k += step, ++tile) {
-        if (!(found >> (tile & 63) & 1)) continue;
-        const int end = min(k + 32 * NK, k1);
-#pragma unroll 1
-        for (int first = k; first < end; first += U) {
-            // (Of a page that is not in the pool the pool's first rows: the result is NaN anyway.)
-            auto values = [&](int key) {
-                return (const T*)c.v + max(key_offset(c, table, min(key, end - 1)), (int64_t)0) + (int64_t)kvh * c.head_stride;
-            };
-            unsigned bad = 0;
+template <typename T, int DP, int NK, int THREADS>
+__device__ __forceinline__ void mark_pass(Rows<T, DP, NK>& w, Loader<T, DP, 32 * NK, THREADS>& ld, char* lds, int k0, int k1,
+                                          int step, const typename Rows<T, DP, NK>::Marks& marks) {
+    static_assert(32 * NK <= 64, "a code's digits");
+    constexpr int B = Loader<T, DP, 32 * NK, THREADS>::kBytes;
+    constexpr bool kShared = THREADS > 64;  // the tile by a workgroup
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const T* v = values(first + u);
-#pragma unroll
-                for (int i = 0; i < kMaxHeadDim / 64; ++i) bad |= (unsigned)!isfinite((float)v[min(lane + 64 * i, d - 1)]) << u;
-            }
+    for (int i = 0; i < Rows<T, DP, NK>::kMarks; ++i) marks(0, i) = 0;
+    const uint32_t at = __builtin_amdgcn_readfirstlane(lds_address(lds));
+    int odd = 0;  // two buffers: a wavefront may still read the one
 #pragma unroll 1
-            for (int u = 0; u < U && first + u < end; ++u)
-                if (__any(bad >> u & 1)) w.add_not_finite(values(first + u), first + u, d);
+    for (int k = k0; k < k1; k += step, odd ^= 1) {
+        auto p = ld.pages(k, k1);
+        ld.load(at + odd * 2 * B, at + odd * 2 * B + B, k, k1, p);
+        loads_done();
+        if (kShared) phase_end();
+        char* const codes = lds + odd * 2 * B + B;
+        const bool found = code_values<T, B, THREADS>(codes, threadIdx.x & (THREADS - 1));
+        bool any;
+        if constexpr (kShared) {
+            any = __syncthreads_or(found);
+            phase_end();
+        } else {
+            any = __any(found);
         }
+        if (any) w.mark(codes, k, marks);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
 }
 
@@ -676,14 +727,6 @@ constexpr int kJoinSplits = 256, kWaveSplits = 16;
 
 // ---- tiles of rows ----------------------------------------------------------
 
-// Ends a phase: nothing is scheduled across it.
-__device__ __forceinline__ void phase_end() {
-    __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-}
-__device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-
 // A workgroup of NW wavefronts takes 32 NW rows of one sequence and kv head, which share tiles of
 // 32 NK keys in two buffers: while one is worked on, the next loads.  Two workgroups share a compute unit (64 KiB of LDS
 // each, up to 256 registers a lane), and while the one has the matrix cores the other has the vector unit: a wavefront's 64
@@ -692,11 +735,11 @@ __device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)"
 // cores 53% and vector unit 55% busy at 1.9 GHz (a large library product: 1094 TFLOP/s); without the loads 3.8.  A prompt of 2048, 32 heads: 52 us,
 // the longest tile's 32 steps one after another.  Measured and not kept: eight wavefronts, half of them a phase behind the other
 // half and barriers between products and softmax (4.8 ms against 4.4: barriers cost more than the units' overlap gave).
-// Heads of 256 leave too few registers: 22 spilled in 16 bits (64 bytes of scratch a lane), 35 (140) in fp32, some in the loop; two wavefronts
+// Heads of 256 leave too few registers: 22 to 23 spilled in 16 bits (60 bytes of scratch a lane), 35 (140) in fp32, some in the loop; two wavefronts
 // a row's columns, or queries in LDS, would mend that.
 template <typename T, int DP, int NW, int NK, bool CLEAN>
-__device__ __forceinline__ uint64_t tile_pass(Rows<T, DP, NK>& w, Loader<T, DP, 32 * NK, 64 * NW>& ld, const Score& sc, char* lds,
-                                              int k0, int k1) {
+__device__ __forceinline__ void tile_pass(Rows<T, DP, NK>& w, Loader<T, DP, 32 * NK, 64 * NW>& ld, const Score& sc, char* lds,
+                                          int k0, int k1) {
     typedef Loader<T, DP, 32 * NK, 64 * NW> L;
     constexpr int kKeys = 32 * NK, B = L::kBytes;
     const uint32_t at = __builtin_amdgcn_readfirstlane(lds_address(lds));  // keys, values; keys, values
@@ -706,12 +749,11 @@ __device__ __forceinline__ uint64_t tile_pass(Rows<T, DP, NK>& w, Loader<T, DP, 
     loads_done();
     phase_end();
     int odd = 0;
-    uint64_t found = 0;
 #pragma unroll 1
     for (int k = k0; k < k1; k += kKeys, odd ^= 1) {
         char* const cur = lds + odd * 2 * B;
         if constexpr (CLEAN) {
-            if (__syncthreads_or(clean_values<T, B, 64 * NW>(cur + B, threadIdx.x))) found |= 1ull << ((k - k0) / kKeys & 63);
+            clean_values<T, B, 64 * NW>(cur + B, threadIdx.x);
             phase_end();
         }
         const uint32_t next = at + (odd ^ 1) * 2 * B;
@@ -730,7 +772,6 @@ __device__ __forceinline__ uint64_t tile_pass(Rows<T, DP, NK>& w, Loader<T, DP, 
         loads_done();
         phase_end();
     }
-    return found;
 }
 
 template <typename T, int DP, int NW, int NK>
@@ -739,6 +780,7 @@ __global__ __launch_bounds__(64 * NW, DP * sizeof(T) <= 512 ? 2 : 1) void k_atte
     typedef Loader<T, DP, 32 * NK, 64 * NW> L;
     constexpr int kRows = kTileRows * NW;
     __shared__ __align__(16) char lds[4 * L::kBytes];
+    __shared__ uint32_t lds_marks[Rows<T, DP, NK>::kMarks * 64 * NW];
     __shared__ int range[2][NW];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = a.heads / c.kv_heads;
@@ -803,9 +845,13 @@ __global__ __launch_bounds__(64 * NW, DP * sizeof(T) <= 512 ? 2 : 1) void k_atte
     if (k0 < k1) tile_pass<T, DP, NW, NK, false>(w, ld, sc, lds, k0, k1);
     const bool bad = __syncthreads_or(ld.bad());
     if (!bad && __builtin_expect(__syncthreads_or(k0 < k1 && on && w.not_finite(other_half(w.l, false))), 0)) {
-        w.again(w.not_finite(other_half(w.l, false)));
-        const uint64_t found = tile_pass<T, DP, NW, NK, true>(w, ld, sc, lds, k0, k1);
-        add_values(w, c, ld.table, kvh, k0, k1, 32 * NK, found);
+        w.set_lower(w.not_finite(other_half(w.l, false)));
+        const typename Rows<T, DP, NK>::Marks marks = {lds_marks + threadIdx.x, 64 * NW};
+        mark_pass(w, ld, lds, k0, k1, 32 * NK, marks);
+        phase_end();
+        w.clear();
+        tile_pass<T, DP, NW, NK, true>(w, ld, sc, lds, k0, k1);
+        w.add(marks);
     }
     const float unit = sc.capped || sc.sloped ? 1.0f : sc.c;
     finish(w, a, parts, unit, split, c.head_dim, row, head, on, bad);
@@ -819,13 +865,12 @@ __global__ __launch_bounds__(64 * NW, DP * sizeof(T) <= 512 ? 2 : 1) void k_atte
 // In fp32 the products are made for 32 rows and take longer than the bytes (64 on 8 heads over 8192 keys 38 us, 1.8 TB/s), most at a head size
 // of 256, where one wavefront fits a compute unit and 36 registers are spilled (113 us, 1.2 TB/s).
 template <typename T, int DP, int NW, bool CLEAN>
-__device__ __forceinline__ uint64_t few_pass(Rows<T, DP, 1>& w, Loader<T, DP, 32, 64>& ld, const Score& sc, char* lds, int k0,
-                                             int k1) {
+__device__ __forceinline__ void few_pass(Rows<T, DP, 1>& w, Loader<T, DP, 32, 64>& ld, const Score& sc, char* lds, int k0,
+                                         int k1) {
     typedef Loader<T, DP, 32, 64> L;
     constexpr int B = L::kBytes, kStep = 32 * NW;
     const uint32_t at = __builtin_amdgcn_readfirstlane(lds_address(lds));  // keys, values; keys, values
-    if (k0 >= k1) return 0;
-    uint64_t found = 0;
+    if (k0 >= k1) return;
     typename L::Pages p = ld.pages(k0, k1);
     ld.load(at, at + B, k0, k1, p);
     p = ld.pages(k0 + kStep, k1);
@@ -839,14 +884,12 @@ __device__ __forceinline__ uint64_t few_pass(Rows<T, DP, 1>& w, Loader<T, DP, 32
         }
         p = ld.pages(k + 2 * kStep, k1);
         char* const cur = lds + odd * 2 * B;
-        if constexpr (CLEAN)
-            if (__any(clean_values<T, B, 64>(cur + B, threadIdx.x & 63))) found |= 1ull << ((k - k0) / kStep & 63);
+        if constexpr (CLEAN) clean_values<T, B, 64>(cur + B, threadIdx.x & 63);
         w.scores(cur, [](int) {});
         w.template softmax<CLEAN>(k, sc);
         w.values(cur + B);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
-    return found;
 }
 
 template <typename T, int DP, int NW>
@@ -855,6 +898,7 @@ __global__ __launch_bounds__(64 * NW) void k_attend_few(const AttendArgs a, cons
     typedef Loader<T, DP, 32, 64> L;
     static_assert(L::kBytes * 4 >= 32 * DP * 4, "a wavefront's buffers hold its result");
     __shared__ __align__(16) char lds[NW][4 * L::kBytes];
+    __shared__ uint32_t lds_marks[Rows<T, DP, 1>::kMarks * 64 * NW];
     __shared__ float ml[2][NW][32];
     __shared__ int wrong[NW];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -884,10 +928,13 @@ __global__ __launch_bounds__(64 * NW) void k_attend_few(const AttendArgs a, cons
     few_pass<T, DP, NW, false>(w, ld, sc, lds[wave], k0 + 32 * wave, k1);
     float l = other_half(w.l, false);
     if (__builtin_expect(__any(on && w.not_finite(l)), 0)) {
-        w.again(w.not_finite(l));
-        const uint64_t found = few_pass<T, DP, NW, true>(w, ld, sc, lds[wave], k0 + 32 * wave, k1);
+        w.set_lower(w.not_finite(l));
+        const typename Rows<T, DP, 1>::Marks marks = {lds_marks + threadIdx.x, 64 * NW};
+        mark_pass(w, ld, lds[wave], k0 + 32 * wave, k1, 32 * NW, marks);
+        w.clear();
+        few_pass<T, DP, NW, true>(w, ld, sc, lds[wave], k0 + 32 * wave, k1);
         l = other_half(w.l, false);
-        add_values(w, c, ld.table, kvh, k0 + 32 * wave, k1, 32 * NW, found);
+        w.add(marks);
     }
     const float unit = sc.capped || sc.sloped ? 1.0f : sc.c;
     const bool bad = __any(ld.bad());
