@@ -84,27 +84,29 @@ __global__ __launch_bounds__(kBlock) void k_norm_rope_append(const RopeArgs a, c
         for (int i = 0; i < N; ++i) u0[i] = (float)x0[i], u1[i] = (float)x1[i];
         const float* g = is_q ? a.q_norm : a.k_norm;
         if (a.q_norm || a.k_norm) {  // the sum by all lanes
-            auto squares = [&](float unit) {  // of the elements times unit
+            auto squares = [&] {
                 float ss = 0.0f;
 #pragma unroll
-                for (int i = 0; i < N; ++i) ss = fmaf(u0[i] * unit, u0[i] * unit, ss);
+                for (int i = 0; i < N; ++i) ss = fmaf(u0[i], u0[i], ss);
 #pragma unroll
-                for (int i = 0; i < N; ++i) ss = fmaf(u1[i] * unit, u1[i] * unit, ss);
+                for (int i = 0; i < N; ++i) ss = fmaf(u1[i], u1[i], ss);
                 for (int o = 1 << lanes_log >> 1; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
                 return ss;
             };
-            float ss = squares(1.0f), unit = 1.0f;
-            // Heads whose squares fp32 does not hold have those of 2^-72 or (where eps does not outweigh them) 2^72 times
-            // their elements taken; where one of a wavefront does, all of it comes along.
-            const bool large = ss == INFINITY, small = ss < 0x1p-90f && a.eps < 0x1p-100f;
-            if (__builtin_expect(__any(large || small), 0)) {
-                const float far = large ? 0x1p-72f : 0x1p72f, ss2 = squares(far);
-                if (large || small) ss = ss2, unit = far;
+            float ss = squares(), eps = a.eps;
+            // Heads whose squares fp32 does not hold are taken 2^-72 or (where eps does not outweigh them) 2^72 times, which the norm
+            // takes out again; where one of a wavefront is, all of it comes along.
+            if (__builtin_expect(__any(!(ss >= 0x1p-90f && ss < INFINITY)), 0)) {
+                const bool large = ss == INFINITY, far = (large || (ss < 0x1p-90f && a.eps < 0x1p-100f)) && g && !is_v;
+                const float unit = !far ? 1.0f : large ? 0x1p-72f : 0x1p72f;
+#pragma unroll
+                for (int i = 0; i < N; ++i) u0[i] *= unit, u1[i] *= unit;
+                ss = squares(), eps = eps * unit * unit;  // (unit * unit by itself would pass fp32)
             }
             if (on && g && !is_v) {
-                const float rstd = 1.0f / sqrtf(ss / (float)d + a.eps * unit * unit);
+                const float rstd = 1.0f / sqrtf(ss / (float)d + eps);
 #pragma unroll
-                for (int i = 0; i < N; ++i) u0[i] = u0[i] * unit * rstd * g[e0 + i], u1[i] = u1[i] * unit * rstd * g[e1 + i];
+                for (int i = 0; i < N; ++i) u0[i] = u0[i] * rstd * g[e0 + i], u1[i] = u1[i] * rstd * g[e1 + i];
             }
         }
         Vec y0 = x0, y1 = x1;  // values as they are
@@ -128,12 +130,9 @@ __global__ __launch_bounds__(kBlock) void k_norm_rope_append(const RopeArgs a, c
         } else if (on && !is_v) {
             if constexpr (P == Pairs::neighbours) {
                 auto two = [&](int e, float p, float q, T& yp, T& yq) {
-                    if (e < 2 * a.half) {  // (else not by an angle of 0: 0 times what is not finite is a NaN)
-                        const float2 w = turn[e / 2];
-                        const float tp = p * w.x - q * w.y, tq = q * w.x + p * w.y;
-                        p = tp, q = tq;
-                    }
-                    yp = (T)p, yq = (T)q;
+                    float2 w = make_float2(1.0f, 0.0f);
+                    if (e < 2 * a.half) w = turn[e / 2];
+                    yp = (T)(p * w.x - q * w.y), yq = (T)(q * w.x + p * w.y);
                 };
 #pragma unroll
                 for (int i = 0; i < N; i += 2) {
@@ -141,16 +140,24 @@ __global__ __launch_bounds__(kBlock) void k_norm_rope_append(const RopeArgs a, c
                     two(e0 + i, u0[i], u0[i + 1], p, q), y0[i] = p, y0[i + 1] = q;
                     two(e1 + i, u1[i], u1[i + 1], p, q), y1[i] = p, y1[i + 1] = q;
                 }
+                if (e1 + N > 2 * a.half)  // as below
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        if (e0 + i >= 2 * a.half) y0[i] = (T)u0[i];
+                        if (e1 + i >= 2 * a.half) y1[i] = (T)u1[i];
+                    }
             } else {
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    float p = u0[i], q = u1[i];
-                    if (t < hc) {
-                        const float2 w = turn[e0 + i];
-                        p = u0[i] * w.x - u1[i] * w.y, q = u1[i] * w.x + u0[i] * w.y;
-                    }
-                    y0[i] = (T)p, y1[i] = (T)q;
+                    float2 w = make_float2(1.0f, 0.0f);
+                    if (t < hc) w = turn[e0 + i];
+                    y0[i] = (T)(u0[i] * w.x - u1[i] * w.y), y1[i] = (T)(u1[i] * w.x + u0[i] * w.y);
                 }
+                // Not by an angle of 0: 0 times what is not finite is a NaN.  (A branch that wavefronts skip whose
+                // heads are turned whole; with one around the products 16384 tokens took 125.4 us instead of 124.9.)
+                if (t >= hc)
+#pragma unroll
+                    for (int i = 0; i < N; ++i) y0[i] = (T)u0[i], y1[i] = (T)u1[i];
             }
         }
         if (!on) continue;
