@@ -96,7 +96,7 @@ __global__ __launch_bounds__(kBlock) void k_norm_rope_append(const RopeArgs a, c
             float ss = squares(), eps = a.eps;
             // Heads whose squares fp32 does not hold are taken 2^-72 or (where eps does not outweigh them) 2^72 times, which the norm
             // takes out again; where one of a wavefront is, all of it comes along.
-            if (__builtin_expect(__any(!(ss >= 0x1p-90f && ss < INFINITY)), 0)) {
+            if (__builtin_expect(__any(h < h1 && !(ss >= 0x1p-90f && ss < INFINITY)), 0)) {
                 const bool large = ss == INFINITY, far = (large || (ss < 0x1p-90f && a.eps < 0x1p-100f)) && g && !is_v;
                 const float unit = !far ? 1.0f : large ? 0x1p-72f : 0x1p72f;
 #pragma unroll
