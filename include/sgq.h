@@ -542,8 +542,8 @@ typedef struct sgq_scores {
 /* out = sum_j exp(s_j - max s) v_j / sum_j exp(s_j - max s) over the keys that a row
  * sees; zeros for a row that sees none.  Sums and softmax in fp32.  What a row does not see does
  * not touch it, infinities and NaN included.  Of the values that it sees, a NaN makes that column of it NaN and an
- * infinity that infinity (of both signs a NaN), whatever their weights and however the keys are shared out.  q, out: [rows, heads, head_dim] as above
- * (out may be q itself).  workspace:
+ * infinity that infinity (of both signs a NaN), whatever their weights and however the keys are shared out.
+ * q, out: [rows, heads, head_dim] as above (out may be q itself; neither shares memory with the cache).  workspace:
  * sgq_paged_attention_workspace_bytes bytes for a device of `compute_units` CUs (0: the
  * calling thread's current device), 16-byte aligned, else SGQ_ERR_WORKSPACE; it needs
  * no initialisation, and calls that overlap in time must not share one. */

@@ -222,7 +222,8 @@ def norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv: Page
     freqs [pairs], float64: pair i of a head is turned by position * freqs[i]
     radians (None: none is); pairs are elements i and i + pairs of a head, or 2i and 2i + 1 where
     interleaved, the elements behind 2 * pairs stay.  positions [rows]: what the rotation takes
-    instead of the tokens' own positions (of 32 bits; what they do not hold is the nearest that they do).  q, k and v may be parts of one projection's rows; out may be q."""
+    instead of the tokens' own positions (of 32 bits; what they do not hold is the nearest that they do).
+    q, k and v may be parts of one projection's rows; out may be q; none shares memory with the cache."""
     dev = _same_device(kv, batch)
     d, KV = kv.head_dim, kv.kv_heads
     T, H, (q, q_at, q_row, q_head) = _queries(q, kv)
@@ -276,7 +277,7 @@ def paged_attention(q: torch.Tensor, kv: PagedKV, batch: SequenceBatch, scale: O
     keys j <= p and those below prefix[b] ([B]; also ahead of it), of them those with j > p - window
     (window > 0) and j >= first_key[row] ([rows], its document's first).  A row that sees
     none is zeros.  A value seen that is not finite makes its column so (NaN, or that infinity), whatever its
-    weight.  out may be q."""
+    weight.  out may be q, but shares no memory with the cache."""
     dev = _same_device(kv, batch)
     d = kv.head_dim
     T, H, (q, q_at, q_row, q_head) = _queries(q, kv)

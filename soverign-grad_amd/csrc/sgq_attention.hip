@@ -383,7 +383,8 @@ struct Rows {
         __device__ __forceinline__ uint32_t& operator()(int kind, int word) const { return at[(kind * kWords + word) * step]; }
     };
     static constexpr int kMarks = 3 * kWords;  // of a lane
-    // Those of the tile of codes (code_values) at vs, whose keys are from k0 on, among the others.  The columns and the weights are lost.
+    // Those of the tile of codes (code_values) at vs, whose keys are from k0 on, among the others.  The columns and the
+    // weights are lost.
     __device__ __forceinline__ void mark(const char* vs, int k0, const Marks& marks) {
         const int kb = k0 + 4 * ((threadIdx.x & 63) >> 5);
         const unsigned width = (unsigned)max(hi - lo, 0);
@@ -567,8 +568,8 @@ __device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)"
 // also pass fp32 where their mean does not.  Where a row's result is not finite, the wavefront (workgroup) goes over its
 // keys twice more: which columns see what that is not finite (mark_pass: codes of the values times who sees whom, on the matrix
 // cores), then everything with such values taken out of the tiles (clean_values); what was marked is added at the end.  (Where all
-// values are NaN, 4 prompts of 8192 tokens take 18.7 ms, one token on 131072 keys 0.42; 305 and 3.7 where the marks were found key by
-// key.)  THREADS threads, all of which come along.
+// values are NaN, 4 prompts of 8192 tokens take 18.6 ms, one token on 131072 keys 0.42; 305 and 3.7 where the marks were
+// found key by key.)  THREADS threads, all of which come along.
 template <typename T, int BYTES, int THREADS>
 __device__ __forceinline__ void clean_values(char* tile, int thread) {
     typedef typename Chunk<T>::type Vec;
@@ -732,10 +733,10 @@ constexpr int kJoinSplits = 256, kWaveSplits = 16;
 // each, up to 256 registers a lane), and while the one has the matrix cores the other has the vector unit: a wavefront's 64
 // keys of 128 in bf16 are 32 products of 32 cycles, 32 exponentials of 16 and some 180 vector instructions of 4, so that neither
 // unit can be busy all the time.  4 prompts of 8192 tokens, 64 on 8 heads of 128 in bf16: 4.17 to 4.46 ms, 986 to 1055 TFLOP/s, matrix
-// cores 53% and vector unit 55% busy at 1.9 GHz (a large library product: 1094 TFLOP/s); without the loads 3.8.  A prompt of 2048, 32 heads: 52 us,
+// cores 54% and vector unit 57% busy at 1.9 GHz (a large library product: 1094 TFLOP/s); without the loads 3.8.  A prompt of 2048, 32 heads: 52 us,
 // the longest tile's 32 steps one after another.  Measured and not kept: eight wavefronts, half of them a phase behind the other
 // half and barriers between products and softmax (4.8 ms against 4.4: barriers cost more than the units' overlap gave).
-// Heads of 256 leave too few registers: 22 to 23 spilled in 16 bits (60 bytes of scratch a lane), 35 (140) in fp32, some in the loop; two wavefronts
+// Heads of 256 leave too few registers: 28 to 30 spilled in 16 bits (72 bytes of scratch a lane), 22 (80) in fp32, some in the loop; two wavefronts
 // a row's columns, or queries in LDS, would mend that.
 template <typename T, int DP, int NW, int NK, bool CLEAN>
 __device__ __forceinline__ void tile_pass(Rows<T, DP, NK>& w, Loader<T, DP, 32 * NK, 64 * NW>& ld, const Score& sc, char* lds,
@@ -863,7 +864,7 @@ __global__ __launch_bounds__(64 * NW, DP * sizeof(T) <= 512 ? 2 : 1) void k_atte
 // have tiles of 32 keys of their own, in two buffers each, and are joined at the end.  The cache's bytes bound it: 64 sequences of up
 // to 8192 keys, 32 on 8 heads of 128 in bf16, 1.05 GB in 218 us, 4.8 TB/s; one of 131072 537 MB in 109 us with its join, 4.9.
 // In fp32 the products are made for 32 rows and take longer than the bytes (64 on 8 heads over 8192 keys 38 us, 1.8 TB/s), most at a head size
-// of 256, where one wavefront fits a compute unit and 36 registers are spilled (113 us, 1.2 TB/s).
+// of 256, where one wavefront fits a compute unit and 35 registers are spilled (114 us, 1.2 TB/s).
 template <typename T, int DP, int NW, bool CLEAN>
 __device__ __forceinline__ void few_pass(Rows<T, DP, 1>& w, Loader<T, DP, 32, 64>& ld, const Score& sc, char* lds, int k0,
                                          int k1) {
@@ -1059,7 +1060,8 @@ __global__ __launch_bounds__(64 * NW) void k_attend_lanes(const AttendArgs a, co
 #pragma unroll
                 for (int e = 0; e < NV; ++e) o[i][e] *= w;
             }
-            const float p = __builtin_amdgcn_exp2f(v - (m[i] == -INFINITY ? 0.0f : m[i]) - (clean() ? kGrowth + lower[i] : kGrowth));  // 1 at most
+            const float less = clean() ? kGrowth + lower[i] : kGrowth;  // so that a weight is 1 at most
+            const float p = __builtin_amdgcn_exp2f(v - (m[i] == -INFINITY ? 0.0f : m[i]) - less);
             l[i] += p;  // each key's in the lanes that have it
 #pragma unroll
             for (int u = 0; u < U; ++u) {
